@@ -19,7 +19,7 @@ extern "C" __attribute__((visibility("hidden"))) int dg_set_error(const char* ms
 namespace dg {
 
 // words[i] != 0: error i happened (DG_ERR_* bit i) since the last dg_take_errors()
-constexpr int kNumStatusWords = 2;
+constexpr int kNumStatusWords = 5;
 
 namespace {
 std::once_flag g_status_once;

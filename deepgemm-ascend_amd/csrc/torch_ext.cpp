@@ -53,8 +53,10 @@ void check_rc(int rc) {
 // Errors that kernels of earlier calls reported through the library's sticky words (read with no
 // synchronisation; the words live in host-mapped memory).
 uint32_t pending_errors() {
-    if (g_words == nullptr || (g_words[0] == 0u && g_words[1] == 0u)) return 0;
-    return g_take();
+    if (g_words == nullptr) return 0;
+    uint32_t any = 0;
+    for (int i = 0; i < 5; ++i) any |= g_words[i];   // (a word per DG_ERR_* bit)
+    return any == 0u ? 0 : g_take();
 }
 
 // The same words as the Python layer's message (deep_gemm/_lib.py, error_message).
@@ -67,6 +69,13 @@ std::string error_message(uint32_t bits) {
         msg += "m_indices is not padded to the M-grouped alignment (every alignment-row block must hold one group "
                "id < num_groups followed only by -1 padding)";
     }
+    const std::pair<uint32_t, const char*> others[] = {
+        {DG_ERR_EXPERT_ID, "topk_idx holds an expert id >= num_groups"},
+        {DG_ERR_MOE_ROWS, "the pairs of topk_idx need more rows than num_rows"},
+        {DG_ERR_TARGET, "target holds an index outside the vocabulary"},
+    };
+    for (const auto& [bit, text] : others)
+        if (bits & bit) msg += (msg.empty() ? "" : "; ") + std::string(text);
     return msg + " [reported by a kernel of an earlier deep_gemm call]";
 }
 

@@ -24,10 +24,12 @@ DG_COMPILED_M, DG_COMPILED_N, DG_COMPILED_K = 1, 2, 4
 EXPORTED_SYMBOLS = ('dg_gemm', 'dg_transform_sf', 'dg_transform_k_grouped_sf', 'dg_transpose_to_k_major', 'dg_fp4_to_k_major', 'dg_device_num_cus', 'dg_select_config',
                     'dg_gemm_workspace_size', 'dg_last_error', 'dg_version', 'dg_jit_compile', 'dg_jit_set_include_dir',
                     'dg_jit_stats', 'dg_launch_plan', 'dg_gemm_noalloc', 'dg_take_errors', 'dg_error_words',
-                    'dg_stream_workspace')
+                    'dg_stream_workspace', 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine',
+                    'dg_moe_combine_backward', 'dg_mx_quantize', 'dg_mx_dequantize')
 
 # Sticky error bits kernels report through host-mapped words (DG_ERR_* in the header)
-DG_ERR_SF_INVALID, DG_ERR_M_INDICES = 1, 2
+DG_ERR_SF_INVALID, DG_ERR_M_INDICES, DG_ERR_EXPERT_ID, DG_ERR_MOE_ROWS, DG_ERR_TARGET = 1, 2, 4, 8, 16
+DG_MX_E2M1, DG_MX_E4M3 = 0, 1
 DG_ENOKERNEL = -3   # dg_gemm: no compiled kernel for the requested configuration
 
 
@@ -60,6 +62,25 @@ class LaunchInfo(ctypes.Structure):
         ('threads', ctypes.c_int32), ('tiles', ctypes.c_int64), ('split_k', ctypes.c_int32),
         ('persistent', ctypes.c_int32), ('skinny', ctypes.c_int32), ('plan_workgroups', ctypes.c_int64),
         ('split_reduce', ctypes.c_int32),
+    ]
+
+
+class MoELayoutArgs(ctypes.Structure):
+    """Mirror of ``dg_moe_layout`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('tokens', ctypes.c_int32), ('topk', ctypes.c_int32), ('num_groups', ctypes.c_int32), ('rows', ctypes.c_int32),
+        ('alignment', ctypes.c_int32), ('slots', ctypes.c_void_p), ('source', ctypes.c_void_p), ('psum', ctypes.c_void_p),
+        ('m_indices', ctypes.c_void_p),
+    ]
+
+
+class MxArgs(ctypes.Structure):
+    """Mirror of ``dg_mx_args`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('format', ctypes.c_int32), ('x_dtype', ctypes.c_int32), ('batches', ctypes.c_int32), ('rows', ctypes.c_int32),
+        ('k', ctypes.c_int32), ('x', ctypes.c_void_p), ('x_ld', ctypes.c_int64), ('x_batch_stride', ctypes.c_int64),
+        ('codes', ctypes.c_void_p), ('codes_ld', ctypes.c_int64), ('codes_batch_stride', ctypes.c_int64),
+        ('sf', ctypes.c_void_p), ('sf_ld', ctypes.c_int64), ('sf_batch_stride', ctypes.c_int64), ('num_cus', ctypes.c_int32),
     ]
 
 
@@ -126,6 +147,18 @@ def load(path=None) -> ctypes.CDLL:
         lib.dg_jit_set_include_dir(str(Path(__file__).resolve().parent.parent / 'csrc').encode())
         lib.dg_stream_workspace.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_int64)]
         lib.dg_stream_workspace.restype = ctypes.c_int
+        i32, i64, ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+        layout = ctypes.POINTER(MoELayoutArgs)
+        for name, argtypes in (
+                ('dg_moe_sort', [ptr, i32, layout, ptr, i64, i32, ptr]),
+                ('dg_moe_sort_workspace_size', [i32, i32, ctypes.POINTER(i64)]),
+                ('dg_moe_dispatch', [ptr, i64, i64, layout, ptr, i64, ptr, i64, i32, ptr, i64, i32, i32, ptr]),
+                ('dg_moe_combine', [ptr, i64, i32, i64, layout, ptr, ptr, i64, i32, ptr]),
+                ('dg_moe_combine_backward', [ptr, i64, ptr, i64, i32, i64, layout, ptr, ptr, i64, ptr, i32, ptr]),
+                ('dg_mx_quantize', [ctypes.POINTER(MxArgs), ptr]),
+                ('dg_mx_dequantize', [ctypes.POINTER(MxArgs), ptr])):
+            getattr(lib, name).argtypes = argtypes
+            getattr(lib, name).restype = ctypes.c_int
         lib.dg_take_errors.restype = ctypes.c_uint32
         lib.dg_take_errors.argtypes = []
         lib.dg_error_words.restype = ctypes.c_void_p
@@ -145,6 +178,12 @@ def error_message(bits: int, where: str = 'an earlier deep_gemm call') -> str:
     if bits & DG_ERR_M_INDICES:
         parts.append('m_indices is not padded to the M-grouped alignment (every alignment-row block must hold one '
                      'group id < num_groups followed only by -1 padding)')
+    if bits & DG_ERR_EXPERT_ID:
+        parts.append('topk_idx holds an expert id >= num_groups')
+    if bits & DG_ERR_MOE_ROWS:
+        parts.append('the pairs of topk_idx need more rows than num_rows')
+    if bits & DG_ERR_TARGET:
+        parts.append('target holds an index outside the vocabulary')
     return '; '.join(parts) + f' [reported by a kernel of {where}]'
 
 

@@ -43,6 +43,11 @@ def set_num_sms(n: int) -> None:
     _num_sms = int(n)
 
 
+def cu_cap() -> int:
+    """Workgroups that may run at a time under set_num_sms; 0 when it does not cap them."""
+    return _num_sms if _num_sms and _num_sms < _device_num_cus() else 0
+
+
 def get_mk_alignment_for_contiguous_layout() -> int:
     return _mk_alignment
 

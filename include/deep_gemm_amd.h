@@ -243,12 +243,18 @@ int dg_gemm_noalloc(const dg_gemm_args *args, void *stream);
  *                      err_flag = NULL) had sign or mantissa bits set;
  *   DG_ERR_M_INDICES   an M-grouped m_indices layout (DG_GEMM_MGROUPED_IDX) was not padded to
  *                      `alignment`: some alignment-row block mixed two group ids, had a group id
- *                      after a padding row, or held an id >= num_groups.
+ *                      after a padding row, or held an id >= num_groups;
+ *   DG_ERR_EXPERT_ID   an expert id given to dg_moe_sort was >= num_groups;
+ *   DG_ERR_MOE_ROWS    the pairs given to dg_moe_sort need more rows than its layout has;
+ *   DG_ERR_TARGET      a target given to the linear cross entropy lay outside the vocabulary.
  * dg_take_errors returns the DG_ERR_* bits set by kernels that completed since the last call and
  * clears them; after a hipStreamSynchronize (or event wait) it covers every call issued before
  * it, which is how a caller checks a given call at a sync point of its choosing.  dg_error_words returns the host address of the words (word i != 0: bit i). */
 #define DG_ERR_SF_INVALID 1u
 #define DG_ERR_M_INDICES 2u
+#define DG_ERR_EXPERT_ID 4u
+#define DG_ERR_MOE_ROWS 8u
+#define DG_ERR_TARGET 16u
 /* The split-K workspace the library holds for (current device, stream) -- see library_workspace in
  * dg_gemm_args -- or NULL / 0 before a call needed one.  Nothing is allocated (inspection). */
 int dg_stream_workspace(void *stream, void **ptr, int64_t *bytes);
@@ -280,6 +286,71 @@ typedef struct dg_launch_info {
                                      32x32 block of D) instead of each tile's last workgroup      */
 } dg_launch_info;
 int dg_launch_plan(const dg_gemm_args *args, dg_launch_info *info);
+
+/*
+ * Tokens sorted by expert, moved into the rows of an M-grouped contiguous layout and back.
+ *
+ * A pair is (token t, choice c), p = t * topk + c.  Pairs of an expert keep their order; expert e's rows start at a
+ * multiple of `alignment`, after those of the experts before it; `rows` (a multiple of the alignment) is the extent of
+ * the layout, and rows that hold no pair are padding.  psum and m_indices are the layout as DG_GEMM_MGROUPED_PSUM /
+ * DG_GEMM_MGROUPED_IDX (and, over K, DG_GEMM_KGROUPED) take it.
+ */
+typedef struct dg_moe_layout {
+    int32_t tokens, topk, num_groups, rows, alignment;
+    int32_t *slots;               /* [tokens][topk] row of a pair, -1 for a dropped one                    */
+    int32_t *source;              /* [rows] pair of a row, -1 for padding                                  */
+    int32_t *psum;                /* [num_groups] end of a group's rows                                    */
+    int32_t *m_indices;           /* [rows] group of a row, -1 for padding                                 */
+} dg_moe_layout;
+
+/* Fills the layout from expert ids [tokens][topk] (id_bytes 4 or 8).  A negative id drops its pair; so does an id past
+ * the last group (DG_ERR_EXPERT_ID) and a row past the layout's extent (DG_ERR_MOE_ROWS).  At most 1024 groups.  The
+ * workspace (dg_moe_sort_workspace_size bytes, NULL where that is 0) holds nothing between calls.
+ * num_cus > 0 here and below: at most that many workgroups at a time. */
+int dg_moe_sort(const void *ids, int32_t id_bytes, const dg_moe_layout *layout, void *workspace, int64_t workspace_bytes,
+                int32_t num_cus, void *stream);
+int dg_moe_sort_workspace_size(int32_t num_pairs, int32_t num_groups, int64_t *bytes);
+
+/* dst row slots[t][c] = src row t, `row_bytes` bytes each (leading dimensions in bytes).  zero_padding: padding rows are
+ * cleared (K-grouped GEMMs need that of their K padding), else left as they are.  sf (optional): required-layout scale
+ * factors [k64][sf_ld] of the tokens go to [k64][sf_out_ld] of the rows, zeros in padding rows. */
+int dg_moe_dispatch(const void *src, int64_t src_ld, int64_t row_bytes, const dg_moe_layout *layout, void *dst, int64_t dst_ld,
+                    const int16_t *sf, int64_t sf_ld, int32_t k64, int16_t *sf_out, int64_t sf_out_ld,
+                    int32_t zero_padding, int32_t num_cus, void *stream);
+
+/* out[t] = sum over c of weights[t][c] * rows[slots[t][c]] (weights NULL: 1), summed in order in fp32; rows and out of
+ * `dtype` (DG_DTYPE_BF16 / F32), leading dimensions in elements.  Also the gradient of dg_moe_dispatch (weights NULL). */
+int dg_moe_combine(const void *rows, int64_t rows_ld, int32_t dtype, int64_t width, const dg_moe_layout *layout,
+                   const float *weights, void *out, int64_t out_ld, int32_t num_cus, void *stream);
+
+/* Gradient of dg_moe_combine: d_rows[slots[t][c]] = weights[t][c] * d_out[t], padding rows zero, and
+ * d_weights[t][c] = <d_out[t], rows[slots[t][c]]> (0 for a dropped pair). */
+int dg_moe_combine_backward(const void *d_out, int64_t d_out_ld, const void *rows, int64_t rows_ld, int32_t dtype,
+                            int64_t width, const dg_moe_layout *layout, const float *weights, void *d_rows,
+                            int64_t d_rows_ld, float *d_weights, int32_t num_cus, void *stream);
+
+/*
+ * Microscaled quantisation of [batches][rows][k] values in blocks of 32 along k (k a multiple of 32) to e2m1 (two to a
+ * byte, even k low) or e4m3 codes and required-layout scale factors.  A block's scale is the smallest power of two, at
+ * least 2^-126, that keeps its values within the format; values round to nearest, ties to even; a block with an infinity
+ * or a NaN gets the exponent byte 255 (NaN) and codes 0.
+ */
+#define DG_MX_E2M1 0
+#define DG_MX_E4M3 1
+typedef struct dg_mx_args {
+    int32_t format;               /* DG_MX_*                                                               */
+    int32_t x_dtype;              /* DG_DTYPE_BF16 or DG_DTYPE_F32                                         */
+    int32_t batches, rows, k;
+    void *x;                      /* read by dg_mx_quantize, written by dg_mx_dequantize                   */
+    int64_t x_ld, x_batch_stride;             /* elements                                                  */
+    void *codes;
+    int64_t codes_ld, codes_batch_stride;     /* bytes, multiples of 8                                     */
+    int16_t *sf;
+    int64_t sf_ld, sf_batch_stride;           /* int16 elements, even                                      */
+    int32_t num_cus;
+} dg_mx_args;
+int dg_mx_quantize(const dg_mx_args *args, void *stream);
+int dg_mx_dequantize(const dg_mx_args *args, void *stream);
 
 /* Message of the last failing call on this thread ("" if none). */
 const char *dg_last_error(void);

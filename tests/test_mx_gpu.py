@@ -1,0 +1,146 @@
+"""Microscaled quantisation and its product against the oracle: codes and scale factors bit for bit, values bit for bit,
+products within their rounding."""
+import pytest
+import torch
+
+import deep_gemm
+from helpers import gen
+from oracle import mx as ox
+
+pytestmark = pytest.mark.gpu
+
+U32, UBF16 = 2.0 ** -24, 2.0 ** -8
+
+
+def _check(x, fmt, dev=None):
+    """mx_quantize of x (two dimensions) against the oracle; (codes, sf) on the device."""
+    codes, sf = deep_gemm.mx_quantize(x.cuda() if dev is None else dev, fmt)
+    m, k = x.shape
+    want, scales = ox.quantize(x, fmt)
+    assert torch.equal(ox.scale_bytes(sf.cpu(), k // 32), scales)
+    assert torch.equal(ox.unpack(codes.cpu()), want)
+    if k % 64:   # the half of the last pair that holds no block
+        assert (sf.cpu()[:, -1].to(torch.int32) >> 8 & 255 == 0).all()
+    return codes, sf
+
+
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('m,k', [(1, 32), (1, 4096), (2, 64), (7, 96), (9, 512), (65, 544), (130, 1440), (33, 7168)])
+def test_quantize(fmt, dtype, m, k):
+    x = (torch.randn(m, k, generator=gen(m + k)) * torch.exp(3 * torch.randn(m, 1, generator=gen(k)))).to(dtype)
+    codes, sf = _check(x, fmt)
+    assert codes.stride(-1) == 1 and (sf.stride(0) == 1 or m == 1)
+    for out in (torch.float32, torch.bfloat16):
+        got = deep_gemm.mx_dequantize((codes, sf), out).cpu()
+        assert torch.equal(got.double(), ox.values(*ox.quantize(x, fmt), fmt).to(out).double())
+
+
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+def test_quantize_many_rows(fmt):
+    """The tall tiles (64 rows)."""
+    x = torch.randn(16400, 2080, generator=gen(1)).bfloat16().cuda()
+    codes, sf = deep_gemm.mx_quantize(x, fmt)
+    for part in (slice(0, 40), slice(8180, 8220), slice(16380, 16400)):
+        want, scales = ox.quantize(x[part].cpu(), fmt)
+        assert torch.equal(ox.unpack(codes[part].cpu()), want) and torch.equal(ox.scale_bytes(sf[part].cpu(), 65), scales)
+    small = deep_gemm.mx_quantize(x[:100], fmt)
+    assert torch.equal(codes[:100].view(torch.int8), small[0].view(torch.int8)) and torch.equal(sf[:100], small[1])
+    back = deep_gemm.mx_dequantize((codes, sf))
+    assert torch.equal(back[:100], deep_gemm.mx_dequantize(small))
+    assert torch.equal(back[-20:].cpu().double(), ox.values(want, scales, fmt))
+
+
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_edges(fmt, dtype):
+    """Ties, block maxima on either side of the format's largest value, zeros of both signs, numbers near the ends of the
+    type's range, and numbers below the smallest normal one."""
+    top = 6.0 if fmt == 'e2m1' else 448.0
+    table = torch.tensor(ox.E2M1 if fmt == 'e2m1' else ox.E4M3[::5])
+    mids = (table[1:] + table[:-1]) / 2
+    rows = []
+    for block in torch.cat((table, mids, -mids, -table)).split(30):
+        rows.append(torch.cat((torch.tensor([top, -top]), torch.nn.functional.pad(block, (0, 30 - block.numel())))))
+    for amax in (top, top * (1 + 2.0 ** -7), top * (1 - 2.0 ** -7), 1.0, 2.0 ** -126, 1.5 * 2.0 ** -125, 2.0 ** -130, 0.0, 3e38, 2.0 ** 127):
+        rows.append(torch.linspace(-amax, amax, 32, dtype=torch.float64).float())
+    x = torch.stack(rows).to(dtype)
+    x = torch.cat((x, -x, torch.zeros_like(x[:1]), -torch.zeros_like(x[:1])))
+    _check(x, fmt)
+
+
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+def test_infinities_and_nan(fmt):
+    """A block with an infinity or a NaN is NaN, its neighbours are not; so is what a product makes of it."""
+    x = torch.randn(5, 128, generator=gen(2))
+    x[1, 40], x[2, 127], x[3, 0] = float('inf'), float('nan'), float('-inf')
+    codes, sf = _check(x, fmt)
+    back = deep_gemm.mx_dequantize((codes, sf), torch.float32).cpu()
+    bad = torch.zeros(5, 4, dtype=torch.bool)
+    bad[1, 1] = bad[2, 3] = bad[3, 0] = True
+    assert torch.equal(back.isnan(), bad.repeat_interleave(32, dim=1))
+    w = deep_gemm.mx_quantize(torch.randn(48, 128, generator=gen(3)).cuda(), 'e2m1')
+    d = torch.empty(5, 48, dtype=torch.float32, device='cuda')
+    deep_gemm.mx_gemm_nt(x.cuda(), w, d, fmt)
+    assert torch.equal(d.cpu().isnan().all(dim=1), bad.any(dim=1)) and not d.cpu()[[0, 4]].isnan().any()
+
+
+def test_strides_and_batches():
+    x = torch.randn(3, 21, 160, generator=gen(4)).bfloat16()
+    for fmt in ('e2m1', 'e4m3'):
+        codes, sf = deep_gemm.mx_quantize(x.cuda(), fmt)
+        for i in range(3):
+            want, scales = ox.quantize(x[i], fmt)
+            assert torch.equal(ox.unpack(codes[i].cpu()), want) and torch.equal(ox.scale_bytes(sf[i].cpu(), 5), scales)
+        assert torch.equal(deep_gemm.mx_dequantize((codes, sf))[1], deep_gemm.mx_dequantize((codes[1], sf[1])))
+        wide = torch.zeros(21, 171, dtype=torch.bfloat16, device='cuda')
+        wide[:, 3:163] = x[0].cuda()
+        _check(x[0], fmt, wide[:, 3:163])
+        _check(x[0], fmt, x[0].t().contiguous().t().cuda())
+        _check(x[0, ::2], fmt, x[0].cuda()[::2])
+        _check(x[0, :, :96], fmt, x[0].cuda()[:, :96])
+
+
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+@pytest.mark.parametrize('m,n,k', [(1, 64, 32), (1, 1000, 4096), (3, 129, 96), (16, 2112, 1440), (17, 300, 7168), (129, 257, 544),
+                                   (300, 512, 2048)])
+def test_product(fmt, m, n, k):
+    x, w = torch.randn(m, k, generator=gen(m)).bfloat16(), torch.randn(n, k, generator=gen(n)) * k ** -0.5
+    q = deep_gemm.mx_quantize(w.cuda(), 'e2m1')
+    a = ox.values(*ox.quantize(x, fmt), fmt)
+    b = ox.values(*ox.quantize(w, 'e2m1'), 'e2m1')
+    ref, mag = a @ b.t(), a.abs() @ b.abs().t()
+    for dtype in (torch.bfloat16, torch.float32):
+        d = torch.full((m, n), float('nan'), dtype=dtype, device='cuda')
+        deep_gemm.mx_gemm_nt(x.cuda(), q, d, fmt)
+        bound = k * U32 * mag
+        if dtype == torch.bfloat16:
+            bound = bound * (1 + UBF16) + UBF16 * ref.abs()
+        assert ((d.cpu().double() - ref).abs() <= bound).all()
+    c = d.clone()
+    deep_gemm.mx_gemm_nt(x.cuda(), q, c, fmt, c=c)
+    assert ((c.cpu().double() - 2 * ref).abs() <= 2 * (k + 1) * U32 * mag).all()
+
+
+def test_quantize_under_a_cu_cap_and_in_a_graph():
+    x = torch.randn(500, 1056, generator=gen(5)).bfloat16().cuda()
+    want = deep_gemm.mx_quantize(x)
+    full = deep_gemm.get_num_sms()
+    try:
+        deep_gemm.set_num_sms(24)
+        got = deep_gemm.mx_quantize(x)
+    finally:
+        deep_gemm.set_num_sms(full)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    stream = torch.cuda.Stream()
+    buf = x.clone()
+    with torch.cuda.stream(stream):
+        stream.wait_stream(torch.cuda.default_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            back = deep_gemm.mx_dequantize(deep_gemm.mx_quantize(buf))
+    for scale in (1.0, 3.0, 0.25):
+        buf.copy_(x * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(back, deep_gemm.mx_dequantize(deep_gemm.mx_quantize(buf)))

@@ -1,0 +1,138 @@
+"""Argument checks of the operators around the GEMMs, through the C ABI and the Python layer (nothing is launched)."""
+import ctypes
+
+import pytest
+import torch
+
+import deep_gemm
+from deep_gemm import _lib
+from oracle import moe as om, mx as ox
+
+
+@pytest.fixture(scope='module')
+def lib():
+    return _lib.load()
+
+
+def _layout(tokens=2, topk=2, groups=4, rows=64, alignment=32, ptr=4096):
+    return _lib.MoELayoutArgs(tokens, topk, groups, rows, alignment, ptr, ptr, ptr, ptr)
+
+
+def _refused(lib, rc, text):
+    assert rc == -1 and text in lib.dg_last_error().decode(), lib.dg_last_error()
+
+
+def test_sort_refusals(lib):
+    sort = lambda layout, ids=4096, size=4, ws=None, n=0: lib.dg_moe_sort(ids, size, layout, ws, n, 0, None)
+    _refused(lib, sort(None), 'null layout')
+    _refused(lib, sort(_layout(), size=2), 'int32 or int64')
+    _refused(lib, sort(_layout(groups=0)), '1024 groups')
+    _refused(lib, sort(_layout(groups=1025)), '1024 groups')
+    _refused(lib, sort(_layout(rows=65)), 'multiple of the alignment')
+    _refused(lib, sort(_layout(alignment=0)), 'multiple of the alignment')
+    _refused(lib, sort(_layout(), ids=None), 'null tensor')
+    _refused(lib, sort(_layout(ptr=None)), 'null tensor')
+    _refused(lib, sort(_layout(tokens=-1)), 'invalid size')
+    _refused(lib, sort(_layout(tokens=1 << 20, topk=1 << 12)), 'invalid size')
+    _refused(lib, sort(_layout(tokens=1 << 28, topk=4, groups=1024, rows=0, alignment=1 << 21)), 'too many rows')
+    _refused(lib, sort(_layout(tokens=1 << 15, topk=8)), 'workspace')
+    need = ctypes.c_int64()
+    assert lib.dg_moe_sort_workspace_size(128, 256, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.dg_moe_sort_workspace_size(1 << 18, 256, ctypes.byref(need)) == 0 and need.value > 0
+    _refused(lib, lib.dg_moe_sort_workspace_size(-1, 4, ctypes.byref(need)), 'invalid size')
+
+
+def test_movement_refusals(lib):
+    d = lambda layout=None, src=4096, sld=64, rb=64, dst=4096, dld=64, sf=None, sfo=None, oload=64: lib.dg_moe_dispatch(
+        src, sld, rb, layout or _layout(), dst, dld, sf, 2, 1, sfo, oload, 1, 0, None)
+    _refused(lib, d(sld=32), 'leading dimension')
+    _refused(lib, d(dld=32), 'leading dimension')
+    _refused(lib, d(src=None), 'null tensor')
+    _refused(lib, d(dst=None), 'null tensor')
+    _refused(lib, d(sf=4096, sfo=4096, oload=65), 'scale factors')
+    _refused(lib, d(sf=4096, sfo=None), 'scale factors')
+    c = lambda dtype=0, rows=4096, ld=64, out=4096: lib.dg_moe_combine(rows, ld, dtype, 64, _layout(), None, out, 64, 0, None)
+    _refused(lib, c(dtype=2), 'bf16 or fp32')
+    _refused(lib, c(ld=8), 'leading dimension')
+    _refused(lib, c(rows=None), 'null tensor')
+    _refused(lib, c(out=None), 'null tensor')
+    b = lambda w=4096, dtype=1, ld=64: lib.dg_moe_combine_backward(4096, 64, 4096, ld, dtype, 64, _layout(), w, 4096, 64, 4096, 0, None)
+    _refused(lib, b(w=None), 'null tensor')
+    _refused(lib, b(dtype=2), 'bf16 or fp32')
+    _refused(lib, b(ld=63), 'leading dimension')
+    # nothing to do
+    assert lib.dg_moe_combine(None, 64, 0, 64, _layout(tokens=0), None, None, 64, 0, None) == 0
+    assert lib.dg_moe_dispatch(None, 64, 64, _layout(rows=0), None, 64, None, 0, 0, None, 0, 1, 0, None) == 0
+
+
+def test_mx_refusals(lib):
+    def run(fn='dg_mx_quantize', **kw):
+        a = _lib.MxArgs(0, 0, 1, 4, 64, 4096, 64, 0, 4096, 32, 0, 4096, 4, 0, 0)
+        for name, v in kw.items():
+            setattr(a, name, v)
+        return getattr(lib, fn)(a, None)
+    for fn in ('dg_mx_quantize', 'dg_mx_dequantize'):
+        _refused(lib, run(fn, format=2), 'unknown format')
+        _refused(lib, run(fn, x_dtype=2), 'bf16 or fp32')
+        _refused(lib, run(fn, k=48), 'block of 32')
+        _refused(lib, run(fn, rows=-1), 'negative size')
+        _refused(lib, run(fn, x=None), 'null tensor')
+        _refused(lib, run(fn, x_ld=63), 'leading dimension')
+        _refused(lib, run(fn, format=1), 'leading dimension')
+        _refused(lib, run(fn, sf_ld=5), 'even')
+        _refused(lib, run(fn, codes_ld=36), '8-byte aligned')
+        assert run(fn, rows=0) == 0 and run(fn, k=0) == 0
+    assert lib.dg_mx_quantize(None, None) == -1
+
+
+def test_python_refusals():
+    with pytest.raises(RuntimeError, match='int32 or int64'):
+        deep_gemm.moe_sort(torch.zeros(2, 2), 4)
+    with pytest.raises(RuntimeError, match='device tensor'):
+        deep_gemm.moe_sort(torch.zeros(2, 2, dtype=torch.int32), 4)
+    with pytest.raises(RuntimeError, match='device tensor'):
+        deep_gemm.mx_quantize(torch.zeros(2, 64))
+    with pytest.raises(RuntimeError, match='unknown format'):
+        deep_gemm.mx_quantize(torch.zeros(2, 64), 'e5m2')
+    with pytest.raises(RuntimeError, match='e2m1 weights'):
+        deep_gemm.mx_gemm_nt(torch.zeros(2, 64), (torch.zeros(4, 64, dtype=torch.float8_e4m3fn), None), torch.zeros(2, 4))
+    layout = deep_gemm.MoELayout(*(torch.zeros(s, dtype=torch.int32) for s in ((2, 2), (64,), (4,), (64,))))
+    with pytest.raises(RuntimeError, match='device tensor'):
+        deep_gemm.moe_dispatch(torch.zeros(2, 64), layout)
+    with pytest.raises(RuntimeError, match='device tensor'):
+        deep_gemm.moe_combine(torch.zeros(64, 64), layout)
+    with pytest.raises(RuntimeError, match='contiguous int32'):
+        deep_gemm.moe_combine(torch.zeros(64, 64), layout._replace(source=torch.zeros(64)))
+
+
+def test_num_rows_bounds_every_routing():
+    g = torch.Generator().manual_seed(0)
+    for pairs, groups, alignment in ((0, 4, 32), (1, 4, 32), (5, 9, 64), (100, 7, 32), (1000, 300, 128)):
+        deep_gemm.set_mk_alignment_for_contiguous_layout(alignment)
+        try:
+            m = deep_gemm.moe_num_rows(pairs, groups)
+        finally:
+            deep_gemm.set_mk_alignment_for_contiguous_layout(256)
+        assert m % alignment == 0
+        for kind in range(3):
+            ids = torch.randint(0, groups, (pairs, 1), generator=g) if kind == 0 else torch.arange(pairs).view(-1, 1) % groups if kind == 1 \
+                else (torch.arange(pairs).view(-1, 1) % groups).clamp(max=min(groups, pairs) - 1)
+            counts = torch.bincount(ids.reshape(-1), minlength=groups)
+            assert int(((counts + alignment - 1) // alignment * alignment).sum()) <= m
+            assert (om.sort(ids, groups, alignment, m)[0] >= 0).all()
+
+
+def test_oracle_quantisation_is_nearest():
+    """No value of the format lies nearer than the one the oracle takes, and its codes decode to multiples of the step."""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, 64, generator=g) * torch.exp(2 * torch.randn(6, 1, generator=g))
+    for fmt, table in (('e2m1', ox.E2M1), ('e4m3', ox.E4M3)):
+        codes, scales = ox.quantize(x, fmt)
+        got = ox.values(codes, scales, fmt)
+        s = torch.exp2(scales.double() - 127).repeat_interleave(32, dim=1)
+        near = (x.double().abs().unsqueeze(-1) - s.unsqueeze(-1) * torch.tensor(table, dtype=torch.float64)).abs().amin(-1)
+        assert torch.equal((x.double() - got).abs(), near)
+        top = 6.0 if fmt == 'e2m1' else 448.0
+        amax = x.double().abs().view(6, 2, 32).amax(-1)
+        blocks = torch.exp2(scales.double() - 127)
+        assert (amax <= top * blocks).all() and (amax > top * blocks / 2).all()
