@@ -771,8 +771,10 @@ std::unique_lock<std::mutex> stream_order(hipStream_t st) {
 }
 
 // Checks, plans and launches one GEMM; with `info` it stops short of the launch and describes it.
+// `k_rows` > 0 (a tile plan of MN-major operands, forced by the caller): K rows that those operands have; k is that, rounded
+// up to whole 16-byte pieces of a K-major operand's rows, which hold zeros past k_rows.
 int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_launch_info* info = nullptr,
-              bool noalloc = false) {
+              bool noalloc = false, int k_rows = 0) {
     using namespace dg;
     if (args == nullptr) return dg_set_error("dg_gemm: null args");
     const dg_gemm_args& a = *args;
@@ -978,7 +980,7 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
     p.sfb = reinterpret_cast<const uint16_t*>(a.sfb);
     p.bias = reinterpret_cast<const uint8_t*>(a.bias);
     p.layout = a.grouped_layout;
-    p.m = a.m; p.n = a.n; p.k = a.k; p.num_groups = a.num_groups;
+    p.m = a.m; p.n = a.n; p.k = k_rows > 0 ? k_rows : a.k; p.num_groups = a.num_groups;
     p.lda = lda_b; p.ldb = ldb_b; p.ldd = a.ldd;
     p.bsa = a.batch_stride_a * esz_a; p.bsb = a.batch_stride_b * esz_b; p.bsd = a.batch_stride_d;
     p.sfa_ld = a.sfa_ld; p.sfb_ld = a.sfb_ld; p.sfa_bs = a.sfa_batch_stride; p.sfb_bs = a.sfb_batch_stride;
@@ -1171,6 +1173,43 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
 }  // namespace
 
 extern "C" int dg_gemm(const dg_gemm_args* args, void* stream) { return gemm_impl(args, stream, false); }
+
+namespace dg {
+
+// The gradient products of the linear cross entropy (linear_xent.hip): a dense bf16 GEMM on the four-wave tile and K split of
+// bf16_tile_plan below.
+int gemm_k_rows(const dg_gemm_args* args, int k_rows, void* stream) { return gemm_impl(args, stream, false, nullptr, false, k_rows); }
+
+// The four-wave tile of a dense bf16 problem (mn: an operand is MN-major) and its K split, at most `most`, by the planner's
+// cost model; the bytes of fp32 partials a split needs.
+void bf16_tile_plan(int m, int n, int k, bool mn, int most, int cus, int& bm, int& bn, int& split, int64_t& partial_bytes) {
+    dg_gemm_args a = {};
+    a.kind = kBF16; a.gemm_type = kNormal; a.m = m; a.n = n; a.k = k; a.num_groups = 1;
+    const int ns = std::max(1, ceil_div(k, 64));
+    double best = 1e300;
+    for (QuadRate q : kQuadBf16) {
+        if (!quad_tile(kBF16, q.bm, q.bn)) continue;
+        if (mn && q.bm == 128) q = kQuadMn128;
+        if (mn) q.fixed += kQuadMnFixedBf16;
+        TileCfg tc = {};
+        tc.bm = q.bm; tc.bn = q.bn;
+        const int64_t tiles = plan_tiles(a, tc), slots = (int64_t)cus * q.occ;
+        for (int sp = 1; sp <= most && sp <= ns; ++sp) {
+            if (sp > 1 && (tiles * sp > slots || tiles > kMaxSplitTiles || ns < 4 * sp)) break;
+            const int sps = ceil_div(ns, sp);
+            if (ceil_div(ns, sps) != sp) continue;
+            double t = quad_time(q, tiles * sp, sps, cus);
+            if (sp > 1) t += 3.5 + 8.0 * sp * m * (double)n / 7e6;
+            if (t < best) {
+                best = t;
+                bm = q.bm; bn = q.bn; split = sp;
+                partial_bytes = sp > 1 ? kCounterBytes + tiles * sp * (int64_t)q.bm * q.bn * 4 : 0;
+            }
+        }
+    }
+}
+
+}  // namespace dg
 
 extern "C" int dg_stream_workspace(void* stream, void** ptr, int64_t* bytes) {
     if (ptr == nullptr || bytes == nullptr) return dg_set_error("dg_stream_workspace: null argument");

@@ -1,0 +1,584 @@
+// Cross entropy of a linear layer over a large vocabulary, without keeping the logits.
+//
+//   z[t][v] = <x[t], w[v]>,  lse[t] = log sum_v exp z[t][v],  loss[t] = lse[t] - z[t][target[t]]
+//   d[t][v] = (exp(z[t][v] - lse[t]) - [v = target[t]]) d_loss[t],  d_x = d w,  d_w = d^T x
+//
+// Forward: the bf16 tile kernel (quad_kernel.hpp) computes a tile of logits, and instead of storing it each row leaves its
+// maximum, the sum of its exponentials under that maximum and, in the one tile that has it, the target's logit; a second
+// kernel joins a row's tiles.  Nothing of tokens x vocabulary is written.
+// Backward, a piece of the vocabulary at a time: the logits are computed again, d leaves the tile in bf16, and two products take
+// it on.  d is rounded to bf16 because the matrix unit takes it so; that error is as large as that of the bf16 inputs and
+// outputs beside it.  It is rounded in units of the largest |d_loss|, which both products multiply their fp32 sums by: with
+// the equal weights of a mean the targets' entries are then p - 1, nearly exact, where 1 / tokens rounded to 8 bits put the
+// same error of up to 0.4 % into all of them (777 tokens: gradients 0.25 % off against 0.17 % of the outputs' rounding alone).
+// Logits, maxima, sums, losses and the sum of d_x over the pieces are fp32.
+#include "op_launch.hpp"
+#include "quad_kernel.hpp"
+
+namespace dg {
+
+int gemm_k_rows(const dg_gemm_args* args, int k_rows, void* stream);
+void bf16_tile_plan(int m, int n, int k, bool mn, int most, int cus, int& bm, int& bn, int& split, int64_t& partial_bytes);
+int device_cus();
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct XentParams {
+    const void* target;        // [tokens] int32 or int64
+    int wide;
+    int tokens, rows;          // rows: tokens rounded up to whole K pieces of the gradient's product (zero rows)
+    int first, vocab;          // first word of the piece, words in all
+    int64_t ignore;
+    float* target_logit;       // [tokens]
+    f32x2* stats;              // forward: [tile columns][tokens] (maximum, sum)
+    const float *lse, *d_loss; // backward
+    const float* unit;         // backward: 1 / u and u, the unit of d
+    uint16_t* d;               // backward: [rows][d_ld] bf16, whole tiles wide
+    int64_t d_ld;
+};
+
+// Target of token t, or -1 where it counts for nothing (ignored, or outside the vocabulary).
+__device__ __forceinline__ int target_of(const void* target, int wide, int64_t ignore, int vocab, int t) {
+    const int64_t v = wide ? reinterpret_cast<const int64_t*>(target)[t] : reinterpret_cast<const int32_t*>(target)[t];
+    return v == ignore || v < 0 || v >= vocab ? -1 : (int)v;
+}
+
+// Columns of a lane within its row of a tile: four runs of four to a 32-column block.
+__device__ __forceinline__ int run_col(int block_col, int q, int e) { return block_col + 4 * q + 8 * (e >> 2) + (e & 3); }
+
+// The logits of one row block that a lane holds: NB blocks of 16, with their first columns within the tile.
+template <typename T, typename TAKE, typename COL, typename HA, typename I, int NB>
+__device__ __forceinline__ void take_row(TAKE& take, COL& col_of, HA ha, I i, f32x16 (&z)[NB], int (&col)[NB]) {
+    using SB = typename T::SB;
+    static_for<NB>([&](auto b_c) {
+        constexpr int b = decltype(b_c)::value, hb = b >= SB::NB0, j = hb ? b - SB::NB0 : b;
+        z[b] = take(ha, Int<hb>{}, i, Int<j>{});
+        col[b] = col_of(Int<hb>{}) + j * 32;
+    });
+}
+
+struct StatsTail {
+    static constexpr bool kOn = true;
+    XentParams x;
+
+    template <typename T, typename TAKE, typename ROW, typename COL>
+    __device__ __forceinline__ void run(TAKE& take, ROW& row_of, COL& col_of, const TileLoc& tl, uint8_t* smem) const {
+        using SA = typename T::SA;
+        using SB = typename T::SB;
+        constexpr int BM = SA::H0 + SA::H1, BN = SB::H0 + SB::H1, NB = SB::NB0 + SB::NB1;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1, r = lane & 31, q = lane >> 5;
+        const int cols = x.vocab - x.first - tl.n0;          // columns of the tile that are words
+        f32x2* const st = reinterpret_cast<f32x2*>(smem);    // [2][BM]: of each wave column
+        __syncthreads();                                     // (every wave has read its last fragments)
+        static_for<2>([&](auto ha_c) {
+            static_for<SA::nb(decltype(ha_c)::value)>([&](auto i_c) {
+                const int m = row_of(ha_c, i_c, wm, r);
+                f32x16 z[NB];
+                int col[NB];
+                take_row<T>(take, col_of, ha_c, i_c, z, col);
+                const int tc = m < x.tokens ? target_of(x.target, x.wide, x.ignore, x.vocab, m) - x.first - tl.n0 : -1;
+                if (cols < BN) {                     // (the last tile: columns past the vocabulary)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (run_col(col[b], q, e) >= cols) z[b][e] = -__builtin_inff();
+                }
+                // (few row blocks have a target among their columns: the search is a branch of the wave)
+                if (__ballot((unsigned)tc < (unsigned)BN) != 0) {
+                    float hit = 0.f;
+                    bool mine = false;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const bool here = run_col(col[b], q, e) == tc;
+                            hit = here ? z[b][e] : hit;
+                            mine = mine || here;
+                        }
+                    if (mine) x.target_logit[m] = hit;
+                }
+                float top[4] = {z[0][0], z[0][1], z[0][2], z[0][3]};
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top[e & 3] = fmaxf(top[e & 3], z[b][e]);
+                float row_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                row_top = fmaxf(row_top, __shfl_xor(row_top, 32, 64));
+                // exponents in units of log 2: one multiply-add each (a row of nothing but -inf: exponentials of zero)
+                const float shift = row_top == -__builtin_inff() ? 0.f : row_top * kLog2e;
+                float sum[4] = {};
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sum[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[b][e], kLog2e, -shift));
+                float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                s += __shfl_xor(s, 32, 64);
+                if (q == 0) st[wn * BM + m - tl.m0] = f32x2{row_top, s};
+            });
+        });
+        __syncthreads();
+        const int m = tl.m0 + (int)threadIdx.x;
+        if ((int)threadIdx.x < BM && m < x.tokens) {
+            const f32x2 a = st[threadIdx.x], b = st[BM + threadIdx.x];
+            const float top = fmaxf(a[0], b[0]), shift = top == -__builtin_inff() ? 0.f : top;
+            const float s = a[1] * __builtin_amdgcn_exp2f((a[0] - shift) * kLog2e) + b[1] * __builtin_amdgcn_exp2f((b[0] - shift) * kLog2e);
+            x.stats[(int64_t)(tl.n0 / BN) * x.tokens + m] = f32x2{top, s};
+        }
+    }
+};
+
+// Runs of four columns of a lane (and its partner in the wave's other half) -> 16 columns in a row, as two pieces of 16 bytes.
+__device__ __forceinline__ void runs_of_16(const i32x2 (&pk)[4], i32x4 (&w)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const auto s02 = __builtin_amdgcn_permlane32_swap(pk[2][h], pk[0][h], false, false);
+        const auto s13 = __builtin_amdgcn_permlane32_swap(pk[3][h], pk[1][h], false, false);
+        w[0][h] = (int)s02[0]; w[0][2 + h] = (int)s02[1];
+        w[1][h] = (int)s13[0]; w[1][2 + h] = (int)s13[1];
+    }
+}
+
+struct GradTail {
+    static constexpr bool kOn = true;
+    XentParams x;
+
+    template <typename T, typename TAKE, typename ROW, typename COL>
+    __device__ __forceinline__ void run(TAKE& take, ROW& row_of, COL& col_of, const TileLoc& tl, uint8_t*) const {
+        using SA = typename T::SA;
+        using SB = typename T::SB;
+        constexpr int BN = SB::H0 + SB::H1, NB = SB::NB0 + SB::NB1;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, r = lane & 31, q = lane >> 5;
+        const int cols = x.vocab - x.first - tl.n0;
+        const float per_unit = x.unit[0];
+        static_for<2>([&](auto ha_c) {
+            static_for<SA::nb(decltype(ha_c)::value)>([&](auto i_c) {
+                const int m = row_of(ha_c, i_c, wm, r);
+                f32x16 z[NB];
+                int col[NB];
+                take_row<T>(take, col_of, ha_c, i_c, z, col);
+                const int target = m < x.tokens ? target_of(x.target, x.wide, x.ignore, x.vocab, m) : -1;
+                const float lse = target >= 0 ? x.lse[m] * kLog2e : 0.f, g = target >= 0 ? x.d_loss[m] * per_unit : 0.f;
+                const int tc = target - x.first - tl.n0;
+                const bool some = __ballot(target >= 0 && (unsigned)tc < (unsigned)BN) != 0;   // (a target among the columns)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float d[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) d[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[b][e], kLog2e, -lse));
+                    if (some) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) d[e] -= run_col(col[b], q, e) == tc ? 1.f : 0.f;
+                    }
+                    if (cols < BN) {                 // (the last tile: columns past the vocabulary)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (run_col(col[b], q, e) >= cols) d[e] = 0.f;
+                    }
+                    i32x2 pk[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        pk[t] = i32x2{(int)pack_bf16x2(d[4 * t] * g, d[4 * t + 1] * g), (int)pack_bf16x2(d[4 * t + 2] * g, d[4 * t + 3] * g)};
+                    if (target < 0) {                // (zeros whatever the logits)
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) pk[t] = i32x2{0, 0};
+                    }
+                    i32x4 w[2];
+                    runs_of_16(pk, w);
+                    if (m < x.rows) {
+                        uint16_t* const d = x.d + (int64_t)m * x.d_ld + tl.n0 + col[b] + (q ? 0 : 16);
+                        *reinterpret_cast<i32x4*>(d) = w[0];
+                        *reinterpret_cast<i32x4*>(d + 8) = w[1];
+                    }
+                }
+            });
+        });
+    }
+};
+
+// d_w's tile: the sums in units of d, as bf16.
+struct WeightTail {
+    static constexpr bool kOn = true;
+    XentParams x;
+    uint16_t* d_w;             // [words][ld]
+    int64_t ld;
+    int words, width;
+
+    template <typename T, typename TAKE, typename ROW, typename COL>
+    __device__ __forceinline__ void run(TAKE& take, ROW& row_of, COL& col_of, const TileLoc& tl, uint8_t*) const {
+        using SA = typename T::SA;
+        using SB = typename T::SB;
+        constexpr int NB = SB::NB0 + SB::NB1;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, r = lane & 31, q = lane >> 5;
+        const float unit = x.unit[1];
+        static_for<2>([&](auto ha_c) {
+            static_for<SA::nb(decltype(ha_c)::value)>([&](auto i_c) {
+                const int m = row_of(ha_c, i_c, wm, r);
+                f32x16 z[NB];
+                int col[NB];
+                take_row<T>(take, col_of, ha_c, i_c, z, col);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    i32x2 pk[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        pk[t] = i32x2{(int)pack_bf16x2(z[b][4 * t] * unit, z[b][4 * t + 1] * unit),
+                                      (int)pack_bf16x2(z[b][4 * t + 2] * unit, z[b][4 * t + 3] * unit)};
+                    i32x4 w[2];
+                    runs_of_16(pk, w);
+                    const int n = tl.n0 + col[b] + (q ? 0 : 16);
+                    uint16_t* const d = d_w + (int64_t)m * ld + n;
+                    // (a row ends after a multiple of 8 values)
+                    if (m < words && n < width) *reinterpret_cast<i32x4*>(d) = w[0];
+                    if (m < words && n + 8 < width) *reinterpret_cast<i32x4*>(d + 8) = w[1];
+                }
+            });
+        });
+    }
+};
+
+template <int BM, int BN, typename TAIL>
+__global__ __launch_bounds__(256, (quad_occupancy<BM, BN, kBF16, false, false>())) void xent_tile_kernel(const KParams p, const XentParams x) {
+    quad_body<BM, BN, kBF16, kEpiBf16, kNormal, 1, 0, 0, 0, false, false, TAIL>(p, blockIdx.x + p.vbase, TAIL{x});
+}
+
+template <int BM, int BN>
+__global__ __launch_bounds__(256, (quad_occupancy<BM, BN, kBF16, true, true>())) void xent_weight_kernel(const KParams p, const WeightTail tail) {
+    quad_body<BM, BN, kBF16, kEpiBf16, kNormal, 1, 0, 0, 0, true, true, WeightTail>(p, blockIdx.x + p.vbase, tail);
+}
+
+struct UnitParams {
+    const float* d_loss;
+    const void* target;
+    int wide, tokens, vocab;
+    int64_t ignore;
+    float* unit;               // 1 / u, u
+    int vbase;
+};
+
+// u = the largest |d_loss| of a token with a target (1 where that, or its reciprocal, is no normal number).
+__global__ __launch_bounds__(1024) void xent_unit_kernel(const UnitParams p) {
+    __shared__ float part[16];
+    float top = 0.f;
+#pragma unroll 8
+    for (int t = threadIdx.x; t < p.tokens; t += 1024)
+        if (target_of(p.target, p.wide, p.ignore, p.vocab, t) >= 0) top = fmaxf(top, fabsf(p.d_loss[t]));
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
+    const bool usable = top >= 0x1p-100f && top <= 0x1p100f;
+    p.unit[0] = usable ? 1.f / top : 1.f;
+    p.unit[1] = usable ? top : 1.f;
+}
+
+struct JoinParams {
+    const f32x2* stats;
+    const float* target_logit;
+    const void* target;
+    int wide, tokens, vocab, tiles;
+    int64_t ignore;
+    float *loss, *lse;
+    uint32_t* status;
+    int vbase;
+};
+
+// A row's tiles joined: TOK rows of a workgroup, 256 / TOK threads a row; their results meet lane by lane, then wave by wave.
+template <int TOK>
+__global__ __launch_bounds__(256) void xent_join_kernel(const JoinParams p) {
+    constexpr int PARTS = 256 / TOK;
+    __shared__ f32x2 part[4][TOK];
+    const int tid = threadIdx.x, tok = tid % TOK, slice = tid / TOK, t = (blockIdx.x + p.vbase) * TOK + tok;
+    float top = -__builtin_inff(), sum = 0.f;
+    auto join = [&](f32x2 v) {
+        const float both = fmaxf(top, v[0]), shift = both == -__builtin_inff() ? 0.f : both;
+        sum = sum * __builtin_amdgcn_exp2f((top - shift) * kLog2e) + v[1] * __builtin_amdgcn_exp2f((v[0] - shift) * kLog2e);
+        top = both;
+    };
+    if (t < p.tokens) {
+        for (int i = slice; i < p.tiles; i += 8 * PARTS) {
+            f32x2 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                v[u] = i + u * PARTS < p.tiles ? p.stats[(int64_t)(i + u * PARTS) * p.tokens + t] : f32x2{-__builtin_inff(), 0.f};
+#pragma unroll
+            for (int u = 0; u < 8; ++u) join(v[u]);
+        }
+    }
+#pragma unroll
+    for (int off = TOK; off < 64; off <<= 1) join(f32x2{__shfl_xor(top, off, 64), __shfl_xor(sum, off, 64)});
+    if ((tid & 63) < TOK) part[tid >> 6][tok] = f32x2{top, sum};
+    __syncthreads();
+    if (slice != 0 || t >= p.tokens) return;
+    for (int i = 1; i < 4; ++i) join(part[i][tok]);
+    const float lse = top + kLn2 * __builtin_amdgcn_logf(sum);
+    const int64_t raw = p.wide ? reinterpret_cast<const int64_t*>(p.target)[t] : reinterpret_cast<const int32_t*>(p.target)[t];
+    const int target = target_of(p.target, p.wide, p.ignore, p.vocab, t);
+    if (raw != p.ignore && target < 0 && p.status != nullptr) p.status[4] = 1u;
+    p.lse[t] = lse;
+    p.loss[t] = target < 0 ? 0.f : lse - p.target_logit[t];
+}
+
+struct CastParams {
+    const float* src;          // [rows][width], whole rows together, in units of d
+    const float* unit;
+    uint16_t* dst;             // [rows][ld]
+    int64_t ld;
+    int rows, chunks;          // eight values each
+    int vbase;
+};
+
+__global__ __launch_bounds__(256) void xent_cast_kernel(const CastParams p) {
+    const int64_t e = (int64_t)(blockIdx.x + p.vbase) * 256 + threadIdx.x;
+    const int64_t row = e / p.chunks;
+    if (row >= p.rows) return;
+    const int c = (int)(e - row * p.chunks) * 8;
+    const float* const s = p.src + row * p.chunks * 8 + c;
+    const float unit = p.unit[1];
+    const f32x4 a = *reinterpret_cast<const f32x4*>(s) * unit, b = *reinterpret_cast<const f32x4*>(s + 4) * unit;
+    *reinterpret_cast<i32x4*>(p.dst + row * p.ld + c) = i32x4{(int)pack_bf16x2(a[0], a[1]), (int)pack_bf16x2(a[2], a[3]),
+                                                             (int)pack_bf16x2(b[0], b[1]), (int)pack_bf16x2(b[2], b[3])};
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// Tokens of one call: the gradient's product reads d MN-major, whose K rows (tokens) times a tile's words stay below 1 GiB.
+constexpr int kMaxTokens = 1 << 20;
+
+int64_t rows_of(int tokens) { return align_up64(tokens, 8); }
+
+// Words of a piece: whole tiles; d and the piece of w stay below 1 GiB each (they are read MN-major).
+int piece_words(const dg_linear_xent_args& a) {
+    // (and 256 rows of d below 2 GiB, a tile's)
+    const int64_t most = (int64_t(1) << 29) - 1;
+    const int64_t fit = std::min({most / rows_of(a.tokens), most / a.w_ld, int64_t(1) << 21}) / 256 * 256;
+    const int64_t pieces = ceil_div64(a.vocab, std::max<int64_t>(256, fit));
+    return (int)align_up64(ceil_div64(a.vocab, pieces), 256);
+}
+
+struct Space {   // the workspace, cut up
+    int64_t bytes = 0;
+    int64_t take(int64_t n) {
+        const int64_t at = bytes;
+        bytes += align_up64(n, 256);
+        return at;
+    }
+};
+
+struct Plan {
+    int bm, bn;                // the logits' tile
+    int words, pieces;
+    int xbm, xbn, xsplit, wbm, wbn;
+    int64_t stats, logit, d, d_x, unit, partial, partial_bytes, bytes;
+};
+
+int cus_of(const dg_linear_xent_args& a) { return a.num_cus > 0 ? a.num_cus : device_cus(); }
+
+Plan plan_of(const dg_linear_xent_args& a, bool backward) {
+    Plan p = {};
+    Space s;
+    int one = 1;
+    int64_t none = 0;
+    const int cus = cus_of(a);
+    if (!backward) {
+        bf16_tile_plan(a.tokens, a.vocab, a.width, false, 1, cus, p.bm, p.bn, one, none);
+        p.stats = s.take((int64_t)ceil_div(a.vocab, p.bn) * a.tokens * 8);
+        p.logit = s.take((int64_t)a.tokens * 4);
+    } else {
+        p.words = piece_words(a);
+        p.pieces = ceil_div(a.vocab, p.words);
+        bf16_tile_plan(a.tokens, std::min(p.words, a.vocab), a.width, false, 1, cus, p.bm, p.bn, one, none);
+        p.d = s.take(rows_of(a.tokens) * p.words * 2);
+        p.d_x = s.take((int64_t)a.tokens * a.width * 4);
+        p.unit = s.take(8);
+        bf16_tile_plan(a.tokens, a.width, p.words, true, 32, cus, p.xbm, p.xbn, p.xsplit, p.partial_bytes);
+        bf16_tile_plan(std::min(p.words, a.vocab), a.width, a.tokens, true, 1, cus, p.wbm, p.wbn, one, none);
+        p.partial = s.take(p.partial_bytes);
+    }
+    p.bytes = s.bytes;
+    return p;
+}
+
+int check(const dg_linear_xent_args* a) {
+    if (a == nullptr) return dg_set_error("dg_linear_xent: null args");
+    if (a->tokens < 0 || a->width < 1 || a->vocab < 1) return dg_set_error("dg_linear_xent: invalid size");
+    if (a->tokens > kMaxTokens) return dg_set_error("dg_linear_xent: at most 2^20 tokens");
+    if (a->width % 8 != 0) return dg_set_error("dg_linear_xent: the width must be a multiple of 8");
+    if (a->target_bytes != 4 && a->target_bytes != 8) return dg_set_error("dg_linear_xent: targets are int32 or int64");
+    if (a->x_ld < a->width || a->w_ld < a->width || a->x_ld % 8 != 0 || a->w_ld % 8 != 0 || !aligned_to(a->x, 16) || !aligned_to(a->w, 16))
+        return dg_set_error("dg_linear_xent: rows of x and w must be 16-byte aligned and hold the width");
+    if (256 * a->x_ld * 2 > 0x7fffffffLL || 256 * a->w_ld * 2 > 0x3fffffffLL)
+        return dg_set_error("dg_linear_xent: row stride too large");
+    return DG_OK;
+}
+
+// The workgroups of a tile kernel over m x n outputs: fn(grid) launches with p, whose vbase is the first one.
+template <typename F>
+int launch_grid(KParams& p, int m, int n, int bm, int bn, int num_cus, F&& fn) {
+    p.num_m_blocks = ceil_div(m, bm);
+    p.num_n_blocks = ceil_div(n, bn);
+    const int64_t grid = (int64_t)p.num_m_blocks * p.num_n_blocks;
+    if (grid > 0x7fffffffLL) return dg_set_error("dg_linear_xent: too many tiles");
+    p.num_tiles = p.vgrid = (int)grid;
+    const int64_t most = num_cus > 0 ? (num_cus >= 8 ? num_cus / 8 * 8 : num_cus) : grid;
+    for (int64_t base = 0; base < grid; base += most) {
+        p.vbase = (int)base;
+        fn(dim3((unsigned)std::min(most, grid - base)));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) {
+            dg_set_error(hipGetErrorString(e));
+            return DG_ELAUNCH;
+        }
+    }
+    return DG_OK;
+}
+
+KParams tile_params() {
+    KParams p = {};
+    p.num_groups = 1;
+    p.out_esize = 2;
+    p.alpha = 1.f;
+    p.group_m = 4;
+    p.split_k = 1;
+    return p;
+}
+
+// Logits of all tokens and `words` words from x.first on.
+int launch_logits(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, bool backward, hipStream_t st) {
+    KParams p = tile_params();
+    p.a = reinterpret_cast<const uint8_t*>(a.x);
+    p.b = reinterpret_cast<const uint8_t*>(a.w) + (int64_t)x.first * a.w_ld * 2;
+    p.m = a.tokens; p.n = words; p.k = a.width;
+    p.lda = a.x_ld * 2; p.ldb = a.w_ld * 2;
+    p.kbytes_a = p.kbytes_b = a.width * 2;
+    return launch_grid(p, a.tokens, words, pl.bm, pl.bn, a.num_cus, [&](dim3 grid) {
+        auto go = [&](auto tail, auto bm, auto bn) {
+            hipLaunchKernelGGL((xent_tile_kernel<decltype(bm)::value, decltype(bn)::value, decltype(tail)>), grid, dim3(256), 0, st, p, x);
+        };
+        auto tile = [&](auto tail) {
+            if (pl.bm == 256 && pl.bn == 256) go(tail, Int<256>{}, Int<256>{});
+            else if (pl.bm == 256) go(tail, Int<256>{}, Int<128>{});
+            else go(tail, Int<128>{}, Int<128>{});
+        };
+        if (backward) tile(GradTail{});
+        else tile(StatsTail{});
+    });
+}
+
+// d_w rows of the piece = d^T x (both read MN-major): K rows past the tokens are not read.
+int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, hipStream_t st) {
+    KParams p = tile_params();
+    p.a = reinterpret_cast<const uint8_t*>(x.d);
+    p.b = reinterpret_cast<const uint8_t*>(a.x);
+    p.m = words; p.n = a.width; p.k = a.tokens;
+    p.lda = x.d_ld * 2; p.ldb = a.x_ld * 2;
+    const WeightTail tail = {x, reinterpret_cast<uint16_t*>(a.d_w) + (int64_t)x.first * a.d_w_ld, a.d_w_ld, words, a.width};
+    return launch_grid(p, words, a.width, pl.wbm, pl.wbn, a.num_cus, [&](dim3 grid) {
+        if (pl.wbm == 256 && pl.wbn == 256) hipLaunchKernelGGL((xent_weight_kernel<256, 256>), grid, dim3(256), 0, st, p, tail);
+        else if (pl.wbm == 256) hipLaunchKernelGGL((xent_weight_kernel<256, 128>), grid, dim3(256), 0, st, p, tail);
+        else hipLaunchKernelGGL((xent_weight_kernel<128, 128>), grid, dim3(256), 0, st, p, tail);
+    });
+}
+
+XentParams xent_params(const dg_linear_xent_args& a) {
+    XentParams x = {};
+    x.target = a.target;
+    x.wide = a.target_bytes == 8;
+    x.tokens = a.tokens;
+    x.rows = (int)rows_of(a.tokens);
+    x.vocab = a.vocab;
+    x.ignore = a.ignore_index;
+    return x;
+}
+
+}  // namespace
+}  // namespace dg
+
+extern "C" int dg_linear_xent_workspace_size(const dg_linear_xent_args* args, int32_t backward, int64_t* bytes) {
+    if (bytes == nullptr) return dg_set_error("dg_linear_xent: null bytes");
+    if (const int rc = dg::check(args)) return rc;
+    *bytes = args->tokens == 0 ? 0 : dg::plan_of(*args, backward != 0).bytes;
+    return DG_OK;
+}
+
+extern "C" int dg_linear_xent_forward(const dg_linear_xent_args* args, void* stream) {
+    using namespace dg;
+    if (const int rc = check(args)) return rc;
+    const dg_linear_xent_args& a = *args;
+    if (a.tokens == 0) return DG_OK;
+    if (a.x == nullptr || a.w == nullptr || a.target == nullptr || a.loss == nullptr || a.lse == nullptr)
+        return dg_set_error("dg_linear_xent: null tensor");
+    const Plan pl = plan_of(a, false);
+    if (a.workspace == nullptr || a.workspace_bytes < pl.bytes)
+        return dg_set_error("dg_linear_xent: workspace smaller than dg_linear_xent_workspace_size() reports");
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
+    XentParams x = xent_params(a);
+    x.stats = reinterpret_cast<f32x2*>(ws + pl.stats);
+    x.target_logit = reinterpret_cast<float*>(ws + pl.logit);
+    if (const int rc = launch_logits(pl, a, x, a.vocab, false, st)) return rc;
+    JoinParams j = {};
+    j.stats = x.stats; j.target_logit = x.target_logit; j.target = a.target; j.wide = x.wide;
+    j.tokens = a.tokens; j.vocab = a.vocab; j.tiles = ceil_div(a.vocab, pl.bn); j.ignore = a.ignore_index;
+    j.loss = a.loss; j.lse = const_cast<float*>(a.lse);
+    j.status = status_words_for(st);
+    // (few tokens: more threads to each)
+    if (a.tokens <= 256) return launch_op(xent_join_kernel<2>, ceil_div(a.tokens, 2), 256, j, st, a.num_cus);
+    return launch_op(xent_join_kernel<16>, ceil_div(a.tokens, 16), 256, j, st, a.num_cus);
+}
+
+extern "C" int dg_linear_xent_backward(const dg_linear_xent_args* args, void* stream) {
+    using namespace dg;
+    if (const int rc = check(args)) return rc;
+    const dg_linear_xent_args& a = *args;
+    if (a.d_x_ld < a.width || a.d_w_ld < a.width || a.d_x_ld % 8 != 0 || a.d_w_ld % 8 != 0 || !aligned_to(a.d_x, 16) || !aligned_to(a.d_w, 16))
+        return dg_set_error("dg_linear_xent: rows of the gradients must be 16-byte aligned and hold the width");
+    if (a.d_w == nullptr) return dg_set_error("dg_linear_xent: null tensor");
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (a.tokens == 0) return dg_set_error("dg_linear_xent: no tokens (the gradient of w is zero)");
+    if (a.x == nullptr || a.w == nullptr || a.target == nullptr || a.lse == nullptr || a.d_loss == nullptr || a.d_x == nullptr)
+        return dg_set_error("dg_linear_xent: null tensor");
+    const Plan pl = plan_of(a, true);
+    if (a.workspace == nullptr || a.workspace_bytes < pl.bytes)
+        return dg_set_error("dg_linear_xent: workspace smaller than dg_linear_xent_workspace_size() reports");
+    uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
+    XentParams x = xent_params(a);
+    x.lse = a.lse;
+    x.d_loss = a.d_loss;
+    x.d = reinterpret_cast<uint16_t*>(ws + pl.d);
+    x.d_ld = pl.words;
+    float* const unit = reinterpret_cast<float*>(ws + pl.unit);
+    x.unit = unit;
+    const UnitParams u = {a.d_loss, a.target, x.wide, a.tokens, a.vocab, a.ignore_index, unit, 0};
+    if (const int rc = launch_op(xent_unit_kernel, 1, 1024, u, st, 0)) return rc;
+    for (int first = 0; first < a.vocab; first += pl.words) {
+        const int words = std::min(pl.words, a.vocab - first);
+        x.first = first;
+        if (const int rc = launch_logits(pl, a, x, words, true, st)) return rc;
+        // d_x (+)= d w: d's rows are zeros past the words, up to a whole tile; w's rows end with the vocabulary
+        dg_gemm_args g = {};
+        g.kind = DG_KIND_BF16; g.gemm_type = DG_GEMM_NORMAL; g.num_groups = 1; g.alpha = 1.f; g.num_cus = a.num_cus;
+        g.a = x.d; g.lda = x.d_ld;
+        g.b = reinterpret_cast<const uint16_t*>(a.w) + (int64_t)first * a.w_ld; g.ldb = a.w_ld; g.b_mn_major = 1;
+        g.d = ws + pl.d_x; g.ldd = a.width; g.d_dtype = DG_DTYPE_F32;
+        g.accumulate = first > 0;
+        g.m = a.tokens; g.n = a.width; g.k = (int)align_up64(words, 8);
+        g.block_m = pl.xbm; g.block_n = pl.xbn; g.split_k = pl.xsplit;
+        if (pl.xsplit > 1) {
+            g.workspace = ws + pl.partial;
+            g.workspace_bytes = pl.partial_bytes;
+        }
+        if (const int rc = gemm_k_rows(&g, words, stream)) return rc;
+        if (const int rc = launch_weight(pl, a, x, words, st)) return rc;
+    }
+    CastParams c = {};
+    c.src = reinterpret_cast<const float*>(ws + pl.d_x);
+    c.unit = unit;
+    c.dst = reinterpret_cast<uint16_t*>(a.d_x);
+    c.ld = a.d_x_ld;
+    c.rows = a.tokens;
+    c.chunks = a.width / 8;
+    return launch_op(xent_cast_kernel, ceil_div64((int64_t)a.tokens * c.chunks, 256), 256, c, st, a.num_cus);
+}

@@ -241,11 +241,14 @@ struct QuadTile {
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
 };
 
+// What a tile does with its sums in place of storing D (linear_xent.hip): run(take, row_of, col_of, tl, smem).
+struct NoTail { static constexpr bool kOn = false; };
+
 // One tile.  LIVE: blocks of A half 1 that hold valid rows; the others are not read and contribute no MFMA, and
 // their sums are zero.  (A tile that takes another LIVE runs a body of its own: loops that join before one epilogue
 // made the register allocator spill the accumulators.)
-template <int BM, int BN, int KIND, int EPI, int CT, int CS, int CM, int CN, int CK, bool AMN, bool BMN, int LIVE>
-__device__ __forceinline__ void quad_tile_body(const KParams& p, const TileLoc& tl, uint8_t* const smem) {
+template <int BM, int BN, int KIND, int EPI, int CT, int CS, int CM, int CN, int CK, bool AMN, bool BMN, int LIVE, typename TAIL>
+__device__ __forceinline__ void quad_tile_body(const KParams& p, const TileLoc& tl, uint8_t* const smem, const TAIL& tail) {
     constexpr bool kBf16 = KIND == kBF16;
     constexpr bool kFp4B = KIND == kFP8FP4;
     using T = QuadTile<BM, BN, KIND, AMN, BMN>;
@@ -694,6 +697,10 @@ __device__ __forceinline__ void quad_tile_body(const KParams& p, const TileLoc& 
         constexpr int hb = decltype(hb_c)::value;
         return hb * SB::H0 + wn * (SB::rows(hb) / 2);
     };
+    if constexpr (TAIL::kOn) {
+        tail.template run<T>(take, row_of, col_of, tl, smem);
+        return;
+    }
     if (split_k > 1) {
         // This workgroup's partial tile, fp32 [BM][BN] (rows past M left out); quad_reduce_kernel sums the
         // ranges in order and runs the epilogue.
@@ -969,15 +976,15 @@ __device__ __forceinline__ void quad_tile_body(const KParams& p, const TileLoc& 
 
 // CT / CS / CM / CN / CK: GEMM type, K split and sizes fixed at compile time (-1 / 0: from the arguments).
 template <int BM, int BN, int KIND, int EPI, int CT = -1, int CS = 0, int CM = 0, int CN = 0, int CK = 0,
-          bool AMN = false, bool BMN = false>
-__device__ __forceinline__ void quad_body(const KParams& p, const int vb) {
+          bool AMN = false, bool BMN = false, typename TAIL = NoTail>
+__device__ __forceinline__ void quad_body(const KParams& p, const int vb, const TAIL& tail = TAIL{}) {
     using T = QuadTile<BM, BN, KIND, AMN, BMN>;
     using SA = typename T::SA;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS_BYTES];
     TileLoc tl;
     if (!locate_tile<BM, BN, 256, KIND, CT, CS, CM, CN, CK, AMN, BMN>(p, vb, -1, threadIdx.x, tl)) return;
     auto run = [&](auto live) {
-        quad_tile_body<BM, BN, KIND, EPI, CT, CS, CM, CN, CK, AMN, BMN, decltype(live)::value>(p, tl, smem);
+        quad_tile_body<BM, BN, KIND, EPI, CT, CS, CM, CN, CK, AMN, BMN, decltype(live)::value>(p, tl, smem, tail);
     };
     if constexpr (T::kWide) {
         // anchored tiles end with their group: of 8192 rows routed to 32 groups, 180 to 333 each, a third of

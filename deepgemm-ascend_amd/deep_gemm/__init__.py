@@ -41,6 +41,7 @@ from .moe import (  # noqa: E402
     MoELayout, moe_num_rows, moe_sort, moe_dispatch, moe_dispatch_backward, moe_combine, moe_combine_backward,
 )
 from .mx import mx_quantize, mx_dequantize, mx_gemm_nt  # noqa: E402
+from .loss import linear_cross_entropy, linear_cross_entropy_backward  # noqa: E402
 from . import epilogue  # noqa: E402
 from ._lib import check_errors  # noqa: E402
 

@@ -25,7 +25,8 @@ EXPORTED_SYMBOLS = ('dg_gemm', 'dg_transform_sf', 'dg_transform_k_grouped_sf', '
                     'dg_gemm_workspace_size', 'dg_last_error', 'dg_version', 'dg_jit_compile', 'dg_jit_set_include_dir',
                     'dg_jit_stats', 'dg_launch_plan', 'dg_gemm_noalloc', 'dg_take_errors', 'dg_error_words',
                     'dg_stream_workspace', 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine',
-                    'dg_moe_combine_backward', 'dg_mx_quantize', 'dg_mx_dequantize')
+                    'dg_moe_combine_backward', 'dg_mx_quantize', 'dg_mx_dequantize', 'dg_linear_xent_workspace_size',
+                    'dg_linear_xent_forward', 'dg_linear_xent_backward')
 
 # Sticky error bits kernels report through host-mapped words (DG_ERR_* in the header)
 DG_ERR_SF_INVALID, DG_ERR_M_INDICES, DG_ERR_EXPERT_ID, DG_ERR_MOE_ROWS, DG_ERR_TARGET = 1, 2, 4, 8, 16
@@ -81,6 +82,18 @@ class MxArgs(ctypes.Structure):
         ('k', ctypes.c_int32), ('x', ctypes.c_void_p), ('x_ld', ctypes.c_int64), ('x_batch_stride', ctypes.c_int64),
         ('codes', ctypes.c_void_p), ('codes_ld', ctypes.c_int64), ('codes_batch_stride', ctypes.c_int64),
         ('sf', ctypes.c_void_p), ('sf_ld', ctypes.c_int64), ('sf_batch_stride', ctypes.c_int64), ('num_cus', ctypes.c_int32),
+    ]
+
+
+class LinearXentArgs(ctypes.Structure):
+    """Mirror of ``dg_linear_xent_args`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('tokens', ctypes.c_int32), ('width', ctypes.c_int32), ('vocab', ctypes.c_int32),
+        ('x', ctypes.c_void_p), ('w', ctypes.c_void_p), ('x_ld', ctypes.c_int64), ('w_ld', ctypes.c_int64),
+        ('target', ctypes.c_void_p), ('target_bytes', ctypes.c_int32), ('ignore_index', ctypes.c_int64),
+        ('loss', ctypes.c_void_p), ('lse', ctypes.c_void_p), ('d_loss', ctypes.c_void_p),
+        ('d_x', ctypes.c_void_p), ('d_w', ctypes.c_void_p), ('d_x_ld', ctypes.c_int64), ('d_w_ld', ctypes.c_int64),
+        ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64), ('num_cus', ctypes.c_int32),
     ]
 
 
@@ -156,7 +169,10 @@ def load(path=None) -> ctypes.CDLL:
                 ('dg_moe_combine', [ptr, i64, i32, i64, layout, ptr, ptr, i64, i32, ptr]),
                 ('dg_moe_combine_backward', [ptr, i64, ptr, i64, i32, i64, layout, ptr, ptr, i64, ptr, i32, ptr]),
                 ('dg_mx_quantize', [ctypes.POINTER(MxArgs), ptr]),
-                ('dg_mx_dequantize', [ctypes.POINTER(MxArgs), ptr])):
+                ('dg_mx_dequantize', [ctypes.POINTER(MxArgs), ptr]),
+                ('dg_linear_xent_workspace_size', [ctypes.POINTER(LinearXentArgs), i32, ctypes.POINTER(i64)]),
+                ('dg_linear_xent_forward', [ctypes.POINTER(LinearXentArgs), ptr]),
+                ('dg_linear_xent_backward', [ctypes.POINTER(LinearXentArgs), ptr])):
             getattr(lib, name).argtypes = argtypes
             getattr(lib, name).restype = ctypes.c_int
         lib.dg_take_errors.restype = ctypes.c_uint32

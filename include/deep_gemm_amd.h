@@ -352,6 +352,34 @@ typedef struct dg_mx_args {
 int dg_mx_quantize(const dg_mx_args *args, void *stream);
 int dg_mx_dequantize(const dg_mx_args *args, void *stream);
 
+/*
+ * Cross entropy of a linear layer over a vocabulary, without keeping the logits:
+ *   z = x w^T, lse[t] = log sum_v exp z[t][v], loss[t] = lse[t] - z[t][target[t]]
+ * and its gradient d_x = d w, d_w = d^T x with d[t][v] = (exp(z[t][v] - lse[t]) - [v = target[t]]) d_loss[t].
+ * x [tokens][width], w [vocab][width], d_x and d_w are bf16 (width a multiple of 8, rows 16-byte aligned, at most 2^20 tokens);
+ * loss, lse, d_loss fp32 [tokens].  A token whose target is ignore_index has loss and gradient 0; so has one whose target lies
+ * outside the vocabulary (DG_ERR_TARGET).  The workspace (dg_linear_xent_workspace_size bytes) holds nothing between calls.
+ */
+typedef struct dg_linear_xent_args {
+    int32_t tokens, width, vocab;
+    const void *x, *w;
+    int64_t x_ld, w_ld;           /* elements                                                              */
+    const void *target;           /* [tokens] int32 or int64                                               */
+    int32_t target_bytes;
+    int64_t ignore_index;
+    float *loss;                  /* forward: written                                                      */
+    float *lse;                   /* forward: written; backward: read                                      */
+    const float *d_loss;          /* backward                                                              */
+    void *d_x, *d_w;              /* backward: written                                                     */
+    int64_t d_x_ld, d_w_ld;
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t num_cus;
+} dg_linear_xent_args;
+int dg_linear_xent_workspace_size(const dg_linear_xent_args *args, int32_t backward, int64_t *bytes);
+int dg_linear_xent_forward(const dg_linear_xent_args *args, void *stream);
+int dg_linear_xent_backward(const dg_linear_xent_args *args, void *stream);
+
 /* Message of the last failing call on this thread ("" if none). */
 const char *dg_last_error(void);
 
