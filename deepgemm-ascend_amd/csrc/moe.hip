@@ -18,6 +18,7 @@ constexpr int kMaxGroups = 1024;
 // blocks of pairs.
 constexpr int kSortOnePass = 8192;
 constexpr int kSortMaxBlocks = 256;
+constexpr int kSortBlock = 8192;   // pairs of a workgroup, at most
 
 struct SortParams {
     const void* ids;
@@ -64,11 +65,14 @@ __device__ __forceinline__ uint64_t same_key(int key, int bits) {
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortParams p) {
     __shared__ int wave_next[kSortWaves][kMaxGroups + 1];   // counts of a wave's pairs, then its next row of each expert
     __shared__ int total[kMaxGroups], before[kMaxGroups], start[kMaxGroups + 1], wave_sum[kSortWaves];
+    __shared__ uint16_t keys[kSortBlock];                   // of this workgroup's pairs (read from memory once)
     const int b = blockIdx.x + p.vbase, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int G = p.groups;
     const int first = b * p.per_block, last = min(p.pairs, first + p.per_block);
     for (int g = tid; g < G; g += kSortThreads) total[g] = before[g] = 0;
-    for (int e = tid; e < kSortWaves * (kMaxGroups + 1); e += kSortThreads) (&wave_next[0][0])[e] = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w)
+        for (int g = tid; g <= G; g += kSortThreads) wave_next[w][g] = 0;
     __syncthreads();
     if (p.counts != nullptr) {
         // a part of the blocks each, so that the loads of all parts are in flight
@@ -76,7 +80,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
         if (G >= kSortThreads) {
             for (int g = tid; g < G; g += kSortThreads) {
                 int all = 0, mine = 0;
-#pragma unroll 8
+#pragma unroll 32
                 for (int i = 0; i < p.blocks; ++i) {
                     const int c = p.counts[(int64_t)i * G + g];
                     all += c;
@@ -88,7 +92,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
         } else if (part < parts) {
             const int g = tid - part * G;
             int all = 0, mine = 0;
-#pragma unroll 8
+#pragma unroll 32
             for (int i = part; i < p.blocks; i += parts) {
                 const int c = p.counts[(int64_t)i * G + g];
                 all += c;
@@ -97,19 +101,23 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
             atomicAdd(&total[g], all);
             atomicAdd(&before[g], mine);
         }
+        for (int i = first + tid; i < last; i += kSortThreads) keys[i - first] = (uint16_t)key_of(p, i);
     } else {
+#pragma unroll 4
         for (int i = tid; i < p.pairs; i += kSortThreads) {
             const int k = key_of(p, i);
             if (k < G) {
                 atomicAdd(&total[k], 1);
                 if (i < first) atomicAdd(&before[k], 1);
             }
+            if (i >= first && i < last) keys[i - first] = (uint16_t)k;
         }
     }
+    __syncthreads();
     // this wave's pairs: a run of whole batches of 64
     const int batches = ceil_div(max(0, last - first), 64), per_wave = ceil_div(batches, kSortWaves);
     const int w0 = first + wave * per_wave * 64, w1 = min(last, w0 + per_wave * 64);
-    for (int i = w0 + lane; i < w1; i += 64) atomicAdd(&wave_next[wave][key_of(p, i)], 1);
+    for (int i = w0 + lane; i < w1; i += 64) atomicAdd(&wave_next[wave][keys[i - first]], 1);
     __syncthreads();
     // first rows of the groups: scan over two groups a thread
     const int g0 = 2 * tid;
@@ -144,7 +152,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
     for (int base_i = w0; base_i < w1; base_i += 64) {
         const int i = base_i + lane;
         const bool on = i < w1;
-        const int key = on ? key_of(p, i) : G;
+        const int key = on ? keys[i - first] : G;
         const uint64_t same = same_key(key, bits);
         const int rank = __popcll(same & ((1ull << lane) - 1));
         const int row = key < G ? wave_next[wave][key] + rank : -1;
@@ -167,16 +175,21 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
         p.source[r] = p.indices[r] = -1;
 }
 
-int sort_blocks(int pairs) {
-    // (one pass: blocks only share out the placing and the padding; a block of pairs has a batch for every wave)
-    if (pairs <= kSortOnePass) return std::max(1, std::min(32, ceil_div(pairs, 512)));
-    return std::min(kSortMaxBlocks, ceil_div(pairs, 2048));
+int sort_blocks(int pairs, int rows) {
+    // One pass: blocks share out the placing (a batch for every wave) and the padding (16 x 8 pairs over 256 groups,
+    // 4096 rows: 7.8 us on one block, 5.3 on eight).
+    if (pairs <= kSortOnePass) return std::max({1, std::min(32, ceil_div(pairs, 512)), std::min(32, ceil_div(rows, 512))});
+    // (every block reads the counts of all, so that more of them cost more than they share out)
+    return std::max(std::min(kSortMaxBlocks, ceil_div(pairs, 2048)), ceil_div(pairs, kSortBlock));
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// A row is cut into chunks of V bytes; `lanes` threads (a power of two up to the workgroup) walk the chunks of one row
+// A row is cut into chunks of 16 bytes; `lanes` threads (a power of two up to the workgroup) walk the chunks of one row
 // and a workgroup holds 256 / lanes rows, so that short rows leave no lane idle and every access of a wave is one run
-// of bytes of a row.
+// of bytes of a row.  The last chunk ends with the row: where the row is no whole number of chunks it overlaps the one
+// before, and both write the same values there.  Rows need no alignment (global memory takes 16 bytes at any address:
+// 1021 x 6 pairs of 1407 fp32 values there and back with gradients: sums 9 us against 19 in single values).  Rows below 16 bytes go
+// value by value.
 constexpr int kRowThreads = 256;
 
 int row_lanes(int64_t chunks) {
@@ -185,34 +198,37 @@ int row_lanes(int64_t chunks) {
     return l;
 }
 
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4_half __attribute__((ext_vector_type(4), aligned(2)));
+
 template <int V> struct Chunk;
-template <> struct Chunk<16> { typedef i32x4 type; };
-template <> struct Chunk<8> { typedef i32x2 type; };
-template <> struct Chunk<4> { typedef int32_t type; };
-template <> struct Chunk<2> { typedef int16_t type; };
-template <> struct Chunk<1> { typedef int8_t type; };
+template <> struct Chunk<16> { typedef i32x4 type; typedef i32x4_any mem; };
+template <> struct Chunk<1> { typedef int8_t type; typedef int8_t mem; };
 
 constexpr int kPadRows = 32;    // rows of a workgroup that clears padding: at the layout's end they come in thousands
 
 // Rows of a layout that hold no pair are cleared by workgroups of kPadRows rows.
 template <int V>
-__device__ __forceinline__ void clear_padding(const int32_t* source, int rows, int first, uint8_t* dst, int64_t dst_ld, int chunks) {
-    typedef typename Chunk<V>::type T;
+__device__ __forceinline__ void clear_padding(const int32_t* source, int rows, int first, uint8_t* dst, int64_t dst_ld,
+                                              int64_t row_bytes) {
+    typedef typename Chunk<V>::mem M;
     const int n = min(kPadRows, rows - first);
     const int mine = (int)(threadIdx.x & 63);
     uint64_t live = __ballot(mine < n && source[first + mine] < 0);
     while (live != 0) {
         const int r = __builtin_ctzll(live);
         live &= live - 1;
-        T* const d = reinterpret_cast<T*>(dst + (int64_t)(first + r) * dst_ld);
-        for (int c = threadIdx.x; c < chunks; c += kRowThreads) d[c] = T{};
+        uint8_t* const d = dst + (int64_t)(first + r) * dst_ld;
+        for (int64_t at = (int64_t)threadIdx.x * V; at < row_bytes; at += kRowThreads * V)
+            *reinterpret_cast<M*>(d + min(at, row_bytes - V)) = typename Chunk<V>::type{};
     }
 }
 
 struct DispatchParams {
     const uint8_t* src;
     uint8_t* dst;
-    int64_t src_ld, dst_ld;    // bytes
+    int64_t src_ld, dst_ld, row_bytes;
     const int32_t *slots, *source;
     int tokens, topk, rows, chunks, lanes;
     int pad_blocks;            // first workgroups: padding rows (0: left as they are)
@@ -230,10 +246,11 @@ constexpr int kSfRows = 512;    // rows of a workgroup that moves scale factors,
 template <int V>
 __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(const DispatchParams p) {
     typedef typename Chunk<V>::type T;
+    typedef typename Chunk<V>::mem M;
     int b = blockIdx.x + p.vbase;
     const int tid = threadIdx.x;
     if (b < p.pad_blocks) {
-        clear_padding<V>(p.source, p.rows, b * kPadRows, p.dst, p.dst_ld, p.chunks);
+        clear_padding<V>(p.source, p.rows, b * kPadRows, p.dst, p.dst_ld, p.row_bytes);
         return;
     }
     b -= p.pad_blocks;
@@ -254,57 +271,66 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(const DispatchPar
     b -= p.sf_blocks;
     const int t = b * (kRowThreads / p.lanes) + tid / p.lanes, c0 = tid % p.lanes;
     if (t >= p.tokens) return;
-    const T* const in = reinterpret_cast<const T*>(p.src + (int64_t)t * p.src_ld);
+    const uint8_t* const in = p.src + (int64_t)t * p.src_ld;
     const int32_t* const slots = p.slots + (int64_t)t * p.topk;
     constexpr int U = 4;
     for (int c = c0; c < p.chunks; c += U * p.lanes) {
         T v[U];
+        int64_t at[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c + u * p.lanes < p.chunks) v[u] = in[c + u * p.lanes];
+        for (int u = 0; u < U; ++u) {
+            at[u] = min((int64_t)(c + u * p.lanes) * V, p.row_bytes - V);
+            if (c + u * p.lanes < p.chunks) v[u] = *reinterpret_cast<const M*>(in + at[u]);
+        }
         for (int k = 0; k < p.topk; ++k) {
             const int s = slots[k];
             if ((u32)s >= (u32)p.rows) continue;    // (dropped: -1)
-            T* const d = reinterpret_cast<T*>(p.dst + (int64_t)s * p.dst_ld);
+            uint8_t* const d = p.dst + (int64_t)s * p.dst_ld;
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (c + u * p.lanes < p.chunks) d[c + u * p.lanes] = v[u];
+                if (c + u * p.lanes < p.chunks) *reinterpret_cast<M*>(d + at[u]) = v[u];
         }
     }
 }
 
-// N values of type E in fp32.
-template <typename E, int N>
-struct Values { float v[N]; };
+// N values of type E as they are loaded (16 bytes, or one value) and in fp32.  They stay as loaded until they are used:
+// unpacked on arrival, the rows in flight took 94 registers of a thread (157 with the gradients) in place of 62 (128), and
+// 8192 x 8 pairs of 4096 bf16 values 288 us with the gradients in place of 226.
+template <typename E, int N> struct Raw;
+template <> struct Raw<float, 4> { typedef f32x4 type; typedef f32x4_any mem; };
+template <> struct Raw<uint16_t, 8> { typedef i32x4 type; typedef i32x4_half mem; };
+template <> struct Raw<float, 1> { typedef float type; typedef float mem; };
+template <> struct Raw<uint16_t, 1> { typedef uint16_t type; typedef uint16_t mem; };
 
 template <typename E, int N>
-__device__ __forceinline__ Values<E, N> load_values(const E* s) {
-    Values<E, N> o;
+__device__ __forceinline__ typename Raw<E, N>::type load_raw(const E* s) {
+    return *reinterpret_cast<const typename Raw<E, N>::mem*>(s);
+}
+
+template <typename E, int N>
+__device__ __forceinline__ void unpack(const typename Raw<E, N>::type w, float (&v)[N]) {
     if constexpr (sizeof(E) == 4 && N == 4) {
-        const f32x4 w = *reinterpret_cast<const f32x4*>(s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o.v[i] = w[i];
-    } else if constexpr (sizeof(E) == 2 && N == 8) {
-        const i32x4 w = *reinterpret_cast<const i32x4*>(s);
+        for (int i = 0; i < 4; ++i) v[i] = w[i];
+    } else if constexpr (N == 8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            o.v[2 * i] = __builtin_bit_cast(float, (u32)w[i] << 16);
-            o.v[2 * i + 1] = __builtin_bit_cast(float, (u32)w[i] & 0xffff0000u);
+            v[2 * i] = __builtin_bit_cast(float, (u32)w[i] << 16);
+            v[2 * i + 1] = __builtin_bit_cast(float, (u32)w[i] & 0xffff0000u);
         }
+    } else if constexpr (sizeof(E) == 4) {
+        v[0] = w;
     } else {
-        static_assert(N == 1, "one value, or 16 bytes of them");
-        if constexpr (sizeof(E) == 4) o.v[0] = *s;
-        else o.v[0] = bf16_to_f32(*s);
+        v[0] = bf16_to_f32(w);
     }
-    return o;
 }
 
 template <typename E, int N>
 __device__ __forceinline__ void store_values(E* d, const float (&v)[N]) {
     if constexpr (sizeof(E) == 4 && N == 4) {
-        *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_any*>(d) = f32x4{v[0], v[1], v[2], v[3]};
     } else if constexpr (sizeof(E) == 2 && N == 8) {
-        *reinterpret_cast<i32x4*>(d) = i32x4{(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]),
+        *reinterpret_cast<i32x4_half*>(d) = i32x4{(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]),
                                             (int)pack_bf16x2(v[4], v[5]), (int)pack_bf16x2(v[6], v[7])};
     } else if constexpr (sizeof(E) == 4) {
         *d = v[0];
@@ -321,7 +347,7 @@ struct CombineParams {
     const float* weights;      // [tokens][topk] or nullptr (ones)
     const int32_t *slots, *source;
     int64_t in_ld, out_ld, d_out_ld;   // elements
-    int tokens, topk, rows, chunks, lanes, pad_blocks;
+    int tokens, topk, rows, width, chunks, lanes, pad_blocks;
     int vbase;
 };
 
@@ -338,9 +364,10 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(const CombineParam
     E* const out = reinterpret_cast<E*>(p.out) + (int64_t)t * p.out_ld;
     const E* const in = reinterpret_cast<const E*>(p.rows_in);
     for (int c = tid % p.lanes; c < p.chunks; c += p.lanes) {
+        const int at = min(c * N, p.width - N);
         float sum[N] = {};
         for (int k0 = 0; k0 < p.topk; k0 += kChoices) {
-            Values<E, N> v[kChoices];
+            typename Raw<E, N>::type v[kChoices];
             float w[kChoices];
 #pragma unroll
             for (int k = 0; k < kChoices; ++k) {
@@ -348,15 +375,18 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(const CombineParam
                 const bool live = (u32)s < (u32)p.rows;
                 // (a dropped pair's weight is not used: whatever it is, it adds nothing)
                 w[k] = !live ? 0.f : p.weights != nullptr ? weights[k0 + k] : 1.f;
-                if (live) v[k] = load_values<E, N>(in + (int64_t)s * p.in_ld + c * N);
-                else v[k] = {};
+                v[k] = typename Raw<E, N>::type{};
+                if (live) v[k] = load_raw<E, N>(in + (int64_t)s * p.in_ld + at);
             }
 #pragma unroll
-            for (int k = 0; k < kChoices; ++k)
+            for (int k = 0; k < kChoices; ++k) {
+                float x[N];
+                unpack<E, N>(v[k], x);
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] = __builtin_fmaf(w[k], v[k].v[i], sum[i]);
+                for (int i = 0; i < N; ++i) sum[i] = __builtin_fmaf(w[k], x[i], sum[i]);
+            }
         }
-        store_values<E, N>(out + c * N, sum);
+        store_values<E, N>(out + at, sum);
     }
 }
 
@@ -369,8 +399,8 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Com
     int b = blockIdx.x + p.vbase;
     const int tid = threadIdx.x;
     if (b < p.pad_blocks) {
-        clear_padding<N * (int)sizeof(E)>(p.source, p.rows, b * kPadRows, reinterpret_cast<uint8_t*>(p.out), p.out_ld * (int)sizeof(E),
-                                          p.chunks);
+        clear_padding<(N == 1 ? 1 : 16)>(p.source, p.rows, b * kPadRows, reinterpret_cast<uint8_t*>(p.out), p.out_ld * (int)sizeof(E),
+                                          (int64_t)p.width * (int)sizeof(E));
         return;
     }
     b -= p.pad_blocks;
@@ -392,21 +422,24 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Com
             dot[k] = 0.f;
         }
         for (int c = c0; on && c < p.chunks; c += p.lanes) {
-            const Values<E, N> g = load_values<E, N>(d_out + c * N);
-            Values<E, N> v[kChoices];
+            const int at = min(c * N, p.width - N), counted = c * N - at;   // (values that the chunk before has counted)
+            float g[N];
+            typename Raw<E, N>::type v[kChoices];
+            unpack<E, N>(load_raw<E, N>(d_out + at), g);
 #pragma unroll
             for (int k = 0; k < kChoices; ++k)
-                if (s[k] >= 0) v[k] = load_values<E, N>(in + (int64_t)s[k] * p.in_ld + c * N);
+                if (s[k] >= 0) v[k] = load_raw<E, N>(in + (int64_t)s[k] * p.in_ld + at);
 #pragma unroll
             for (int k = 0; k < kChoices; ++k) {
                 if (s[k] < 0) continue;
-                float d[N];
+                float x[N], d[N];
+                unpack<E, N>(v[k], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    dot[k] = __builtin_fmaf(g.v[i], v[k].v[i], dot[k]);
-                    d[i] = w[k] * g.v[i];
+                    if (i >= counted) dot[k] = __builtin_fmaf(g[i], x[i], dot[k]);
+                    d[i] = w[k] * g[i];
                 }
-                store_values<E, N>(out + (int64_t)s[k] * p.out_ld + c * N, d);
+                store_values<E, N>(out + (int64_t)s[k] * p.out_ld + at, d);
             }
         }
 #pragma unroll
@@ -441,25 +474,12 @@ int layout_ok(const dg_moe_layout* l, const char* who) {
     return DG_OK;
 }
 
-// A row of `bytes` at the given strides: the widest chunk that divides everything (16, 4, 2 or 1 bytes).
-int chunk_bytes(int64_t bytes, int64_t ld0, int64_t ld1, const void* a, const void* b) {
-    for (int v : {16, 8, 4, 2})
-        if (bytes % v == 0 && ld0 % v == 0 && ld1 % v == 0 && aligned_to(a, v) && aligned_to(b, v)) return v;
-    return 1;
-}
-
-template <typename E>
-bool vector_rows(int64_t width, int64_t l0, int64_t l1, int64_t l2, const void* a, const void* b, const void* c) {
-    constexpr int n = 16 / (int)sizeof(E);
-    return width % n == 0 && l0 % n == 0 && l1 % n == 0 && l2 % n == 0 && aligned_to(a, 16) && aligned_to(b, 16) && aligned_to(c, 16);
-}
-
 }  // namespace
 }  // namespace dg
 
 extern "C" int dg_moe_sort_workspace_size(int32_t num_pairs, int32_t num_groups, int64_t* bytes) {
     if (bytes == nullptr || num_pairs < 0 || num_groups < 1) return dg_set_error("dg_moe_sort: invalid size");
-    *bytes = num_pairs <= dg::kSortOnePass ? 0 : (int64_t)dg::sort_blocks(num_pairs) * num_groups * 4;
+    *bytes = num_pairs <= dg::kSortOnePass ? 0 : (int64_t)dg::sort_blocks(num_pairs, 0) * num_groups * 4;
     return DG_OK;
 }
 
@@ -486,7 +506,7 @@ extern "C" int dg_moe_sort(const void* ids, int32_t id_bytes, const dg_moe_layou
     p.ids = ids;
     p.wide = id_bytes == 8;
     p.pairs = (int)pairs; p.groups = l->num_groups; p.alignment = l->alignment; p.rows = l->rows;
-    p.blocks = sort_blocks(p.pairs);
+    p.blocks = sort_blocks(p.pairs, p.rows);
     p.per_block = ceil_div(std::max(1, p.pairs), p.blocks);
     p.slots = l->slots; p.source = l->source; p.indices = l->m_indices; p.psum = l->psum;
     p.counts = need > 0 ? reinterpret_cast<int32_t*>(workspace) : nullptr;
@@ -508,14 +528,15 @@ extern "C" int dg_moe_dispatch(const void* src, int64_t src_ld, int64_t row_byte
     if (l->rows == 0 || row_bytes == 0) return DG_OK;
     if (dst == nullptr || l->source == nullptr || (l->tokens > 0 && (src == nullptr || l->slots == nullptr)))
         return dg_set_error("dg_moe_dispatch: null tensor");
-    const int v = chunk_bytes(row_bytes, src_ld, dst_ld, src, dst);
-    if (row_bytes / v > 0x3fffffffLL) return dg_set_error("dg_moe_dispatch: row too long");
+    const int v = row_bytes >= 16 ? 16 : 1;
+    if (row_bytes > 0x7fffffffLL) return dg_set_error("dg_moe_dispatch: row too long");
     DispatchParams p = {};
     p.src = reinterpret_cast<const uint8_t*>(src); p.dst = reinterpret_cast<uint8_t*>(dst);
     p.src_ld = src_ld; p.dst_ld = dst_ld;
     p.slots = l->slots; p.source = l->source;
     p.tokens = l->tokens; p.topk = l->topk; p.rows = l->rows;
-    p.chunks = (int)(row_bytes / v);
+    p.row_bytes = row_bytes;
+    p.chunks = (int)ceil_div64(row_bytes, v);
     p.lanes = row_lanes(p.chunks);
     p.pad_blocks = zero_padding ? ceil_div(l->rows, kPadRows) : 0;
     if (sf != nullptr && k64 > 0) {
@@ -526,24 +547,19 @@ extern "C" int dg_moe_dispatch(const void* src, int64_t src_ld, int64_t row_byte
     }
     const int64_t grid = p.pad_blocks + (int64_t)p.sf_blocks + (l->topk > 0 ? ceil_div(l->tokens, kRowThreads / p.lanes) : 0);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    switch (v) {
-        case 16: return launch_op(dispatch_kernel<16>, grid, kRowThreads, p, st, num_cus);
-        case 8: return launch_op(dispatch_kernel<8>, grid, kRowThreads, p, st, num_cus);
-        case 4: return launch_op(dispatch_kernel<4>, grid, kRowThreads, p, st, num_cus);
-        case 2: return launch_op(dispatch_kernel<2>, grid, kRowThreads, p, st, num_cus);
-        default: return launch_op(dispatch_kernel<1>, grid, kRowThreads, p, st, num_cus);
-    }
+    return launch_op(v == 16 ? dispatch_kernel<16> : dispatch_kernel<1>, grid, kRowThreads, p, st, num_cus);
 }
 
 namespace dg {
 namespace {
 
-int combine_params(const dg_moe_layout* l, int64_t width, bool vec, int n, CombineParams& p) {
+// n: values of a chunk
+int combine_params(const dg_moe_layout* l, int64_t width, int n, CombineParams& p) {
     p.slots = l->slots; p.source = l->source;
     p.tokens = l->tokens; p.topk = l->topk; p.rows = l->rows;
-    const int64_t chunks = vec ? width / n : width;
-    if (chunks > 0x3fffffffLL) return dg_set_error("dg_moe_combine: row too long");
-    p.chunks = (int)chunks;
+    if (width > 0x3fffffffLL) return dg_set_error("dg_moe_combine: row too long");
+    p.width = (int)width;
+    p.chunks = ceil_div(p.width, n);
     p.lanes = row_lanes(p.chunks);
     return DG_OK;
 }
@@ -560,12 +576,13 @@ extern "C" int dg_moe_combine(const void* rows, int64_t rows_ld, int32_t dtype, 
         return dg_set_error("dg_moe_combine: leading dimension smaller than the row");
     if (l->tokens == 0 || width == 0) return DG_OK;
     if (out == nullptr || (l->topk > 0 && l->slots == nullptr) || (l->rows > 0 && rows == nullptr)) return dg_set_error("dg_moe_combine: null tensor");
+    const int64_t e = dtype == DG_DTYPE_F32 ? 4 : 2;
+    if (!aligned_to(rows, e) || !aligned_to(out, e)) return dg_set_error("dg_moe_combine: values must be aligned");
     CombineParams p = {};
     p.rows_in = rows; p.out = out; p.weights = weights; p.in_ld = rows_ld; p.out_ld = out_ld;
     const bool f32 = dtype == DG_DTYPE_F32;
-    const bool vec = f32 ? vector_rows<float>(width, rows_ld, out_ld, 0, rows, out, nullptr)
-                         : vector_rows<uint16_t>(width, rows_ld, out_ld, 0, rows, out, nullptr);
-    if (const int rc = combine_params(l, width, vec, f32 ? 4 : 8, p)) return rc;
+    const bool vec = width >= (f32 ? 4 : 8);
+    if (const int rc = combine_params(l, width, !vec ? 1 : f32 ? 4 : 8, p)) return rc;
     const int64_t grid = ceil_div(l->tokens, kRowThreads / p.lanes);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (f32) return launch_op(vec ? combine_kernel<float, 4> : combine_kernel<float, 1>, grid, kRowThreads, p, st, num_cus);
@@ -584,13 +601,14 @@ extern "C" int dg_moe_combine_backward(const void* d_out, int64_t d_out_ld, cons
     if ((pairs > 0 && (d_out == nullptr || l->slots == nullptr || weights == nullptr || d_weights == nullptr)) ||
         (l->rows > 0 && width > 0 && (rows == nullptr || d_rows == nullptr || l->source == nullptr)))
         return dg_set_error("dg_moe_combine_backward: null tensor");
+    const int64_t e = dtype == DG_DTYPE_F32 ? 4 : 2;
+    if (!aligned_to(rows, e) || !aligned_to(d_rows, e) || !aligned_to(d_out, e)) return dg_set_error("dg_moe_combine_backward: values must be aligned");
     CombineParams p = {};
     p.rows_in = rows; p.d_out = d_out; p.out = d_rows; p.weights = weights; p.d_weights = d_weights;
     p.in_ld = rows_ld; p.out_ld = d_rows_ld; p.d_out_ld = d_out_ld;
     const bool f32 = dtype == DG_DTYPE_F32;
-    const bool vec = f32 ? vector_rows<float>(width, rows_ld, d_rows_ld, d_out_ld, rows, d_rows, d_out)
-                         : vector_rows<uint16_t>(width, rows_ld, d_rows_ld, d_out_ld, rows, d_rows, d_out);
-    if (const int rc = combine_params(l, width, vec, f32 ? 4 : 8, p)) return rc;
+    const bool vec = width >= (f32 ? 4 : 8);
+    if (const int rc = combine_params(l, width, !vec ? 1 : f32 ? 4 : 8, p)) return rc;
     p.pad_blocks = width > 0 ? ceil_div(l->rows, kPadRows) : 0;
     const int64_t grid = p.pad_blocks + (int64_t)(l->topk > 0 ? ceil_div(l->tokens, kRowThreads / p.lanes) : 0);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);

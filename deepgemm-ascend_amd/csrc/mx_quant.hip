@@ -30,46 +30,18 @@ struct MxParams {
     int vbase;
 };
 
-// Eight values from x (16-byte aligned, or not: element by element).
-template <typename E, bool VEC>
-__device__ __forceinline__ void load8(const E* x, float (&v)[8]) {
-    if constexpr (VEC && sizeof(E) == 2) {
-        const i32x4 w = *reinterpret_cast<const i32x4*>(x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __builtin_bit_cast(float, (u32)w[i] << 16);
-            v[2 * i + 1] = __builtin_bit_cast(float, (u32)w[i] & 0xffff0000u);
-        }
-    } else if constexpr (VEC) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(x), b = *reinterpret_cast<const f32x4*>(x + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (sizeof(E) == 2) v[i] = bf16_to_f32(x[i]);
-            else v[i] = x[i];
-        }
-    }
-}
+// (rows need no alignment: global memory takes 16 bytes at any address)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4_half __attribute__((ext_vector_type(4), aligned(2)));
 
-template <typename E, bool VEC>
+template <typename E>
 __device__ __forceinline__ void store8(E* x, const float (&v)[8]) {
-    if constexpr (VEC && sizeof(E) == 2) {
-        *reinterpret_cast<i32x4*>(x) = i32x4{(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]),
-                                            (int)pack_bf16x2(v[4], v[5]), (int)pack_bf16x2(v[6], v[7])};
-    } else if constexpr (VEC) {
-        *reinterpret_cast<f32x4*>(x) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(x + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    if constexpr (sizeof(E) == 2) {
+        *reinterpret_cast<i32x4_half*>(x) = i32x4{(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]),
+                                                 (int)pack_bf16x2(v[4], v[5]), (int)pack_bf16x2(v[6], v[7])};
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (sizeof(E) == 2) x[i] = f32_to_bf16_rne(v[i]);
-            else x[i] = v[i];
-        }
+        *reinterpret_cast<f32x4_any*>(x) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_any*>(x + 4) = f32x4{v[4], v[5], v[6], v[7]};
     }
 }
 
@@ -82,10 +54,91 @@ __device__ __forceinline__ u32 scale_byte(u32 a) {
     return max(e, FP4 ? 3u : 9u) - (FP4 ? 2u : 8u);
 }
 
+// Largest of a value's over a block's four lanes and the partner block's value: lane exchanges within a row of the wave
+// (xor 1, xor 2; in a half row mirrored, which is xor 4 for what four lanes share), cheaper than through LDS.
+template <int CTRL>
+__device__ __forceinline__ u32 dpp(u32 v) { return (u32)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kMirror8 = 0x141;   // quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror
+
+// Eight values of a lane: as loaded, their largest magnitude's fp32 bits, and their codes under the scale 2^(s - 127).
+template <typename E> struct Eight;
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* x) {
+        const f32x4 a = *reinterpret_cast<const f32x4_any*>(x), b = *reinterpret_cast<const f32x4_any*>(x + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+    __device__ __forceinline__ u32 top() const {
+        u32 a = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = max(a, __builtin_bit_cast(u32, v[i]) & 0x7fffffffu);
+        return a;
+    }
+    __device__ __forceinline__ u32 e2m1(float s) const {
+        u32 w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], s, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], s, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], s, 3);
+    }
+    __device__ __forceinline__ i32x2 e4m3(float inv) const {
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
+        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
+        return i32x2{lo, hi};
+    }
+};
+
+// bf16 stays packed: the maximum on pairs of 16-bit integers, e2m1 from pairs of bf16.
+template <>
+struct Eight<uint16_t> {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    i32x4 w;
+    __device__ __forceinline__ void load(const uint16_t* x) { w = *reinterpret_cast<const i32x4_half*>(x); }
+    __device__ __forceinline__ void zero() { w = i32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ u32 top() const {
+        u16x2 a = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fff);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fff));
+        return (u32)max(a[0], a[1]) << 16;
+    }
+    // (through a value of its own: the compiler takes element 0 of any element that is bit-cast in place)
+    __device__ __forceinline__ bf16x2 pair(int i) const {
+        const int v = w[i];
+        return __builtin_bit_cast(bf16x2, v);
+    }
+    __device__ __forceinline__ u32 e2m1(float s) const {
+        u32 c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, pair(0), s, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, pair(1), s, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, pair(2), s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, pair(3), s, 3);
+    }
+    __device__ __forceinline__ i32x2 e4m3(float inv) const {
+        Eight<float> f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f.v[2 * i] = __builtin_bit_cast(float, (u32)w[i] << 16);
+            f.v[2 * i + 1] = __builtin_bit_cast(float, (u32)w[i] & 0xffff0000u);
+        }
+        return f.e4m3(inv);
+    }
+};
+
 // A workgroup quantises ROWS rows x 512 values, a wave a row at a time: eight values a lane (1 KB of bf16 a wave), the
 // block's maximum over four lanes, and the exponent bytes of the tile collected in LDS so that they leave as runs
-// of rows.  Bound by the bytes of x: 32 rows a wave are in flight two at a time.
-template <typename E, bool FP4, bool VEC, int ROWS>
+// of rows.  Bound by the bytes of x; four rows of a wave are in flight.
+template <typename E, bool FP4, int ROWS>
 __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxParams p) {
     __shared__ uint16_t pairs[8][ROWS + 2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -94,51 +147,36 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxParams p)
     t /= p.col_tiles;
     const int rt = t % p.row_tiles, batch = t / p.row_tiles;
     const int row0 = rt * ROWS, col = ct * 512 + lane * 8;
-    const bool on = col < p.k;
-    const E* const x = reinterpret_cast<const E*>(p.x) + batch * p.x_bs;
-    uint8_t* const codes = reinterpret_cast<uint8_t*>(p.codes) + batch * p.codes_bs;
+    const bool on = col < p.k, paired = col + 32 < p.k;
+    const E* const x = reinterpret_cast<const E*>(p.x) + batch * p.x_bs + col;
+    uint8_t* const codes = reinterpret_cast<uint8_t*>(p.codes) + batch * p.codes_bs + (FP4 ? col / 2 : col);
     constexpr int PER = ROWS / 4, U = PER < 4 ? PER : 4;
 #pragma unroll 1
     for (int r0 = 0; r0 < PER; r0 += U) {
-        float v[U][8];
+        Eight<E> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int row = row0 + (r0 + u) * 4 + wave;
-            if (on && row < p.rows) load8<E, VEC>(x + (int64_t)row * p.x_ld + col, v[u]);
-            else
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+            v[u].zero();
+            if (on && row < p.rows) v[u].load(x + (int64_t)row * p.x_ld);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int at = (r0 + u) * 4 + wave, row = row0 + at;
-            u32 a = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a = max(a, __builtin_bit_cast(u32, v[u][i]) & 0x7fffffffu);
-            a = max(a, (u32)__shfl_xor((int)a, 1, 64));
-            a = max(a, (u32)__shfl_xor((int)a, 2, 64));
-            const u32 s = scale_byte<FP4>(a);
-            const u32 other = (u32)__shfl_xor((int)s, 4, 64);
-            if ((lane & 7) == 0) pairs[lane >> 3][at] = (uint16_t)(s | (col + 32 < p.k ? other << 8 : 0u));
+            u32 a = v[u].top();
+            a = max(a, dpp<kXor1>(a));
+            a = max(a, dpp<kXor2>(a));
+            const u32 s = scale_byte<FP4>(a), other = dpp<kMirror8>(s);
+            if ((lane & 7) == 0) pairs[lane >> 3][at] = (uint16_t)(s | (paired ? other << 8 : 0u));
             if (!on || row >= p.rows) continue;
-            // (s lies in [1, 254 - p] for finite blocks: its reciprocal is a normal number)
-            const float inv = s == 255u ? 0.f : __builtin_bit_cast(float, (254u - s) << 23);
-            uint8_t* const d = codes + (int64_t)row * p.codes_ld + (FP4 ? col / 2 : col);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = s == 255u ? 0.f : v[u][i] * inv;
+            uint8_t* const d = codes + (int64_t)row * p.codes_ld;
+            // (s lies in [1, 254 - p] for finite blocks: 2^(s - 127) and its reciprocal are normal numbers)
             if constexpr (FP4) {
-                u32 w = 0;
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][0], v[u][1], 1.f, 0);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][2], v[u][3], 1.f, 1);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][4], v[u][5], 1.f, 2);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[u][6], v[u][7], 1.f, 3);
-                *reinterpret_cast<u32*>(d) = w;
+                const u32 c = v[u].e2m1(__builtin_bit_cast(float, s << 23));
+                *reinterpret_cast<u32*>(d) = s == 255u ? 0u : c;
             } else {
-                int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][0], v[u][1], 0, false);
-                lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][2], v[u][3], lo, true);
-                int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][4], v[u][5], 0, false);
-                hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][6], v[u][7], hi, true);
-                *reinterpret_cast<i32x2*>(d) = i32x2{lo, hi};
+                const i32x2 c = v[u].e4m3(__builtin_bit_cast(float, (254u - s) << 23));
+                *reinterpret_cast<i32x2*>(d) = s == 255u ? i32x2{0, 0} : c;
             }
         }
     }
@@ -155,7 +193,7 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxParams p)
 }
 
 // The values of codes under their scale factors; the same tiles, with the exponent pairs read into LDS first.
-template <typename E, bool FP4, bool VEC, int ROWS>
+template <typename E, bool FP4, int ROWS>
 __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const MxParams p) {
     __shared__ uint16_t pairs[8][ROWS + 2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -208,22 +246,22 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const MxParams 
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] *= scale;
-            store8<E, VEC>(x + (int64_t)row * p.x_ld + col, v);
+            store8<E>(x + (int64_t)row * p.x_ld + col, v);
         }
     }
 }
 
 typedef void (*MxKernel)(const MxParams);
 
-template <bool QUANT, typename E, bool FP4, bool VEC>
-MxKernel pick_rows(bool tall) {
-    if constexpr (QUANT) return tall ? &mx_quantize_kernel<E, FP4, VEC, 64> : &mx_quantize_kernel<E, FP4, VEC, 8>;
-    else return tall ? &mx_dequantize_kernel<E, FP4, VEC, 64> : &mx_dequantize_kernel<E, FP4, VEC, 8>;
-}
 template <bool QUANT, typename E>
-MxKernel pick(bool fp4, bool vec, bool tall) {
-    if (fp4) return vec ? pick_rows<QUANT, E, true, true>(tall) : pick_rows<QUANT, E, true, false>(tall);
-    return vec ? pick_rows<QUANT, E, false, true>(tall) : pick_rows<QUANT, E, false, false>(tall);
+MxKernel pick(bool fp4, bool tall) {
+    if constexpr (QUANT) {
+        if (fp4) return tall ? &mx_quantize_kernel<E, true, 64> : &mx_quantize_kernel<E, true, 8>;
+        return tall ? &mx_quantize_kernel<E, false, 64> : &mx_quantize_kernel<E, false, 8>;
+    } else {
+        if (fp4) return tall ? &mx_dequantize_kernel<E, true, 64> : &mx_dequantize_kernel<E, true, 8>;
+        return tall ? &mx_dequantize_kernel<E, false, 64> : &mx_dequantize_kernel<E, false, 8>;
+    }
 }
 
 template <bool QUANT>
@@ -242,8 +280,7 @@ int mx_run(const dg_mx_args* a, void* stream) {
         return dg_set_error("dg_mx: scale factors need an even leading dimension and 4-byte alignment");
     if (a->codes_ld % 8 != 0 || a->codes_batch_stride % 8 != 0 || !aligned_to(a->codes, 8))
         return dg_set_error("dg_mx: rows of codes must be 8-byte aligned");
-    const int n = f32 ? 4 : 8;
-    const bool vec = a->x_ld % n == 0 && a->x_batch_stride % n == 0 && aligned_to(a->x, 16);
+    if (!aligned_to(a->x, f32 ? 4 : 2)) return dg_set_error("dg_mx: values must be aligned");
     MxParams p = {};
     p.x = a->x; p.codes = a->codes; p.sf = a->sf;
     p.x_ld = a->x_ld; p.x_bs = a->x_batch_stride;
@@ -255,7 +292,7 @@ int mx_run(const dg_mx_args* a, void* stream) {
     const bool tall = (int64_t)ceil_div(a->rows, 64) * p.col_tiles * a->batches >= 1024;
     p.row_tiles = ceil_div(a->rows, tall ? 64 : 8);
     const int64_t grid = (int64_t)p.row_tiles * p.col_tiles * a->batches;
-    return launch_op(f32 ? pick<QUANT, float>(fp4, vec, tall) : pick<QUANT, uint16_t>(fp4, vec, tall), grid, kThreads, p,
+    return launch_op(f32 ? pick<QUANT, float>(fp4, tall) : pick<QUANT, uint16_t>(fp4, tall), grid, kThreads, p,
                      reinterpret_cast<hipStream_t>(stream), a->num_cus);
 }
 

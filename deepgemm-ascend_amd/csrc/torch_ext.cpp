@@ -247,10 +247,206 @@ bool gemm(int64_t gemm_type, const at::Tensor& a, const c10::optional<at::Tensor
     return true;
 }
 
+// ------------------------------------------------------------------------------------------------ operators around the GEMMs
+// The same calls as deep_gemm/moe.py and mx.py make; an empty result sends the call to their general path, which converts what
+// these checks do not take or raises.
+decltype(&dg_moe_sort) g_moe_sort = nullptr;
+decltype(&dg_moe_sort_workspace_size) g_moe_sort_workspace_size = nullptr;
+decltype(&dg_moe_dispatch) g_moe_dispatch = nullptr;
+decltype(&dg_moe_combine) g_moe_combine = nullptr;
+decltype(&dg_moe_combine_backward) g_moe_combine_backward = nullptr;
+decltype(&dg_mx_quantize) g_mx_quantize = nullptr;
+decltype(&dg_mx_dequantize) g_mx_dequantize = nullptr;
+
+void init_operators(int64_t sort, int64_t sort_workspace, int64_t dispatch, int64_t combine, int64_t combine_backward,
+                    int64_t quantize, int64_t dequantize) {
+    g_moe_sort = reinterpret_cast<decltype(g_moe_sort)>(sort);
+    g_moe_sort_workspace_size = reinterpret_cast<decltype(g_moe_sort_workspace_size)>(sort_workspace);
+    g_moe_dispatch = reinterpret_cast<decltype(g_moe_dispatch)>(dispatch);
+    g_moe_combine = reinterpret_cast<decltype(g_moe_combine)>(combine);
+    g_moe_combine_backward = reinterpret_cast<decltype(g_moe_combine_backward)>(combine_backward);
+    g_mx_quantize = reinterpret_cast<decltype(g_mx_quantize)>(quantize);
+    g_mx_dequantize = reinterpret_cast<decltype(g_mx_dequantize)>(dequantize);
+}
+
+using Tensors = std::vector<at::Tensor>;
+
+void raise_pending() {
+    if (const uint32_t bits = pending_errors()) throw std::runtime_error(error_message(bits));
+}
+
+void* stream_ptr(int64_t stream) { return reinterpret_cast<void*>(stream); }
+
+bool int32_rows(const at::Tensor& t, int64_t dim, const at::Device& device) {
+    return t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == device && t.numel() < (int64_t(1) << 31);
+}
+
+// The layout of a MoELayout's four tensors beside rows on `device`.
+bool layout_of(const Tensors& l, const at::Device& device, dg_moe_layout& out) {
+    if (l.size() != 4 || !int32_rows(l[0], 2, device) || !int32_rows(l[1], 1, device) || !int32_rows(l[2], 1, device) ||
+        !int32_rows(l[3], 1, device) || l[3].numel() != l[1].numel())
+        return false;
+    out = {(int32_t)l[0].size(0), (int32_t)l[0].size(1), 0, (int32_t)l[1].numel(), 1, l[0].data_ptr<int32_t>(), l[1].data_ptr<int32_t>(),
+           l[2].data_ptr<int32_t>(), l[3].data_ptr<int32_t>()};
+    return true;
+}
+
+Tensors moe_sort(const at::Tensor& ids, int64_t groups, int64_t rows, int64_t alignment, int64_t num_cus, int64_t stream) {
+    if (g_moe_sort == nullptr || ids.dim() != 2 || !ids.is_cuda() || !ids.is_contiguous() || groups < 1 || groups > 1024 || rows < 0 ||
+        rows % alignment != 0 || rows >= (int64_t(1) << 31) || ids.numel() >= (int64_t(1) << 31) ||
+        !(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong))
+        return {};
+    raise_pending();
+    const auto options = ids.options().dtype(at::kInt);
+    Tensors l = {at::empty(ids.sizes(), options), at::empty({rows}, options), at::empty({groups}, options), at::empty({rows}, options)};
+    dg_moe_layout a;
+    if (!layout_of(l, ids.device(), a)) return {};
+    a.num_groups = (int32_t)groups;
+    a.alignment = (int32_t)alignment;
+    int64_t need = 0;
+    check_rc(g_moe_sort_workspace_size((int32_t)ids.numel(), (int32_t)groups, &need));
+    at::Tensor ws;
+    if (need > 0) ws = at::empty({need}, ids.options().dtype(at::kByte));
+    check_rc(g_moe_sort(ids.data_ptr(), (int32_t)ids.element_size(), &a, need > 0 ? ws.data_ptr() : nullptr, need, (int32_t)num_cus,
+                        stream_ptr(stream)));
+    return l;
+}
+
+Tensors moe_dispatch(const at::Tensor& x, const c10::optional<at::Tensor>& sf, const Tensors& layout, bool zero_padding, int64_t num_cus,
+                     int64_t stream) {
+    dg_moe_layout a;
+    const int64_t e = x.element_size();
+    if (g_moe_dispatch == nullptr || x.dim() != 2 || !x.is_cuda() || !(e == 1 || e == 2 || e == 4) || !layout_of(layout, x.device(), a) ||
+        x.size(0) != a.tokens || !(x.stride(1) == 1 || x.size(1) <= 1))
+        return {};
+    int64_t k64 = 0, sf_ld = 0;
+    const int64_t out_ld = align_up(a.rows, 2);
+    if (sf.has_value()) {
+        if (sf->scalar_type() != at::kShort || sf->dim() != 2 || sf->size(0) != a.tokens || sf->device() != x.device() ||
+            !(a.tokens <= 1 || sf->stride(0) == 1))
+            return {};
+        k64 = sf->size(1);
+        sf_ld = k64 > 1 ? sf->stride(1) : a.tokens;
+    }
+    raise_pending();
+    Tensors out = {at::empty({a.rows, x.size(1)}, x.options())};
+    if (sf.has_value()) out.push_back(at::empty({k64, out_ld}, sf->options()));
+    check_rc(g_moe_dispatch(x.data_ptr(), x.stride(0) * e, x.size(1) * e, &a, out[0].data_ptr(), x.size(1) * e,
+                            sf.has_value() ? static_cast<const int16_t*>(sf->data_ptr()) : nullptr, sf_ld, (int32_t)k64,
+                            sf.has_value() ? static_cast<int16_t*>(out[1].data_ptr()) : nullptr, out_ld, zero_padding, (int32_t)num_cus,
+                            stream_ptr(stream)));
+    if (sf.has_value()) out[1] = out[1].slice(1, 0, a.rows).transpose(0, 1);
+    return out;
+}
+
+int rows_dtype(const at::Tensor& t) {
+    return t.scalar_type() == at::kBFloat16 ? DG_DTYPE_BF16 : t.scalar_type() == at::kFloat ? DG_DTYPE_F32 : -1;
+}
+
+bool plain_rows(const at::Tensor& t, int64_t rows) {
+    return t.dim() == 2 && t.is_cuda() && rows_dtype(t) >= 0 && t.size(0) == rows && (t.stride(1) == 1 || t.size(1) <= 1);
+}
+
+bool plain_weights(const at::Tensor& w, const dg_moe_layout& a, const at::Device& device) {
+    return w.scalar_type() == at::kFloat && w.dim() == 2 && w.size(0) == a.tokens && w.size(1) == a.topk && w.is_contiguous() &&
+           w.device() == device;
+}
+
+Tensors moe_combine(const at::Tensor& rows, const Tensors& layout, const c10::optional<at::Tensor>& weights, int64_t num_cus,
+                    int64_t stream) {
+    dg_moe_layout a;
+    if (g_moe_combine == nullptr || !layout_of(layout, rows.device(), a) || !plain_rows(rows, a.rows) ||
+        (weights.has_value() && !plain_weights(*weights, a, rows.device())))
+        return {};
+    raise_pending();
+    Tensors out = {at::empty({a.tokens, rows.size(1)}, rows.options())};
+    check_rc(g_moe_combine(rows.data_ptr(), rows.stride(0), rows_dtype(rows), rows.size(1), &a,
+                           weights.has_value() ? weights->data_ptr<float>() : nullptr, out[0].data_ptr(), rows.size(1), (int32_t)num_cus,
+                           stream_ptr(stream)));
+    return out;
+}
+
+Tensors moe_combine_backward(const at::Tensor& d_out, const at::Tensor& rows, const Tensors& layout, const at::Tensor& weights,
+                             int64_t num_cus, int64_t stream) {
+    dg_moe_layout a;
+    if (g_moe_combine_backward == nullptr || !layout_of(layout, rows.device(), a) || !plain_rows(rows, a.rows) || !plain_rows(d_out, a.tokens) ||
+        d_out.scalar_type() != rows.scalar_type() || d_out.size(1) != rows.size(1) || d_out.device() != rows.device() ||
+        !plain_weights(weights, a, rows.device()))
+        return {};
+    raise_pending();
+    Tensors out = {at::empty({a.rows, rows.size(1)}, rows.options()), at::empty({a.tokens, a.topk}, weights.options())};
+    check_rc(g_moe_combine_backward(d_out.data_ptr(), d_out.stride(0), rows.data_ptr(), rows.stride(0), rows_dtype(rows), rows.size(1), &a,
+                                    weights.data_ptr<float>(), out[0].data_ptr(), rows.size(1), out[1].data_ptr<float>(), (int32_t)num_cus,
+                                    stream_ptr(stream)));
+    return out;
+}
+
+// A two-dimensional x [M, K] to codes and scale factors.
+Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stream) {
+    if (g_mx_quantize == nullptr || x.dim() != 2 || !x.is_cuda() || rows_dtype(x) < 0 || x.size(1) % 32 != 0 || x.numel() == 0 ||
+        x.stride(1) != 1 || x.size(0) >= (int64_t(1) << 31) || x.size(1) >= (int64_t(1) << 31))
+        return {};
+    raise_pending();
+    const int64_t m = x.size(0), k = x.size(1), ld = align_up(m, 2), k64 = ceil_div(k, 64);
+    Tensors out = {at::empty({m, fp4 ? k / 2 : k}, x.options().dtype(fp4 ? at::kChar : at::kFloat8_e4m3fn)),
+                   at::empty({k64, ld}, x.options().dtype(at::kShort))};
+    dg_mx_args a = {};
+    a.format = fp4 ? DG_MX_E2M1 : DG_MX_E4M3;
+    a.x_dtype = rows_dtype(x);
+    a.batches = 1;
+    a.rows = (int32_t)m;
+    a.k = (int32_t)k;
+    a.x = x.data_ptr();
+    a.x_ld = m > 1 ? x.stride(0) : k;
+    a.codes = out[0].data_ptr();
+    a.codes_ld = out[0].stride(0);
+    a.sf = static_cast<int16_t*>(out[1].data_ptr());
+    a.sf_ld = ld;
+    a.num_cus = (int32_t)num_cus;
+    check_rc(g_mx_quantize(&a, stream_ptr(stream)));
+    out[1] = out[1].slice(1, 0, m).transpose(0, 1);
+    return out;
+}
+
+Tensors mx_dequantize(const at::Tensor& codes, const at::Tensor& sf, bool f32, int64_t num_cus, int64_t stream) {
+    const bool fp4 = codes.scalar_type() == at::kChar;
+    if (g_mx_dequantize == nullptr || codes.dim() != 2 || !codes.is_cuda() || !(fp4 || codes.scalar_type() == at::kFloat8_e4m3fn) ||
+        codes.numel() == 0 || codes.stride(1) != 1)
+        return {};
+    const int64_t m = codes.size(0), k = codes.size(1) * (fp4 ? 2 : 1), k64 = ceil_div(k, 64);
+    if (k % 32 != 0 || m >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || sf.scalar_type() != at::kShort || sf.dim() != 2 ||
+        sf.size(0) != m || sf.size(1) != k64 || sf.device() != codes.device() || !(m <= 1 || sf.stride(0) == 1))
+        return {};
+    raise_pending();
+    Tensors out = {at::empty({m, k}, codes.options().dtype(f32 ? at::kFloat : at::kBFloat16))};
+    dg_mx_args a = {};
+    a.format = fp4 ? DG_MX_E2M1 : DG_MX_E4M3;
+    a.x_dtype = f32 ? DG_DTYPE_F32 : DG_DTYPE_BF16;
+    a.batches = 1;
+    a.rows = (int32_t)m;
+    a.k = (int32_t)k;
+    a.x = out[0].data_ptr();
+    a.x_ld = k;
+    a.codes = codes.data_ptr();
+    a.codes_ld = m > 1 ? codes.stride(0) : codes.size(1);
+    a.sf = static_cast<int16_t*>(sf.data_ptr());
+    a.sf_ld = k64 > 1 ? sf.stride(1) : align_up(m, 2);
+    a.num_cus = (int32_t)num_cus;
+    check_rc(g_mx_dequantize(&a, stream_ptr(stream)));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "deep_gemm C++ host path (validation, scale-factor pass-through and launch)";
     m.def("init", &init, "hand over the library's entry points");
+    m.def("init_operators", &init_operators, "hand over the entry points of the operators around the GEMMs");
+    m.def("moe_sort", &moe_sort, "slots, source, psum and m_indices; empty (here and below): the general path must handle the call");
+    m.def("moe_dispatch", &moe_dispatch, "rows (and their scale factors) from tokens");
+    m.def("moe_combine", &moe_combine, "weighted sums of the tokens' rows");
+    m.def("moe_combine_backward", &moe_combine_backward, "gradients of rows and weights");
+    m.def("mx_quantize", &mx_quantize, "codes and scale factors of a matrix");
+    m.def("mx_dequantize", &mx_dequantize, "values of codes and scale factors");
     m.def("gemm", &gemm, "validate and launch one GEMM; false: the general path must handle the call");
 }

@@ -255,6 +255,9 @@ def ext():
             addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value
             mod.init(addr(lib.dg_gemm), addr(lib.dg_transform_sf), addr(lib.dg_take_errors), addr(lib.dg_last_error),
                      lib.dg_error_words() or 0)
+            mod.init_operators(*(addr(getattr(lib, f)) for f in (
+                'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine', 'dg_moe_combine_backward',
+                'dg_mx_quantize', 'dg_mx_dequantize')))
         _ext = mod
         _ext_tried = True
         return _ext

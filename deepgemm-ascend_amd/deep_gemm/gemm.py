@@ -221,6 +221,12 @@ def _fast():
     return _lib.ext()
 
 
+def _operators(t: torch.Tensor):
+    """The extension when it may serve an operator call on t, else None (csrc/torch_ext.cpp; DG_CHECK_SF and the GEMMs' tuning
+    overrides do not concern these)."""
+    return None if get_dry_run() or not t.is_cuda else _lib.ext()
+
+
 def _fast_recipes(recipe, recipe_a, recipe_b):
     """operand_recipes flattened to (gran_a_mn, gran_a_k, gran_b_mn, gran_b_k), memoised."""
     key = (recipe, recipe_a, recipe_b)

@@ -16,6 +16,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
+from .gemm import _operators, _stream
 from .layout import _assert, _align
 from .runtime import cu_cap, get_dry_run, get_mk_alignment_for_contiguous_layout
 
@@ -54,10 +55,6 @@ def _check_layout(layout: MoELayout, device) -> Tuple[int, int, int]:
     return layout.slots.size(0), layout.slots.size(1), layout.source.numel()
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
 def moe_sort(topk_idx: torch.Tensor, num_groups: int, num_rows: Optional[int] = None) -> MoELayout:
     """The layout of the pairs of ``topk_idx`` [T, K] (int32 or int64 expert ids; a negative id drops its pair).
 
@@ -70,6 +67,11 @@ def moe_sort(topk_idx: torch.Tensor, num_groups: int, num_rows: Optional[int] = 
     alignment = get_mk_alignment_for_contiguous_layout()
     t, k = topk_idx.shape
     rows = moe_num_rows(t * k, num_groups) if num_rows is None else int(num_rows)
+    ext = _operators(topk_idx)
+    if ext is not None:
+        made = ext.moe_sort(topk_idx, num_groups, rows, alignment, cu_cap(), _stream(topk_idx))
+        if made:
+            return MoELayout(*made)
     _assert(rows >= 0 and rows % alignment == 0, f'num_rows must be a multiple of the alignment {alignment}')
     _assert(max(t * k, rows) < 2 ** 31, 'a layout has less than 2^31 pairs and rows')
     topk_idx = topk_idx.contiguous()
@@ -97,6 +99,11 @@ def moe_dispatch(x, layout: MoELayout, zero_padding: bool = True):
     sf = None
     if isinstance(x, tuple):
         x, sf = x
+    ext = _operators(x)
+    if ext is not None:
+        made = ext.moe_dispatch(x, sf, layout, zero_padding, cu_cap(), _stream(x))
+        if made:
+            return made[0] if sf is None else (made[0], made[1])
     _assert(x.dim() == 2 and x.is_cuda, 'x must be a [T, H] device tensor')
     _assert(x.element_size() in (1, 2, 4), 'x must have elements of 1, 2 or 4 bytes')
     t, _, m = _check_layout(layout, x.device)
@@ -141,6 +148,11 @@ def _check_weights(weights: torch.Tensor, layout: MoELayout) -> torch.Tensor:
 def moe_combine(rows: torch.Tensor, layout: MoELayout, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, H] sums over a token's choices of ``weights[t, c] * rows[slots[t, c]]`` (no weights: 1), in fp32 in order, rounded
     once to the type of ``rows`` (bf16 or fp32).  Dropped pairs add nothing, whatever their weight."""
+    ext = _operators(rows)
+    if ext is not None:
+        made = ext.moe_combine(rows, layout, weights, cu_cap(), _stream(rows))
+        if made:
+            return made[0]
     t, _, m = _check_layout(layout, rows.device)
     rows = _check_rows('rows', rows, m, 'rows')
     if weights is not None:
@@ -164,6 +176,11 @@ def moe_combine_backward(d_out: torch.Tensor, rows: torch.Tensor, layout: MoELay
                          weights: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Gradients of ``moe_combine``: (d_rows [M, H] = weights[t, c] * d_out[t] in the pairs' rows, zeros in padding rows;
     d_weights [T, K] fp32 = <d_out[t], rows[slots[t, c]]>, 0 for dropped pairs)."""
+    ext = _operators(rows)
+    if ext is not None:
+        made = ext.moe_combine_backward(d_out, rows, layout, weights, cu_cap(), _stream(rows))
+        if made:
+            return made[0], made[1]
     t, k, m = _check_layout(layout, rows.device)
     rows = _check_rows('rows', rows, m, 'rows')
     d_out = _check_rows('d_out', d_out, t, 'tokens')

@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .gemm import _is_fp4, _stream, fp8_fp4_gemm_nt
+from .gemm import _is_fp4, _operators, _stream, fp8_fp4_gemm_nt
 from .layout import _align, _assert, _ceil_div
 from .runtime import cu_cap, get_dry_run
 
@@ -43,6 +43,11 @@ def mx_quantize(x: torch.Tensor, fmt: str = 'e2m1') -> Tuple[torch.Tensor, torch
     saturates; values round to nearest, ties to even.  A block that holds an infinity or a NaN becomes NaN (scale byte 255)
     and so does every product that reads it."""
     _assert(fmt in _FORMATS, f'unknown format {fmt}: e2m1 or e4m3')
+    ext = _operators(x)
+    if ext is not None:
+        made = ext.mx_quantize(x, fmt == 'e2m1', cu_cap(), _stream(x))
+        if made:
+            return made[0], made[1]
     _assert(x.dim() in (2, 3) and x.is_cuda, 'x must be a [M, K] or [B, M, K] device tensor')
     _assert(x.dtype in _DTYPES, 'x must be bf16 or fp32')
     m, k = x.size(-2), x.size(-1)
@@ -62,6 +67,11 @@ def mx_dequantize(q: Tuple[torch.Tensor, torch.Tensor], dtype: torch.dtype = tor
     """The values [.., M, K] of (codes, sf) as ``mx_quantize`` gives them, exact in bf16 and fp32 down to the type's
     smallest numbers."""
     codes, sf = q
+    ext = _operators(codes)
+    if ext is not None and dtype in _DTYPES:
+        made = ext.mx_dequantize(codes, sf, dtype == torch.float32, cu_cap(), _stream(codes))
+        if made:
+            return made[0]
     fmt = 'e2m1' if _is_fp4(codes) else 'e4m3'
     _assert(fmt == 'e2m1' or codes.dtype == torch.float8_e4m3fn, 'codes must be packed e2m1 (int8) or float8_e4m3fn')
     _assert(codes.dim() in (2, 3) and codes.is_cuda and sf.device == codes.device, 'codes and sf must be device tensors')

@@ -205,6 +205,25 @@ def test_under_a_cu_cap():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_python_path_matches_the_extension(monkeypatch, dtype):
+    assert _lib.ext() is not None
+    g = gen(5)
+    ids, x, w = _ids(200, 4, 9, g, 'dropped').cuda(), torch.randn(200, 72, generator=g).to(dtype).cuda(), torch.rand(200, 4, generator=g).cuda()
+    q = deep_gemm.mx_quantize(torch.randn(200, 160, generator=g).to(dtype).cuda())
+    deep_gemm.set_mk_alignment_for_contiguous_layout(32)
+
+    def everything():
+        layout = deep_gemm.moe_sort(ids, 9)
+        rows = deep_gemm.moe_dispatch(x, layout)
+        return (*layout, rows, *deep_gemm.moe_dispatch(q, layout), deep_gemm.moe_combine(rows, layout, w),
+                deep_gemm.moe_dispatch_backward(rows, layout), *deep_gemm.moe_combine_backward(x, rows, layout, w))
+    fast = everything()
+    monkeypatch.setattr('deep_gemm.moe._operators', lambda t: None)
+    for a, b in zip(everything(), fast):
+        assert a.dtype == b.dtype and a.stride() == b.stride() and torch.equal(a, b)
+
+
 def test_rows_feed_the_grouped_gemms():
     """moe_sort's layouts are what the M-grouped and K-grouped GEMMs take."""
     g = gen(11)

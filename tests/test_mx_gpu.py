@@ -85,6 +85,17 @@ def test_infinities_and_nan(fmt):
     assert torch.equal(d.cpu().isnan().all(dim=1), bad.any(dim=1)) and not d.cpu()[[0, 4]].isnan().any()
 
 
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+def test_python_path_matches_the_extension(monkeypatch, fmt):
+    x = torch.randn(77, 160, generator=gen(6)).cuda()
+    run = lambda: (*deep_gemm.mx_quantize(x, fmt), deep_gemm.mx_dequantize(deep_gemm.mx_quantize(x, fmt)))
+    fast = run()
+    monkeypatch.setattr('deep_gemm.mx._operators', lambda t: None)
+    for a, b in zip(run(), fast):
+        assert a.dtype == b.dtype and a.stride() == b.stride()
+        assert torch.equal(a.view(torch.int8) if a.dtype == torch.float8_e4m3fn else a, b.view(torch.int8) if a.dtype == torch.float8_e4m3fn else b)
+
+
 def test_strides_and_batches():
     x = torch.randn(3, 21, 160, generator=gen(4)).bfloat16()
     for fmt in ('e2m1', 'e4m3'):
