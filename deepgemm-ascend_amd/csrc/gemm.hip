@@ -55,6 +55,10 @@ int check_m_indices(const int32_t* idx, int m, int alignment, int num_groups, hi
 // csrc/status.hip: the run table of an m_indices layout (for anchored tiles)
 int m_indices_runs(const int32_t* idx, int m, int alignment, int32_t* runs, const int32_t* blk_end, hipStream_t st);
 
+// csrc/mx_product.hip: M-grouped psum GEMMs of e2m1 rows, a few to an expert
+bool mx_experts_fit(const dg_gemm_args& a);
+int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* info);
+
 KernelFn lookup_quad_fp8(int bm, int bn, int epi);
 KernelFn lookup_quad_fp8_mn_a(int bm, int bn, int epi);
 KernelFn lookup_quad_fp8_mn_b(int bm, int bn, int epi);
@@ -850,6 +854,12 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
     }
 
     const int cus = a.num_cus > 0 ? a.num_cus : device_cus();
+    // Few rows to an expert, e2m1 on both sides: the weights' bytes are all (32 x 8 pairs over 32 experts, N = 2048 K = 4096:
+    // 33 us against 56 on the 384-row tiles and 59 on 32-row ones).
+    if (mx_experts_fit(a) && k_rows == 0) {
+        if (compile_only && info == nullptr) return DG_OK;
+        return mx_experts(a, cus_capped(cus) ? cus : 0, reinterpret_cast<hipStream_t>(stream), info);
+    }
     if (a.split_k < 0) return dg_set_error("dg_gemm: split_k must be >= 0");
     const bool lib_ws = a.workspace == nullptr && a.library_workspace != 0;
     Plan plan = choose(a, cus, a.workspace != nullptr || lib_ws);

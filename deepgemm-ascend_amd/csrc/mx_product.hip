@@ -1,0 +1,347 @@
+// Products of few rows with e2m1 weights: a token, or an expert's few tokens, against all rows of w.
+//
+//   D[m][n] = sum over blocks b of 2^(sa[m][b] + sw[n][b] - 254) sum_{k in b} a[m][k] w[n][k]
+// Bound by the bytes of w, which is read once, straight into registers: a lane of v_mfma_scale_f32_16x16x128_f8f6f4 holds the
+// 16 bytes of one block of 32 codes of one row, so a wave's load is 16 rows x 64 bytes as they lie in memory, no two lanes
+// need the same bytes, and neither LDS nor a barrier stands between memory and the matrix unit.  A wave owns 32 rows of w and
+// a range of K, a few steps of 128 ahead in registers; the waves of a workgroup that share rows join their sums in LDS, in
+// order.  The few rows of a come the same way (from the caches).
+//
+// The rows of a are e2m1 codes (an M-grouped layout: each expert's rows with its weights), or bf16 / fp32 values that each wave
+// quantises as it loads them: the 32 values of a block are one lane's, so its scale needs no other lane.
+#include "gemm_kernel.hpp"
+#include "op_launch.hpp"
+#include "mx_scale.hpp"
+
+namespace dg {
+namespace {
+
+struct MxProductParams {
+    const uint8_t* a;          // codes [rows][lda], or values
+    const uint8_t* w;          // codes [groups][n][ldw]
+    uint8_t* d;
+    const uint16_t *sfa, *sfw; // [k64][ld]; sfa: codes only
+    const int* psum;           // M-grouped layout, or nullptr: one group of m rows
+    int m, n, k, groups, alignment;
+    int64_t lda, ldw, ldd;     // bytes, bytes, elements
+    int64_t w_bs, sfw_bs;      // bytes, int16 elements
+    int64_t sfa_ld, sfw_ld;
+    int f32, accumulate;       // of D
+    int strips, grid;
+    int vbase;
+};
+
+enum Rows : int { kCodes = 0, kBf16Rows = 1, kF32Rows = 2 };
+
+// The 32 values of a block as e2m1 codes and their exponent byte (mx_quant.hip's).
+__device__ __forceinline__ void quantise_block(const float (&v)[32], i32x4& codes, int& scale) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+    const uint32_t s = scale_byte<true>(top);
+    const float f = __builtin_bit_cast(float, s << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j], v[8 * j + 1], f, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 2], v[8 * j + 3], f, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 4], v[8 * j + 5], f, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 6], v[8 * j + 7], f, 3);
+        codes[j] = s == 255u ? 0 : (int)c;
+    }
+    scale = (int)s;
+}
+
+// x >> sh, kept where it stands (with the two wait states that an MFMA wants after a write of its operand: the compiler does
+// not see into the asm).
+__device__ __forceinline__ int shifted(int x, int sh) {
+    int y;
+    asm volatile("v_lshrrev_b32 %0, %1, %2\n\ts_nop 1" : "=v"(y) : "v"(sh), "v"(x));
+    return y;
+}
+
+constexpr int kNB = 2;         // 16-row blocks of w of a wave
+constexpr int kStrip = 16 * kNB;
+
+// MT: 16-row blocks of a in flight together; DEPTH: steps of 128 values of K ahead.
+template <int ROWS, int MT, int DEPTH, int KS>
+__device__ __forceinline__ void product_rows(const MxProductParams& p, const uint8_t* a, const uint16_t* sfa, const uint8_t* w,
+                                             const uint16_t* sfw, uint8_t* d, int rows, int n0, float* red) {
+    constexpr int EA = ROWS == kCodes ? 0 : ROWS == kBf16Rows ? 2 : 4;       // bytes of a value of a
+    constexpr int A_REGS = ROWS == kCodes ? 1 : ROWS == kBf16Rows ? 4 : 8;   // 16-byte loads of a block of 32
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);       // of K (KS waves share the strip)
+    const int blocks = p.k / 32, steps = ceil_div(blocks, 4), per = ceil_div(steps, KS);
+    const int s0 = part * per, s1 = min(steps, s0 + per);
+    const int cols = min(kStrip, p.n - n0);
+    const __amdgpu_buffer_rsrc_t rs_w = make_rsrc(w, (int64_t)cols * p.ldw);
+    const __amdgpu_buffer_rsrc_t rs_a = make_rsrc(a, (int64_t)rows * p.lda);
+    const int k64 = ceil_div(p.k, 64);
+    // Scales: a lane loads the dword of its row pair (leading dimensions are even) and shifts its byte down where it is used.
+    // (Of a byte load the compiler clears the upper bytes, all at the head of the loop, behind a wait for every load in flight.)
+    const __amdgpu_buffer_rsrc_t rs_sw = make_rsrc(sfw, ((int64_t)(k64 - 1) * p.sfw_ld + align_up(cols, 2)) * 2);
+    const __amdgpu_buffer_rsrc_t rs_sa = make_rsrc(sfa, ROWS == kCodes ? ((int64_t)(k64 - 1) * p.sfa_ld + align_up(rows, 2)) * 2 : 0);
+    const int shift = 8 * ((r & 1) * 2 + (g & 1));
+    uint32_t vw[kNB], vsw[kNB], va[MT], vsa[MT];    // (rows past the end: out of range, zeros)
+#pragma unroll
+    for (int j = 0; j < kNB; ++j) {
+        const bool on = 16 * j + r < cols;
+        vw[j] = on ? (uint32_t)((16 * j + r) * p.ldw + 16 * g) : kOOBOffset;
+        vsw[j] = on ? (uint32_t)(((g >> 1) * p.sfw_ld + 16 * j + (r & ~1)) * 2) : kOOBOffset;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const bool on = 16 * i + r < rows;
+        va[i] = on ? (uint32_t)((16 * i + r) * p.lda + (ROWS == kCodes ? 16 : 32 * EA) * g) : kOOBOffset;
+        vsa[i] = on ? (uint32_t)(((g >> 1) * p.sfa_ld + 16 * i + (r & ~1)) * 2) : kOOBOffset;
+    }
+    i32x4 fw[DEPTH][kNB], fa[DEPTH][MT][A_REGS];
+    int sw[DEPTH][kNB], sa[DEPTH][MT];
+    auto load = [&](auto slot, int s) {
+        constexpr int S = decltype(slot)::value;
+        const bool on = s < s1 && 4 * s + g < blocks;   // (past K: zeros)
+        const int step_w = __builtin_amdgcn_readfirstlane(s * 64), step_sw = __builtin_amdgcn_readfirstlane((int)(s * 4 * p.sfw_ld));
+#pragma unroll
+        for (int j = 0; j < kNB; ++j) {
+            fw[S][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_w, on ? vw[j] : kOOBOffset, step_w, 0));
+            sw[S][j] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sw, on ? vsw[j] : kOOBOffset, step_sw, 0);
+        }
+        const int step_a = __builtin_amdgcn_readfirstlane(ROWS == kCodes ? s * 64 : s * 128 * EA);
+        const int step_sa = __builtin_amdgcn_readfirstlane((int)(s * 4 * p.sfa_ld));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int x = 0; x < A_REGS; ++x)
+                fa[S][i][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_a, on ? va[i] + 16 * x : kOOBOffset, step_a, 0));
+            if constexpr (ROWS == kCodes) sa[S][i] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sa, on ? vsa[i] : kOOBOffset, step_sa, 0);
+        }
+    };
+    f32x4 acc[kNB][MT];
+#pragma unroll
+    for (int j = 0; j < kNB; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        int scale_w[kNB];
+#pragma unroll
+        for (int j = 0; j < kNB; ++j) scale_w[j] = shifted(sw[S][j], shift);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            i32x4 c;
+            int scale;
+            if constexpr (ROWS == kCodes) {
+                c = fa[S][i][0];
+                scale = shifted(sa[S][i], shift);
+            } else {
+                float v[32];
+#pragma unroll
+                for (int x = 0; x < A_REGS; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t b = (uint32_t)fa[S][i][x][e];
+                        if constexpr (ROWS == kBf16Rows) {
+                            v[8 * x + 2 * e] = __builtin_bit_cast(float, b << 16);
+                            v[8 * x + 2 * e + 1] = __builtin_bit_cast(float, b & 0xffff0000u);
+                        } else {
+                            v[4 * x + e] = __builtin_bit_cast(float, b);
+                        }
+                    }
+                quantise_block(v, c, scale);
+            }
+            const i32x8 fa8 = {c[0], c[1], c[2], c[3], 0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < kNB; ++j) {
+                const i32x4 b = fw[S][j];
+                const i32x8 fb8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+                acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb8, fa8, acc[j][i], kFmtE2M1, kFmtE2M1, 0, scale_w[j], 0, scale);
+            }
+        }
+    };
+    static_for<DEPTH>([&](auto s) {
+        load(s, s0 + decltype(s)::value);
+        __builtin_amdgcn_sched_barrier(0);
+    });
+    for (int s = s0; s < s1; s += DEPTH) {
+        static_for<DEPTH>([&](auto x) {
+            multiply(x);   // (a step past the range holds zeros and adds nothing)
+            __builtin_amdgcn_sched_barrier(0);
+            load(x, s + DEPTH + decltype(x)::value);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+    // sums of the K ranges, in order: red[part][block][lane]
+    if constexpr (KS > 1) {
+        __syncthreads();       // (an earlier chunk's sums have been read)
+#pragma unroll
+        for (int j = 0; j < kNB; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(red + ((part * kNB * MT + j * MT + i) * 64 + lane) * 4) = acc[j][i];
+        __syncthreads();
+        if (part != 0) return;
+        for (int w2 = 1; w2 < KS; ++w2)
+#pragma unroll
+            for (int j = 0; j < kNB; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i] += *reinterpret_cast<const f32x4*>(red + ((w2 * kNB * MT + j * MT + i) * 64 + lane) * 4);
+    }
+    // lane (r, g): columns 4 g .. + 3 of block j, row 16 i + r of a
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int row = 16 * i + r;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < kNB; ++j) {
+            const int n = n0 + 16 * j + 4 * g, live = min(4, p.n - n);
+            const int64_t at = row * p.ldd + n;
+            f32x4 v = acc[j][i];
+            if (p.f32) {
+                float* const out = reinterpret_cast<float*>(d) + at;
+                for (int x = 0; x < live; ++x) out[x] = p.accumulate ? out[x] + v[x] : v[x];
+            } else {
+                uint16_t* const out = reinterpret_cast<uint16_t*>(d) + at;
+                if (!p.accumulate && live == 4 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+                    *reinterpret_cast<i32x2*>(out) = i32x2{(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3])};
+                } else {
+                    for (int x = 0; x < live; ++x) out[x] = f32_to_bf16_rne(p.accumulate ? v[x] + bf16_to_f32(out[x]) : v[x]);
+                }
+            }
+        }
+    }
+}
+
+// Zeros in columns [n0, n0 + cols) of row `row`, by the lanes of a wave.
+__device__ __forceinline__ void clear_row(const MxProductParams& p, int64_t row, int n0, int cols, int lane) {
+    for (int c = lane; c < cols; c += 64) {
+        if (p.f32) reinterpret_cast<float*>(p.d)[row * p.ldd + n0 + c] = 0.f;
+        else reinterpret_cast<uint16_t*>(p.d)[row * p.ldd + n0 + c] = 0;
+    }
+}
+
+template <int ROWS, int KS>
+__global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductParams p) {
+    __shared__ __attribute__((aligned(16))) float red[KS > 1 ? KS * kNB * 2 * 256 : 4];
+    // (neighbouring strips, whose scale factors share lines, on one XCD)
+    const int t = xcd_remap(blockIdx.x + p.vbase, p.grid);
+    const int e = t / p.strips, n0 = (t - e * p.strips) * kStrip, cols = min(kStrip, p.n - n0);
+    const uint8_t* const w = p.w + (int64_t)e * p.w_bs + (int64_t)n0 * p.ldw;
+    const uint16_t* const sfw = p.sfw + (int64_t)e * p.sfw_bs + n0;
+    if constexpr (ROWS != kCodes) {
+        product_rows<ROWS, 1, ROWS == kBf16Rows ? 4 : 2, KS>(p, p.a, nullptr, w, sfw, p.d, p.m, n0, red);
+    } else {
+        int first = 0, rows = p.m, end = p.m;
+        if (p.psum != nullptr) {
+            first = e == 0 ? 0 : max(0, align_up(p.psum[e - 1], p.alignment));
+            rows = min(p.m, p.psum[e]) - first;
+            end = min(p.m, align_up(p.psum[e], p.alignment));
+            first = __builtin_amdgcn_readfirstlane(first);
+            rows = __builtin_amdgcn_readfirstlane(rows);
+        }
+        const int esize = p.f32 ? 4 : 2;
+        // (an expert with more rows than fit reads its weights again, from the caches)
+        for (int m0 = 0; m0 < rows; m0 += 32) {
+            const uint8_t* const a = p.a + (int64_t)(first + m0) * p.lda;
+            const uint16_t* const sfa = p.sfa + first + m0;
+            uint8_t* const d = p.d + (int64_t)(first + m0) * p.ldd * esize;
+            if (rows - m0 <= 16) product_rows<ROWS, 1, 6, KS>(p, a, sfa, w, sfw, d, rows - m0, n0, red);
+            else product_rows<ROWS, 2, 4, KS>(p, a, sfa, w, sfw, d, min(32, rows - m0), n0, red);
+        }
+        if (p.psum != nullptr) {
+            // padding rows of the group, and every groups-th row past the last group, are zeros
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+            for (int m = first + max(rows, 0) + wave; m < end; m += KS) clear_row(p, m, n0, cols, lane);
+            for (int64_t m = (int64_t)align_up(p.psum[p.groups - 1], p.alignment) + e + (int64_t)wave * p.groups; m < p.m; m += (int64_t)KS * p.groups)
+                clear_row(p, m, n0, cols, lane);
+        }
+    }
+}
+
+// Waves that share a strip: as many as give the card about eight waves a CU, while each keeps two steps.
+int k_waves(int64_t strips, int k) {
+    int ks = 1;
+    while (ks < 8 && strips * ks < 2048 && ceil_div(k, 128) >= 4 * ks) ks *= 2;
+    return ks;
+}
+
+template <int ROWS>
+int launch_product(MxProductParams p, hipStream_t st, int cus) {
+    p.strips = ceil_div(p.n, kStrip);
+    const int64_t grid = (int64_t)p.strips * p.groups;
+    if (grid > 0x7fffffffLL) return dg_set_error("dg_mx_gemm: too many workgroups");
+    p.grid = (int)grid;
+    switch (k_waves(grid, p.k)) {
+        case 1: return launch_op(mx_product_kernel<ROWS, 1>, grid, 64, p, st, cus);
+        case 2: return launch_op(mx_product_kernel<ROWS, 2>, grid, 128, p, st, cus);
+        case 4: return launch_op(mx_product_kernel<ROWS, 4>, grid, 256, p, st, cus);
+        default: return launch_op(mx_product_kernel<ROWS, 8>, grid, 512, p, st, cus);
+    }
+}
+
+bool span32(int64_t rows, int64_t ld_bytes) { return rows * ld_bytes < 0x40000000LL; }
+
+}  // namespace
+
+// csrc/gemm.hip: an M-grouped psum GEMM of e2m1 rows, a few to an expert.  Whether this kernel serves it.
+bool mx_experts_fit(const dg_gemm_args& a) {
+    return a.gemm_type == kMGroupedPsum && a.kind == kFP4FP4 && a.k > 0 && a.k % 32 == 0 && a.m <= 64 * a.num_groups &&
+           (a.d_dtype == DG_DTYPE_BF16 || a.d_dtype == DG_DTYPE_F32) && a.epilogue == DG_EPI_DEFAULT && !a.accumulate &&
+           a.bias == nullptr && a.alpha == 1.0f && a.block_m == 0 && a.block_n == 0 && a.split_k <= 1 && !a.jit && span32(32, a.lda) &&
+           span32(kStrip, a.ldb) && span32(ceil_div(a.k, 64), a.sfa_ld * 2) && span32(ceil_div(a.k, 64), a.sfb_ld * 2);
+}
+
+int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* info) {
+    MxProductParams p = {};
+    p.a = reinterpret_cast<const uint8_t*>(a.a); p.w = reinterpret_cast<const uint8_t*>(a.b); p.d = reinterpret_cast<uint8_t*>(a.d);
+    p.sfa = reinterpret_cast<const uint16_t*>(a.sfa); p.sfw = reinterpret_cast<const uint16_t*>(a.sfb);
+    p.psum = a.grouped_layout;
+    p.m = a.m; p.n = a.n; p.k = a.k; p.groups = a.num_groups; p.alignment = a.alignment;
+    p.lda = a.lda; p.ldw = a.ldb; p.ldd = a.ldd;
+    p.w_bs = a.batch_stride_b; p.sfw_bs = a.sfb_batch_stride;
+    p.sfa_ld = a.sfa_ld; p.sfw_ld = a.sfb_ld;
+    p.f32 = a.d_dtype == DG_DTYPE_F32;
+    if (info != nullptr) {
+        const int64_t grid = (int64_t)ceil_div(a.n, kStrip) * a.num_groups;
+        info->block_m = 32;
+        info->block_n = kStrip;
+        info->plan_workgroups = info->tiles = grid;
+        info->grid = cus > 0 ? std::min<int64_t>(grid, cus) : grid;
+        info->threads = 64 * k_waves(grid, a.k);
+        info->split_k = 1;
+        info->skinny = 4;
+        return DG_OK;
+    }
+    return launch_product<kCodes>(p, st, cus);
+}
+
+}  // namespace dg
+
+extern "C" int dg_mx_gemm(const void* x, int32_t x_dtype, int64_t x_ld, const void* w, int64_t w_ld, const int16_t* sfw, int64_t sfw_ld,
+                          void* d, int32_t d_dtype, int64_t ldd, int32_t m, int32_t n, int32_t k, int32_t accumulate, int32_t num_cus,
+                          void* stream) {
+    using namespace dg;
+    if (m < 0 || n < 0 || k < 0) return dg_set_error("dg_mx_gemm: negative size");
+    if (x_dtype != DG_DTYPE_BF16 && x_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx_gemm: x is bf16 or fp32");
+    if (d_dtype != DG_DTYPE_BF16 && d_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx_gemm: D is bf16 or fp32");
+    if (m > 16) {
+        dg_set_error("dg_mx_gemm: more than 16 rows (quantise them with dg_mx_quantize, then dg_gemm)");
+        return DG_ENOKERNEL;
+    }
+    if (k % 32 != 0 || k == 0) return dg_set_error("dg_mx_gemm: K must be a multiple of the block of 32 values");
+    if (m == 0 || n == 0) return DG_OK;
+    const int64_t e = x_dtype == DG_DTYPE_F32 ? 4 : 2;
+    if (x == nullptr || w == nullptr || sfw == nullptr || d == nullptr) return dg_set_error("dg_mx_gemm: null tensor");
+    if ((m > 1 && x_ld < k) || w_ld < k / 2 || sfw_ld < n || (m > 1 && ldd < n)) return dg_set_error("dg_mx_gemm: leading dimension smaller than the row");
+    if (x_ld * e % 4 != 0 || !aligned_to(x, 4) || w_ld % 4 != 0 || !aligned_to(w, 4) || !aligned_to(d, d_dtype == DG_DTYPE_F32 ? 4 : 2))
+        return dg_set_error("dg_mx_gemm: rows of x and w must be 4-byte aligned");
+    if (sfw_ld % 2 != 0 || !aligned_to(sfw, 4)) return dg_set_error("dg_mx_gemm: scale factors need an even leading dimension and 4-byte alignment");
+    if (!span32(16, x_ld * e) || !span32(kStrip, w_ld) || !span32(ceil_div(k, 64), sfw_ld * 2)) return dg_set_error("dg_mx_gemm: row stride too large");
+    MxProductParams p = {};
+    p.a = reinterpret_cast<const uint8_t*>(x); p.w = reinterpret_cast<const uint8_t*>(w); p.d = reinterpret_cast<uint8_t*>(d);
+    p.sfw = reinterpret_cast<const uint16_t*>(sfw);
+    p.m = m; p.n = n; p.k = k; p.groups = 1; p.alignment = 1;
+    p.lda = x_ld * e; p.ldw = w_ld; p.ldd = ldd; p.sfw_ld = sfw_ld;
+    p.f32 = d_dtype == DG_DTYPE_F32;
+    p.accumulate = accumulate != 0;
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return x_dtype == DG_DTYPE_F32 ? launch_product<kF32Rows>(p, st, num_cus) : launch_product<kBf16Rows>(p, st, num_cus);
+}

@@ -10,6 +10,7 @@
 // Scale factors come out as the GEMMs read them: int16 pairs of exponent bytes (even block low), [k64][ld], rows
 // contiguous.
 #include "op_launch.hpp"
+#include "mx_scale.hpp"
 
 namespace dg {
 namespace {
@@ -43,15 +44,6 @@ __device__ __forceinline__ void store8(E* x, const float (&v)[8]) {
         *reinterpret_cast<f32x4_any*>(x) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4_any*>(x + 4) = f32x4{v[4], v[5], v[6], v[7]};
     }
-}
-
-// Exponent byte of a block whose largest magnitude has the fp32 bits `a`.
-template <bool FP4>
-__device__ __forceinline__ u32 scale_byte(u32 a) {
-    if (a >= 0x7f800000u) return 255u;
-    // (adding what lies between l and 2 carries into the exponent where the mantissa passes l)
-    const u32 e = (a + (FP4 ? 0x3fffffu : 0x1fffffu)) >> 23;
-    return max(e, FP4 ? 3u : 9u) - (FP4 ? 2u : 8u);
 }
 
 // Largest of a value's over a block's four lanes and the partner block's value: lane exchanges within a row of the wave

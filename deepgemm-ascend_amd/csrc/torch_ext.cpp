@@ -257,9 +257,10 @@ decltype(&dg_moe_combine) g_moe_combine = nullptr;
 decltype(&dg_moe_combine_backward) g_moe_combine_backward = nullptr;
 decltype(&dg_mx_quantize) g_mx_quantize = nullptr;
 decltype(&dg_mx_dequantize) g_mx_dequantize = nullptr;
+decltype(&dg_mx_gemm) g_mx_gemm = nullptr;
 
 void init_operators(int64_t sort, int64_t sort_workspace, int64_t dispatch, int64_t combine, int64_t combine_backward,
-                    int64_t quantize, int64_t dequantize) {
+                    int64_t quantize, int64_t dequantize, int64_t mx_gemm) {
     g_moe_sort = reinterpret_cast<decltype(g_moe_sort)>(sort);
     g_moe_sort_workspace_size = reinterpret_cast<decltype(g_moe_sort_workspace_size)>(sort_workspace);
     g_moe_dispatch = reinterpret_cast<decltype(g_moe_dispatch)>(dispatch);
@@ -267,6 +268,7 @@ void init_operators(int64_t sort, int64_t sort_workspace, int64_t dispatch, int6
     g_moe_combine_backward = reinterpret_cast<decltype(g_moe_combine_backward)>(combine_backward);
     g_mx_quantize = reinterpret_cast<decltype(g_mx_quantize)>(quantize);
     g_mx_dequantize = reinterpret_cast<decltype(g_mx_dequantize)>(dequantize);
+    g_mx_gemm = reinterpret_cast<decltype(g_mx_gemm)>(mx_gemm);
 }
 
 using Tensors = std::vector<at::Tensor>;
@@ -436,6 +438,38 @@ Tensors mx_dequantize(const at::Tensor& codes, const at::Tensor& sf, bool f32, i
     return out;
 }
 
+// D (+)= quantised(x) w^T: rows of e2m1 codes in one launch up to 16 of them, otherwise quantised first.  false: the general path.
+// cus: what the GEMMs take (set_num_sms, 0 = all); num_cus: the cap, 0 = none.
+bool mx_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sfw, const at::Tensor& d, const c10::optional<at::Tensor>& c,
+             bool fp4, int64_t cus, int64_t num_cus, int64_t alignment, int64_t stream) {
+    if (g_mx_gemm == nullptr || x.dim() != 2 || w.dim() != 2 || d.dim() != 2 || sfw.dim() != 2 || !x.is_cuda() || rows_dtype(x) < 0 ||
+        rows_dtype(d) < 0 || w.scalar_type() != at::kChar || sfw.scalar_type() != at::kShort || w.device() != x.device() ||
+        sfw.device() != x.device() || d.device() != x.device())
+        return false;
+    const int64_t m = x.size(0), k = x.size(1), n = w.size(0), k64 = ceil_div(k, 64);
+    if (m > 16 || !fp4) {
+        const Tensors q = mx_quantize(x, fp4, num_cus, stream);
+        return !q.empty() && gemm(kNormal, q[0], q[1], w, sfw, d, c, c10::nullopt, 1, 32, 1, 32, cus, alignment, stream);
+    }
+    if (m == 0 || n == 0 || k == 0 || k % 32 != 0 || k >= (int64_t(1) << 31) || n >= (int64_t(1) << 31) || w.size(1) * 2 != k ||
+        sfw.size(0) != n || sfw.size(1) != k64 || d.size(0) != m || d.size(1) != n || x.stride(1) != 1 || w.stride(1) != 1 ||
+        d.stride(1) != 1 || !(n <= 1 || sfw.stride(0) == 1))
+        return false;
+    const int64_t sf_ld = k64 > 1 ? sfw.stride(1) : align_up(n, 2), e = x.element_size();
+    if (sf_ld % 2 != 0 || sf_ld < n || (reinterpret_cast<uintptr_t>(sfw.data_ptr()) & 3) || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 3) ||
+        (reinterpret_cast<uintptr_t>(w.data_ptr()) & 3) || (m > 1 && (x.stride(0) < k || (x.stride(0) * e) % 4 || d.stride(0) < n)) ||
+        (n > 1 && (w.stride(0) < k / 2 || w.stride(0) % 4)))
+        return false;
+    if (c.has_value() && (c->data_ptr() != d.data_ptr() || c->sizes() != d.sizes() || c->strides() != d.strides() ||
+                          c->scalar_type() != d.scalar_type()))
+        return false;
+    raise_pending();
+    check_rc(g_mx_gemm(x.data_ptr(), rows_dtype(x), m > 1 ? x.stride(0) : k, w.data_ptr(), n > 1 ? w.stride(0) : k / 2,
+                       static_cast<const int16_t*>(sfw.data_ptr()), sf_ld, d.data_ptr(), rows_dtype(d), m > 1 ? d.stride(0) : n,
+                       (int32_t)m, (int32_t)n, (int32_t)k, c.has_value(), (int32_t)num_cus, stream_ptr(stream)));
+    return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -448,5 +482,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("moe_combine_backward", &moe_combine_backward, "gradients of rows and weights");
     m.def("mx_quantize", &mx_quantize, "codes and scale factors of a matrix");
     m.def("mx_dequantize", &mx_dequantize, "values of codes and scale factors");
+    m.def("mx_gemm", &mx_gemm, "product of rows quantised on the way; false: the general path must handle the call");
     m.def("gemm", &gemm, "validate and launch one GEMM; false: the general path must handle the call");
 }

@@ -25,7 +25,7 @@ EXPORTED_SYMBOLS = ('dg_gemm', 'dg_transform_sf', 'dg_transform_k_grouped_sf', '
                     'dg_gemm_workspace_size', 'dg_last_error', 'dg_version', 'dg_jit_compile', 'dg_jit_set_include_dir',
                     'dg_jit_stats', 'dg_launch_plan', 'dg_gemm_noalloc', 'dg_take_errors', 'dg_error_words',
                     'dg_stream_workspace', 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine',
-                    'dg_moe_combine_backward', 'dg_mx_quantize', 'dg_mx_dequantize', 'dg_linear_xent_workspace_size',
+                    'dg_moe_combine_backward', 'dg_mx_quantize', 'dg_mx_dequantize', 'dg_mx_gemm', 'dg_linear_xent_workspace_size',
                     'dg_linear_xent_forward', 'dg_linear_xent_backward')
 
 # Sticky error bits kernels report through host-mapped words (DG_ERR_* in the header)
@@ -170,6 +170,7 @@ def load(path=None) -> ctypes.CDLL:
                 ('dg_moe_combine_backward', [ptr, i64, ptr, i64, i32, i64, layout, ptr, ptr, i64, ptr, i32, ptr]),
                 ('dg_mx_quantize', [ctypes.POINTER(MxArgs), ptr]),
                 ('dg_mx_dequantize', [ctypes.POINTER(MxArgs), ptr]),
+                ('dg_mx_gemm', [ptr, i32, i64, ptr, i64, ptr, i64, ptr, i32, i64, i32, i32, i32, i32, i32, ptr]),
                 ('dg_linear_xent_workspace_size', [ctypes.POINTER(LinearXentArgs), i32, ctypes.POINTER(i64)]),
                 ('dg_linear_xent_forward', [ctypes.POINTER(LinearXentArgs), ptr]),
                 ('dg_linear_xent_backward', [ctypes.POINTER(LinearXentArgs), ptr])):
@@ -257,7 +258,7 @@ def ext():
                      lib.dg_error_words() or 0)
             mod.init_operators(*(addr(getattr(lib, f)) for f in (
                 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine', 'dg_moe_combine_backward',
-                'dg_mx_quantize', 'dg_mx_dequantize')))
+                'dg_mx_quantize', 'dg_mx_dequantize', 'dg_mx_gemm')))
         _ext = mod
         _ext_tried = True
         return _ext

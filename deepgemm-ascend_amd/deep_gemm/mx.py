@@ -11,7 +11,8 @@ import torch
 from . import _lib
 from .gemm import _is_fp4, _operators, _stream, fp8_fp4_gemm_nt
 from .layout import _align, _assert, _ceil_div
-from .runtime import cu_cap, get_dry_run
+from . import runtime as _rt
+from .runtime import cu_cap, get_dry_run, get_jit
 
 _FORMATS = {'e2m1': _lib.DG_MX_E2M1, 'e4m3': _lib.DG_MX_E4M3}
 _DTYPES = {torch.bfloat16: _lib.DG_DTYPE_BF16, torch.float32: _lib.DG_DTYPE_F32}
@@ -91,4 +92,9 @@ def mx_gemm_nt(x: torch.Tensor, w: Tuple[torch.Tensor, torch.Tensor], d: torch.T
     """D = quantised(x) @ w^T (+ C): ``x`` [M, K] bf16 or fp32 is quantised to ``fmt`` on the way, ``w`` = (codes, sf) holds [N, K]
     weights in e2m1 as ``mx_quantize`` gives them; ``d`` [M, N] bf16 or fp32 and ``c`` as in ``fp8_fp4_gemm_nt``."""
     _assert(_is_fp4(w[0]), 'mx_gemm_nt takes e2m1 weights (for e4m3 ones: mx_quantize, then fp8_gemm_nt)')
+    _assert(fmt in _FORMATS, f'unknown format {fmt}: e2m1 or e4m3')
+    ext = _operators(x)
+    if ext is not None and not get_jit() and \
+            ext.mx_gemm(x, w[0], w[1], d, c, fmt == 'e2m1', _rt._num_sms, cu_cap(), _rt._mk_alignment, _stream(x)):
+        return
     fp8_fp4_gemm_nt(mx_quantize(x, fmt), w, d, c, recipe_a=(1, 32), recipe_b=(1, 32))

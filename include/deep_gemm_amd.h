@@ -277,7 +277,7 @@ typedef struct dg_launch_info {
     int64_t tiles;                /* output tiles (strips) of the problem                         */
     int32_t split_k;              /* K ranges per tile (1 = unsplit)                              */
     int32_t persistent;           /* 1: workgroups walk tiles (grid < tiles possible)             */
-    int32_t skinny;               /* 1: the decode-shape kernel, 2: its shared-ring variant, 3: the decode GEMV kernel (block_m = M rows served, block_n = rows of B per workgroup, 64 / its K split) */
+    int32_t skinny;               /* 1: the decode-shape kernel, 2: its shared-ring variant, 3: the decode GEMV kernel (block_m = M rows served, block_n = rows of B per workgroup, 64 / its K split), 4: the kernel of few e2m1 rows to an expert */
     int64_t plan_workgroups;      /* workgroups of the plan; under a CU cap (num_cus below the
                                      device's CUs) they go out in stream-ordered launches of at
                                      most `grid` <= num_cus workgroups each (the persistent kernel:
@@ -351,6 +351,13 @@ typedef struct dg_mx_args {
 } dg_mx_args;
 int dg_mx_quantize(const dg_mx_args *args, void *stream);
 int dg_mx_dequantize(const dg_mx_args *args, void *stream);
+
+/* D[m][n] (+)= x w^T with the rows of x (bf16 or fp32) quantised to e2m1 on the way, as dg_mx_quantize does it, and e2m1 weights
+ * [n][k] with required-layout scale factors; D bf16 or fp32.  One launch for at most 16 rows (DG_ENOKERNEL above: quantise, then
+ * dg_gemm).  x_ld and ldd in elements, w_ld in bytes; rows of x and w 4-byte aligned. */
+int dg_mx_gemm(const void *x, int32_t x_dtype, int64_t x_ld, const void *w, int64_t w_ld, const int16_t *sfw, int64_t sfw_ld,
+               void *d, int32_t d_dtype, int64_t ldd, int32_t m, int32_t n, int32_t k, int32_t accumulate, int32_t num_cus,
+               void *stream);
 
 /*
  * Cross entropy of a linear layer over a vocabulary, without keeping the logits:

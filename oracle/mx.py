@@ -11,15 +11,13 @@ E2M1 = [float(v) for v in quant.FP4_VALUES[:8]]
 E4M3 = [float(v) for v in quant.e4m3_decode_table()[:0x7f]]   # (positive, finite; ascending)
 
 
-def scale_byte(amax: float, fmt: str) -> int:
-    """Exponent byte of the smallest power of two, at least 2^-126, under which amax stays inside the format."""
-    if not math.isfinite(amax):
-        return 255
-    largest = 6.0 if fmt == 'e2m1' else 448.0
-    e = -126
-    while amax > largest * 2.0 ** e:
-        e += 1
-    return e + 127
+def scale_bytes_of(amax: np.ndarray, fmt: str) -> np.ndarray:
+    """Exponent bytes of the smallest powers of two, at least 2^-126, under which amax stays inside the format (255: no
+    finite number).  With amax = m 2^e and the largest value l 2^p, m and l in [0.5, 1): e - p, and one more where m > l."""
+    l, p = math.frexp(6.0 if fmt == 'e2m1' else 448.0)
+    m, e = np.frexp(amax)
+    e = np.where(amax == 0, -1000, e)
+    return np.where(np.isfinite(amax), np.maximum(e - p + (m > l), -126) + 127, 255).astype(np.int64)
 
 
 def quantize(x: torch.Tensor, fmt: str):
@@ -28,8 +26,8 @@ def quantize(x: torch.Tensor, fmt: str):
     m, k = x.shape
     v = x.double().numpy().reshape(m, k // 32, 32)
     with np.errstate(invalid='ignore'):
-        amax = np.where(np.isnan(v).any(-1), np.nan, np.abs(v).max(-1))
-    scales = np.array([[scale_byte(float(a), fmt) for a in row] for row in amax], dtype=np.int64).reshape(m, k // 32)
+        amax = np.abs(v).max(-1)   # (NaN where a value is)
+    scales = scale_bytes_of(amax, fmt)
     nan = (scales == 255)[..., None]
     a = np.where(nan, 0.0, np.abs(v)) / np.exp2((np.where(scales == 255, 127, scales) - 127).astype(np.float64))[..., None]
     hi = np.searchsorted(table, a).clip(max=len(table) - 1)          # first table value >= a

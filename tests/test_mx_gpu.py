@@ -155,3 +155,84 @@ def test_quantize_under_a_cu_cap_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(back, deep_gemm.mx_dequantize(deep_gemm.mx_quantize(buf)))
+
+
+def _layout(counts, alignment):
+    """psum and extent of groups of these sizes, with a spare block of padding rows at the end."""
+    psum, at = [], 0
+    for c in counts:
+        psum.append(at + c)
+        at += -(-c // alignment) * alignment
+    return torch.tensor(psum, dtype=torch.int32), at + alignment
+
+
+@pytest.mark.parametrize('counts,alignment', [
+    ([1], 32), ([0, 1, 0, 0, 5], 32), ([16, 17, 0, 33, 3], 32), ([32, 64, 100, 1, 1, 1, 1], 32), ([0, 0, 0], 64), ([2] * 40, 32), ([40, 1, 1], 128),
+])
+@pytest.mark.parametrize('n,k', [(32, 32), (100, 96), (257, 544), (512, 4096)])
+def test_experts_of_few_rows(counts, alignment, n, k):
+    """M-grouped products of e2m1 rows, few to a group: each group's rows with its weights, zeros in padding rows, whatever
+    the padding rows of A and its scales hold."""
+    g, groups = gen(n + k + len(counts)), len(counts)
+    psum, m = _layout(counts, alignment)
+    x, w = torch.randn(m, k, generator=g).bfloat16(), torch.randn(groups, n, k, generator=g) * k ** -0.5
+    codes, sf = deep_gemm.mx_quantize(x.cuda(), 'e2m1')
+    starts = [0] + [-(-int(p) // alignment) * alignment for p in psum[:-1]]
+    live = torch.zeros(m, dtype=torch.bool)
+    for s, p in zip(starts, psum.tolist()):
+        live[s:p] = True
+    dead = (~live).cuda()
+    codes[dead] = -1
+    held = torch.full((sf.size(1), m + m % 2), -1, dtype=torch.int16, device='cuda')[:, :m].transpose(0, 1)
+    held.copy_(sf)
+    held[dead] = -1                       # (scale bytes 255: NaN)
+    q = deep_gemm.mx_quantize(w.cuda(), 'e2m1')
+    a = ox.values(*ox.quantize(x, 'e2m1'), 'e2m1')
+    ref, mag = torch.zeros(m, n, dtype=torch.float64), torch.zeros(m, n, dtype=torch.float64)
+    for e, (s, p) in enumerate(zip(starts, psum.tolist())):
+        b = ox.values(*ox.quantize(w[e], 'e2m1'), 'e2m1')
+        ref[s:p], mag[s:p] = a[s:p] @ b.t(), a[s:p].abs() @ b.abs().t()
+    deep_gemm.set_mk_alignment_for_contiguous_layout(alignment)
+    try:
+        for dtype in (torch.bfloat16, torch.float32):
+            d = torch.full((m, n), float('nan'), dtype=dtype, device='cuda')
+            deep_gemm.m_grouped_fp8_fp4_gemm_nt_contiguous((codes, held), q, d, psum.cuda())
+            bound = k * U32 * mag
+            if dtype == torch.bfloat16:
+                bound = bound * (1 + UBF16) + UBF16 * ref.abs()
+            assert ((d.cpu().double() - ref).abs() <= bound).all()
+            wide = torch.full((m, n + 3), 7.0, dtype=dtype, device='cuda')
+            deep_gemm.m_grouped_fp8_fp4_gemm_nt_contiguous((codes, held), q, wide[:, 1:n + 1], psum.cuda())
+            assert torch.equal(wide[:, 1:n + 1], d) and (wide[:, 0] == 7).all() and (wide[:, n + 1:] == 7).all()
+    finally:
+        deep_gemm.set_mk_alignment_for_contiguous_layout(256)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('m,n,k', [(1, 1, 32), (1, 64, 8192), (2, 33, 160), (15, 500, 1056), (16, 2112, 7168), (16, 16, 64)])
+def test_few_rows_quantised_inside(dtype, m, n, k):
+    """The product that quantises its rows itself against the quantiser followed by the GEMM's oracle."""
+    x, w = torch.randn(m, k, generator=gen(m)).to(dtype), torch.randn(n, k, generator=gen(n)) * k ** -0.5
+    x[0, :32] = 0
+    if k > 64:
+        x[m - 1, 40:50] *= 1e-6
+    q = deep_gemm.mx_quantize(w.cuda(), 'e2m1')
+    a, b = ox.values(*ox.quantize(x, 'e2m1'), 'e2m1'), ox.values(*ox.quantize(w, 'e2m1'), 'e2m1')
+    ref, mag = a @ b.t(), a.abs() @ b.abs().t()
+    wide = torch.full((m, k + 8), float('nan'), dtype=dtype, device='cuda')
+    wide[:, 4:k + 4] = x.cuda()
+    for inp in (x.cuda(), wide[:, 4:k + 4]):
+        d = torch.full((m, n), float('nan'), device='cuda')
+        deep_gemm.mx_gemm_nt(inp, q, d)
+        assert ((d.cpu().double() - ref).abs() <= k * U32 * mag).all()
+        deep_gemm.mx_gemm_nt(inp, q, d, c=d)
+        assert ((d.cpu().double() - 2 * ref).abs() <= 2 * (k + 1) * U32 * mag).all()
+
+
+def test_few_rows_matches_the_general_path(monkeypatch):
+    x, w = torch.randn(5, 256, generator=gen(7)).bfloat16().cuda(), deep_gemm.mx_quantize(torch.randn(96, 256, generator=gen(8)).cuda())
+    fast, general = (torch.empty(5, 96, dtype=torch.bfloat16, device='cuda') for _ in range(2))
+    deep_gemm.mx_gemm_nt(x, w, fast)
+    monkeypatch.setattr('deep_gemm.mx._operators', lambda t: None)
+    deep_gemm.mx_gemm_nt(x, w, general)
+    assert (fast.float() - general.float()).abs().max() <= 2 * UBF16 * general.float().abs().max()

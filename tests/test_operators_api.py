@@ -85,6 +85,39 @@ def test_mx_refusals(lib):
     assert lib.dg_mx_quantize(None, None) == -1
 
 
+def test_mx_gemm_refusals(lib):
+    def run(m=4, n=64, k=64, x=4096, xt=0, xld=64, w=4096, wld=32, sf=4096, sfld=64, d=4096, dt=0, ldd=64):
+        return lib.dg_mx_gemm(x, xt, xld, w, wld, sf, sfld, d, dt, ldd, m, n, k, 0, 0, None)
+    _refused(lib, run(k=-1), 'negative size')
+    _refused(lib, run(xt=2), 'x is bf16')
+    _refused(lib, run(dt=2), 'D is bf16')
+    assert run(m=17) == _lib.DG_ENOKERNEL and b'16 rows' in lib.dg_last_error()
+    _refused(lib, run(k=48), 'block of 32')
+    _refused(lib, run(k=0), 'block of 32')
+    _refused(lib, run(w=None), 'null tensor')
+    _refused(lib, run(wld=16), 'leading dimension')
+    _refused(lib, run(xld=63), 'leading dimension')
+    _refused(lib, run(ldd=32), 'leading dimension')
+    _refused(lib, run(xld=65), '4-byte aligned')
+    _refused(lib, run(sfld=65), 'even')
+    _refused(lib, run(wld=1 << 28), 'stride too large')
+    assert run(m=0) == 0 and run(n=0) == 0
+
+
+def test_few_rows_to_an_expert_plan(lib):
+    """M-grouped psum layouts of e2m1 rows, 64 or fewer to a group on average, take their own kernel; others do not."""
+    info = _lib.LaunchInfo()
+    def plan(m, kind=_lib.DG_KIND_FP4_FP4, gemm_type=_lib.DG_GEMM_MGROUPED_PSUM):
+        a = _lib.GemmArgs()
+        a.kind, a.gemm_type, a.m, a.n, a.k, a.num_groups, a.alignment, a.alpha = kind, gemm_type, m, 2048, 4096, 32, 32, 1.0
+        a.lda = a.ldb = 2048 if kind == _lib.DG_KIND_FP4_FP4 else 4096
+        a.ldd, a.batch_stride_b, a.sfa_ld, a.sfb_ld, a.num_cus = 2048, 2048 * a.ldb, m, 2048, 256
+        assert lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)) == 0, lib.dg_last_error()
+        return info.skinny
+    assert plan(1248) == 4 and plan(2048) == 4
+    assert plan(2080) != 4 and plan(1248, _lib.DG_KIND_FP8_FP8) != 4 and plan(1248, gemm_type=_lib.DG_GEMM_MGROUPED_IDX) != 4
+
+
 def test_python_refusals():
     with pytest.raises(RuntimeError, match='int32 or int64'):
         deep_gemm.moe_sort(torch.zeros(2, 2), 4)
