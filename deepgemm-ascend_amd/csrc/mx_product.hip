@@ -7,8 +7,8 @@
 // a range of K, a few steps of 128 ahead in registers; the waves of a workgroup that share rows join their sums in LDS, in
 // order.  The few rows of a come the same way (from the caches).
 //
-// The rows of a are e2m1 codes (an M-grouped layout: each expert's rows with its weights), or bf16 / fp32 values that each wave
-// quantises as it loads them: the 32 values of a block are one lane's, so its scale needs no other lane.
+// The rows of a are e2m1 codes (an M-grouped layout: each expert's rows with its weights), or a few rows of bf16 / fp32 values
+// that every workgroup quantises into LDS, a block of 32 a thread, while its first weights are on their way.
 #include "gemm_kernel.hpp"
 #include "op_launch.hpp"
 #include "mx_scale.hpp"
@@ -33,23 +33,61 @@ struct MxProductParams {
 
 enum Rows : int { kCodes = 0, kBf16Rows = 1, kF32Rows = 2 };
 
-// The 32 values of a block as e2m1 codes and their exponent byte (mx_quant.hip's).
-__device__ __forceinline__ void quantise_block(const float (&v)[32], i32x4& codes, int& scale) {
-    uint32_t top = 0;
+// Quantised rows in LDS: codes [row][kPad + K / 2], then exponent bytes [row][K / 32].  (The pad sets the rows that a read of 16
+// rows x 16 bytes touches 16 bytes apart.)
+constexpr int kPad = 16;
+__host__ __device__ __forceinline__ int row_pitch(int k) { return k / 2 + kPad; }
+__host__ __device__ __forceinline__ int rows_lds(int m, int k) { return align_up(m * (row_pitch(k) + k / 32), 16); }
+// Values quantised inside, at most (17.6 KB of LDS).  Every workgroup quantises all of them; beyond, the quantiser's own launch
+// costs less (with the quantiser's launch in brackets, us: 1x7168x4096 7.3 (9.5), 4x7168x4096 8.3 (9.6), 4x2112x7168 9.4
+// (10.6), 8x2112x7168 10.5 (10.7), 16x7168x4096 10.4 (10.0), 4x7168x16384 21.6 (21.1)).
+constexpr int kInside = 32768;
+
+template <typename E, int THREADS>
+__device__ __forceinline__ void quantise_rows(const MxProductParams& p, uint8_t* lds) {
+    typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+    typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+    const int blocks = p.k / 32;
+    for (int b = threadIdx.x; b < p.m * blocks; b += THREADS) {
+        const int row = b / blocks, block = b - row * blocks;
+        const uint8_t* const x = p.a + row * p.lda + block * 32 * (int)sizeof(E);
+        float v[32];
+        uint32_t top = 0;
+        if constexpr (sizeof(E) == 2) {
+            i32x4 w[4];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
-    const uint32_t s = scale_byte<true>(top);
-    const float f = __builtin_bit_cast(float, s << 23);
+            for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const i32x4_any*>(x)[i];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t c = 0;
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j], v[8 * j + 1], f, 0);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 2], v[8 * j + 3], f, 1);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 4], v[8 * j + 5], f, 2);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 6], v[8 * j + 7], f, 3);
-        codes[j] = s == 255u ? 0 : (int)c;
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t u = (uint32_t)w[i / 4][i % 4];
+                v[2 * i] = __builtin_bit_cast(float, u << 16);
+                v[2 * i + 1] = __builtin_bit_cast(float, u & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const f32x4 w = reinterpret_cast<const f32x4_any*>(x)[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * i + e] = w[e];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+        const uint32_t s = scale_byte<true>(top);
+        const float f = __builtin_bit_cast(float, s << 23);
+        i32x4 codes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t c = 0;
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j], v[8 * j + 1], f, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 2], v[8 * j + 3], f, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 4], v[8 * j + 5], f, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 6], v[8 * j + 7], f, 3);
+            codes[j] = s == 255u ? 0 : (int)c;
+        }
+        *reinterpret_cast<i32x4*>(lds + row * row_pitch(p.k) + block * 16) = codes;
+        lds[p.m * row_pitch(p.k) + row * blocks + block] = (uint8_t)s;
     }
-    scale = (int)s;
 }
 
 // x >> sh, kept where it stands (with the two wait states that an MFMA wants after a write of its operand: the compiler does
@@ -66,21 +104,20 @@ constexpr int kStrip = 16 * kNB;
 // MT: 16-row blocks of a in flight together; DEPTH: steps of 128 values of K ahead.
 template <int ROWS, int MT, int DEPTH, int KS>
 __device__ __forceinline__ void product_rows(const MxProductParams& p, const uint8_t* a, const uint16_t* sfa, const uint8_t* w,
-                                             const uint16_t* sfw, uint8_t* d, int rows, int n0, float* red) {
-    constexpr int EA = ROWS == kCodes ? 0 : ROWS == kBf16Rows ? 2 : 4;       // bytes of a value of a
-    constexpr int A_REGS = ROWS == kCodes ? 1 : ROWS == kBf16Rows ? 4 : 8;   // 16-byte loads of a block of 32
+                                             const uint16_t* sfw, uint8_t* d, int rows, int n0, float* red, uint8_t* lds) {
+    constexpr bool kLoaded = ROWS == kCodes;                                 // (else in LDS)
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);       // of K (KS waves share the strip)
     const int blocks = p.k / 32, steps = ceil_div(blocks, 4), per = ceil_div(steps, KS);
     const int s0 = part * per, s1 = min(steps, s0 + per);
     const int cols = min(kStrip, p.n - n0);
     const __amdgpu_buffer_rsrc_t rs_w = make_rsrc(w, (int64_t)cols * p.ldw);
-    const __amdgpu_buffer_rsrc_t rs_a = make_rsrc(a, (int64_t)rows * p.lda);
+    const __amdgpu_buffer_rsrc_t rs_a = make_rsrc(a, kLoaded ? (int64_t)rows * p.lda : 0);
     const int k64 = ceil_div(p.k, 64);
     // Scales: a lane loads the dword of its row pair (leading dimensions are even) and shifts its byte down where it is used.
     // (Of a byte load the compiler clears the upper bytes, all at the head of the loop, behind a wait for every load in flight.)
     const __amdgpu_buffer_rsrc_t rs_sw = make_rsrc(sfw, ((int64_t)(k64 - 1) * p.sfw_ld + align_up(cols, 2)) * 2);
-    const __amdgpu_buffer_rsrc_t rs_sa = make_rsrc(sfa, ROWS == kCodes ? ((int64_t)(k64 - 1) * p.sfa_ld + align_up(rows, 2)) * 2 : 0);
+    const __amdgpu_buffer_rsrc_t rs_sa = make_rsrc(sfa, kLoaded ? ((int64_t)(k64 - 1) * p.sfa_ld + align_up(rows, 2)) * 2 : 0);
     const int shift = 8 * ((r & 1) * 2 + (g & 1));
     uint32_t vw[kNB], vsw[kNB], va[MT], vsa[MT];    // (rows past the end: out of range, zeros)
 #pragma unroll
@@ -92,10 +129,10 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const bool on = 16 * i + r < rows;
-        va[i] = on ? (uint32_t)((16 * i + r) * p.lda + (ROWS == kCodes ? 16 : 32 * EA) * g) : kOOBOffset;
+        va[i] = on ? (uint32_t)((16 * i + r) * p.lda + 16 * g) : kOOBOffset;
         vsa[i] = on ? (uint32_t)(((g >> 1) * p.sfa_ld + 16 * i + (r & ~1)) * 2) : kOOBOffset;
     }
-    i32x4 fw[DEPTH][kNB], fa[DEPTH][MT][A_REGS];
+    i32x4 fw[DEPTH][kNB], fa[DEPTH][MT];
     int sw[DEPTH][kNB], sa[DEPTH][MT];
     auto load = [&](auto slot, int s) {
         constexpr int S = decltype(slot)::value;
@@ -106,14 +143,13 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
             fw[S][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_w, on ? vw[j] : kOOBOffset, step_w, 0));
             sw[S][j] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sw, on ? vsw[j] : kOOBOffset, step_sw, 0);
         }
-        const int step_a = __builtin_amdgcn_readfirstlane(ROWS == kCodes ? s * 64 : s * 128 * EA);
-        const int step_sa = __builtin_amdgcn_readfirstlane((int)(s * 4 * p.sfa_ld));
+        if constexpr (kLoaded) {
+            const int step_sa = __builtin_amdgcn_readfirstlane((int)(s * 4 * p.sfa_ld));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-#pragma unroll
-            for (int x = 0; x < A_REGS; ++x)
-                fa[S][i][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_a, on ? va[i] + 16 * x : kOOBOffset, step_a, 0));
-            if constexpr (ROWS == kCodes) sa[S][i] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sa, on ? vsa[i] : kOOBOffset, step_sa, 0);
+            for (int i = 0; i < MT; ++i) {
+                fa[S][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_a, on ? va[i] : kOOBOffset, step_w, 0));
+                sa[S][i] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sa, on ? vsa[i] : kOOBOffset, step_sa, 0);
+            }
         }
     };
     f32x4 acc[kNB][MT];
@@ -121,33 +157,21 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
     for (int j = 0; j < kNB; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](auto slot) {
+    auto multiply = [&](auto slot, int s) {
         constexpr int S = decltype(slot)::value;
         int scale_w[kNB];
 #pragma unroll
         for (int j = 0; j < kNB; ++j) scale_w[j] = shifted(sw[S][j], shift);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            i32x4 c;
-            int scale;
-            if constexpr (ROWS == kCodes) {
-                c = fa[S][i][0];
+            i32x4 c = {0, 0, 0, 0};
+            int scale = 0;
+            if constexpr (kLoaded) {
+                c = fa[S][i];
                 scale = shifted(sa[S][i], shift);
-            } else {
-                float v[32];
-#pragma unroll
-                for (int x = 0; x < A_REGS; ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t b = (uint32_t)fa[S][i][x][e];
-                        if constexpr (ROWS == kBf16Rows) {
-                            v[8 * x + 2 * e] = __builtin_bit_cast(float, b << 16);
-                            v[8 * x + 2 * e + 1] = __builtin_bit_cast(float, b & 0xffff0000u);
-                        } else {
-                            v[4 * x + e] = __builtin_bit_cast(float, b);
-                        }
-                    }
-                quantise_block(v, c, scale);
+            } else if (r < rows && 4 * s + g < blocks) {
+                c = *reinterpret_cast<const i32x4*>(lds + r * row_pitch(p.k) + s * 64 + g * 16);
+                scale = lds[rows * row_pitch(p.k) + r * blocks + 4 * s + g];
             }
             const i32x8 fa8 = {c[0], c[1], c[2], c[3], 0, 0, 0, 0};
 #pragma unroll
@@ -162,9 +186,14 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
         load(s, s0 + decltype(s)::value);
         __builtin_amdgcn_sched_barrier(0);
     });
+    if constexpr (!kLoaded) {
+        if constexpr (ROWS == kBf16Rows) quantise_rows<uint16_t, 64 * KS>(p, lds);
+        else quantise_rows<float, 64 * KS>(p, lds);
+        __syncthreads();
+    }
     for (int s = s0; s < s1; s += DEPTH) {
         static_for<DEPTH>([&](auto x) {
-            multiply(x);   // (a step past the range holds zeros and adds nothing)
+            multiply(x, s + decltype(x)::value);   // (a step past the range holds zero weights and adds nothing)
             __builtin_amdgcn_sched_barrier(0);
             load(x, s + DEPTH + decltype(x)::value);
             __builtin_amdgcn_sched_barrier(0);
@@ -226,8 +255,9 @@ __global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductPara
     const int e = t / p.strips, n0 = (t - e * p.strips) * kStrip, cols = min(kStrip, p.n - n0);
     const uint8_t* const w = p.w + (int64_t)e * p.w_bs + (int64_t)n0 * p.ldw;
     const uint16_t* const sfw = p.sfw + (int64_t)e * p.sfw_bs + n0;
+    extern __shared__ __attribute__((aligned(16))) uint8_t rows_in_lds[];
     if constexpr (ROWS != kCodes) {
-        product_rows<ROWS, 1, ROWS == kBf16Rows ? 4 : 2, KS>(p, p.a, nullptr, w, sfw, p.d, p.m, n0, red);
+        product_rows<ROWS, 1, KS == 8 ? 8 : 4, KS>(p, nullptr, nullptr, w, sfw, p.d, p.m, n0, red, rows_in_lds);
     } else {
         int first = 0, rows = p.m, end = p.m;
         if (p.psum != nullptr) {
@@ -243,8 +273,8 @@ __global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductPara
             const uint8_t* const a = p.a + (int64_t)(first + m0) * p.lda;
             const uint16_t* const sfa = p.sfa + first + m0;
             uint8_t* const d = p.d + (int64_t)(first + m0) * p.ldd * esize;
-            if (rows - m0 <= 16) product_rows<ROWS, 1, 6, KS>(p, a, sfa, w, sfw, d, rows - m0, n0, red);
-            else product_rows<ROWS, 2, 4, KS>(p, a, sfa, w, sfw, d, min(32, rows - m0), n0, red);
+            if (rows - m0 <= 16) product_rows<ROWS, 1, 6, KS>(p, a, sfa, w, sfw, d, rows - m0, n0, red, nullptr);
+            else product_rows<ROWS, 2, 4, KS>(p, a, sfa, w, sfw, d, min(32, rows - m0), n0, red, nullptr);
         }
         if (p.psum != nullptr) {
             // padding rows of the group, and every groups-th row past the last group, are zeros
@@ -269,11 +299,12 @@ int launch_product(MxProductParams p, hipStream_t st, int cus) {
     const int64_t grid = (int64_t)p.strips * p.groups;
     if (grid > 0x7fffffffLL) return dg_set_error("dg_mx_gemm: too many workgroups");
     p.grid = (int)grid;
+    const unsigned lds = ROWS == kCodes ? 0 : (unsigned)rows_lds(p.m, p.k);
     switch (k_waves(grid, p.k)) {
-        case 1: return launch_op(mx_product_kernel<ROWS, 1>, grid, 64, p, st, cus);
-        case 2: return launch_op(mx_product_kernel<ROWS, 2>, grid, 128, p, st, cus);
-        case 4: return launch_op(mx_product_kernel<ROWS, 4>, grid, 256, p, st, cus);
-        default: return launch_op(mx_product_kernel<ROWS, 8>, grid, 512, p, st, cus);
+        case 1: return launch_op(mx_product_kernel<ROWS, 1>, grid, 64, p, st, cus, lds);
+        case 2: return launch_op(mx_product_kernel<ROWS, 2>, grid, 128, p, st, cus, lds);
+        case 4: return launch_op(mx_product_kernel<ROWS, 4>, grid, 256, p, st, cus, lds);
+        default: return launch_op(mx_product_kernel<ROWS, 8>, grid, 512, p, st, cus, lds);
     }
 }
 
@@ -322,8 +353,8 @@ extern "C" int dg_mx_gemm(const void* x, int32_t x_dtype, int64_t x_ld, const vo
     if (m < 0 || n < 0 || k < 0) return dg_set_error("dg_mx_gemm: negative size");
     if (x_dtype != DG_DTYPE_BF16 && x_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx_gemm: x is bf16 or fp32");
     if (d_dtype != DG_DTYPE_BF16 && d_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx_gemm: D is bf16 or fp32");
-    if (m > 16) {
-        dg_set_error("dg_mx_gemm: more than 16 rows (quantise them with dg_mx_quantize, then dg_gemm)");
+    if (m > 16 || (int64_t)m * k > kInside) {
+        dg_set_error("dg_mx_gemm: more than 16 rows or 32768 values (quantise them with dg_mx_quantize, then dg_gemm)");
         return DG_ENOKERNEL;
     }
     if (k % 32 != 0 || k == 0) return dg_set_error("dg_mx_gemm: K must be a multiple of the block of 32 values");

@@ -29,12 +29,12 @@ inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<u
 // Workgroups [0, grid) of a kernel whose parameters hold the first one of a launch (vbase).  `cus` > 0 (set_num_sms
 // below the device's count): at most that many at a time, in launches one after another.
 template <typename P>
-int launch_op(void (*kernel)(const P), int64_t grid, unsigned threads, P p, hipStream_t st, int cus) {
+int launch_op(void (*kernel)(const P), int64_t grid, unsigned threads, P p, hipStream_t st, int cus, unsigned lds = 0) {
     if (grid > 0x7fffffffLL) return dg_set_error("too many workgroups");
     const int64_t most = cus > 0 ? cus : std::max<int64_t>(grid, 1);
     for (int64_t base = 0; base < grid; base += most) {
         p.vbase = (int)base;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(most, grid - base)), dim3(threads), 0, st, p);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(most, grid - base)), dim3(threads), lds, st, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
             dg_set_error(hipGetErrorString(e));

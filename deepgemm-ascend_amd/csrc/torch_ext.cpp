@@ -438,7 +438,7 @@ Tensors mx_dequantize(const at::Tensor& codes, const at::Tensor& sf, bool f32, i
     return out;
 }
 
-// D (+)= quantised(x) w^T: rows of e2m1 codes in one launch up to 16 of them, otherwise quantised first.  false: the general path.
+// D (+)= quantised(x) w^T: a few rows to e2m1 in one launch, otherwise quantised first.  false: the general path.
 // cus: what the GEMMs take (set_num_sms, 0 = all); num_cus: the cap, 0 = none.
 bool mx_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sfw, const at::Tensor& d, const c10::optional<at::Tensor>& c,
              bool fp4, int64_t cus, int64_t num_cus, int64_t alignment, int64_t stream) {
@@ -447,7 +447,7 @@ bool mx_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sfw, co
         sfw.device() != x.device() || d.device() != x.device())
         return false;
     const int64_t m = x.size(0), k = x.size(1), n = w.size(0), k64 = ceil_div(k, 64);
-    if (m > 16 || !fp4) {
+    if (m > 16 || m * k > 32768 || !fp4) {   // (what dg_mx_gemm takes)
         const Tensors q = mx_quantize(x, fp4, num_cus, stream);
         return !q.empty() && gemm(kNormal, q[0], q[1], w, sfw, d, c, c10::nullopt, 1, 32, 1, 32, cus, alignment, stream);
     }

@@ -353,8 +353,8 @@ int dg_mx_quantize(const dg_mx_args *args, void *stream);
 int dg_mx_dequantize(const dg_mx_args *args, void *stream);
 
 /* D[m][n] (+)= x w^T with the rows of x (bf16 or fp32) quantised to e2m1 on the way, as dg_mx_quantize does it, and e2m1 weights
- * [n][k] with required-layout scale factors; D bf16 or fp32.  One launch for at most 16 rows (DG_ENOKERNEL above: quantise, then
- * dg_gemm).  x_ld and ldd in elements, w_ld in bytes; rows of x and w 4-byte aligned. */
+ * [n][k] with required-layout scale factors; D bf16 or fp32.  One launch for at most 16 rows of together at most 32768 values
+ * (DG_ENOKERNEL above: quantise, then dg_gemm).  x_ld and ldd in elements, w_ld in bytes; rows of x and w 4-byte aligned. */
 int dg_mx_gemm(const void *x, int32_t x_dtype, int64_t x_ld, const void *w, int64_t w_ld, const int16_t *sfw, int64_t sfw_ld,
                void *d, int32_t d_dtype, int64_t ldd, int32_t m, int32_t n, int32_t k, int32_t accumulate, int32_t num_cus,
                void *stream);

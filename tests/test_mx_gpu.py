@@ -209,7 +209,8 @@ def test_experts_of_few_rows(counts, alignment, n, k):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize('m,n,k', [(1, 1, 32), (1, 64, 8192), (2, 33, 160), (15, 500, 1056), (16, 2112, 7168), (16, 16, 64)])
+@pytest.mark.parametrize('m,n,k', [(1, 1, 32), (1, 64, 8192), (2, 33, 160), (15, 500, 1056), (16, 2112, 2048), (16, 2112, 7168), (16, 16, 64),
+                                   (1, 10000, 512), (1, 129, 32768)])
 def test_few_rows_quantised_inside(dtype, m, n, k):
     """The product that quantises its rows itself against the quantiser followed by the GEMM's oracle."""
     x, w = torch.randn(m, k, generator=gen(m)).to(dtype), torch.randn(n, k, generator=gen(n)) * k ** -0.5

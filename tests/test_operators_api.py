@@ -92,6 +92,7 @@ def test_mx_gemm_refusals(lib):
     _refused(lib, run(xt=2), 'x is bf16')
     _refused(lib, run(dt=2), 'D is bf16')
     assert run(m=17) == _lib.DG_ENOKERNEL and b'16 rows' in lib.dg_last_error()
+    assert run(m=16, k=2080, xld=2080, wld=1040) == _lib.DG_ENOKERNEL and b'32768' in lib.dg_last_error()
     _refused(lib, run(k=48), 'block of 32')
     _refused(lib, run(k=0), 'block of 32')
     _refused(lib, run(w=None), 'null tensor')
