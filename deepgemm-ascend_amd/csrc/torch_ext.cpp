@@ -248,7 +248,7 @@ bool gemm(int64_t gemm_type, const at::Tensor& a, const c10::optional<at::Tensor
 }
 
 // ------------------------------------------------------------------------------------------------ operators around the GEMMs
-// The same calls as deep_gemm/moe.py and mx.py make; an empty result sends the call to their general path, which converts what
+// The same calls as deep_gemm/moe.py, mx.py and loss.py make; an empty result sends the call to their general path, which converts what
 // these checks do not take or raises.
 decltype(&dg_moe_sort) g_moe_sort = nullptr;
 decltype(&dg_moe_sort_workspace_size) g_moe_sort_workspace_size = nullptr;
@@ -258,9 +258,13 @@ decltype(&dg_moe_combine_backward) g_moe_combine_backward = nullptr;
 decltype(&dg_mx_quantize) g_mx_quantize = nullptr;
 decltype(&dg_mx_dequantize) g_mx_dequantize = nullptr;
 decltype(&dg_mx_gemm) g_mx_gemm = nullptr;
+decltype(&dg_linear_xent_workspace_size) g_xent_workspace_size = nullptr;
+decltype(&dg_linear_xent_forward) g_xent_forward = nullptr;
+decltype(&dg_linear_xent_backward) g_xent_backward = nullptr;
 
 void init_operators(int64_t sort, int64_t sort_workspace, int64_t dispatch, int64_t combine, int64_t combine_backward,
-                    int64_t quantize, int64_t dequantize, int64_t mx_gemm) {
+                    int64_t quantize, int64_t dequantize, int64_t mx_gemm, int64_t xent_workspace, int64_t xent_forward,
+                    int64_t xent_backward) {
     g_moe_sort = reinterpret_cast<decltype(g_moe_sort)>(sort);
     g_moe_sort_workspace_size = reinterpret_cast<decltype(g_moe_sort_workspace_size)>(sort_workspace);
     g_moe_dispatch = reinterpret_cast<decltype(g_moe_dispatch)>(dispatch);
@@ -269,6 +273,9 @@ void init_operators(int64_t sort, int64_t sort_workspace, int64_t dispatch, int6
     g_mx_quantize = reinterpret_cast<decltype(g_mx_quantize)>(quantize);
     g_mx_dequantize = reinterpret_cast<decltype(g_mx_dequantize)>(dequantize);
     g_mx_gemm = reinterpret_cast<decltype(g_mx_gemm)>(mx_gemm);
+    g_xent_workspace_size = reinterpret_cast<decltype(g_xent_workspace_size)>(xent_workspace);
+    g_xent_forward = reinterpret_cast<decltype(g_xent_forward)>(xent_forward);
+    g_xent_backward = reinterpret_cast<decltype(g_xent_backward)>(xent_backward);
 }
 
 using Tensors = std::vector<at::Tensor>;
@@ -332,12 +339,12 @@ Tensors moe_dispatch(const at::Tensor& x, const c10::optional<at::Tensor>& sf, c
     }
     raise_pending();
     Tensors out = {at::empty({a.rows, x.size(1)}, x.options())};
-    if (sf.has_value()) out.push_back(at::empty({k64, out_ld}, sf->options()));
+    if (sf.has_value()) out.push_back(at::empty({k64 * out_ld}, sf->options()));
     check_rc(g_moe_dispatch(x.data_ptr(), x.stride(0) * e, x.size(1) * e, &a, out[0].data_ptr(), x.size(1) * e,
                             sf.has_value() ? static_cast<const int16_t*>(sf->data_ptr()) : nullptr, sf_ld, (int32_t)k64,
                             sf.has_value() ? static_cast<int16_t*>(out[1].data_ptr()) : nullptr, out_ld, zero_padding, (int32_t)num_cus,
                             stream_ptr(stream)));
-    if (sf.has_value()) out[1] = out[1].slice(1, 0, a.rows).transpose(0, 1);
+    if (sf.has_value()) out[1] = out[1].as_strided({a.rows, k64}, {1, out_ld});
     return out;
 }
 
@@ -391,7 +398,7 @@ Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stre
     raise_pending();
     const int64_t m = x.size(0), k = x.size(1), ld = align_up(m, 2), k64 = ceil_div(k, 64);
     Tensors out = {at::empty({m, fp4 ? k / 2 : k}, x.options().dtype(fp4 ? at::kChar : at::kFloat8_e4m3fn)),
-                   at::empty({k64, ld}, x.options().dtype(at::kShort))};
+                   at::empty({k64 * ld}, x.options().dtype(at::kShort))};
     dg_mx_args a = {};
     a.format = fp4 ? DG_MX_E2M1 : DG_MX_E4M3;
     a.x_dtype = rows_dtype(x);
@@ -406,7 +413,7 @@ Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stre
     a.sf_ld = ld;
     a.num_cus = (int32_t)num_cus;
     check_rc(g_mx_quantize(&a, stream_ptr(stream)));
-    out[1] = out[1].slice(1, 0, m).transpose(0, 1);
+    out[1] = out[1].as_strided({m, k64}, {1, ld});
     return out;
 }
 
@@ -470,6 +477,73 @@ bool mx_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sfw, co
     return true;
 }
 
+bool xent_rows(const at::Tensor& t, const at::Device& device) {
+    return t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.is_cuda() && t.device() == device && t.stride(1) == 1 &&
+           t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+}
+
+bool xent_vector(const at::Tensor& t, int64_t tokens, const at::Device& device) {
+    return t.dim() == 1 && t.size(0) == tokens && t.is_contiguous() && t.device() == device;
+}
+
+// Arguments of a cross entropy of x [T, H], w [V, H] and their targets; false: the general path.
+bool xent_args(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore, int64_t num_cus, dg_linear_xent_args& a) {
+    if (g_xent_forward == nullptr || !xent_rows(x, x.device()) || !xent_rows(w, x.device()) || x.size(1) != w.size(1) || x.size(1) == 0 ||
+        x.size(1) % 8 != 0 || x.size(0) == 0 || x.size(0) > (1 << 20) || w.size(0) == 0 || w.size(0) >= (int64_t(1) << 31) - 256 ||
+        !xent_vector(target, x.size(0), x.device()) || !(target.scalar_type() == at::kInt || target.scalar_type() == at::kLong))
+        return false;
+    a = {};
+    a.tokens = (int32_t)x.size(0);
+    a.width = (int32_t)x.size(1);
+    a.vocab = (int32_t)w.size(0);
+    a.x = x.data_ptr();
+    a.w = w.data_ptr();
+    a.x_ld = x.stride(0);
+    a.w_ld = w.stride(0);
+    a.target = target.data_ptr();
+    a.target_bytes = (int32_t)target.element_size();
+    a.ignore_index = ignore;
+    a.num_cus = (int32_t)num_cus;
+    return true;
+}
+
+void xent_run(decltype(g_xent_forward) fn, dg_linear_xent_args& a, int32_t backward, const at::Tensor& x, int64_t stream) {
+    int64_t need = 0;
+    check_rc(g_xent_workspace_size(&a, backward, &need));
+    const at::Tensor ws = at::empty({need}, x.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = need;
+    check_rc(fn(&a, stream_ptr(stream)));
+}
+
+Tensors linear_xent(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore, int64_t num_cus, int64_t stream) {
+    dg_linear_xent_args a;
+    if (!xent_args(x, w, target, ignore, num_cus, a)) return {};
+    raise_pending();
+    Tensors out = {at::empty({x.size(0)}, x.options().dtype(at::kFloat)), at::empty({x.size(0)}, x.options().dtype(at::kFloat))};
+    a.loss = out[0].data_ptr<float>();
+    a.lse = out[1].data_ptr<float>();
+    xent_run(g_xent_forward, a, 0, x, stream);
+    return out;
+}
+
+Tensors linear_xent_backward(const at::Tensor& d_loss, const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
+                             const at::Tensor& lse, int64_t ignore, int64_t num_cus, int64_t stream) {
+    dg_linear_xent_args a;
+    if (!xent_args(x, w, target, ignore, num_cus, a) || d_loss.scalar_type() != at::kFloat || lse.scalar_type() != at::kFloat ||
+        !xent_vector(d_loss, x.size(0), x.device()) || !xent_vector(lse, x.size(0), x.device()))
+        return {};
+    raise_pending();
+    Tensors out = {at::empty(x.sizes(), x.options()), at::empty(w.sizes(), w.options())};
+    a.lse = lse.data_ptr<float>();
+    a.d_loss = d_loss.data_ptr<float>();
+    a.d_x = out[0].data_ptr();
+    a.d_w = out[1].data_ptr();
+    a.d_x_ld = a.d_w_ld = a.width;
+    xent_run(g_xent_backward, a, 1, x, stream);
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -483,5 +557,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("mx_quantize", &mx_quantize, "codes and scale factors of a matrix");
     m.def("mx_dequantize", &mx_dequantize, "values of codes and scale factors");
     m.def("mx_gemm", &mx_gemm, "product of rows quantised on the way; false: the general path must handle the call");
+    m.def("linear_xent", &linear_xent, "loss and log sums of a linear cross entropy");
+    m.def("linear_xent_backward", &linear_xent_backward, "gradients of x and the weight");
     m.def("gemm", &gemm, "validate and launch one GEMM; false: the general path must handle the call");
 }

@@ -258,7 +258,8 @@ def ext():
                      lib.dg_error_words() or 0)
             mod.init_operators(*(addr(getattr(lib, f)) for f in (
                 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine', 'dg_moe_combine_backward',
-                'dg_mx_quantize', 'dg_mx_dequantize', 'dg_mx_gemm')))
+                'dg_mx_quantize', 'dg_mx_dequantize', 'dg_mx_gemm', 'dg_linear_xent_workspace_size', 'dg_linear_xent_forward',
+                'dg_linear_xent_backward')))
         _ext = mod
         _ext_tried = True
         return _ext

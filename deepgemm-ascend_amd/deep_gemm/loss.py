@@ -12,7 +12,7 @@ from typing import Tuple
 import torch
 
 from . import _lib
-from .gemm import _stream
+from .gemm import _operators, _stream
 from .layout import _assert
 from .runtime import cu_cap, get_dry_run
 
@@ -62,6 +62,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     A token whose target is ``ignore_index`` has loss 0; a target outside the vocabulary counts as ignored and is reported
     (``check_errors``)."""
+    ext = _operators(x)
+    if ext is not None:
+        made = ext.linear_xent(x, weight, target, ignore_index, cu_cap(), _stream(x))
+        if made:
+            return made[0], made[1]
     keep, a = _args(x, weight, target, ignore_index)
     loss, lse = (torch.empty(x.size(0), dtype=torch.float32, device=x.device) for _ in range(2))
     if x.size(0) == 0 or get_dry_run():
@@ -75,6 +80,11 @@ def linear_cross_entropy_backward(d_loss: torch.Tensor, x: torch.Tensor, weight:
                                   lse: torch.Tensor, ignore_index: int = -100) -> Tuple[torch.Tensor, torch.Tensor]:
     """Gradients (d_x [T, H], d_weight [V, H]) in bf16 of the losses weighted by ``d_loss`` [T] fp32 (1 / T for a mean over T
     tokens), with ``lse`` as ``linear_cross_entropy`` gave it."""
+    ext = _operators(x)
+    if ext is not None:
+        made = ext.linear_xent_backward(d_loss, x, weight, target, lse, ignore_index, cu_cap(), _stream(x))
+        if made:
+            return made[0], made[1]
     keep, a = _args(x, weight, target, ignore_index)
     for name, t in (('d_loss', d_loss), ('lse', lse)):
         _assert(t.dtype == torch.float32 and t.shape == x.shape[:1] and t.device == x.device, f'{name} must be a [T] fp32 tensor')

@@ -130,6 +130,26 @@ def test_strided_rows_and_what_lies_beside_them():
     _check(x, w, target, d_loss, (x.t().contiguous().t().cuda(), held[1], target.cuda(), d_loss.cuda()))
 
 
+def test_python_path_matches_the_extension(monkeypatch):
+    x, w, target, d_loss = (a.cuda() for a in _inputs(70, 64, 400))
+    def both():
+        loss, lse = deep_gemm.linear_cross_entropy(x, w, target)
+        return loss, lse, *deep_gemm.linear_cross_entropy_backward(d_loss, x, w, target, lse)
+    fast = both()
+    monkeypatch.setattr('deep_gemm.loss._operators', lambda t: None)
+    for a, b in zip(both(), fast):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_no_tokens():
+    w = torch.ones(30, 64, dtype=torch.bfloat16, device='cuda')
+    x, target, d_loss = w[:0], torch.zeros(0, dtype=torch.int64, device='cuda'), torch.zeros(0, device='cuda')
+    loss, lse = deep_gemm.linear_cross_entropy(x, w, target)
+    assert loss.shape == lse.shape == (0,)
+    d_x, d_w = deep_gemm.linear_cross_entropy_backward(d_loss, x, w, target, lse)
+    assert d_x.shape == (0, 64) and (d_w == 0).all() and d_w.shape == w.shape
+
+
 def test_pieces_of_the_vocabulary():
     """More words than one piece holds: d_x is summed over the pieces (against fp32 products on this device)."""
     t, h, v = 8200, 128, 70001

@@ -119,6 +119,36 @@ def test_few_rows_to_an_expert_plan(lib):
     assert plan(2080) != 4 and plan(1248, _lib.DG_KIND_FP8_FP8) != 4 and plan(1248, gemm_type=_lib.DG_GEMM_MGROUPED_IDX) != 4
 
 
+def test_linear_xent_refusals(lib):
+    def run(fn='dg_linear_xent_forward', **kw):
+        a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 40, 0)
+        for name, v in kw.items():
+            setattr(a, name, v)
+        return getattr(lib, fn)(a, None)
+    for fn in ('dg_linear_xent_forward', 'dg_linear_xent_backward'):
+        _refused(lib, run(fn, tokens=-1), 'invalid size')
+        _refused(lib, run(fn, vocab=0), 'invalid size')
+        _refused(lib, run(fn, tokens=(1 << 20) + 1), '2^20 tokens')
+        _refused(lib, run(fn, width=60), 'multiple of 8')
+        _refused(lib, run(fn, target_bytes=2), 'int32 or int64')
+        _refused(lib, run(fn, x_ld=32), '16-byte aligned')
+        _refused(lib, run(fn, w=4100), '16-byte aligned')
+        _refused(lib, run(fn, w_ld=1 << 22), 'stride too large')
+        _refused(lib, run(fn, x=None), 'null tensor')
+        _refused(lib, run(fn, lse=None), 'null tensor')
+        _refused(lib, run(fn, workspace=None), 'workspace')
+        _refused(lib, run(fn, workspace_bytes=16), 'workspace')
+    _refused(lib, run('dg_linear_xent_backward', d_w_ld=32), 'gradients')
+    _refused(lib, run('dg_linear_xent_backward', d_loss=None), 'null tensor')
+    _refused(lib, run('dg_linear_xent_backward', tokens=0), 'no tokens')
+    assert run(tokens=0) == 0
+    need = ctypes.c_int64()
+    a = _lib.LinearXentArgs(8192, 4096, 131072, 4096, 4096, 4096, 4096, 4096, 8)
+    assert lib.dg_linear_xent_workspace_size(a, 1, ctypes.byref(need)) == 0
+    assert 0 < need.value < 8192 * 131072 * 2          # (a piece of the vocabulary, not all of it)
+    assert lib.dg_linear_xent_workspace_size(a, 0, ctypes.byref(need)) == 0 and need.value < 8192 * 131072 // 8
+
+
 def test_python_refusals():
     with pytest.raises(RuntimeError, match='int32 or int64'):
         deep_gemm.moe_sort(torch.zeros(2, 2), 4)
@@ -130,6 +160,9 @@ def test_python_refusals():
         deep_gemm.mx_quantize(torch.zeros(2, 64), 'e5m2')
     with pytest.raises(RuntimeError, match='e2m1 weights'):
         deep_gemm.mx_gemm_nt(torch.zeros(2, 64), (torch.zeros(4, 64, dtype=torch.float8_e4m3fn), None), torch.zeros(2, 4))
+    x, w, t = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(9, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match='device tensors'):
+        deep_gemm.linear_cross_entropy(x, w, t)
     layout = deep_gemm.MoELayout(*(torch.zeros(s, dtype=torch.int32) for s in ((2, 2), (64,), (4,), (64,))))
     with pytest.raises(RuntimeError, match='device tensor'):
         deep_gemm.moe_dispatch(torch.zeros(2, 64), layout)
