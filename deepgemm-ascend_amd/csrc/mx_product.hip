@@ -4,7 +4,7 @@
 // Bound by the bytes of w, which is read once, straight into registers: a lane of v_mfma_scale_f32_16x16x128_f8f6f4 holds the
 // 16 bytes of one block of 32 codes of one row, so a wave's load is 16 rows x 64 bytes as they lie in memory, no two lanes
 // need the same bytes, and neither LDS nor a barrier stands between memory and the matrix unit.  A wave owns 32 rows of w and
-// a range of K, a few steps of 128 ahead in registers; the waves of a workgroup that share rows join their sums in LDS, in
+// a range of K, two to eight steps of 128 ahead in registers; the waves of a workgroup that share rows join their sums in LDS, in
 // order.  The few rows of a come the same way (from the caches).
 //
 // The rows of a are e2m1 codes (an M-grouped layout: each expert's rows with its weights), or a few rows of bf16 / fp32 values
@@ -21,13 +21,13 @@ struct MxProductParams {
     const uint8_t* w;          // codes [groups][n][ldw]
     uint8_t* d;
     const uint16_t *sfa, *sfw; // [k64][ld]; sfa: codes only
-    const int* psum;           // M-grouped layout, or nullptr: one group of m rows
+    const int* psum;           // M-grouped layout (codes); values are one group of m rows
     int m, n, k, groups, alignment;
     int64_t lda, ldw, ldd;     // bytes, bytes, elements
     int64_t w_bs, sfw_bs;      // bytes, int16 elements
     int64_t sfa_ld, sfw_ld;
     int f32, accumulate;       // of D
-    int strips, grid;
+    int strips;
     int vbase;
 };
 
@@ -90,14 +90,6 @@ __device__ __forceinline__ void quantise_rows(const MxProductParams& p, uint8_t*
     }
 }
 
-// x >> sh, kept where it stands (with the two wait states that an MFMA wants after a write of its operand: the compiler does
-// not see into the asm).
-__device__ __forceinline__ int shifted(int x, int sh) {
-    int y;
-    asm volatile("v_lshrrev_b32 %0, %1, %2\n\ts_nop 1" : "=v"(y) : "v"(sh), "v"(x));
-    return y;
-}
-
 constexpr int kNB = 2;         // 16-row blocks of w of a wave
 constexpr int kStrip = 16 * kNB;
 
@@ -114,43 +106,60 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
     const __amdgpu_buffer_rsrc_t rs_w = make_rsrc(w, (int64_t)cols * p.ldw);
     const __amdgpu_buffer_rsrc_t rs_a = make_rsrc(a, kLoaded ? (int64_t)rows * p.lda : 0);
     const int k64 = ceil_div(p.k, 64);
-    // Scales: a lane loads the dword of its row pair (leading dimensions are even) and shifts its byte down where it is used.
-    // (Of a byte load the compiler clears the upper bytes, all at the head of the loop, behind a wait for every load in flight.)
+    // Scales: one load holds the dwords (a row pair's exponents of 64 K) of all the wave's rows for several steps, lane l the pair
+    // l % P of the (l / P)-th 64 K, and every lane fetches its own from there.  (With a load for each 16 rows and step, 32 x 8
+    // pairs over 32 experts, N = 2048 K = 4096, took 40 us in place of 37; without scales 33, without rows of a too 28.)
+    constexpr int kPairsW = kStrip / 2, kStepsW = 64 / kPairsW / 2, kPairsA = 8 * MT, kStepsA = 64 / kPairsA / 2;
+    static_assert(DEPTH % kStepsW == 0 && DEPTH % kStepsA == 0, "steps in flight");
     const __amdgpu_buffer_rsrc_t rs_sw = make_rsrc(sfw, ((int64_t)(k64 - 1) * p.sfw_ld + align_up(cols, 2)) * 2);
     const __amdgpu_buffer_rsrc_t rs_sa = make_rsrc(sfa, kLoaded ? ((int64_t)(k64 - 1) * p.sfa_ld + align_up(rows, 2)) * 2 : 0);
     const int shift = 8 * ((r & 1) * 2 + (g & 1));
-    uint32_t vw[kNB], vsw[kNB], va[MT], vsa[MT];    // (rows past the end: out of range, zeros)
+    const uint32_t vsw = lane % kPairsW * 2 < cols ? (uint32_t)((lane / kPairsW * p.sfw_ld + lane % kPairsW * 2) * 2) : kOOBOffset;
+    const uint32_t vsa = lane % kPairsA * 2 < rows ? (uint32_t)((lane / kPairsA * p.sfa_ld + lane % kPairsA * 2) * 2) : kOOBOffset;
+    uint32_t vw[kNB], va[MT];                       // (rows past the end: out of range, zeros)
 #pragma unroll
     for (int j = 0; j < kNB; ++j) {
         const bool on = 16 * j + r < cols;
         vw[j] = on ? (uint32_t)((16 * j + r) * p.ldw + 16 * g) : kOOBOffset;
-        vsw[j] = on ? (uint32_t)(((g >> 1) * p.sfw_ld + 16 * j + (r & ~1)) * 2) : kOOBOffset;
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const bool on = 16 * i + r < rows;
         va[i] = on ? (uint32_t)((16 * i + r) * p.lda + 16 * g) : kOOBOffset;
-        vsa[i] = on ? (uint32_t)(((g >> 1) * p.sfa_ld + 16 * i + (r & ~1)) * 2) : kOOBOffset;
     }
     i32x4 fw[DEPTH][kNB], fa[DEPTH][MT];
-    int sw[DEPTH][kNB], sa[DEPTH][MT];
+    int sw[DEPTH / kStepsW], sa[DEPTH / kStepsA];
     auto load = [&](auto slot, int s) {
         constexpr int S = decltype(slot)::value;
         const bool on = s < s1 && 4 * s + g < blocks;   // (past K: zeros)
-        const int step_w = __builtin_amdgcn_readfirstlane(s * 64), step_sw = __builtin_amdgcn_readfirstlane((int)(s * 4 * p.sfw_ld));
+        const int step_w = __builtin_amdgcn_readfirstlane(s * 64);
 #pragma unroll
-        for (int j = 0; j < kNB; ++j) {
+        for (int j = 0; j < kNB; ++j)
             fw[S][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_w, on ? vw[j] : kOOBOffset, step_w, 0));
-            sw[S][j] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sw, on ? vsw[j] : kOOBOffset, step_sw, 0);
-        }
         if constexpr (kLoaded) {
-            const int step_sa = __builtin_amdgcn_readfirstlane((int)(s * 4 * p.sfa_ld));
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
+            for (int i = 0; i < MT; ++i)
                 fa[S][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_a, on ? va[i] : kOOBOffset, step_w, 0));
-                sa[S][i] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sa, on ? vsa[i] : kOOBOffset, step_sa, 0);
-            }
         }
+    };
+    // the scales that slot S is the last to need (s: its next step), or, at the start, those that it is the first to need
+    auto load_scales = [&](auto slot, int s, auto start) {
+        constexpr int S = decltype(slot)::value;
+        constexpr bool kStart = decltype(start)::value != 0;
+        if constexpr ((S + (kStart ? 0 : 1)) % kStepsW == 0) {
+            const int first = s - (kStart ? 0 : kStepsW - 1);
+            sw[S / kStepsW] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sw, vsw, __builtin_amdgcn_readfirstlane((int)(first * 4 * p.sfw_ld)), 0);
+        }
+        if constexpr (kLoaded && (S + (kStart ? 0 : 1)) % kStepsA == 0) {
+            const int first = s - (kStart ? 0 : kStepsA - 1);
+            sa[S / kStepsA] = (int)__builtin_amdgcn_raw_buffer_load_b32(rs_sa, vsa, __builtin_amdgcn_readfirstlane((int)(first * 4 * p.sfa_ld)), 0);
+        }
+    };
+    // Exponent byte of block g of row 16 `blk` + r in the step-th step of a load (0 past K, where the codes are zeros too)
+    auto scale_of = [&](int held, int pairs, int step, int blk, bool on) -> int {
+        const int from = (2 * step + (g >> 1)) * pairs + 8 * blk + (r >> 1);
+        const int v = __builtin_amdgcn_ds_bpermute(from * 4, held);
+        return on ? (v >> shift) & 255 : 0;
     };
     f32x4 acc[kNB][MT];
 #pragma unroll
@@ -159,17 +168,18 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](auto slot, int s) {
         constexpr int S = decltype(slot)::value;
+        const bool on = 4 * s + g < blocks;
         int scale_w[kNB];
 #pragma unroll
-        for (int j = 0; j < kNB; ++j) scale_w[j] = shifted(sw[S][j], shift);
+        for (int j = 0; j < kNB; ++j) scale_w[j] = scale_of(sw[S / kStepsW], kPairsW, S % kStepsW, j, on);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             i32x4 c = {0, 0, 0, 0};
             int scale = 0;
             if constexpr (kLoaded) {
                 c = fa[S][i];
-                scale = shifted(sa[S][i], shift);
-            } else if (r < rows && 4 * s + g < blocks) {
+                scale = scale_of(sa[S / kStepsA], kPairsA, S % kStepsA, i, on);
+            } else if (r < rows && on) {
                 c = *reinterpret_cast<const i32x4*>(lds + r * row_pitch(p.k) + s * 64 + g * 16);
                 scale = lds[rows * row_pitch(p.k) + r * blocks + 4 * s + g];
             }
@@ -183,6 +193,7 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
         }
     };
     static_for<DEPTH>([&](auto s) {
+        load_scales(s, s0 + decltype(s)::value, Int<1>{});
         load(s, s0 + decltype(s)::value);
         __builtin_amdgcn_sched_barrier(0);
     });
@@ -196,6 +207,7 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
             multiply(x, s + decltype(x)::value);   // (a step past the range holds zero weights and adds nothing)
             __builtin_amdgcn_sched_barrier(0);
             load(x, s + DEPTH + decltype(x)::value);
+            load_scales(x, s + DEPTH + decltype(x)::value, Int<0>{});
             __builtin_amdgcn_sched_barrier(0);
         });
     }
@@ -239,57 +251,65 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
     }
 }
 
-// Zeros in columns [n0, n0 + cols) of row `row`, by the lanes of a wave.
-__device__ __forceinline__ void clear_row(const MxProductParams& p, int64_t row, int n0, int cols, int lane) {
-    for (int c = lane; c < cols; c += 64) {
-        if (p.f32) reinterpret_cast<float*>(p.d)[row * p.ldd + n0 + c] = 0.f;
-        else reinterpret_cast<uint16_t*>(p.d)[row * p.ldd + n0 + c] = 0;
+// Zeros in columns [n0, n0 + cols) of rows first, first + step, ... below end, by a workgroup: four columns a thread.
+template <int THREADS, int COLS>
+__device__ __forceinline__ void clear_rows(const MxProductParams& p, int64_t first, int64_t end, int step, int n0, int cols) {
+    constexpr int PER = COLS / 4;
+    const int c = threadIdx.x % PER * 4, live = min(4, cols - c);
+    for (int64_t row = first + (int64_t)(threadIdx.x / PER) * step; row < end; row += (int64_t)(THREADS / PER) * step) {
+        const int64_t at = row * p.ldd + n0 + c;
+        if (p.f32) {
+            float* const d = reinterpret_cast<float*>(p.d) + at;
+            if (live == 4 && (reinterpret_cast<uintptr_t>(d) & 15) == 0) *reinterpret_cast<f32x4*>(d) = f32x4{0.f, 0.f, 0.f, 0.f};
+            else for (int x = 0; x < live; ++x) d[x] = 0.f;
+        } else {
+            uint16_t* const d = reinterpret_cast<uint16_t*>(p.d) + at;
+            if (live == 4 && (reinterpret_cast<uintptr_t>(d) & 7) == 0) *reinterpret_cast<i32x2*>(d) = i32x2{0, 0};
+            else for (int x = 0; x < live; ++x) d[x] = 0;
+        }
     }
 }
 
 template <int ROWS, int KS>
 __global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductParams p) {
-    __shared__ __attribute__((aligned(16))) float red[KS > 1 ? KS * kNB * 2 * 256 : 4];
-    // (neighbouring strips, whose scale factors share lines, on one XCD)
-    const int t = xcd_remap(blockIdx.x + p.vbase, p.grid);
-    const int e = t / p.strips, n0 = (t - e * p.strips) * kStrip, cols = min(kStrip, p.n - n0);
+    __shared__ __attribute__((aligned(16))) float red[KS > 1 ? KS * kNB * (ROWS == kCodes ? 4 : 1) * 256 : 4];
+    // (strips dealt over the XCDs one by one: an expert without rows, or with many, is then spread over all of them; with an
+    // expert's strips on one XCD 16 x 8 pairs over 64 experts took 49 us in place of 41.  Four strips to a workgroup, whose
+    // waves would share their rows of a in the CU's cache, were no faster, and 128 x 8 pairs over 32 77 us in place of 64.)
+    const int t = blockIdx.x + p.vbase;
+    const int e = t / p.strips, n0 = (t - e * p.strips) * kStrip;
     const uint8_t* const w = p.w + (int64_t)e * p.w_bs + (int64_t)n0 * p.ldw;
     const uint16_t* const sfw = p.sfw + (int64_t)e * p.sfw_bs + n0;
     extern __shared__ __attribute__((aligned(16))) uint8_t rows_in_lds[];
     if constexpr (ROWS != kCodes) {
         product_rows<ROWS, 1, KS == 8 ? 8 : 4, KS>(p, nullptr, nullptr, w, sfw, p.d, p.m, n0, red, rows_in_lds);
     } else {
-        int first = 0, rows = p.m, end = p.m;
-        if (p.psum != nullptr) {
-            first = e == 0 ? 0 : max(0, align_up(p.psum[e - 1], p.alignment));
-            rows = min(p.m, p.psum[e]) - first;
-            end = min(p.m, align_up(p.psum[e], p.alignment));
-            first = __builtin_amdgcn_readfirstlane(first);
-            rows = __builtin_amdgcn_readfirstlane(rows);
-        }
+        const int first = __builtin_amdgcn_readfirstlane(e == 0 ? 0 : max(0, align_up(p.psum[e - 1], p.alignment)));
+        const int rows = __builtin_amdgcn_readfirstlane(min(p.m, p.psum[e]) - first), end = min(p.m, align_up(p.psum[e], p.alignment));
         const int esize = p.f32 ? 4 : 2;
-        // (an expert with more rows than fit reads its weights again, from the caches)
-        for (int m0 = 0; m0 < rows; m0 += 32) {
+        // (an expert with more than 64 rows reads its weights again, from the caches; with 64 in two passes, 128 x 8 pairs over 32
+        // experts took 64 us in place of 56)
+        for (int m0 = 0; m0 < rows; m0 += 64) {
             const uint8_t* const a = p.a + (int64_t)(first + m0) * p.lda;
             const uint16_t* const sfa = p.sfa + first + m0;
             uint8_t* const d = p.d + (int64_t)(first + m0) * p.ldd * esize;
-            if (rows - m0 <= 16) product_rows<ROWS, 1, 6, KS>(p, a, sfa, w, sfw, d, rows - m0, n0, red, nullptr);
-            else product_rows<ROWS, 2, 4, KS>(p, a, sfa, w, sfw, d, min(32, rows - m0), n0, red, nullptr);
+            const int live = min(64, rows - m0);
+            if (live <= 16) product_rows<ROWS, 1, 8, KS>(p, a, sfa, w, sfw, d, live, n0, red, nullptr);
+            else if (live <= 32) product_rows<ROWS, 2, 4, KS>(p, a, sfa, w, sfw, d, live, n0, red, nullptr);
+            else product_rows<ROWS, 4, 2, KS>(p, a, sfa, w, sfw, d, live, n0, red, nullptr);
         }
-        if (p.psum != nullptr) {
-            // padding rows of the group, and every groups-th row past the last group, are zeros
-            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-            for (int m = first + max(rows, 0) + wave; m < end; m += KS) clear_row(p, m, n0, cols, lane);
-            for (int64_t m = (int64_t)align_up(p.psum[p.groups - 1], p.alignment) + e + (int64_t)wave * p.groups; m < p.m; m += (int64_t)KS * p.groups)
-                clear_row(p, m, n0, cols, lane);
-        }
+        // padding rows of the group, and every groups-th row past the last group, are zeros
+        const int cols = min(kStrip, p.n - n0);
+        clear_rows<64 * KS, kStrip>(p, first + max(rows, 0), end, 1, n0, cols);
+        clear_rows<64 * KS, kStrip>(p, (int64_t)max(0, align_up(p.psum[p.groups - 1], p.alignment)) + e, p.m, p.groups, n0, cols);
     }
 }
 
-// Waves that share a strip: as many as give the card about eight waves a CU, while each keeps two steps.
-int k_waves(int64_t strips, int k) {
+// Waves that share a strip: as many as give the card about eight waves a CU, while each keeps four steps.  (Codes: at most four,
+// eight would share a SIMD's registers by twos and spill.)
+int k_waves(int64_t strips, int k, bool codes) {
     int ks = 1;
-    while (ks < 8 && strips * ks < 2048 && ceil_div(k, 128) >= 4 * ks) ks *= 2;
+    while (ks < (codes ? 4 : 8) && strips * ks < 2048 && ceil_div(k, 128) >= 4 * ks) ks *= 2;
     return ks;
 }
 
@@ -298,14 +318,13 @@ int launch_product(MxProductParams p, hipStream_t st, int cus) {
     p.strips = ceil_div(p.n, kStrip);
     const int64_t grid = (int64_t)p.strips * p.groups;
     if (grid > 0x7fffffffLL) return dg_set_error("dg_mx_gemm: too many workgroups");
-    p.grid = (int)grid;
     const unsigned lds = ROWS == kCodes ? 0 : (unsigned)rows_lds(p.m, p.k);
-    switch (k_waves(grid, p.k)) {
-        case 1: return launch_op(mx_product_kernel<ROWS, 1>, grid, 64, p, st, cus, lds);
-        case 2: return launch_op(mx_product_kernel<ROWS, 2>, grid, 128, p, st, cus, lds);
-        case 4: return launch_op(mx_product_kernel<ROWS, 4>, grid, 256, p, st, cus, lds);
-        default: return launch_op(mx_product_kernel<ROWS, 8>, grid, 512, p, st, cus, lds);
-    }
+    const int ks = k_waves(grid, p.k, ROWS == kCodes);
+    if (ks == 1) return launch_op(mx_product_kernel<ROWS, 1>, grid, 64, p, st, cus, lds);
+    if (ks == 2) return launch_op(mx_product_kernel<ROWS, 2>, grid, 128, p, st, cus, lds);
+    if constexpr (ROWS != kCodes)
+        if (ks == 8) return launch_op(mx_product_kernel<ROWS, 8>, grid, 512, p, st, cus, lds);
+    return launch_op(mx_product_kernel<ROWS, 4>, grid, 256, p, st, cus, lds);
 }
 
 bool span32(int64_t rows, int64_t ld_bytes) { return rows * ld_bytes < 0x40000000LL; }
@@ -316,7 +335,7 @@ bool span32(int64_t rows, int64_t ld_bytes) { return rows * ld_bytes < 0x4000000
 bool mx_experts_fit(const dg_gemm_args& a) {
     return a.gemm_type == kMGroupedPsum && a.kind == kFP4FP4 && a.k > 0 && a.k % 32 == 0 && a.m <= 64 * a.num_groups &&
            (a.d_dtype == DG_DTYPE_BF16 || a.d_dtype == DG_DTYPE_F32) && a.epilogue == DG_EPI_DEFAULT && !a.accumulate &&
-           a.bias == nullptr && a.alpha == 1.0f && a.block_m == 0 && a.block_n == 0 && a.split_k <= 1 && !a.jit && span32(32, a.lda) &&
+           a.bias == nullptr && a.alpha == 1.0f && a.block_m == 0 && a.block_n == 0 && a.split_k <= 1 && !a.jit && span32(64, a.lda) &&
            span32(kStrip, a.ldb) && span32(ceil_div(a.k, 64), a.sfa_ld * 2) && span32(ceil_div(a.k, 64), a.sfb_ld * 2);
 }
 
@@ -332,11 +351,11 @@ int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* i
     p.f32 = a.d_dtype == DG_DTYPE_F32;
     if (info != nullptr) {
         const int64_t grid = (int64_t)ceil_div(a.n, kStrip) * a.num_groups;
-        info->block_m = 32;
+        info->block_m = 64;
         info->block_n = kStrip;
         info->plan_workgroups = info->tiles = grid;
         info->grid = cus > 0 ? std::min<int64_t>(grid, cus) : grid;
-        info->threads = 64 * k_waves(grid, a.k);
+        info->threads = 64 * k_waves(grid, a.k, true);
         info->split_k = 1;
         info->skinny = 4;
         return DG_OK;
