@@ -290,6 +290,11 @@ bool int32_rows(const at::Tensor& t, int64_t dim, const at::Device& device) {
     return t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == device && t.numel() < (int64_t(1) << 31);
 }
 
+// Rows of contiguous values that do not overlap (an expanded row goes to the general path).
+bool plain(const at::Tensor& t) {
+    return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+
 // The layout of a MoELayout's four tensors beside rows on `device`.
 bool layout_of(const Tensors& l, const at::Device& device, dg_moe_layout& out) {
     if (l.size() != 4 || !int32_rows(l[0], 2, device) || !int32_rows(l[1], 1, device) || !int32_rows(l[2], 1, device) ||
@@ -326,7 +331,7 @@ Tensors moe_dispatch(const at::Tensor& x, const c10::optional<at::Tensor>& sf, c
     dg_moe_layout a;
     const int64_t e = x.element_size();
     if (g_moe_dispatch == nullptr || x.dim() != 2 || !x.is_cuda() || !(e == 1 || e == 2 || e == 4) || !layout_of(layout, x.device(), a) ||
-        x.size(0) != a.tokens || !(x.stride(1) == 1 || x.size(1) <= 1))
+        x.size(0) != a.tokens || !plain(x))
         return {};
     int64_t k64 = 0, sf_ld = 0;
     const int64_t out_ld = align_up(a.rows, 2);
@@ -353,7 +358,7 @@ int rows_dtype(const at::Tensor& t) {
 }
 
 bool plain_rows(const at::Tensor& t, int64_t rows) {
-    return t.dim() == 2 && t.is_cuda() && rows_dtype(t) >= 0 && t.size(0) == rows && (t.stride(1) == 1 || t.size(1) <= 1);
+    return t.dim() == 2 && t.is_cuda() && rows_dtype(t) >= 0 && t.size(0) == rows && plain(t);
 }
 
 bool plain_weights(const at::Tensor& w, const dg_moe_layout& a, const at::Device& device) {
@@ -393,7 +398,7 @@ Tensors moe_combine_backward(const at::Tensor& d_out, const at::Tensor& rows, co
 // A two-dimensional x [M, K] to codes and scale factors.
 Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stream) {
     if (g_mx_quantize == nullptr || x.dim() != 2 || !x.is_cuda() || rows_dtype(x) < 0 || x.size(1) % 32 != 0 || x.numel() == 0 ||
-        x.stride(1) != 1 || x.size(0) >= (int64_t(1) << 31) || x.size(1) >= (int64_t(1) << 31))
+        !plain(x) || x.size(0) >= (int64_t(1) << 31) || x.size(1) >= (int64_t(1) << 31))
         return {};
     raise_pending();
     const int64_t m = x.size(0), k = x.size(1), ld = align_up(m, 2), k64 = ceil_div(k, 64);
@@ -420,7 +425,7 @@ Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stre
 Tensors mx_dequantize(const at::Tensor& codes, const at::Tensor& sf, bool f32, int64_t num_cus, int64_t stream) {
     const bool fp4 = codes.scalar_type() == at::kChar;
     if (g_mx_dequantize == nullptr || codes.dim() != 2 || !codes.is_cuda() || !(fp4 || codes.scalar_type() == at::kFloat8_e4m3fn) ||
-        codes.numel() == 0 || codes.stride(1) != 1)
+        codes.numel() == 0 || !plain(codes) || codes.stride(0) % 8 || (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 7))
         return {};
     const int64_t m = codes.size(0), k = codes.size(1) * (fp4 ? 2 : 1), k64 = ceil_div(k, 64);
     if (k % 32 != 0 || m >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || sf.scalar_type() != at::kShort || sf.dim() != 2 ||

@@ -108,8 +108,7 @@ def moe_dispatch(x, layout: MoELayout, zero_padding: bool = True):
     _assert(x.element_size() in (1, 2, 4), 'x must have elements of 1, 2 or 4 bytes')
     t, _, m = _check_layout(layout, x.device)
     _assert(x.size(0) == t, f'x has {x.size(0)} rows, the layout {t} tokens')
-    if x.size(1) > 1 and x.stride(1) != 1:
-        x = x.contiguous()
+    x = _plain(x)
     h, esize = x.size(1), x.element_size()
     out = torch.empty((m, h), dtype=x.dtype, device=x.device)
     sf_out, k64, sf_ld, out_ld = None, 0, 0, _align(m, 2)
@@ -132,11 +131,16 @@ def moe_dispatch(x, layout: MoELayout, zero_padding: bool = True):
 _DTYPES = {torch.bfloat16: _lib.DG_DTYPE_BF16, torch.float32: _lib.DG_DTYPE_F32}
 
 
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    """t with rows of contiguous values that do not overlap (an expanded row is written out)."""
+    return t if (t.size(1) <= 1 or t.stride(1) == 1) and (t.size(0) <= 1 or t.stride(0) >= t.size(1)) else t.contiguous()
+
+
 def _check_rows(name: str, t: torch.Tensor, size: int, what: str) -> torch.Tensor:
     _assert(t.dim() == 2 and t.is_cuda, f'{name} must be a 2D device tensor')
     _assert(t.dtype in _DTYPES, f'{name} must be bf16 or fp32')
     _assert(t.size(0) == size, f'{name} has {t.size(0)} rows, the layout {size} {what}')
-    return t if t.size(1) <= 1 or t.stride(1) == 1 else t.contiguous()
+    return _plain(t)
 
 
 def _check_weights(weights: torch.Tensor, layout: MoELayout) -> torch.Tensor:

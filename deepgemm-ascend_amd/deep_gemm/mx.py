@@ -54,7 +54,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = 'e2m1') -> Tuple[torch.Tensor, torch
     m, k = x.size(-2), x.size(-1)
     _assert(max(x.shape) < 2 ** 31, 'every extent must be below 2^31')
     _assert(k % 32 == 0, f'K must be a multiple of the block of 32 values, got {k}')
-    if x.stride(-1) != 1 and k > 1:
+    if k > 1 and (x.stride(-1) != 1 or (m > 1 and x.stride(-2) < k)):   # (an expanded row is written out)
         x = x.contiguous()
     lead = x.shape[:-2]
     codes = torch.empty((*lead, m, k // 2), dtype=torch.int8, device=x.device) if fmt == 'e2m1' else \
@@ -81,7 +81,9 @@ def mx_dequantize(q: Tuple[torch.Tensor, torch.Tensor], dtype: torch.dtype = tor
     _assert(k % 32 == 0, f'K must be a multiple of the block of 32 values, got {k}')
     _assert(sf.dtype == torch.int16 and sf.shape == (*codes.shape[:-1], _ceil_div(k, 64)), 'sf must be int16 [.., M, ceil(K / 64)]')
     _assert(m <= 1 or sf.stride(-2) == 1, 'sf must be in the required layout (rows contiguous)')
-    codes = codes if codes.stride(-1) == 1 or codes.size(-1) <= 1 else codes.contiguous()
+    if codes.size(-1) > 1 and (codes.stride(-1) != 1 or codes.stride(-2) % 8 or codes.data_ptr() % 8 or
+                               (m > 1 and codes.stride(-2) < codes.size(-1))):
+        codes = codes.contiguous()
     out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=codes.device)
     _run('dg_mx_dequantize', out, codes, sf, fmt)
     return out
