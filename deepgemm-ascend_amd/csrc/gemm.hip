@@ -379,7 +379,7 @@ bool skinny_kernel_plan(const dg_gemm_args& a, int cus, bool allow_split, const 
             sp = std::max(1, std::min(sp, std::min(16, nk64)));
         }
         const int ss = ceil_div(nk64, sp);
-        out = {{32 * env.rmt, 32 * env.rnb, 0, env.rmt * env.rnb, 0, 0, 0, 0, 0}, ceil_div(nk64, ss), ss,
+        out = {{32 * env.rmt, 32 * env.rnb, 0, env.rmt * env.rnb, 0, 0, 0, 0}, ceil_div(nk64, ss), ss,
                env.rmt * env.rnb, env.rd, 32 * env.rmt, 1, 0, 0};
         out.split_reduce = (out.split > 1 && env.rreduce == 1) || (out.split > 2 && env.rreduce == 2) ? 1 : 0;
         return true;
@@ -414,7 +414,7 @@ bool skinny_kernel_plan(const dg_gemm_args& a, int cus, bool allow_split, const 
         sp = std::max(1, std::min(sp, std::min(16, nk64)));
     }
     const int ss = ceil_div(nk64, sp);
-    out = {{32 * mt, 32 * nb, 0, nw, 0, 0, 0, 0, 0}, ceil_div(nk64, ss), ss, nw, d, ar};
+    out = {{32 * mt, 32 * nb, 0, nw, 0, 0, 0, 0}, ceil_div(nk64, ss), ss, nw, d, ar};
     return true;
 }
 
@@ -444,6 +444,13 @@ constexpr QuadRate kQuadBf16[] = {{256, 256, 1, 0.87, 0.0058, 9.0}, {256, 128, 1
 // MN-major operands of a 128-row tile come in half lines and fill the LDS of a whole CU (bf16 tn 4096^3: 163 us
 // against 115 on 256x256 tiles)
 constexpr QuadRate kQuadMn128 = {128, 128, 1, 0.48, 0.0022, 7.0};
+// FP4 x FP4 tiles, all on the eight-wave kernel: its matrix instructions take half the time, so a stage waits on its
+// loads whatever the tile, and few rows gain from small tiles on many CUs.  Measured (M 200 .. 2048 at N x K 4096x4096,
+// 7168x2048, 2112x7168, 4096x768, every tile, unsplit, us): 512x4096x4096 128x128 18.9, 64x128 19.6, 256x128 27.5, 256x256
+// 30.4; 2048x4096x4096 41.1, 55.7, 37.8, 34.7, 256x160 33.5; 200x2112x7168 27.0, 28.9, 42.5, 45.4.
+constexpr QuadRate kTileFp4[] = {{256, 256, 1, 0.64, 0.0051, 9.7}, {256, 224, 1, 0.72, 0.0041, 10.6}, {256, 160, 1, 0.58, 0.0036, 8.6},
+                                 {256, 128, 1, 0.625, 0.0037, 7.2}, {128, 128, 1, 0.36, 0.0018, 6.3}, {64, 128, 2, 0.40, 0.0011, 6.0},
+                                 {32, 128, 2, 0.385, 0.0008, 5.6}};
 
 // The last two bf16 tiles run the eight-wave kernel: two waves a SIMD cover more of a tile's fill and epilogue, while a
 // stage takes longer.  They win where 256x256 tiles leave CUs idle (nt 1000x9000x1024 23.8 us against 26.2, 3000x3000x512
@@ -482,22 +489,24 @@ double quad_time(const QuadRate& q, int64_t tiles, int stages, int cus) {
 
 // Best tile plan by that model.  K is split while the ranges still run at once; their fp32 partials are
 // written and read back (7 TB/s, mostly from the caches) and summed by a second launch (3.5 us).
-bool quad_plan(const dg_gemm_args& a, int cus, bool allow_split, Plan& out) {
-    if (a.kind == kFP4FP4) return false;
-    const bool bf16 = a.kind == kBF16, mn = a.a_mn_major || a.b_mn_major;
+// (The plan does not depend on D's dtype: a bf16 D is then exactly the RNE rounding of the fp32 D of the same
+// call, with the same K split and summation order.)
+Plan quad_plan(const dg_gemm_args& a, int cus, bool allow_split) {
+    const bool fp4 = a.kind == kFP4FP4, bf16 = a.kind == kBF16, mn = a.a_mn_major || a.b_mn_major;
     const int groups = (a.gemm_type == kBatched || a.gemm_type == kMasked || a.gemm_type == kKGrouped) ? a.num_groups : 1;
     const int k_tile = a.gemm_type == kKGrouped ? ceil_div(a.k, std::max(1, a.num_groups)) : a.k;
     const int ns = std::max(1, ceil_div(k_tile, bf16 ? 64 : 128));
-    const QuadRate* const rates = bf16 ? kQuadBf16 : kQuadFp8;
-    const int num = bf16 ? (int)(sizeof(kQuadBf16) / sizeof(QuadRate)) : (int)(sizeof(kQuadFp8) / sizeof(QuadRate));
+    const QuadRate* const rates = bf16 ? kQuadBf16 : fp4 ? kTileFp4 : kQuadFp8;
+    const int num = (int)((bf16 ? sizeof(kQuadBf16) : fp4 ? sizeof(kTileFp4) : sizeof(kQuadFp8)) / sizeof(QuadRate));
     const bool dense = a.gemm_type == kNormal || a.gemm_type == kBatched;
-    const bool small = dense && !mn && !cus_capped(cus) && ns <= kSmallStages, cut = a.n % (bf16 ? 32 : 16) != 0;
+    const bool small = dense && !fp4 && !mn && !cus_capped(cus) && ns <= kSmallStages, cut = a.n % (bf16 ? 32 : 16) != 0;
+    Plan out = {};
     double best = 1e300;
     for (int i = small ? -1 : 0; i < num; ++i) {
         QuadRate q = i < 0 ? kSmall[bf16 ? 2 : a.kind == kFP8FP4 ? 1 : 0] : mn && rates[i].bm == 128 ? kQuadMn128 : rates[i];
         if (!tile_allowed(a, q.bm, q.bn)) continue;
         const bool quad = quad_tile(a.kind, q.bm, q.bn);
-        if (mn && !quad && ns > kEightWaveMnStages) continue;
+        if (mn && !quad && !fp4 && ns > kEightWaveMnStages) continue;
         TileCfg tc = {};
         for (const TileCfg& c : kTiles)
             if (c.bm == q.bm && c.bn == q.bn) tc = c;
@@ -524,7 +533,7 @@ bool quad_plan(const dg_gemm_args& a, int cus, bool allow_split, Plan& out) {
             }
         }
     }
-    return best < 1e300;
+    return out;
 }
 
 Plan select_plan(const dg_gemm_args& a, int cus, bool allow_split) {
@@ -546,38 +555,7 @@ Plan select_plan(const dg_gemm_args& a, int cus, bool allow_split) {
         for (const TileCfg& tc : kTiles)
             if (tc.bm == 384 && tc.bn == (fp4_b ? 128 : 192)) return {tc, 1, ceil_div(a.k, k_stage_elems(a.kind, tc)), 0, 0, 0};
     }
-    Plan quad;
-    if (quad_plan(a, cus, allow_split, quad)) return quad;
-    // FP4 x FP4, which the four-wave kernel does not serve: waves of workgroups, unsplit (wide problems fill the CUs).
-    const int groups = (a.gemm_type == kBatched || a.gemm_type == kMasked || a.gemm_type == kKGrouped) ? a.num_groups : 1;
-    // (K-grouped: each tile contracts one group's share of K)
-    const int k_tile = a.gemm_type == kKGrouped ? ceil_div(a.k, std::max(1, a.num_groups)) : a.k;
-    // HBM floor: operands once, D once (8 TB/s at ~2.1 GHz is ~3800 bytes per cycle).
-    const double esz = a.kind == kBF16 ? 2.0 : 1.0;
-    // (The plan must not depend on D's dtype: a bf16 D is then exactly the RNE rounding of the
-    // fp32 D of the same call, with the same K split and summation order.)
-    const double hbm_bytes = esz * ((double)a.m + a.n) * a.k * groups + 2.0 * a.m * a.n * groups;
-    double best = 1e300;
-    Plan pick = {{0, 0, 0, 0, 0, 0, 0, 0, 0}, 1, 1, 0, 0, 0};
-    for (int i = 0; i < kNumTiles; ++i) {
-        const TileCfg& tc = kTiles[i];
-        // (anchored tiles only where the alignment rules out 256-row tiles, above: at alignment 256 they
-        // measured behind, 526 vs 443 us for 256x224 at G=32 N=4096 K=7168, and FP8 x FP4 G=8 x 4096
-        // rows N=7168 K=3072 took 2546 us on 384x192)
-        if (!tile_allowed(a, tc.bm, tc.bn) || tile_anchored(tc.bm)) continue;
-        const int ns = ceil_div(k_tile, k_stage_elems(a.kind, tc));
-        const int64_t rounds = ceil_div64(plan_tiles(a, tc), (int64_t)cus * tc.occ);
-        // Waves of workgroups x (their K stages at the tile's measured stage time + the
-        // fixed cost of a tile: pipeline fill and the epilogue's stores).
-        // (co-resident workgroups share the CU's MFMAs but overlap each other's fixed costs)
-        double t = (double)rounds * ((double)tc.occ * ns * tc.km * tc.stage_cycles + 6000.0 + tc.bm * tc.bn / 8.0);
-        t = std::max(t, hbm_bytes / 3800.0);
-        if (t < best * 0.97) {
-            best = t;
-            pick = {tc, 1, ns, 0, 0, 0};
-        }
-    }
-    return pick;
+    return quad_plan(a, cus, allow_split);
 }
 
 struct MemoKey {
@@ -600,7 +578,7 @@ std::unordered_map<MemoKey, Plan, MemoHash> g_memo;
 Plan choose_plan(const dg_gemm_args& a, int cus, bool allow_split) {
     allow_split = allow_split && split_capable(a);
     if (a.block_m > 0 && a.block_n > 0) {
-        TileCfg t = {a.block_m, a.block_n, 0, 0, 0, 0, 0, 0, 0};
+        TileCfg t = {a.block_m, a.block_n, 0, 0, 0, 0, 0, 0};
         for (const TileCfg& c : kTiles)
             if (c.bm == a.block_m && c.bn == a.block_n) t = c;
         const int ns = ceil_div(a.k, k_stage_elems(a.kind, t));

@@ -22,7 +22,6 @@ struct TileCfg {
     int km;       // MFMA K-steps per stage: 2 = 128-byte fp8 rows (whole-line loads), 1 = 64
     int occ;      // workgroups per CU (2: LDS ring and registers sized for two co-resident
                   // workgroups, whose prologues and epilogues then overlap each other's main loops)
-    int stage_cycles;   // measured cycles per 64 K with every CU busy (fp8, MI355X)
     int nsb = 0;        // 3: B rows get a ring of three slots beside the two of A + SF, where that fits
                         // the LDS for the kind (0: one shared ring)
 };
@@ -32,11 +31,11 @@ struct TileCfg {
 // experts, ~257 rows each, alignment 128) N=4096 K=7168: 128x256 as 8 waves / one workgroup per CU 572 us, as
 // 4 waves / two workgroups per CU 509 us; skinny M=128, N=7168, K=16384: 128x128 split 4 57 us.
 constexpr TileCfg kTiles[] = {
-    {256, 256, 4, 8, 4, 2, 2, 1, 1380, 3}, {256, 224, 4, 8, 4, 2, 2, 1, 1250, 3}, {256, 128, 4, 8, 8, 4, 1, 1, 937},
-    {128, 256, 2, 4, 4, 3, 1, 2, 985},  {128, 128, 2, 4, 4, 4, 1, 1, 1056}, {64, 128, 2, 4, 4, 6, 1, 2, 588},
-    {32, 128, 1, 4, 4, 6, 1, 2, 643},  {256, 160, 4, 8, 4, 2, 2, 1, 950, 3},
+    {256, 256, 4, 8, 4, 2, 2, 1, 3}, {256, 224, 4, 8, 4, 2, 2, 1, 3}, {256, 128, 4, 8, 8, 4, 1, 1},
+    {128, 256, 2, 4, 4, 3, 1, 2},  {128, 128, 2, 4, 4, 4, 1, 1}, {64, 128, 2, 4, 4, 6, 1, 2},
+    {32, 128, 1, 4, 4, 6, 1, 2},  {256, 160, 4, 8, 4, 2, 2, 1, 3},
     // tiles anchored at each group's first row (M-grouped psum layouts only)
-    {384, 192, 4, 8, 8, 2, 2, 1, 1250}, {384, 128, 4, 8, 4, 2, 2, 1, 1000},
+    {384, 192, 4, 8, 8, 2, 2, 1}, {384, 128, 4, 8, 4, 2, 2, 1},
 };
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 

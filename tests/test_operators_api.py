@@ -203,3 +203,13 @@ def test_oracle_quantisation_is_nearest():
         amax = x.double().abs().view(6, 2, 32).amax(-1)
         blocks = torch.exp2(scales.double() - 127)
         assert (amax <= top * blocks).all() and (amax > top * blocks / 2).all()
+
+
+@pytest.mark.parametrize('m,n,k,bm', [(200, 4096, 4096, 128), (512, 2112, 7168, 128), (4096, 7168, 2048, 256)])
+def test_fp4_products_of_few_rows_take_small_tiles(lib, m, n, k, bm):
+    """A large tile would leave most CUs idle at a few hundred rows."""
+    args = _lib.GemmArgs()
+    args.kind, args.m, args.n, args.k, args.num_groups, args.num_cus = 2, m, n, k, 1, 256
+    block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.dg_select_config(ctypes.byref(args), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
+    assert block_m.value <= bm if bm < 256 else block_m.value == bm
