@@ -305,6 +305,20 @@ bool layout_of(const Tensors& l, const at::Device& device, dg_moe_layout& out) {
     return true;
 }
 
+// A contiguous piece of `whole` from element `at` on, without the dispatcher and the allocator.
+at::Tensor piece(const at::Tensor& whole, int64_t at, at::IntArrayRef sizes) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
+
+// Scale factors [rows][k64] as they lie in a flat tensor: rows contiguous, `ld` apart.
+at::Tensor scale_view(at::Tensor flat, int64_t rows, int64_t k64, int64_t ld) {
+    flat.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef{rows, k64}, at::IntArrayRef{1, ld});
+    return flat;
+}
+
 Tensors moe_sort(const at::Tensor& ids, int64_t groups, int64_t rows, int64_t alignment, int64_t num_cus, int64_t stream) {
     if (g_moe_sort == nullptr || ids.dim() != 2 || !ids.is_cuda() || !ids.is_contiguous() || groups < 1 || groups > 1024 || rows < 0 ||
         rows % alignment != 0 || rows >= (int64_t(1) << 31) || ids.numel() >= (int64_t(1) << 31) ||
@@ -312,7 +326,11 @@ Tensors moe_sort(const at::Tensor& ids, int64_t groups, int64_t rows, int64_t al
         return {};
     raise_pending();
     const auto options = ids.options().dtype(at::kInt);
-    Tensors l = {at::empty(ids.sizes(), options), at::empty({rows}, options), at::empty({groups}, options), at::empty({rows}, options)};
+    // One allocation for the four, which live and die together (each would cost the host 0.8 us of a latency-bound call); pieces
+    // start at 128 bytes.
+    const int64_t at_source = align_up(ids.numel(), 32), at_psum = at_source + align_up(rows, 32), at_indices = at_psum + align_up(groups, 32);
+    const at::Tensor whole = at::empty({at_indices + rows}, options);
+    Tensors l = {piece(whole, 0, ids.sizes()), piece(whole, at_source, {rows}), piece(whole, at_psum, {groups}), piece(whole, at_indices, {rows})};
     dg_moe_layout a;
     if (!layout_of(l, ids.device(), a)) return {};
     a.num_groups = (int32_t)groups;
@@ -349,7 +367,7 @@ Tensors moe_dispatch(const at::Tensor& x, const c10::optional<at::Tensor>& sf, c
                             sf.has_value() ? static_cast<const int16_t*>(sf->data_ptr()) : nullptr, sf_ld, (int32_t)k64,
                             sf.has_value() ? static_cast<int16_t*>(out[1].data_ptr()) : nullptr, out_ld, zero_padding, (int32_t)num_cus,
                             stream_ptr(stream)));
-    if (sf.has_value()) out[1] = out[1].as_strided({a.rows, k64}, {1, out_ld});
+    if (sf.has_value()) out[1] = scale_view(std::move(out[1]), a.rows, k64, out_ld);
     return out;
 }
 
@@ -418,7 +436,7 @@ Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stre
     a.sf_ld = ld;
     a.num_cus = (int32_t)num_cus;
     check_rc(g_mx_quantize(&a, stream_ptr(stream)));
-    out[1] = out[1].as_strided({m, k64}, {1, ld});
+    out[1] = scale_view(std::move(out[1]), m, k64, ld);
     return out;
 }
 
