@@ -436,6 +436,7 @@ struct QuadRate {
     int bm, bn, occ;
     double light, share, fixed;
     double mn_stage = 1.0;   // a stage's factor where an operand is MN-major
+    double paired = 0.0;     // `fixed` of two tiles that share a CU, where one's fill and epilogue go under the other's stages (0: no less)
 };
 constexpr QuadRate kQuadFp8[] = {{256, 256, 1, 0.94, 0.0045, 7.5}, {256, 224, 1, 0.815, 0.0040, 8.2}, {256, 160, 1, 0.64, 0.0030, 7.5},
                                  {256, 128, 1, 0.54, 0.00245, 6.5}, {128, 128, 2, 0.353, 0.00172, 6.5}};
@@ -482,7 +483,7 @@ double quad_time(const QuadRate& q, int64_t tiles, int stages, int cus) {
     auto round = [&](int64_t running) {
         // (two tiles on a CU share its path to the L2)
         const double one = q.light * (running > cus ? 2 : 1), l = one * one, c = q.share * running * q.share * running;
-        return stages * std::sqrt(std::sqrt(l * l + c * c)) + q.fixed;
+        return stages * std::sqrt(std::sqrt(l * l + c * c)) + (running > cus && q.paired > 0 ? q.paired : q.fixed);
     };
     return full * round(slots) + (rest ? round(rest) : 0.0);
 }
@@ -1168,9 +1169,13 @@ namespace dg {
 // bf16_tile_plan below.
 int gemm_k_rows(const dg_gemm_args* args, int k_rows, void* stream) { return gemm_impl(args, stream, false, nullptr, false, k_rows); }
 
+constexpr double kPairedStats = 2.7;
+
 // The four-wave tile of a dense bf16 problem (mn: an operand is MN-major) and its K split, at most `most`, by the planner's
-// cost model; the bytes of fp32 partials a split needs.
-void bf16_tile_plan(int m, int n, int k, bool mn, int most, int cus, int& bm, int& bn, int& split, int64_t& partial_bytes) {
+// cost model; the bytes of fp32 partials a split needs.  `stats`: the tile stores no D but a pair of numbers a row (the
+// forward pass): two 128x128 tiles on a CU then cover each other's fill and tail (1000 x 50257, K = 512: 68 us against 78
+// with 256x256; 777 x 32003, K = 1536: 89 and 86; 300 x 131072, K = 2048: 228 and 216).
+void bf16_tile_plan(int m, int n, int k, bool mn, bool stats, int most, int cus, int& bm, int& bn, int& split, int64_t& partial_bytes) {
     dg_gemm_args a = {};
     a.kind = kBF16; a.gemm_type = kNormal; a.m = m; a.n = n; a.k = k; a.num_groups = 1;
     const int ns = std::max(1, ceil_div(k, 64));
@@ -1179,6 +1184,7 @@ void bf16_tile_plan(int m, int n, int k, bool mn, int most, int cus, int& bm, in
         if (!quad_tile(kBF16, q.bm, q.bn)) continue;
         if (mn && q.bm == 128) q = kQuadMn128;
         if (mn) q.fixed += kQuadMnFixedBf16;
+        if (stats && q.occ == 2) q.paired = kPairedStats;
         TileCfg tc = {};
         tc.bm = q.bm; tc.bn = q.bn;
         const int64_t tiles = plan_tiles(a, tc), slots = (int64_t)cus * q.occ;
