@@ -215,7 +215,6 @@ __device__ __forceinline__ void product_rows(const MxProductParams& p, const uin
     }
     // sums of the K ranges, in order: red[part][block][lane]
     if constexpr (KS > 1) {
-        __syncthreads();       // (an earlier chunk's sums have been read)
 #pragma unroll
         for (int j = 0; j < kNB; ++j)
 #pragma unroll
@@ -272,6 +271,45 @@ __device__ __forceinline__ void clear_rows(const MxProductParams& p, int64_t fir
     }
 }
 
+// Chunk `x` of 64 rows among those past their group's first, groups in order: its group and number (0: there is none).  A lane
+// takes four groups, so that up to 256 are read at once (most launches have no such chunk, and their workgroups only look).
+__device__ __forceinline__ int later_chunk(const MxProductParams& p, int x, int& group) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < p.groups; base += 256) {
+        const int e = base + 4 * lane;
+        int start = e > 0 && e < p.groups ? max(0, align_up(p.psum[e - 1], p.alignment)) : 0, later[4], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int end = e + j < p.groups ? p.psum[e + j] : start;
+            later[j] = max(0, ceil_div(min(p.m, end) - start, 64) - 1);
+            start = max(0, align_up(end, p.alignment));
+            sum += later[j];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int v = __shfl_up(incl, off, 64);
+            if (lane >= off) incl += v;
+        }
+        const uint64_t hit = __ballot(x < incl);
+        if (hit != 0) {
+            const int src = __builtin_ctzll(hit);
+            x -= __shfl(incl - sum, src, 64);
+            for (int j = 0; j < 4; ++j) {
+                const int n = __shfl(later[j], src, 64);
+                if (x < n) {
+                    group = base + 4 * src + j;
+                    break;
+                }
+                x -= n;
+            }
+            return x + 1;
+        }
+        x -= __shfl(incl, 63, 64);
+    }
+    return 0;
+}
+
 template <int ROWS, int KS>
 __global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductParams p) {
     __shared__ __attribute__((aligned(16))) float red[KS > 1 ? KS * kNB * (ROWS == kCodes ? 4 : 1) * 256 : 4];
@@ -279,7 +317,15 @@ __global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductPara
     // expert's strips on one XCD 16 x 8 pairs over 64 experts took 49 us in place of 41.  Four strips to a workgroup, whose
     // waves would share their rows of a in the CU's cache, were no faster, and 128 x 8 pairs over 32 77 us in place of 64.)
     const int t = blockIdx.x + p.vbase;
-    const int e = t / p.strips, n0 = (t - e * p.strips) * kStrip;
+    int e = t / p.strips, chunk = 0;
+    const int n0 = (t - e * p.strips) * kStrip;
+    if (ROWS == kCodes && e >= p.groups) {
+        // (workgroups of their own, behind the others: 256 rows of one of 32 experts, 16 of the others, N = 2048 K = 4096 50 us where a
+        // strip's one workgroup took its chunks in turn for 77; 2048 rows in one 51 and 467)
+        chunk = __builtin_amdgcn_readfirstlane(later_chunk(p, e - p.groups, e));
+        e = __builtin_amdgcn_readfirstlane(e);
+        if (chunk == 0) return;
+    }
     const uint8_t* const w = p.w + (int64_t)e * p.w_bs + (int64_t)n0 * p.ldw;
     const uint16_t* const sfw = p.sfw + (int64_t)e * p.sfw_bs + n0;
     extern __shared__ __attribute__((aligned(16))) uint8_t rows_in_lds[];
@@ -289,17 +335,18 @@ __global__ __launch_bounds__(64 * KS) void mx_product_kernel(const MxProductPara
         const int first = __builtin_amdgcn_readfirstlane(e == 0 ? 0 : max(0, align_up(p.psum[e - 1], p.alignment)));
         const int rows = __builtin_amdgcn_readfirstlane(min(p.m, p.psum[e]) - first), end = min(p.m, align_up(p.psum[e], p.alignment));
         const int esize = p.f32 ? 4 : 2;
-        // (an expert with more than 64 rows reads its weights again, from the caches; with 64 in two passes, 128 x 8 pairs over 32
+        // (every 64 rows of an expert read its weights, the later ones from the caches; with 32 at a time, 128 x 8 pairs over 32
         // experts took 64 us in place of 56)
-        for (int m0 = 0; m0 < rows; m0 += 64) {
+        const int m0 = 64 * chunk, live = min(64, rows - m0);
+        if (live > 0) {
             const uint8_t* const a = p.a + (int64_t)(first + m0) * p.lda;
             const uint16_t* const sfa = p.sfa + first + m0;
             uint8_t* const d = p.d + (int64_t)(first + m0) * p.ldd * esize;
-            const int live = min(64, rows - m0);
             if (live <= 16) product_rows<ROWS, 1, 8, KS>(p, a, sfa, w, sfw, d, live, n0, red, nullptr);
             else if (live <= 32) product_rows<ROWS, 2, 4, KS>(p, a, sfa, w, sfw, d, live, n0, red, nullptr);
             else product_rows<ROWS, 4, 2, KS>(p, a, sfa, w, sfw, d, live, n0, red, nullptr);
         }
+        if (chunk > 0) return;
         // padding rows of the group, and every groups-th row past the last group, are zeros
         const int cols = min(kStrip, p.n - n0);
         clear_rows<64 * KS, kStrip>(p, first + max(rows, 0), end, 1, n0, cols);
@@ -318,10 +365,11 @@ int k_waves(int64_t strips, int k, bool codes) {
 template <int ROWS>
 int launch_product(MxProductParams p, hipStream_t st, int cus) {
     p.strips = ceil_div(p.n, kStrip);
-    const int64_t grid = (int64_t)p.strips * p.groups;
+    // (chunks of 64 rows past a group's first: m / 64 at most)
+    const int64_t grid = (int64_t)p.strips * (p.groups + (ROWS == kCodes ? p.m / 64 : 0));
     if (grid > 0x7fffffffLL) return dg_set_error("dg_mx_gemm: too many workgroups");
     const unsigned lds = ROWS == kCodes ? 0 : (unsigned)rows_lds(p.m, p.k);
-    const int ks = k_waves(grid, p.k, ROWS == kCodes);
+    const int ks = k_waves((int64_t)p.strips * p.groups, p.k, ROWS == kCodes);
     if (ks == 1) return launch_op(mx_product_kernel<ROWS, 1>, grid, 64, p, st, cus, lds);
     if (ks == 2) return launch_op(mx_product_kernel<ROWS, 2>, grid, 128, p, st, cus, lds);
     if constexpr (ROWS != kCodes)
@@ -352,12 +400,12 @@ int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* i
     p.sfa_ld = a.sfa_ld; p.sfw_ld = a.sfb_ld;
     p.f32 = a.d_dtype == DG_DTYPE_F32;
     if (info != nullptr) {
-        const int64_t grid = (int64_t)ceil_div(a.n, kStrip) * a.num_groups;
+        const int64_t strips = ceil_div(a.n, kStrip), grid = strips * (a.num_groups + a.m / 64);
         info->block_m = 64;
         info->block_n = kStrip;
         info->plan_workgroups = info->tiles = grid;
         info->grid = cus > 0 ? std::min<int64_t>(grid, cus) : grid;
-        info->threads = 64 * k_waves(grid, a.k, true);
+        info->threads = 64 * k_waves(strips * a.num_groups, a.k, true);
         info->split_k = 1;
         info->skinny = 4;
         return DG_OK;

@@ -208,6 +208,15 @@ def test_experts_of_few_rows(counts, alignment, n, k):
         deep_gemm.set_mk_alignment_for_contiguous_layout(256)
 
 
+@pytest.mark.parametrize('counts,n,k', [
+    ([300] + [0] * 9, 70, 160), ([64, 65, 128, 129, 0, 1, 192], 100, 96), ([70] + [0] * 257 + [130, 1, 66] + [0] * 3 + [64], 33, 64),
+    ([65] * 5 + [1] * 7, 257, 2048), ([0] * 255 + [200] + [0] * 20 + [90], 32, 32),
+])
+def test_groups_of_more_rows_than_one_pass(counts, n, k):
+    """Groups of more than 64 rows among few: the later rows are work of their own, found by scanning the layout."""
+    test_experts_of_few_rows(counts, 32, n, k)
+
+
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('m,n,k', [(1, 1, 32), (1, 64, 8192), (2, 33, 160), (15, 500, 1056), (16, 2112, 2048), (16, 2112, 7168), (16, 16, 64),
                                    (1, 10000, 512), (1, 129, 32768)])
