@@ -552,6 +552,19 @@ Plan select_plan(const dg_gemm_args& a, int cus, bool allow_split) {
     // alignment 128, cold us: N=4096 K=7168 1011 vs 370 on 384x128 and 410 on the scored 128x256, N=7168
     // K=2048 532 vs 217 / 219)
     const bool fp4_b = a.kind == kFP8FP4 || a.kind == kFP4FP4;
+    // FP4 x FP4 in psum layouts of hardly more rows than one small tile a group takes that tile, 128x128 or 64x128 as the alignment
+    // allows: a group's weights then come by more workgroups at once.  Top-8 routings, rows of the layout a group in
+    // brackets, us, small tile and 384x128: 64 x 8 pairs over 32 experts, N=2048 K=4096, alignment 64 (78) 48 and 76, 128 (140) 61
+    // and 76; N=4096 K=7168 188 and 247, 230 and 250; 16 x 8 over 64, N=2048 K=512 (65, 128) 20 and 30, 24 and 32; full groups of
+    // 128, 64 of them, N=K=2048 50 and 70.  (Behind: 64 x 8 over 64, N=1024 K=2048, alignment 128 (134) 38 and 34.)  Past one and
+    // a half tiles: 256 x 8 over 32, N=4096 K=7168, alignment 64 (126) 266 and 254, 768 x 8, N=2048 K=4096, 64 (254) 104 and
+    // 86, 128 (316) 95 and 90.
+    if (a.kind == kFP4FP4 && a.gemm_type == kMGroupedPsum && a.alignment % 256 != 0 && a.alignment % 64 == 0) {
+        const int rows = a.alignment % 128 == 0 ? 128 : 64;
+        if (2 * (int64_t)a.m <= 3 * (int64_t)rows * a.num_groups)
+            for (const TileCfg& tc : kTiles)
+                if (tc.bm == rows && tc.bn == 128) return {tc, 1, ceil_div(a.k, k_stage_elems(a.kind, tc)), 0, 0, 0};
+    }
     if ((a.gemm_type == kMGroupedPsum || a.gemm_type == kMGroupedIdx) && a.alignment % 256 != 0) {
         for (const TileCfg& tc : kTiles)
             if (tc.bm == 384 && tc.bn == (fp4_b ? 128 : 192)) return {tc, 1, ceil_div(a.k, k_stage_elems(a.kind, tc)), 0, 0, 0};

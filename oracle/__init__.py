@@ -15,6 +15,9 @@ It restates, in plain CPU torch / numpy, the reference's own reference math:
 * ``gemm``    -- dequantise-to-fp32 then matmul then cast (``tests/generators.py:320-322``),
                  grouped, masked, batched, K-grouped and einsum variants, and ``calc_diff``
                  (``tests/utils.py:36-43``).
+* ``moe``, ``mx``, ``loss`` -- the operators around the GEMMs (tokens sorted by expert and moved, quantisation in
+                 blocks of 32, cross entropy of a linear layer) from their definitions in 64 bits; the
+                 reference has none of them.
 * ``epilogue`` -- stochastic bf16 rounding (``tests/utils.py:70-92``) and FP8 output
                  quantisation (``tests/test_einsum.py:70-86``).
 

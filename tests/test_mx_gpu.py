@@ -217,6 +217,15 @@ def test_groups_of_more_rows_than_one_pass(counts, n, k):
     test_experts_of_few_rows(counts, 32, n, k)
 
 
+@pytest.mark.parametrize('counts,alignment', [
+    ([1, 64, 0, 65], 64), ([0, 3, 40, 128, 1], 64), ([0] * 3 + [5], 64), ([1, 128, 0, 129, 7], 128), ([2] * 70, 128), ([100, 192, 30], 192),
+])
+@pytest.mark.parametrize('n,k', [(100, 96), (257, 544), (512, 2048)])
+def test_experts_on_small_tiles(counts, alignment, n, k):
+    """Layouts of a small tile to a group or little more."""
+    test_experts_of_few_rows(counts, alignment, n, k)
+
+
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('m,n,k', [(1, 1, 32), (1, 64, 8192), (2, 33, 160), (15, 500, 1056), (16, 2112, 2048), (16, 2112, 7168), (16, 16, 64),
                                    (1, 10000, 512), (1, 129, 32768)])
