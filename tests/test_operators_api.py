@@ -213,3 +213,13 @@ def test_fp4_products_of_few_rows_take_small_tiles(lib, m, n, k, bm):
     block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
     assert lib.dg_select_config(ctypes.byref(args), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
     assert block_m.value <= bm if bm < 256 else block_m.value == bm
+
+
+@pytest.mark.parametrize('m,alignment,tile', [(2240, 64, (64, 128)), (4224, 128, (128, 128)), (8192, 128, (384, 128)), (4096, 96, (384, 128))])
+def test_fp4_psum_layouts_of_little_more_than_a_tile_a_group(lib, m, alignment, tile):
+    args = _lib.GemmArgs()
+    args.kind, args.gemm_type, args.m, args.n, args.k, args.num_groups = 2, 2, m, 2048, 4096, 32
+    args.alignment, args.num_cus = alignment, 256
+    block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.dg_select_config(ctypes.byref(args), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
+    assert (block_m.value, block_n.value) == tile
