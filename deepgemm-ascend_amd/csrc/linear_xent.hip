@@ -413,6 +413,7 @@ Plan plan_of(const dg_linear_xent_args& a, bool backward) {
 int check(const dg_linear_xent_args* a) {
     if (a == nullptr) return dg_set_error("dg_linear_xent: null args");
     if (a->tokens < 0 || a->width < 1 || a->vocab < 1) return dg_set_error("dg_linear_xent: invalid size");
+    if (a->vocab > kMaxExtent || a->width > kMaxExtent) return dg_set_error("dg_linear_xent: at most 2^30 words and values of a row");
     if (a->tokens > kMaxTokens) return dg_set_error("dg_linear_xent: at most 2^20 tokens");
     if (a->width % 8 != 0) return dg_set_error("dg_linear_xent: the width must be a multiple of 8");
     if (a->target_bytes != 4 && a->target_bytes != 8) return dg_set_error("dg_linear_xent: targets are int32 or int64");

@@ -477,7 +477,9 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Com
 
 int layout_ok(const dg_moe_layout* l, const char* who) {
     if (l == nullptr) return dg_set_error("dg_moe: null layout");
-    if (l->tokens < 0 || l->topk < 0 || l->rows < 0 || (int64_t)l->tokens * l->topk > 0x7fffffffLL) return dg_set_error(who);
+    if (l->tokens < 0 || l->topk < 0 || l->rows < 0 || l->tokens > kMaxExtent || l->rows > kMaxExtent ||
+        (int64_t)l->tokens * l->topk > kMaxExtent)
+        return dg_set_error(who);
     return DG_OK;
 }
 

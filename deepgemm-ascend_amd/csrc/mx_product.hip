@@ -383,7 +383,7 @@ bool span32(int64_t rows, int64_t ld_bytes) { return rows * ld_bytes < 0x4000000
 
 // csrc/gemm.hip: an M-grouped psum GEMM of e2m1 rows, a few to an expert.  Whether this kernel serves it.
 bool mx_experts_fit(const dg_gemm_args& a) {
-    return a.gemm_type == kMGroupedPsum && a.kind == kFP4FP4 && a.k > 0 && a.k % 32 == 0 && a.m <= 64 * a.num_groups &&
+    return a.gemm_type == kMGroupedPsum && a.kind == kFP4FP4 && a.k > 0 && a.k % 32 == 0 && a.m <= (int64_t)64 * a.num_groups &&
            (a.d_dtype == DG_DTYPE_BF16 || a.d_dtype == DG_DTYPE_F32) && a.epilogue == DG_EPI_DEFAULT && !a.accumulate &&
            a.bias == nullptr && a.alpha == 1.0f && a.block_m == 0 && a.block_n == 0 && a.split_k <= 1 && !a.jit && span32(64, a.lda) &&
            span32(kStrip, a.ldb) && span32(ceil_div(a.k, 64), a.sfa_ld * 2) && span32(ceil_div(a.k, 64), a.sfb_ld * 2);
@@ -420,6 +420,7 @@ extern "C" int dg_mx_gemm(const void* x, int32_t x_dtype, int64_t x_ld, const vo
                           void* stream) {
     using namespace dg;
     if (m < 0 || n < 0 || k < 0) return dg_set_error("dg_mx_gemm: negative size");
+    if (n > kMaxExtent) return dg_set_error("dg_mx_gemm: at most 2^30 columns");
     if (x_dtype != DG_DTYPE_BF16 && x_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx_gemm: x is bf16 or fp32");
     if (d_dtype != DG_DTYPE_BF16 && d_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx_gemm: D is bf16 or fp32");
     if (m > 16 || (int64_t)m * k > kInside) {

@@ -264,6 +264,7 @@ int mx_run(const dg_mx_args* a, void* stream) {
     if (a->format != DG_MX_E2M1 && a->format != DG_MX_E4M3) return dg_set_error("dg_mx: unknown format");
     if (a->x_dtype != DG_DTYPE_BF16 && a->x_dtype != DG_DTYPE_F32) return dg_set_error("dg_mx: values are bf16 or fp32");
     if (a->batches < 0 || a->rows < 0 || a->k < 0) return dg_set_error("dg_mx: negative size");
+    if (a->rows > kMaxExtent || a->k > kMaxExtent) return dg_set_error("dg_mx: at most 2^30 rows and values of a row");
     if (a->k % 32 != 0) return dg_set_error("dg_mx: K must be a multiple of the block of 32 values");
     if (a->batches == 0 || a->rows == 0 || a->k == 0) return DG_OK;
     const bool fp4 = a->format == DG_MX_E2M1, f32 = a->x_dtype == DG_DTYPE_F32;

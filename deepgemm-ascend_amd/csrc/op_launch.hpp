@@ -24,6 +24,9 @@ inline uint32_t* status_words_for(hipStream_t st) {
     return s == hipStreamCaptureStatusNone ? status_words() : status_words_if_ready();
 }
 
+// Extents of the operators: indices of tiles that end past an extent stay within 32 bits.
+constexpr int64_t kMaxExtent = int64_t(1) << 30;
+
 inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // Workgroups [0, grid) of a kernel whose parameters hold the first one of a launch (vbase).  `cus` > 0 (set_num_sms

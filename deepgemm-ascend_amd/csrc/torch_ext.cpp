@@ -280,6 +280,9 @@ void init_operators(int64_t sort, int64_t sort_workspace, int64_t dispatch, int6
 
 using Tensors = std::vector<at::Tensor>;
 
+// (as the library: larger extents go to the general path, which refuses them)
+constexpr int64_t kMaxExtent = int64_t(1) << 30;
+
 void raise_pending() {
     if (const uint32_t bits = pending_errors()) throw std::runtime_error(error_message(bits));
 }
@@ -287,7 +290,7 @@ void raise_pending() {
 void* stream_ptr(int64_t stream) { return reinterpret_cast<void*>(stream); }
 
 bool int32_rows(const at::Tensor& t, int64_t dim, const at::Device& device) {
-    return t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == device && t.numel() < (int64_t(1) << 31);
+    return t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == device && t.numel() <= kMaxExtent;
 }
 
 // Rows of contiguous values that do not overlap (an expanded row goes to the general path).
@@ -321,7 +324,7 @@ at::Tensor scale_view(at::Tensor flat, int64_t rows, int64_t k64, int64_t ld) {
 
 Tensors moe_sort(const at::Tensor& ids, int64_t groups, int64_t rows, int64_t alignment, int64_t num_cus, int64_t stream) {
     if (g_moe_sort == nullptr || ids.dim() != 2 || !ids.is_cuda() || !ids.is_contiguous() || groups < 1 || groups > 1024 || rows < 0 ||
-        rows % alignment != 0 || rows >= (int64_t(1) << 31) || ids.numel() >= (int64_t(1) << 31) ||
+        rows % alignment != 0 || rows > kMaxExtent || ids.numel() > kMaxExtent ||
         !(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong))
         return {};
     raise_pending();
@@ -416,7 +419,7 @@ Tensors moe_combine_backward(const at::Tensor& d_out, const at::Tensor& rows, co
 // A two-dimensional x [M, K] to codes and scale factors.
 Tensors mx_quantize(const at::Tensor& x, bool fp4, int64_t num_cus, int64_t stream) {
     if (g_mx_quantize == nullptr || x.dim() != 2 || !x.is_cuda() || rows_dtype(x) < 0 || x.size(1) % 32 != 0 || x.numel() == 0 ||
-        !plain(x) || x.size(0) >= (int64_t(1) << 31) || x.size(1) >= (int64_t(1) << 31))
+        !plain(x) || x.size(0) > kMaxExtent || x.size(1) > kMaxExtent)
         return {};
     raise_pending();
     const int64_t m = x.size(0), k = x.size(1), ld = align_up(m, 2), k64 = ceil_div(k, 64);
@@ -446,7 +449,7 @@ Tensors mx_dequantize(const at::Tensor& codes, const at::Tensor& sf, bool f32, i
         codes.numel() == 0 || !plain(codes) || codes.stride(0) % 8 || (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 7))
         return {};
     const int64_t m = codes.size(0), k = codes.size(1) * (fp4 ? 2 : 1), k64 = ceil_div(k, 64);
-    if (k % 32 != 0 || m >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || sf.scalar_type() != at::kShort || sf.dim() != 2 ||
+    if (k % 32 != 0 || m > kMaxExtent || k > kMaxExtent || sf.scalar_type() != at::kShort || sf.dim() != 2 ||
         sf.size(0) != m || sf.size(1) != k64 || sf.device() != codes.device() || !(m <= 1 || sf.stride(0) == 1))
         return {};
     raise_pending();
@@ -481,7 +484,7 @@ bool mx_gemm(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sfw, co
         const Tensors q = mx_quantize(x, fp4, num_cus, stream);
         return !q.empty() && gemm(kNormal, q[0], q[1], w, sfw, d, c, c10::nullopt, 1, 32, 1, 32, cus, alignment, stream);
     }
-    if (m == 0 || n == 0 || k == 0 || k % 32 != 0 || k >= (int64_t(1) << 31) || n >= (int64_t(1) << 31) || w.size(1) * 2 != k ||
+    if (m == 0 || n == 0 || k == 0 || k % 32 != 0 || k > kMaxExtent || n > kMaxExtent || w.size(1) * 2 != k ||
         sfw.size(0) != n || sfw.size(1) != k64 || d.size(0) != m || d.size(1) != n || x.stride(1) != 1 || w.stride(1) != 1 ||
         d.stride(1) != 1 || !(n <= 1 || sfw.stride(0) == 1))
         return false;
@@ -512,7 +515,7 @@ bool xent_vector(const at::Tensor& t, int64_t tokens, const at::Device& device) 
 // Arguments of a cross entropy of x [T, H], w [V, H] and their targets; false: the general path.
 bool xent_args(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore, int64_t num_cus, dg_linear_xent_args& a) {
     if (g_xent_forward == nullptr || !xent_rows(x, x.device()) || !xent_rows(w, x.device()) || x.size(1) != w.size(1) || x.size(1) == 0 ||
-        x.size(1) % 8 != 0 || x.size(0) == 0 || x.size(0) > (1 << 20) || w.size(0) == 0 || w.size(0) >= (int64_t(1) << 31) - 256 ||
+        x.size(1) % 8 != 0 || x.size(0) == 0 || x.size(0) > (1 << 20) || w.size(0) == 0 || w.size(0) > kMaxExtent ||
         !xent_vector(target, x.size(0), x.device()) || !(target.scalar_type() == at::kInt || target.scalar_type() == at::kLong))
         return false;
     a = {};

@@ -32,7 +32,7 @@ def _args(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_in
     _assert(x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16, 'x and weight must be bf16')
     _assert(x.size(1) == weight.size(1), f"Conflicting shape dimension 'h': x gives {x.size(1)}, weight gives {weight.size(1)}")
     _assert(x.size(1) > 0 and x.size(1) % 8 == 0, f'H must be a multiple of 8, got {x.size(1)}')
-    _assert(0 < weight.size(0) < 2 ** 31 - 256, 'the vocabulary must have between 1 and 2^31 - 257 words')
+    _assert(0 < weight.size(0) <= 2 ** 30, 'the vocabulary must have between 1 and 2^30 words')
     _assert(x.size(0) <= MAX_TOKENS, f'at most {MAX_TOKENS} tokens')
     _assert(target.dtype in (torch.int32, torch.int64) and target.shape == x.shape[:1], 'target must be a [T] int32 or int64 tensor')
     _assert(weight.device == x.device and target.device == x.device, 'x, weight and target must be on the same device')

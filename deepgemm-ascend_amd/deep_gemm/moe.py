@@ -50,7 +50,7 @@ def _check_layout(layout: MoELayout, device) -> Tuple[int, int, int]:
     for name, t, dim in zip(MoELayout._fields, layout, (2, 1, 1, 1)):
         _assert(t.dtype == torch.int32 and t.dim() == dim and t.is_contiguous(), f'layout.{name} must be a contiguous int32 tensor')
         _assert(t.device == device, f'layout.{name} must be on the same device as the rows')
-    _assert(max(layout.slots.numel(), layout.source.numel()) < 2 ** 31, 'a layout has less than 2^31 pairs and rows')
+    _assert(max(layout.slots.numel(), layout.source.numel()) <= 2 ** 30, 'a layout has at most 2^30 pairs and rows')
     _assert(layout.m_indices.numel() == layout.source.numel(), 'layout.source and layout.m_indices must have one entry per row')
     return layout.slots.size(0), layout.slots.size(1), layout.source.numel()
 
@@ -73,7 +73,7 @@ def moe_sort(topk_idx: torch.Tensor, num_groups: int, num_rows: Optional[int] = 
         if made:
             return MoELayout(*made)
     _assert(rows >= 0 and rows % alignment == 0, f'num_rows must be a multiple of the alignment {alignment}')
-    _assert(max(t * k, rows) < 2 ** 31, 'a layout has less than 2^31 pairs and rows')
+    _assert(max(t * k, rows) <= 2 ** 30, 'a layout has at most 2^30 pairs and rows')
     topk_idx = topk_idx.contiguous()
     new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=topk_idx.device)
     layout = MoELayout(new(t, k), new(rows), new(num_groups), new(rows))

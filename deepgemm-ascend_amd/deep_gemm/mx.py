@@ -52,7 +52,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = 'e2m1') -> Tuple[torch.Tensor, torch
     _assert(x.dim() in (2, 3) and x.is_cuda, 'x must be a [M, K] or [B, M, K] device tensor')
     _assert(x.dtype in _DTYPES, 'x must be bf16 or fp32')
     m, k = x.size(-2), x.size(-1)
-    _assert(max(x.shape) < 2 ** 31, 'every extent must be below 2^31')
+    _assert(max(x.shape) <= 2 ** 30, 'every extent must be at most 2^30')
     _assert(k % 32 == 0, f'K must be a multiple of the block of 32 values, got {k}')
     if k > 1 and (x.stride(-1) != 1 or (m > 1 and x.stride(-2) < k)):   # (an expanded row is written out)
         x = x.contiguous()

@@ -363,7 +363,8 @@ int dg_mx_gemm(const void *x, int32_t x_dtype, int64_t x_ld, const void *w, int6
  * Cross entropy of a linear layer over a vocabulary, without keeping the logits:
  *   z = x w^T, lse[t] = log sum_v exp z[t][v], loss[t] = lse[t] - z[t][target[t]]
  * and its gradient d_x = d w, d_w = d^T x with d[t][v] = (exp(z[t][v] - lse[t]) - [v = target[t]]) d_loss[t].
- * x [tokens][width], w [vocab][width], d_x and d_w are bf16 (width a multiple of 8, rows 16-byte aligned, at most 2^20 tokens);
+ * x [tokens][width], w [vocab][width], d_x and d_w are bf16 (width a multiple of 8, rows 16-byte aligned, at most 2^20 tokens and
+ * 2^30 words);
  * loss, lse, d_loss fp32 [tokens].  A token whose target is ignore_index has loss and gradient 0; so has one whose target lies
  * outside the vocabulary (DG_ERR_TARGET).  The workspace (dg_linear_xent_workspace_size bytes) holds nothing between calls.
  */

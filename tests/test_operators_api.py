@@ -223,3 +223,23 @@ def test_fp4_psum_layouts_of_little_more_than_a_tile_a_group(lib, m, alignment, 
     block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
     assert lib.dg_select_config(ctypes.byref(args), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
     assert (block_m.value, block_n.value) == tile
+
+
+def test_extents_past_2_to_the_30(lib):
+    """Indices of tiles that end past an extent are 32-bit: larger extents are refused before anything is launched."""
+    big = (1 << 30) + 32
+    layout = _layout(tokens=big, topk=1)
+    _refused(lib, lib.dg_moe_sort(4096, 4, layout, None, 0, 0, None), 'invalid size')
+    _refused(lib, lib.dg_moe_combine(4096, 64, 0, 64, _layout(rows=big), None, 4096, 64, 0, None), 'invalid size')
+    _refused(lib, lib.dg_moe_dispatch(4096, 64, 64, layout, 4096, 64, None, 0, 0, None, 0, 1, 0, None), 'invalid size')
+    for kw in (dict(rows=big, sf_ld=big), dict(k=big, x_ld=big, codes_ld=big)):
+        a = _lib.MxArgs(0, 0, 1, 4, 64, 4096, 64, 0, 4096, 32, 0, 4096, 4, 0, 0)
+        for name, v in kw.items():
+            setattr(a, name, v)
+        _refused(lib, lib.dg_mx_quantize(a, None), '2^30')
+        _refused(lib, lib.dg_mx_dequantize(a, None), '2^30')
+    _refused(lib, lib.dg_mx_gemm(4096, 0, 64, 4096, 32, 4096, big, 4096, 0, big, 1, big, 64, 0, 0, None), '2^30')
+    a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 60, 0)
+    a.vocab = (1 << 30) + 1
+    _refused(lib, lib.dg_linear_xent_forward(a, None), '2^30')
+    _refused(lib, lib.dg_linear_xent_backward(a, None), '2^30')
