@@ -255,6 +255,125 @@ __global__ __launch_bounds__(256, (quad_occupancy<BM, BN, kBF16, true, true>()))
     quad_body<BM, BN, kBF16, kEpiBf16, kNormal, 1, 0, 0, 0, true, true, WeightTail>(p, blockIdx.x + p.vbase, tail);
 }
 
+// d_w of few tokens: a product of short K, where a tile's fill and stores are more than its stages, so that several workgroups share
+// a CU and run them beside each other: 128 words x 128 values, four waves of 64 x 64, 32 tokens a stage in two slots of LDS (32 KB a
+// workgroup, four to a CU).  Both operands are MN-major: 16-byte pieces of a token's row go to LDS as they are (swizzled so that a
+// transposing read of four rows meets every bank once), and the reads hand each lane consecutive tokens of a word.
+// Bound by the bytes of d_w, or by its LDS reads where there are more tokens.  The whole backward pass with it and with the four-wave
+// tiles, us: 16 tokens, 131072 words of width 4096 757 and 799, 50257 of 1024 73 and 87, 100000 of 512 82 and 97, 32000 of 2048 85 and
+// 97; 128 tokens 930 and 937, 100 and 114, 117 and 131, 107 and 119; 200 tokens, 50257 of 1024 124 and 141; 300 tokens 1365 and
+// 1340, 170 and 189, 188 and 205, 182 and 189; 512 tokens 1665 and 1575, 209 and 220, 271 and 278, 221 and 223; 777 tokens 2581 and 2410.
+constexpr int kShortTile = 128, kShortK = 32, kShortTokens = 256;
+
+struct ShortParams {
+    const uint16_t *d, *x;
+    int64_t d_ld, x_ld, ld;
+    const float* unit;
+    uint16_t* d_w;
+    int tokens, words, width;
+    int col_tiles, tiles;
+    int vbase;
+};
+
+__global__ __launch_bounds__(256, 4) void xent_weight_short_kernel(const ShortParams p) {
+    constexpr int PITCH = kShortTile * 2, SIDE = kShortK * PITCH, SLOT = 2 * SIDE, LOADS = SIDE / (256 * 16);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SLOT];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, q = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
+    // (neighbours in a row of tiles share their d, on one XCD)
+    const int t = xcd_remap(blockIdx.x + p.vbase, p.tiles);
+    const int m0 = t / p.col_tiles * kShortTile, n0 = t % p.col_tiles * kShortTile;
+    // tokens past the last, and values past the width in the last row, lie past the ranges and read zeros
+    const __amdgpu_buffer_rsrc_t rs_d = make_rsrc(p.d + m0, (p.tokens * p.d_ld - m0) * 2);
+    const __amdgpu_buffer_rsrc_t rs_x = make_rsrc(p.x + n0, ((p.tokens - 1) * p.x_ld + p.width - n0) * 2);
+    const int k_of = tid / (PITCH / 16), piece = (tid % (PITCH / 16)) ^ ((k_of & 3) << 2);
+    const uint32_t at_d = (uint32_t)(k_of * p.d_ld * 2 + piece * 16), at_x = (uint32_t)(k_of * p.x_ld * 2 + piece * 16);
+    const int row_d = __builtin_amdgcn_readfirstlane((int)(p.d_ld * 2)), row_x = __builtin_amdgcn_readfirstlane((int)(p.x_ld * 2));
+    constexpr int KSTEP = 256 / (PITCH / 16);          // tokens of one load of the workgroup
+    static_assert(KSTEP % 4 == 0, "a thread's piece of the swizzle is the same in each of its loads");
+    auto issue = [&](int s, int slot) {
+        uint8_t* const to = lds + slot * SLOT + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int k = s * kShortK + i * KSTEP;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_d, (lds_void*)(to + i * 4096), 16, at_d, k * row_d, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_x, (lds_void*)(to + SIDE + i * 4096), 16, at_x, k * row_x, 0, 0);
+        }
+    };
+    // K [8 q, + 8) of 16 tokens from `k0` of MN row R0 + (lane & 31): two transposing reads
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s lds_v4s;
+    const int s16 = lane & 15, h = (lane >> 4) & 1;
+    auto fragment = [&](const uint8_t* side, int R0, int k0) {
+        const int col = R0 + 16 * h + 4 * (s16 & 3), k = k0 + 8 * q + (s16 >> 2);
+        const uint8_t* const at = side + k * PITCH + (((col >> 3) ^ ((k & 3) << 2)) << 4) + ((col >> 2) & 1) * 8;
+        const i32x2 a = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at));
+        const i32x2 b = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 4 * PITCH)));
+        const i32x4 both = {a[0], a[1], b[0], b[1]};
+        return __builtin_bit_cast(bf16x8, both);
+    };
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+    const int ns = ceil_div(p.tokens, kShortK);
+    issue(0, 0);
+    if (ns > 1) issue(1, 1);
+    for (int s = 0; s < ns; ++s) {
+        if (s + 1 < ns) wait_vmcnt<2 * LOADS>();
+        else wait_vmcnt<0>();
+        stage_barrier();
+        const uint8_t* const side = lds + (s & 1) * SLOT;
+#pragma unroll
+        for (int k0 = 0; k0 < kShortK; k0 += 16) {
+            bf16x8 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i] = fragment(side, wm * 64 + 32 * i, k0);
+                b[i] = fragment(side + SIDE, wn * 64 + 32 * i, k0);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        }
+        if (s + 2 < ns) {
+            __builtin_amdgcn_s_waitcnt(0xc07f);        // (lgkmcnt 0: this wave's reads of the slot have returned)
+            stage_barrier();
+            issue(s + 2, s & 1);
+        }
+    }
+    // through LDS, so that 16 lanes store a row's 256 bytes (16-byte pieces, each row's in an order of its own)
+    const float unit = p.unit[1];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = wm * 64 + 32 * i + r;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            i32x2 pk[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                pk[e] = i32x2{(int)pack_bf16x2(acc[i][j][4 * e] * unit, acc[i][j][4 * e + 1] * unit),
+                              (int)pack_bf16x2(acc[i][j][4 * e + 2] * unit, acc[i][j][4 * e + 3] * unit)};
+            i32x4 w[2];
+            runs_of_16(pk, w);
+            const int at = wn * 8 + 4 * j + (q ? 0 : 2);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) *reinterpret_cast<i32x4*>(lds + row * PITCH + (((at + x) ^ (row & 15)) << 4)) = w[x];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kShortTile / 16; ++i) {
+        const int row = i * 16 + tid / 16, n = n0 + ((tid % 16) ^ (row & 15)) * 8;
+        // (a row ends after a multiple of 8 values)
+        if (m0 + row < p.words && n < p.width)
+            *reinterpret_cast<i32x4*>(p.d_w + (int64_t)(m0 + row) * p.ld + n) = *reinterpret_cast<const i32x4*>(lds + row * PITCH + (tid % 16) * 16);
+    }
+}
+
 struct UnitParams {
     const float* d_loss;
     const void* target;
@@ -479,6 +598,17 @@ int launch_logits(const Plan& pl, const dg_linear_xent_args& a, const XentParams
 
 // d_w rows of the piece = d^T x (both read MN-major): K rows past the tokens are not read.
 int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, hipStream_t st) {
+    if (a.tokens <= kShortTokens && (int64_t)(a.tokens + kShortK) * a.x_ld * 2 <= 0x7fffffffLL) {   // (32-bit offsets into x)
+        ShortParams s = {};
+        s.d = x.d; s.d_ld = x.d_ld; s.x = reinterpret_cast<const uint16_t*>(a.x); s.x_ld = a.x_ld;
+        s.unit = x.unit; s.d_w = reinterpret_cast<uint16_t*>(a.d_w) + (int64_t)x.first * a.d_w_ld; s.ld = a.d_w_ld;
+        s.tokens = a.tokens; s.words = words; s.width = a.width;
+        s.col_tiles = ceil_div(a.width, kShortTile);
+        const int64_t tiles = (int64_t)ceil_div(words, kShortTile) * s.col_tiles;
+        if (tiles > 0x7fffffffLL) return dg_set_error("dg_linear_xent: too many tiles");
+        s.tiles = (int)tiles;
+        return launch_op(xent_weight_short_kernel, tiles, 256, s, st, a.num_cus);
+    }
     KParams p = tile_params();
     p.a = reinterpret_cast<const uint8_t*>(x.d);
     p.b = reinterpret_cast<const uint8_t*>(a.x);

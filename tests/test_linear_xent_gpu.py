@@ -66,6 +66,37 @@ def test_loss_and_gradient(t, h, v, dtype):
     _check(*_inputs(t, h, v, dtype=dtype))
 
 
+@pytest.mark.parametrize('t', [16, 31, 32, 33, 64, 65, 96, 255, 256])
+@pytest.mark.parametrize('h,v', [(8, 130), (136, 127), (392, 300), (1024, 2049)])
+def test_gradients_of_few_tokens(t, h, v):
+    """Up to 256 tokens the gradient of w is a kernel of short K: whole and cut stages of 32 tokens, tiles of 128 words and values."""
+    _check(*_inputs(t, h, v, seed=1))
+
+
+@pytest.mark.parametrize('t', [5, 40, 300])
+@pytest.mark.parametrize('h,v', [(72, 257), (136, 128)])
+def test_gradients_stay_within_their_rows(t, h, v):
+    """Leading dimensions past the width: nothing but the rows' values is written, and nothing behind the inputs is read."""
+    x, w, target, d_loss = _inputs(t, h, v, seed=2)
+    wide = [torch.full((n + 2, h + 24), float('nan'), dtype=torch.bfloat16, device='cuda') for n in (t, v)]
+    for buf, rows in zip(wide, (x, w)):
+        buf[1:-1, 8:8 + h] = rows.cuda()
+    dx, dw, dt, dl = wide[0][1:-1, 8:8 + h], wide[1][1:-1, 8:8 + h], target.cuda(), d_loss.cuda()
+    _check(x, w, target, d_loss, (dx, dw, dt, dl))
+    _, lse = deep_gemm.linear_cross_entropy(dx, dw, dt)
+    want = deep_gemm.linear_cross_entropy_backward(dl, dx, dw, dt, lse)
+    keep, a = deep_gemm.loss._args(dx, dw, dt, -100)
+    assert a.x_ld == a.w_ld == h + 24
+    out = [torch.full((n + 2, h + 24), 7.0, dtype=torch.bfloat16, device='cuda') for n in (t, v)]
+    a.lse, a.d_loss, a.d_x_ld, a.d_w_ld = lse.data_ptr(), dl.data_ptr(), h + 24, h + 24
+    a.d_x, a.d_w = out[0][1:, 8:].data_ptr(), out[1][1:, 8:].data_ptr()
+    deep_gemm.loss._run('dg_linear_xent_backward', a, 1, dx)
+    for buf, ref in zip(out, want):
+        assert torch.equal(buf[1:-1, 8:8 + h], ref)
+        buf[1:-1, 8:8 + h] = 7.0
+        assert (buf == 7.0).all()
+
+
 def test_large_logits_and_sharp_rows():
     """Logits of several hundred: exponentials of anything but the largest vanish, and nothing overflows.  (The gradient's
     entries below the smallest normal fp32 number, which the matrix unit flushes, have no relative bound: gradients are
