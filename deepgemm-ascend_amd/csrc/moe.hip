@@ -451,7 +451,7 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Com
         }
 #pragma unroll
         for (int k = 0; k < kChoices; ++k)
-            for (int off = min(p.lanes, 64) / 2; off > 0; off >>= 1) dot[k] += __shfl_xor(dot[k], off, 64);
+            for (int off = k0 + k < p.topk ? min(p.lanes, 64) / 2 : 0; off > 0; off >>= 1) dot[k] += __shfl_xor(dot[k], off, 64);
         if (p.lanes > 64) {
             if (k0 > 0) __syncthreads();            // (the last group's sums have been read)
             if ((tid & 63) == 0) {
@@ -562,6 +562,15 @@ extern "C" int dg_moe_dispatch(const void* src, int64_t src_ld, int64_t row_byte
 namespace dg {
 namespace {
 
+// Threads of a token in the gradient, at most: eight chunks of its rows to each, where there are tokens enough, so that the sums
+// over the threads stay small beside them (us with 64 and 256 threads: 8192 x 2 pairs of 2048 bf16 values 36 and 49, 8192 x 1 of
+// 4096 48 and 57, 32768 x 4 of 1024 127 and 138; 8192 x 8 of 4096 261 and 250, 16 x 8 of 7168 39 and 27).
+int backward_lanes(int tokens, int topk, int chunks) {
+    int lanes = kRowThreads;
+    while (tokens >= 1024 && lanes > 64 && (int64_t)chunks * topk < 8 * (int64_t)lanes) lanes /= 2;
+    return lanes;
+}
+
 // n: values of a chunk
 int combine_params(const dg_moe_layout* l, int64_t width, int n, CombineParams& p) {
     p.slots = l->slots; p.source = l->source;
@@ -618,6 +627,7 @@ extern "C" int dg_moe_combine_backward(const void* d_out, int64_t d_out_ld, cons
     const bool f32 = dtype == DG_DTYPE_F32;
     const bool vec = width >= (f32 ? 4 : 8);
     if (const int rc = combine_params(l, width, !vec ? 1 : f32 ? 4 : 8, p)) return rc;
+    p.lanes = std::min(p.lanes, backward_lanes(l->tokens, l->topk, p.chunks));
     p.pad_blocks = width > 0 ? ceil_div(l->rows, kPadRows) : 0;
     const int64_t grid = p.pad_blocks + (int64_t)(l->topk > 0 ? ceil_div(l->tokens, kRowThreads / p.lanes) : 0);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
