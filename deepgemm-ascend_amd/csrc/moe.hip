@@ -202,6 +202,14 @@ int row_lanes(int64_t chunks) {
     return l;
 }
 
+// Workgroups that share the rows of `blocks` ones: for few tokens a row's chunks go beside each other rather than after each other
+// (sums of 16 x 8 pairs of 7168 bf16 values 4.2 us, 9.5 with one workgroup a token; 256 x 8 7.0 and 14.2, 512 x 8 12.5 and 17.6), up to
+// `most` workgroups in all: moving keeps four chunks of a thread in flight already (16 x 8 of 7168 fp32 values 4.5 and 6.9, but 256 x 8
+// of bf16 8.4 and 7.8 with 1024 workgroups).
+int row_parts(int64_t blocks, int chunks, int lanes, int most) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(chunks, lanes), most / std::max<int64_t>(blocks, 1)));
+}
+
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int i32x4_half __attribute__((ext_vector_type(4), aligned(2)));
@@ -235,6 +243,7 @@ struct DispatchParams {
     int64_t src_ld, dst_ld, row_bytes;
     const int32_t *slots, *source;
     int tokens, topk, rows, chunks, lanes;
+    int parts;                 // workgroups that share a token's row
     int pad_blocks;            // first workgroups: padding rows (0: left as they are)
     int sf_blocks;             // next workgroups: scale factors (0: none)
     const int16_t* sf;         // [k64][sf_ld]
@@ -274,18 +283,19 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(const DispatchPar
         return;
     }
     b -= p.sf_blocks;
-    const int t = b * (kRowThreads / p.lanes) + tid / p.lanes, c0 = tid % p.lanes;
+    const int part = b % p.parts, step = p.lanes * p.parts;
+    const int t = b / p.parts * (kRowThreads / p.lanes) + tid / p.lanes, c0 = part * p.lanes + tid % p.lanes;
     if (t >= p.tokens) return;
     const uint8_t* const in = p.src + (int64_t)t * p.src_ld;
     const int32_t* const slots = p.slots + (int64_t)t * p.topk;
     constexpr int U = 4;
-    for (int c = c0; c < p.chunks; c += U * p.lanes) {
+    for (int c = c0; c < p.chunks; c += U * step) {
         T v[U];
         int64_t at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            at[u] = min((int64_t)(c + u * p.lanes) * V, p.row_bytes - V);
-            if (c + u * p.lanes < p.chunks) v[u] = *reinterpret_cast<const M*>(in + at[u]);
+            at[u] = min((int64_t)(c + u * step) * V, p.row_bytes - V);
+            if (c + u * step < p.chunks) v[u] = *reinterpret_cast<const M*>(in + at[u]);
         }
         for (int k = 0; k < p.topk; ++k) {
             const int s = slots[k];
@@ -293,7 +303,7 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(const DispatchPar
             uint8_t* const d = p.dst + (int64_t)s * p.dst_ld;
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (c + u * p.lanes < p.chunks) *reinterpret_cast<M*>(d + at[u]) = v[u];
+                if (c + u * step < p.chunks) *reinterpret_cast<M*>(d + at[u]) = v[u];
         }
     }
 }
@@ -353,6 +363,7 @@ struct CombineParams {
     const int32_t *slots, *source;
     int64_t in_ld, out_ld, d_out_ld;   // elements
     int tokens, topk, rows, width, chunks, lanes, pad_blocks;
+    int parts;                 // forward: workgroups that share a token's row
     int vbase;
 };
 
@@ -362,14 +373,14 @@ constexpr int kChoices = 8;     // choices whose rows are in flight together
 // bytes: 8192 x 8 pairs of 4096 bf16 values 124 us (604 MB: 4.9 TB/s), 140 to 160 behind a kernel whose stores are still going out.
 template <typename E, int N>
 __global__ __launch_bounds__(kRowThreads) void combine_kernel(const CombineParams p) {
-    const int b = blockIdx.x + p.vbase, tid = threadIdx.x;
+    const int b = (blockIdx.x + p.vbase) / p.parts, part = (blockIdx.x + p.vbase) % p.parts, tid = threadIdx.x;
     const int t = b * (kRowThreads / p.lanes) + tid / p.lanes;
     if (t >= p.tokens) return;
     const int32_t* const slots = p.slots + (int64_t)t * p.topk;
     const float* const weights = p.weights + (int64_t)t * p.topk;
     E* const out = reinterpret_cast<E*>(p.out) + (int64_t)t * p.out_ld;
     const E* const in = reinterpret_cast<const E*>(p.rows_in);
-    for (int c = tid % p.lanes; c < p.chunks; c += p.lanes) {
+    for (int c = part * p.lanes + tid % p.lanes; c < p.chunks; c += p.parts * p.lanes) {
         const int at = min(c * N, p.width - N);
         float sum[N] = {};
         for (int k0 = 0; k0 < p.topk; k0 += kChoices) {
@@ -554,7 +565,9 @@ extern "C" int dg_moe_dispatch(const void* src, int64_t src_ld, int64_t row_byte
         if (n > 0x3fffffffLL) return dg_set_error("dg_moe_dispatch: too many scale factors");
         p.sf_blocks = (int)n;
     }
-    const int64_t grid = p.pad_blocks + (int64_t)p.sf_blocks + (l->topk > 0 ? ceil_div(l->tokens, kRowThreads / p.lanes) : 0);
+    const int64_t blocks = l->topk > 0 ? ceil_div(l->tokens, kRowThreads / p.lanes) : 0;
+    p.parts = row_parts(blocks, p.chunks, p.lanes, 256);
+    const int64_t grid = p.pad_blocks + (int64_t)p.sf_blocks + blocks * p.parts;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     return launch_op(v == 16 ? dispatch_kernel<16> : dispatch_kernel<1>, grid, kRowThreads, p, st, num_cus);
 }
@@ -601,7 +614,9 @@ extern "C" int dg_moe_combine(const void* rows, int64_t rows_ld, int32_t dtype, 
     const bool f32 = dtype == DG_DTYPE_F32;
     const bool vec = width >= (f32 ? 4 : 8);
     if (const int rc = combine_params(l, width, !vec ? 1 : f32 ? 4 : 8, p)) return rc;
-    const int64_t grid = ceil_div(l->tokens, kRowThreads / p.lanes);
+    const int64_t blocks = ceil_div(l->tokens, kRowThreads / p.lanes);
+    p.parts = row_parts(blocks, p.chunks, p.lanes, 1024);
+    const int64_t grid = blocks * p.parts;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (f32) return launch_op(vec ? combine_kernel<float, 4> : combine_kernel<float, 1>, grid, kRowThreads, p, st, num_cus);
     return launch_op(vec ? combine_kernel<uint16_t, 8> : combine_kernel<uint16_t, 1>, grid, kRowThreads, p, st, num_cus);
