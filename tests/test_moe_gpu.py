@@ -162,6 +162,27 @@ def test_combine_and_gradients(dtype, h, k):
     assert torch.equal(deep_gemm.moe_combine(wide[:, 1:h + 1], layout, w_in.cuda()), deep_gemm.moe_combine(dev, layout, w_in.cuda()))
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('t,k,h', [(1, 8, 7168), (3, 2, 16001), (70, 3, 5003), (130, 9, 4100), (600, 2, 2050), (1030, 1, 2048), (1100, 3, 700)])
+def test_wide_rows_of_few_tokens_and_short_ones_of_many(dtype, t, k, h):
+    """Rows that several workgroups share, and gradients that fewer threads than a workgroup take."""
+    g = gen(h + k)
+    layout, (slots, source, _, _) = _sort(_ids(t, k, 13, g), 13, 32)
+    m = source.numel()
+    x, rows, d_out = (torch.randn(n, h, generator=g).to(dtype) for n in (t, m, t))
+    moved = deep_gemm.moe_dispatch(x.cuda(), layout).cpu()
+    live = source >= 0
+    assert torch.equal(moved[live], x[(source[live] // k).long()]) and (moved[~live] == 0).all()
+    rows[~live] = float('nan')
+    w = torch.randn(t, k, generator=g)
+    ref, mag = om.combine(rows, slots, w)
+    assert _close(deep_gemm.moe_combine(rows.cuda(), layout, w.cuda()).cpu(), ref, mag, k, dtype)
+    d_rows, d_w = deep_gemm.moe_combine_backward(d_out.cuda(), rows.cuda(), layout, w.cuda())
+    ref_rows, ref_w, mag_w = om.combine_backward(d_out, rows, slots, w)
+    assert _close(d_rows.cpu(), ref_rows, ref_rows.abs(), 1, dtype)
+    assert ((d_w.cpu().double() - ref_w).abs() <= (h + 8) * U32 * mag_w).all()
+
+
 def test_gradients_against_differences():
     """<d/ds loss(s), direction> of a weighted there-and-back movement against central differences in 64 bits."""
     g = gen(7)
