@@ -1043,7 +1043,11 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
     if (plan.split > 1) {
         // DG_SPLIT_SPREAD=1 (test knob): the splits of a tile run on different XCDs
         const char* spread = std::getenv("DG_SPLIT_SPREAD");
-        p.split_spread = spread != nullptr && spread[0] == '1';
+        // (the cross entropy's d_x, whose K ranges are summed by a launch of their own: with a multiple of eight of them the tiles of
+        // a range run on one XCD and read its rows of d and w into that L2 once; its backward pass, us, with the ranges of a tile
+        // on one XCD in brackets: 785 tokens, 63000 words of width 1680 605 (724), 1200 x 131072 of 1024 1024 (1152), 600 x
+        // 131072 of 256 246 (278), 128 x 32000 of 2048 105 (111))
+        p.split_spread = (spread != nullptr && spread[0] == '1') || (k_rows > 0 && plan.split % kXcds == 0);
         p.counters = reinterpret_cast<int*>(workspace);
         p.ws = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + kCounterBytes);
         p.split_reduce = plan.split_reduce || quad;
@@ -1207,6 +1211,9 @@ void bf16_tile_plan(int m, int n, int k, bool mn, bool stats, int most, int cus,
             if (ceil_div(ns, sps) != sp) continue;
             double t = quad_time(q, tiles * sp, sps, cus);
             if (sp > 1) t += 3.5 + 8.0 * sp * m * (double)n / 7e6;
+            // (a range's tiles meet on one XCD where there are a multiple of eight ranges, see split_spread: worth a few idle CUs where
+            // the operands pass the last-level cache)
+            if (sp % kXcds == 0 && 2.0 * ((double)m + n) * k > 200e6) t *= 0.85;
             if (t < best) {
                 best = t;
                 bm = q.bm; bn = q.bn; split = sp;
