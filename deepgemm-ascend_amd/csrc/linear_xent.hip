@@ -255,6 +255,29 @@ __global__ __launch_bounds__(256, (quad_occupancy<BM, BN, kBF16, true, true>()))
     quad_body<BM, BN, kBF16, kEpiBf16, kNormal, 1, 0, 0, 0, true, true, WeightTail>(p, blockIdx.x + p.vbase, tail);
 }
 
+struct CastParams {
+    const float* src;          // [rows][width], whole rows together, in units of d
+    const float* unit;
+    uint16_t* dst;             // [rows][ld]
+    int64_t ld;
+    int rows, chunks;          // eight values each
+    int vbase;
+};
+
+// d_x: the fp32 sums over the pieces as bf16, a chunk a thread (8192 x 4096: 31 us, 201 MB).  In the launch of few tokens' d_w it
+// saves its own: backward of 1 token, 4000 words of width 512 24.2 -> 22.6 us, 90, 11000 of 704 38.0 -> 36.4, 256, 1000 of 4096 56.5 -> 54.6.
+__device__ __forceinline__ void cast_chunks(const CastParams& p, int block) {
+    const int64_t e = (int64_t)block * 256 + threadIdx.x;
+    const int64_t row = e / p.chunks;
+    if (row >= p.rows) return;
+    const int c = (int)(e - row * p.chunks) * 8;
+    const float* const s = p.src + row * p.chunks * 8 + c;
+    const float unit = p.unit[1];
+    const f32x4 a = *reinterpret_cast<const f32x4*>(s) * unit, b = *reinterpret_cast<const f32x4*>(s + 4) * unit;
+    *reinterpret_cast<i32x4*>(p.dst + row * p.ld + c) = i32x4{(int)pack_bf16x2(a[0], a[1]), (int)pack_bf16x2(a[2], a[3]),
+                                                             (int)pack_bf16x2(b[0], b[1]), (int)pack_bf16x2(b[2], b[3])};
+}
+
 // d_w of few tokens: a product of short K, where a tile's fill and stores are more than its stages, so that several workgroups share
 // a CU and run them beside each other: 128 words x 128 values, four waves of 64 x 64, 32 tokens a stage in two slots of LDS (32 KB a
 // workgroup, four to a CU).  Both operands are MN-major: 16-byte pieces of a token's row go to LDS as they are (swizzled so that a
@@ -272,6 +295,7 @@ struct ShortParams {
     uint16_t* d_w;
     int tokens, words, width;
     int col_tiles, tiles;
+    CastParams cast;           // d_x, by the workgroups past the tiles (the last piece's launch: d_x is complete there)
     int vbase;
 };
 
@@ -279,6 +303,10 @@ __global__ __launch_bounds__(256, 4) void xent_weight_short_kernel(const ShortPa
     constexpr int PITCH = kShortTile * 2, SIDE = kShortK * PITCH, SLOT = 2 * SIDE, LOADS = SIDE / (256 * 16);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SLOT];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, q = lane >> 5;
+    if ((int)blockIdx.x + p.vbase >= p.tiles) {
+        cast_chunks(p.cast, blockIdx.x + p.vbase - p.tiles);
+        return;
+    }
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
     // (neighbours in a row of tiles share their d, on one XCD)
     const int t = xcd_remap(blockIdx.x + p.vbase, p.tiles);
@@ -449,27 +477,8 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const JoinParams p) {
     p.loss[t] = target < 0 ? 0.f : lse - p.target_logit[t];
 }
 
-struct CastParams {
-    const float* src;          // [rows][width], whole rows together, in units of d
-    const float* unit;
-    uint16_t* dst;             // [rows][ld]
-    int64_t ld;
-    int rows, chunks;          // eight values each
-    int vbase;
-};
-
-// d_x: the fp32 sums over the pieces as bf16 (8192 x 4096: 31 us, 201 MB).
-__global__ __launch_bounds__(256) void xent_cast_kernel(const CastParams p) {
-    const int64_t e = (int64_t)(blockIdx.x + p.vbase) * 256 + threadIdx.x;
-    const int64_t row = e / p.chunks;
-    if (row >= p.rows) return;
-    const int c = (int)(e - row * p.chunks) * 8;
-    const float* const s = p.src + row * p.chunks * 8 + c;
-    const float unit = p.unit[1];
-    const f32x4 a = *reinterpret_cast<const f32x4*>(s) * unit, b = *reinterpret_cast<const f32x4*>(s + 4) * unit;
-    *reinterpret_cast<i32x4*>(p.dst + row * p.ld + c) = i32x4{(int)pack_bf16x2(a[0], a[1]), (int)pack_bf16x2(a[2], a[3]),
-                                                             (int)pack_bf16x2(b[0], b[1]), (int)pack_bf16x2(b[2], b[3])};
-}
+// d_x by itself, behind more tokens than the short kernel takes.
+__global__ __launch_bounds__(256) void xent_cast_kernel(const CastParams p) { cast_chunks(p, blockIdx.x + p.vbase); }
 
 // ------------------------------------------------------------------------------------------------ host
 // Tokens of one call: the gradient's product reads d MN-major, whose K rows (tokens) times a tile's words stay below 1 GiB.
@@ -596,18 +605,23 @@ int launch_logits(const Plan& pl, const dg_linear_xent_args& a, const XentParams
     });
 }
 
-// d_w rows of the piece = d^T x (both read MN-major): K rows past the tokens are not read.
-int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, hipStream_t st) {
+int64_t cast_blocks(const CastParams& c) { return ceil_div64((int64_t)c.rows * c.chunks, 256); }
+
+// d_w rows of the piece = d^T x (both read MN-major): K rows past the tokens are not read.  Behind the last piece, d_x from
+// its sums: for few tokens in the same launch.
+int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, const CastParams& cast, hipStream_t st) {
+    const bool last = x.first + words == a.vocab;
     if (a.tokens <= kShortTokens && (int64_t)(a.tokens + kShortK) * a.x_ld * 2 <= 0x7fffffffLL) {   // (32-bit offsets into x)
         ShortParams s = {};
         s.d = x.d; s.d_ld = x.d_ld; s.x = reinterpret_cast<const uint16_t*>(a.x); s.x_ld = a.x_ld;
         s.unit = x.unit; s.d_w = reinterpret_cast<uint16_t*>(a.d_w) + (int64_t)x.first * a.d_w_ld; s.ld = a.d_w_ld;
         s.tokens = a.tokens; s.words = words; s.width = a.width;
         s.col_tiles = ceil_div(a.width, kShortTile);
-        const int64_t tiles = (int64_t)ceil_div(words, kShortTile) * s.col_tiles;
-        if (tiles > 0x7fffffffLL) return dg_set_error("dg_linear_xent: too many tiles");
+        const int64_t tiles = (int64_t)ceil_div(words, kShortTile) * s.col_tiles, grid = tiles + (last ? cast_blocks(cast) : 0);
+        if (grid > 0x7fffffffLL) return dg_set_error("dg_linear_xent: too many tiles");
         s.tiles = (int)tiles;
-        return launch_op(xent_weight_short_kernel, tiles, 256, s, st, a.num_cus);
+        s.cast = cast;
+        return launch_op(xent_weight_short_kernel, grid, 256, s, st, a.num_cus);
     }
     KParams p = tile_params();
     p.a = reinterpret_cast<const uint8_t*>(x.d);
@@ -615,11 +629,12 @@ int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams
     p.m = words; p.n = a.width; p.k = a.tokens;
     p.lda = x.d_ld * 2; p.ldb = a.x_ld * 2;
     const WeightTail tail = {x, reinterpret_cast<uint16_t*>(a.d_w) + (int64_t)x.first * a.d_w_ld, a.d_w_ld, words, a.width};
-    return launch_grid(p, words, a.width, pl.wbm, pl.wbn, a.num_cus, [&](dim3 grid) {
+    const int rc = launch_grid(p, words, a.width, pl.wbm, pl.wbn, a.num_cus, [&](dim3 grid) {
         if (pl.wbm == 256 && pl.wbn == 256) hipLaunchKernelGGL((xent_weight_kernel<256, 256>), grid, dim3(256), 0, st, p, tail);
         else if (pl.wbm == 256) hipLaunchKernelGGL((xent_weight_kernel<256, 128>), grid, dim3(256), 0, st, p, tail);
         else hipLaunchKernelGGL((xent_weight_kernel<128, 128>), grid, dim3(256), 0, st, p, tail);
     });
+    return rc != DG_OK || !last ? rc : launch_op(xent_cast_kernel, cast_blocks(cast), 256, cast, st, a.num_cus);
 }
 
 XentParams xent_params(const dg_linear_xent_args& a) {
@@ -691,6 +706,8 @@ extern "C" int dg_linear_xent_backward(const dg_linear_xent_args* args, void* st
     x.d_ld = pl.words;
     float* const unit = reinterpret_cast<float*>(ws + pl.unit);
     x.unit = unit;
+    const CastParams cast = {reinterpret_cast<const float*>(ws + pl.d_x), unit, reinterpret_cast<uint16_t*>(a.d_x), a.d_x_ld, a.tokens,
+                             a.width / 8, 0};
     const UnitParams u = {a.d_loss, a.target, x.wide, a.tokens, a.vocab, a.ignore_index, unit, 0};
     if (const int rc = launch_op(xent_unit_kernel, 1, 1024, u, st, 0)) return rc;
     for (int first = 0; first < a.vocab; first += pl.words) {
@@ -711,14 +728,7 @@ extern "C" int dg_linear_xent_backward(const dg_linear_xent_args* args, void* st
             g.workspace_bytes = pl.partial_bytes;
         }
         if (const int rc = gemm_k_rows(&g, words, stream)) return rc;
-        if (const int rc = launch_weight(pl, a, x, words, st)) return rc;
+        if (const int rc = launch_weight(pl, a, x, words, cast, st)) return rc;
     }
-    CastParams c = {};
-    c.src = reinterpret_cast<const float*>(ws + pl.d_x);
-    c.unit = unit;
-    c.dst = reinterpret_cast<uint16_t*>(a.d_x);
-    c.ld = a.d_x_ld;
-    c.rows = a.tokens;
-    c.chunks = a.width / 8;
-    return launch_op(xent_cast_kernel, ceil_div64((int64_t)a.tokens * c.chunks, 256), 256, c, st, a.num_cus);
+    return DG_OK;
 }
