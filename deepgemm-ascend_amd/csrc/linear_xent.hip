@@ -34,7 +34,8 @@ struct XentParams {
     float* target_logit;       // [tokens]
     f32x2* stats;              // forward: [tile columns][tokens] (maximum, sum)
     const float *lse, *d_loss; // backward
-    const float* unit;         // backward: 1 / u and u, the unit of d
+    float* unit;               // backward: 1 / u and u, the unit of d
+    int own_unit;              // found by every tile itself (else ahead of them)
     uint16_t* d;               // backward: [rows][d_ld] bf16, whole tiles wide
     int64_t d_ld;
 };
@@ -44,6 +45,14 @@ __device__ __forceinline__ int target_of(const void* target, int wide, int64_t i
     const int64_t v = wide ? reinterpret_cast<const int64_t*>(target)[t] : reinterpret_cast<const int32_t*>(target)[t];
     return v == ignore || v < 0 || v >= vocab ? -1 : (int)v;
 }
+
+// u = the largest |d_loss| of a token with a target (1 where that, or its reciprocal, is no normal number), as (1 / u, u).
+__device__ __forceinline__ f32x2 unit_of(float top) {
+    return top >= 0x1p-100f && top <= 0x1p100f ? f32x2{1.f / top, top} : f32x2{1.f, 1.f};
+}
+
+// Tokens whose d_loss a tile's 256 threads take one each: past that a launch of one workgroup finds u.
+constexpr int kOwnUnit = 256;
 
 // Columns of a lane within its row of a tile: four runs of four to a 32-column block.
 __device__ __forceinline__ int run_col(int block_col, int q, int e) { return block_col + 4 * q + 8 * (e >> 2) + (e & 3); }
@@ -65,6 +74,8 @@ __device__ __forceinline__ void take_row(TAKE& take, COL& col_of, HA ha, I i, f3
 struct StatsTail {
     static constexpr bool kOn = true;
     XentParams x;
+
+    __device__ __forceinline__ void begin() {}
 
     template <typename T, typename TAKE, typename ROW, typename COL>
     __device__ __forceinline__ void run(TAKE& take, ROW& row_of, COL& col_of, const TileLoc& tl, uint8_t* smem) const {
@@ -149,15 +160,44 @@ __device__ __forceinline__ void runs_of_16(const i32x2 (&pk)[4], i32x4 (&w)[2]) 
 struct GradTail {
     static constexpr bool kOn = true;
     XentParams x;
+    float top;                 // own_unit: |d_loss| of this thread's token
+
+    // (loaded ahead of the tile's stages.  The backward pass with it and with the unit's own launch, us: 1 token, 4000 words of width
+    // 512 22.9 and 25.1, 90, 11000 of 704 34.5 and 36.9, 256, 1000 of 4096 52.4 and 54.5, 128, 131072 of 4096 906 and 909, but 16,
+    // 131072 of 4096 737 and 735.)
+    __device__ __forceinline__ void begin() {
+        const int t = threadIdx.x;
+        top = 0.f;
+        if (x.own_unit && t < x.tokens) {
+            const float g = fabsf(x.d_loss[t]);
+            top = target_of(x.target, x.wide, x.ignore, x.vocab, t) >= 0 ? fmaxf(g, 0.f) : 0.f;
+        }
+    }
+
+    __device__ __forceinline__ float own_unit(const TileLoc& tl, uint8_t* smem) const {
+        float* const part = reinterpret_cast<float*>(smem);
+        float all = top;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor(all, off, 64));
+        __syncthreads();                             // (every wave has read its last fragments)
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = all;
+        __syncthreads();
+        const f32x2 u = unit_of(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+        if (threadIdx.x == 0 && tl.m0 == 0 && tl.n0 == 0) {   // (for the kernels behind)
+            x.unit[0] = u[0];
+            x.unit[1] = u[1];
+        }
+        return u[0];
+    }
 
     template <typename T, typename TAKE, typename ROW, typename COL>
-    __device__ __forceinline__ void run(TAKE& take, ROW& row_of, COL& col_of, const TileLoc& tl, uint8_t*) const {
+    __device__ __forceinline__ void run(TAKE& take, ROW& row_of, COL& col_of, const TileLoc& tl, uint8_t* smem) const {
         using SA = typename T::SA;
         using SB = typename T::SB;
         constexpr int BN = SB::H0 + SB::H1, NB = SB::NB0 + SB::NB1;
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, r = lane & 31, q = lane >> 5;
         const int cols = x.vocab - x.first - tl.n0;
-        const float per_unit = x.unit[0];
+        const float per_unit = x.own_unit ? own_unit(tl, smem) : x.unit[0];
         static_for<2>([&](auto ha_c) {
             static_for<SA::nb(decltype(ha_c)::value)>([&](auto i_c) {
                 const int m = row_of(ha_c, i_c, wm, r);
@@ -247,7 +287,9 @@ struct WeightTail {
 
 template <int BM, int BN, typename TAIL>
 __global__ __launch_bounds__(256, (quad_occupancy<BM, BN, kBF16, false, false>())) void xent_tile_kernel(const KParams p, const XentParams x) {
-    quad_body<BM, BN, kBF16, kEpiBf16, kNormal, 1, 0, 0, 0, false, false, TAIL>(p, blockIdx.x + p.vbase, TAIL{x});
+    TAIL tail = {x};
+    tail.begin();
+    quad_body<BM, BN, kBF16, kEpiBf16, kNormal, 1, 0, 0, 0, false, false, TAIL>(p, blockIdx.x + p.vbase, tail);
 }
 
 template <int BM, int BN>
@@ -265,7 +307,7 @@ struct CastParams {
 };
 
 // d_x: the fp32 sums over the pieces as bf16, a chunk a thread (8192 x 4096: 31 us, 201 MB).  In the launch of few tokens' d_w it
-// saves its own: backward of 1 token, 4000 words of width 512 24.2 -> 22.6 us, 90, 11000 of 704 38.0 -> 36.4, 256, 1000 of 4096 56.5 -> 54.6.
+// saves its own: the backward pass of 1 token, 4000 words of width 512 1.6 us, of 90, 11000 of 704 1.6, of 256, 1000 of 4096 1.9.
 __device__ __forceinline__ void cast_chunks(const CastParams& p, int block) {
     const int64_t e = (int64_t)block * 256 + threadIdx.x;
     const int64_t row = e / p.chunks;
@@ -411,8 +453,7 @@ struct UnitParams {
     int vbase;
 };
 
-// u = the largest |d_loss| of a token with a target (1 where that, or its reciprocal, is no normal number).  One workgroup: 3 to 8
-// us up to 8192 tokens, next to at least a hundred of products.
+// u by one workgroup: 3 to 8 us up to 8192 tokens, next to at least a hundred of products.
 __global__ __launch_bounds__(1024) void xent_unit_kernel(const UnitParams p) {
     __shared__ float part[16];
     float top = 0.f;
@@ -424,9 +465,9 @@ __global__ __launch_bounds__(1024) void xent_unit_kernel(const UnitParams p) {
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
-    const bool usable = top >= 0x1p-100f && top <= 0x1p100f;
-    p.unit[0] = usable ? 1.f / top : 1.f;
-    p.unit[1] = usable ? top : 1.f;
+    const f32x2 u = unit_of(top);
+    p.unit[0] = u[0];
+    p.unit[1] = u[1];
 }
 
 struct JoinParams {
@@ -708,8 +749,10 @@ extern "C" int dg_linear_xent_backward(const dg_linear_xent_args* args, void* st
     x.unit = unit;
     const CastParams cast = {reinterpret_cast<const float*>(ws + pl.d_x), unit, reinterpret_cast<uint16_t*>(a.d_x), a.d_x_ld, a.tokens,
                              a.width / 8, 0};
+    x.own_unit = a.tokens <= kOwnUnit;
     const UnitParams u = {a.d_loss, a.target, x.wide, a.tokens, a.vocab, a.ignore_index, unit, 0};
-    if (const int rc = launch_op(xent_unit_kernel, 1, 1024, u, st, 0)) return rc;
+    if (!x.own_unit)
+        if (const int rc = launch_op(xent_unit_kernel, 1, 1024, u, st, 0)) return rc;
     for (int first = 0; first < a.vocab; first += pl.words) {
         const int words = std::min(pl.words, a.vocab - first);
         x.first = first;
