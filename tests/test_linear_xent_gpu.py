@@ -205,6 +205,36 @@ def test_pieces_of_the_vocabulary():
         assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize('t', [1, 40, 256, 257])
+def test_gradients_follow_the_weights_of_the_losses(t):
+    """d is held in units of the largest |d_loss|: a power of two times all of them is that times the gradients, to the last bit, and
+    an ignored token's d_loss has no part in it.  (Another sign is not: the matrix unit's sums round differently for it.)"""
+    x, w, target, d_loss = (a.cuda() for a in _inputs(t, 72, 1025, seed=3))
+    target[0] = 1024
+    lse = deep_gemm.linear_cross_entropy(x, w, target)[1]
+    want = deep_gemm.linear_cross_entropy_backward(d_loss, x, w, target, lse)
+    for times in (2.0 ** 20, 2.0 ** -20):
+        got = deep_gemm.linear_cross_entropy_backward(d_loss * times, x, w, target, lse)
+        for a, b in zip(got, want):
+            assert torch.equal(a.float(), b.float() * times)
+    for loud in (1e30, float('inf'), float('nan')):
+        got = deep_gemm.linear_cross_entropy_backward(torch.where(target < 0, loud, d_loss), x, w, target, lse)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    for d in deep_gemm.linear_cross_entropy_backward(torch.zeros_like(d_loss), x, w, target, lse):
+        assert (d == 0).all()
+
+
+@pytest.mark.parametrize('t', [5, 256, 257])
+def test_pieces_of_strided_words(t):
+    """Rows of w so far apart that 9000 of them are two pieces: d_x is complete, and rounded once, behind the second."""
+    x, w, target, d_loss = _inputs(t, 64, 9000, seed=4)
+    target[0], target[1] = 8999, 0
+    held = torch.empty((9000, 1 << 16), dtype=torch.bfloat16, device='cuda')[:, :64]
+    held.copy_(w)
+    _check(x, w, target, d_loss, (x.cuda(), held, target.cuda(), d_loss.cuda()))
+
+
 def test_gradient_against_differences():
     g = gen(9)
     t, h, v = 24, 64, 200
