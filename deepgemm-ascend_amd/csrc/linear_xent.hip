@@ -527,11 +527,21 @@ constexpr int kMaxTokens = 1 << 20;
 
 int64_t rows_of(int tokens) { return align_up64(tokens, 8); }
 
+// Whether d_w's tiles read x, MN-major, through one range of 32-bit offsets.  Where its rows span more, the tokens go in pieces
+// whose products are summed in fp32 (a range of 2^31 - 1 bytes would end inside x, and the tokens past it read as zeros).
+bool x_in_one_range(const dg_linear_xent_args& a) { return (int64_t)a.tokens * a.x_ld * 2 <= 0x7fffffffLL; }
+
+// Tokens of such a piece: below 1 GiB of x and of d, as dg_gemm takes MN-major operands; whole stages.
+int piece_tokens(const dg_linear_xent_args& a, int words) {
+    const int64_t row = 2 * std::max<int64_t>(a.x_ld, words);
+    return (int)std::min<int64_t>(0x3fffffffLL / row / 64 * 64, a.tokens);
+}
+
 // Words of a piece: whole tiles; d and the piece of w stay below 1 GiB each (they are read MN-major).
 int piece_words(const dg_linear_xent_args& a) {
-    // (and 256 rows of d below 2 GiB, a tile's)
-    const int64_t most = (int64_t(1) << 29) - 1;
-    const int64_t fit = std::min({most / rows_of(a.tokens), most / a.w_ld, int64_t(1) << 21}) / 256 * 256;
+    // (and 256 rows of d below 2 GiB, a tile's; d_w's fp32 sums below 1 GiB)
+    const int64_t most = (int64_t(1) << 29) - 1, sums = x_in_one_range(a) ? most : (int64_t(1) << 28) / a.width;
+    const int64_t fit = std::min({most / rows_of(a.tokens), most / a.w_ld, int64_t(1) << 21, sums}) / 256 * 256;
     const int64_t pieces = ceil_div64(a.vocab, std::max<int64_t>(256, fit));
     return (int)align_up64(ceil_div64(a.vocab, pieces), 256);
 }
@@ -549,7 +559,7 @@ struct Plan {
     int bm, bn;                // the logits' tile
     int words, pieces;
     int xbm, xbn, xsplit, wbm, wbn;
-    int64_t stats, logit, d, d_x, unit, partial, partial_bytes, bytes;
+    int64_t stats, logit, d, d_x, d_w, unit, partial, partial_bytes, bytes;
 };
 
 int cus_of(const dg_linear_xent_args& a) { return a.num_cus > 0 ? a.num_cus : device_cus(); }
@@ -570,6 +580,7 @@ Plan plan_of(const dg_linear_xent_args& a, bool backward) {
         bf16_tile_plan(a.tokens, std::min(p.words, a.vocab), a.width, false, false, 1, cus, p.bm, p.bn, one, none);
         p.d = s.take(rows_of(a.tokens) * p.words * 2);
         p.d_x = s.take((int64_t)a.tokens * a.width * 4);
+        p.d_w = s.take(x_in_one_range(a) ? 0 : (int64_t)p.words * a.width * 4);
         p.unit = s.take(8);
         bf16_tile_plan(a.tokens, a.width, p.words, true, false, 32, cus, p.xbm, p.xbn, p.xsplit, p.partial_bytes);
         bf16_tile_plan(std::min(p.words, a.vocab), a.width, a.tokens, true, false, 1, cus, p.wbm, p.wbn, one, none);
@@ -650,7 +661,8 @@ int64_t cast_blocks(const CastParams& c) { return ceil_div64((int64_t)c.rows * c
 
 // d_w rows of the piece = d^T x (both read MN-major): K rows past the tokens are not read.  Behind the last piece, d_x from
 // its sums: for few tokens in the same launch.
-int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, const CastParams& cast, hipStream_t st) {
+// `sums`: fp32 [words][width], used only where x spans more than one range.
+int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams& x, int words, float* sums, const CastParams& cast, hipStream_t st) {
     const bool last = x.first + words == a.vocab;
     if (a.tokens <= kShortTokens && (int64_t)(a.tokens + kShortK) * a.x_ld * 2 <= 0x7fffffffLL) {   // (32-bit offsets into x)
         ShortParams s = {};
@@ -664,12 +676,31 @@ int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams
         s.cast = cast;
         return launch_op(xent_weight_short_kernel, grid, 256, s, st, a.num_cus);
     }
+    uint16_t* const d_w = reinterpret_cast<uint16_t*>(a.d_w) + (int64_t)x.first * a.d_w_ld;
+    if (!x_in_one_range(a)) {
+        const int step = piece_tokens(a, pl.words);
+        for (int t = 0; t < a.tokens; t += step) {
+            const int tokens = std::min(step, a.tokens - t);
+            dg_gemm_args g = {};
+            g.kind = DG_KIND_BF16; g.gemm_type = DG_GEMM_NORMAL; g.num_groups = 1; g.alpha = 1.f; g.num_cus = a.num_cus;
+            g.a = x.d + (int64_t)t * x.d_ld; g.lda = x.d_ld; g.a_mn_major = 1;
+            g.b = reinterpret_cast<const uint16_t*>(a.x) + (int64_t)t * a.x_ld; g.ldb = a.x_ld; g.b_mn_major = 1;
+            g.d = sums; g.ldd = a.width; g.d_dtype = DG_DTYPE_F32;
+            g.accumulate = t > 0;
+            g.m = words; g.n = a.width; g.k = (int)align_up64(tokens, 8);
+            g.block_m = pl.wbm; g.block_n = pl.wbn; g.split_k = 1;
+            if (const int rc = gemm_k_rows(&g, tokens, reinterpret_cast<void*>(st))) return rc;
+        }
+        const CastParams rounded = {sums, x.unit, d_w, a.d_w_ld, words, a.width / 8, 0};
+        if (const int rc = launch_op(xent_cast_kernel, cast_blocks(rounded), 256, rounded, st, a.num_cus)) return rc;
+        return last ? launch_op(xent_cast_kernel, cast_blocks(cast), 256, cast, st, a.num_cus) : DG_OK;
+    }
     KParams p = tile_params();
     p.a = reinterpret_cast<const uint8_t*>(x.d);
     p.b = reinterpret_cast<const uint8_t*>(a.x);
     p.m = words; p.n = a.width; p.k = a.tokens;
     p.lda = x.d_ld * 2; p.ldb = a.x_ld * 2;
-    const WeightTail tail = {x, reinterpret_cast<uint16_t*>(a.d_w) + (int64_t)x.first * a.d_w_ld, a.d_w_ld, words, a.width};
+    const WeightTail tail = {x, d_w, a.d_w_ld, words, a.width};
     const int rc = launch_grid(p, words, a.width, pl.wbm, pl.wbn, a.num_cus, [&](dim3 grid) {
         if (pl.wbm == 256 && pl.wbn == 256) hipLaunchKernelGGL((xent_weight_kernel<256, 256>), grid, dim3(256), 0, st, p, tail);
         else if (pl.wbm == 256) hipLaunchKernelGGL((xent_weight_kernel<256, 128>), grid, dim3(256), 0, st, p, tail);
@@ -771,7 +802,7 @@ extern "C" int dg_linear_xent_backward(const dg_linear_xent_args* args, void* st
             g.workspace_bytes = pl.partial_bytes;
         }
         if (const int rc = gemm_k_rows(&g, words, stream)) return rc;
-        if (const int rc = launch_weight(pl, a, x, words, cast, st)) return rc;
+        if (const int rc = launch_weight(pl, a, x, words, reinterpret_cast<float*>(ws + pl.d_w), cast, st)) return rc;
     }
     return DG_OK;
 }

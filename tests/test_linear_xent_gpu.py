@@ -235,6 +235,40 @@ def test_pieces_of_strided_words(t):
     _check(x, w, target, d_loss, (x.cuda(), held, target.cuda(), d_loss.cuda()))
 
 
+@pytest.mark.parametrize('t', [1020, 1030, 1100, 2200])
+def test_gradient_of_rows_past_2_and_4_gib(t):
+    """Rows of x 2 MiB apart, 1024 of them to 2 GiB: every token takes part in d_w, and with its own row."""
+    x, w, target, d_loss = _inputs(t, 72, 300, seed=5)
+    target[-1], target[1024 % t] = 299, 7
+    held = torch.empty((t, 1 << 20), dtype=torch.bfloat16, device='cuda')[:, :72]
+    held.copy_(x)
+    _check(x, w, target, d_loss, (held, w.cuda(), target.cuda(), d_loss.cuda()))
+
+
+def test_gradient_of_the_most_tokens():
+    """2^20 whole rows of width 1032 (2.16 GB), against fp32 products on this device."""
+    t, h, v = 1 << 20, 1032, 40
+    x = torch.empty(t, h, dtype=torch.bfloat16, device='cuda').normal_()
+    w = torch.empty(v, h, dtype=torch.bfloat16, device='cuda').normal_().mul_(h ** -0.5)
+    target = torch.randint(0, v, (t,), generator=gen(6)).cuda()
+    d_loss = (torch.rand(t, generator=gen(7)) / t).cuda()
+    lse = deep_gemm.linear_cross_entropy(x, w, target)[1]
+    got_x, got_w = deep_gemm.linear_cross_entropy_backward(d_loss, x, w, target, lse)
+    ref_w = torch.zeros(v, h, dtype=torch.float64, device='cuda')
+    wf = w.float()
+    for i in range(0, t, 1 << 16):
+        part = slice(i, i + (1 << 16))
+        xf = x[part].float()
+        p = torch.softmax(xf @ wf.t(), dim=1)
+        p[torch.arange(1 << 16, device='cuda'), target[part]] -= 1
+        p *= d_loss[part].unsqueeze(1)
+        ref_w += (p.t().contiguous() @ xf).double()
+        ref_x = p @ wf
+        # (bf16 in d and in the result: each within 2^-8 of a value, 2^-8 / sqrt(3) at random)
+        assert (got_x[part].float() - ref_x).norm() < 2 * UBF16 / 3 ** 0.5 * ref_x.norm()
+    assert (got_w.double() - ref_w).norm() < 2 * UBF16 / 3 ** 0.5 * ref_w.norm()
+
+
 def test_gradient_against_differences():
     g = gen(9)
     t, h, v = 24, 64, 200

@@ -149,6 +149,17 @@ def test_linear_xent_refusals(lib):
     assert lib.dg_linear_xent_workspace_size(a, 0, ctypes.byref(need)) == 0 and need.value < 8192 * 131072 // 8
 
 
+@pytest.mark.parametrize('tokens,x_ld,pieces', [(262143, 4096, False), (262144, 4096, True), (1023, 1 << 20, False), (1100, 1 << 20, True)])
+def test_linear_xent_sums_pieces_of_tokens_past_2_gib(lib, tokens, x_ld, pieces):
+    """Where the rows of x span 2 GiB, the gradient's workspace holds fp32 sums of d_w besides d and d_x."""
+    need, small = ctypes.c_int64(), 64 * 1024
+    a = _lib.LinearXentArgs(tokens, 256, 512, 4096, 4096, x_ld, 256, 4096, 8)
+    a.num_cus = 8   # (no ranges of K)
+    assert lib.dg_linear_xent_workspace_size(a, 1, ctypes.byref(need)) == 0
+    rest = need.value - (tokens + 8) * 512 * 2 - tokens * 256 * 4
+    assert (rest > 512 * 256 * 4 - small) == pieces and rest < 512 * 256 * 4 + small
+
+
 def test_python_refusals():
     with pytest.raises(RuntimeError, match='int32 or int64'):
         deep_gemm.moe_sort(torch.zeros(2, 2), 4)
