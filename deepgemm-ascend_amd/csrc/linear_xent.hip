@@ -11,6 +11,8 @@
 // outputs beside it.  It is rounded in units of the largest |d_loss|, which both products multiply their fp32 sums by: with
 // the equal weights of a mean the targets' entries are then p - 1, nearly exact, where 1 / tokens rounded to 8 bits put the
 // same error of up to 0.4 % into all of them (777 tokens: gradients 0.25 % off against 0.17 % of the outputs' rounding alone).
+// With unequal weights d_x gets what rounding took from the target's entry (one row of w a token); d_w, whose sums run over
+// the tokens, would need it inside the product, and keeps that error.
 // Logits, maxima, sums, losses and the sum of d_x over the pieces are fp32.
 #include "op_launch.hpp"
 #include "quad_kernel.hpp"
@@ -36,6 +38,7 @@ struct XentParams {
     const float *lse, *d_loss; // backward
     float* unit;               // backward: 1 / u and u, the unit of d
     int own_unit;              // found by every tile itself (else ahead of them)
+    float* left;               // backward: [tokens] what rounding took from d at the target, in units of d
     uint16_t* d;               // backward: [rows][d_ld] bf16, whole tiles wide
     int64_t d_ld;
 };
@@ -214,8 +217,16 @@ struct GradTail {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) d[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[b][e], kLog2e, -lse));
                     if (some) {
+                        // (columns of the block that this lane holds: bit 2 of their number is the lane's half)
+                        const bool mine = (unsigned)(tc - col[b]) < 32u && (tc - col[b] >> 2 & 1) == q;
+                        float v = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) d[e] -= run_col(col[b], q, e) == tc ? 1.f : 0.f;
+                        for (int e = 0; e < 16; ++e) {
+                            const bool here = run_col(col[b], q, e) == tc;
+                            d[e] -= here ? 1.f : 0.f;
+                            v = here ? d[e] * g : v;
+                        }
+                        if (mine) x.left[m] = v - bf16_to_f32(f32_to_bf16_rne(v));   // (m has a target: a token's row)
                     }
                     if (cols < BN) {                 // (the last tile: columns past the vocabulary)
 #pragma unroll
@@ -304,9 +315,16 @@ struct CastParams {
     int64_t ld;
     int rows, chunks;          // eight values each
     int vbase;
+    const uint16_t* w;         // d_x: what rounding left of d at the targets times their words' rows (else nullptr)
+    int64_t w_ld;
+    const float* left;
+    const void* target;
+    int wide, vocab;
+    int64_t ignore;
 };
 
-// d_x: the fp32 sums over the pieces as bf16, a chunk a thread (8192 x 4096: 31 us, 201 MB).  In the launch of few tokens' d_w it
+// d_x: the fp32 sums over the pieces as bf16, a chunk a thread (8192 x 4096: 31 us, 201 MB).  The target's entry of d, most of
+// its row, is joined by what its rounding left, so that it counts in fp32 whatever the weights of the losses.  In the launch of few tokens' d_w it
 // saves its own: the backward pass of 1 token, 4000 words of width 512 1.6 us, of 90, 11000 of 704 1.6, of 256, 1000 of 4096 1.9.
 __device__ __forceinline__ void cast_chunks(const CastParams& p, int block) {
     const int64_t e = (int64_t)block * 256 + threadIdx.x;
@@ -315,7 +333,20 @@ __device__ __forceinline__ void cast_chunks(const CastParams& p, int block) {
     const int c = (int)(e - row * p.chunks) * 8;
     const float* const s = p.src + row * p.chunks * 8 + c;
     const float unit = p.unit[1];
-    const f32x4 a = *reinterpret_cast<const f32x4*>(s) * unit, b = *reinterpret_cast<const f32x4*>(s + 4) * unit;
+    f32x4 a = *reinterpret_cast<const f32x4*>(s), b = *reinterpret_cast<const f32x4*>(s + 4);
+    const int target = p.w != nullptr ? target_of(p.target, p.wide, p.ignore, p.vocab, (int)row) : -1;
+    if (target >= 0) {
+        const float left = p.left[row];
+        const i32x4 w = *reinterpret_cast<const i32x4*>(p.w + (int64_t)target * p.w_ld + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f32x4& v = i < 2 ? a : b;
+            v[2 * (i & 1)] += left * __builtin_bit_cast(float, (uint32_t)w[i] << 16);
+            v[2 * (i & 1) + 1] += left * __builtin_bit_cast(float, (uint32_t)w[i] & 0xffff0000u);
+        }
+    }
+    a *= unit;
+    b *= unit;
     *reinterpret_cast<i32x4*>(p.dst + row * p.ld + c) = i32x4{(int)pack_bf16x2(a[0], a[1]), (int)pack_bf16x2(a[2], a[3]),
                                                              (int)pack_bf16x2(b[0], b[1]), (int)pack_bf16x2(b[2], b[3])};
 }
@@ -559,7 +590,7 @@ struct Plan {
     int bm, bn;                // the logits' tile
     int words, pieces;
     int xbm, xbn, xsplit, wbm, wbn;
-    int64_t stats, logit, d, d_x, d_w, unit, partial, partial_bytes, bytes;
+    int64_t stats, logit, d, d_x, d_w, unit, left, partial, partial_bytes, bytes;
 };
 
 int cus_of(const dg_linear_xent_args& a) { return a.num_cus > 0 ? a.num_cus : device_cus(); }
@@ -582,6 +613,7 @@ Plan plan_of(const dg_linear_xent_args& a, bool backward) {
         p.d_x = s.take((int64_t)a.tokens * a.width * 4);
         p.d_w = s.take(x_in_one_range(a) ? 0 : (int64_t)p.words * a.width * 4);
         p.unit = s.take(8);
+        p.left = s.take((int64_t)a.tokens * 4);
         bf16_tile_plan(a.tokens, a.width, p.words, true, false, 32, cus, p.xbm, p.xbn, p.xsplit, p.partial_bytes);
         bf16_tile_plan(std::min(p.words, a.vocab), a.width, a.tokens, true, false, 1, cus, p.wbm, p.wbn, one, none);
         p.partial = s.take(p.partial_bytes);
@@ -691,7 +723,7 @@ int launch_weight(const Plan& pl, const dg_linear_xent_args& a, const XentParams
             g.block_m = pl.wbm; g.block_n = pl.wbn; g.split_k = 1;
             if (const int rc = gemm_k_rows(&g, tokens, reinterpret_cast<void*>(st))) return rc;
         }
-        const CastParams rounded = {sums, x.unit, d_w, a.d_w_ld, words, a.width / 8, 0};
+        const CastParams rounded = {sums, x.unit, d_w, a.d_w_ld, words, a.width / 8};
         if (const int rc = launch_op(xent_cast_kernel, cast_blocks(rounded), 256, rounded, st, a.num_cus)) return rc;
         return last ? launch_op(xent_cast_kernel, cast_blocks(cast), 256, cast, st, a.num_cus) : DG_OK;
     }
@@ -778,8 +810,10 @@ extern "C" int dg_linear_xent_backward(const dg_linear_xent_args* args, void* st
     x.d_ld = pl.words;
     float* const unit = reinterpret_cast<float*>(ws + pl.unit);
     x.unit = unit;
+    x.left = reinterpret_cast<float*>(ws + pl.left);
     const CastParams cast = {reinterpret_cast<const float*>(ws + pl.d_x), unit, reinterpret_cast<uint16_t*>(a.d_x), a.d_x_ld, a.tokens,
-                             a.width / 8, 0};
+                             a.width / 8, 0, reinterpret_cast<const uint16_t*>(a.w), a.w_ld, x.left, a.target, x.wide, a.vocab,
+                             a.ignore_index};
     x.own_unit = a.tokens <= kOwnUnit;
     const UnitParams u = {a.d_loss, a.target, x.wide, a.tokens, a.vocab, a.ignore_index, unit, 0};
     if (!x.own_unit)

@@ -269,6 +269,39 @@ def test_gradient_of_the_most_tokens():
     assert (got_w.double() - ref_w).norm() < 2 * UBF16 / 3 ** 0.5 * ref_w.norm()
 
 
+@pytest.mark.parametrize('t', [1, 5, 255, 257, 600])
+@pytest.mark.parametrize('v,ld', [(1000, 72), (9000, 1 << 16)])
+def test_targets_count_in_full_whatever_the_weights(t, v, ld):
+    """d_x where the words that are targets are 32 times as large as the others (in columns that x does not have, so that they are as
+    likely as any): the target's term is all but alone in its sum, and nothing but the result's rounding may be left of it."""
+    x, w, target, d_loss = _inputs(t, 72, v, seed=8)
+    x[:, 36:] = 0
+    words = torch.tensor([0, 3, 130, 255, 256, 511, v // 2, v - 1])
+    w[words, 36:] = torch.randn(8, 36, generator=gen(t)).bfloat16() * 32
+    target = torch.where(target >= 0, words[target % 8], target)
+    target[0] = v - 1
+    held = torch.empty((v, ld), dtype=torch.bfloat16, device='cuda')[:, :72]
+    held.copy_(w)
+    args = x.cuda(), held, target.cuda()
+    lse = deep_gemm.linear_cross_entropy(*args)[1]
+    got = deep_gemm.linear_cross_entropy_backward(d_loss.cuda(), *args, lse)[0].cpu().double()
+    d = ol.d_logits(x, w, target, d_loss)
+    _, want_lse, z = ol.forward(x, w, target)
+    live, at, u = target >= 0, torch.where(target >= 0, target, 0), UBF16   # (u: a rounding to bf16, eight bits)
+    e = _logit_error(x, w)
+    span = (z.amax(1) - z.amin(1)).unsqueeze(1)
+    lse_error = e.amax(1) + EXP + (4 + span.squeeze(1)) * U32 + v * U32 + 4 * U32 * (want_lse.abs() + z.abs().amax(1) + 1)
+    p = torch.exp(z - want_lse.unsqueeze(1)) * torch.where(live, d_loss.double(), 0.0).unsqueeze(1)
+    err = p * (e + lse_error.unsqueeze(1) + EXP + (4 + span) * U32) + 8 * U32 * d.abs()
+    rounded = u * d.abs() * (1 + u)
+    rounded[torch.arange(t), at] = 0
+    ref = d @ w.double()
+    # (products and sums in fp32, in pieces and ranges: as many additions as words)
+    bound = (err + rounded) @ w.double().abs() + (v + 16) * U32 * (d.abs() @ w.double().abs())
+    bound = bound * (1 + u) + u * ref.abs()
+    assert ((got - ref).abs() <= bound + 1e-40).all()
+
+
 def test_gradient_against_differences():
     g = gen(9)
     t, h, v = 24, 64, 200
