@@ -30,7 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct XentParams {
     const void* target;        // [tokens] int32 or int64
     int wide;
-    int tokens, rows;          // rows: tokens rounded up to whole K pieces of the gradient's product (zero rows)
+    int tokens;
     int first, vocab;          // first word of the piece, words in all
     int64_t ignore;
     float* target_logit;       // [tokens]
@@ -39,7 +39,7 @@ struct XentParams {
     float* unit;               // backward: 1 / u and u, the unit of d
     int own_unit;              // found by every tile itself (else ahead of them)
     float* left;               // backward: [tokens] what rounding took from d at the target, in units of d
-    uint16_t* d;               // backward: [rows][d_ld] bf16, whole tiles wide
+    uint16_t* d;               // backward: [tokens][d_ld] bf16, whole tiles wide
     int64_t d_ld;
 };
 
@@ -243,7 +243,7 @@ struct GradTail {
                     }
                     i32x4 w[2];
                     runs_of_16(pk, w);
-                    if (m < x.rows) {
+                    if (m < x.tokens) {
                         uint16_t* const d = x.d + (int64_t)m * x.d_ld + tl.n0 + col[b] + (q ? 0 : 16);
                         *reinterpret_cast<i32x4*>(d) = w[0];
                         *reinterpret_cast<i32x4*>(d + 8) = w[1];
@@ -556,8 +556,6 @@ __global__ __launch_bounds__(256) void xent_cast_kernel(const CastParams p) { ca
 // Tokens of one call: the gradient's product reads d MN-major, whose K rows (tokens) times a tile's words stay below 1 GiB.
 constexpr int kMaxTokens = 1 << 20;
 
-int64_t rows_of(int tokens) { return align_up64(tokens, 8); }
-
 // Whether d_w's tiles read x, MN-major, through one range of 32-bit offsets.  Where its rows span more, the tokens go in pieces
 // whose products are summed in fp32 (a range of 2^31 - 1 bytes would end inside x, and the tokens past it read as zeros).
 bool x_in_one_range(const dg_linear_xent_args& a) { return (int64_t)a.tokens * a.x_ld * 2 <= 0x7fffffffLL; }
@@ -572,7 +570,7 @@ int piece_tokens(const dg_linear_xent_args& a, int words) {
 int piece_words(const dg_linear_xent_args& a) {
     // (and 256 rows of d below 2 GiB, a tile's; d_w's fp32 sums below 1 GiB)
     const int64_t most = (int64_t(1) << 29) - 1, sums = x_in_one_range(a) ? most : (int64_t(1) << 28) / a.width;
-    const int64_t fit = std::min({most / rows_of(a.tokens), most / a.w_ld, int64_t(1) << 21, sums}) / 256 * 256;
+    const int64_t fit = std::min({most / a.tokens, most / a.w_ld, int64_t(1) << 21, sums}) / 256 * 256;
     const int64_t pieces = ceil_div64(a.vocab, std::max<int64_t>(256, fit));
     return (int)align_up64(ceil_div64(a.vocab, pieces), 256);
 }
@@ -609,7 +607,7 @@ Plan plan_of(const dg_linear_xent_args& a, bool backward) {
         p.words = piece_words(a);
         p.pieces = ceil_div(a.vocab, p.words);
         bf16_tile_plan(a.tokens, std::min(p.words, a.vocab), a.width, false, false, 1, cus, p.bm, p.bn, one, none);
-        p.d = s.take(rows_of(a.tokens) * p.words * 2);
+        p.d = s.take((int64_t)a.tokens * p.words * 2);
         p.d_x = s.take((int64_t)a.tokens * a.width * 4);
         p.d_w = s.take(x_in_one_range(a) ? 0 : (int64_t)p.words * a.width * 4);
         p.unit = s.take(8);
@@ -746,7 +744,6 @@ XentParams xent_params(const dg_linear_xent_args& a) {
     x.target = a.target;
     x.wide = a.target_bytes == 8;
     x.tokens = a.tokens;
-    x.rows = (int)rows_of(a.tokens);
     x.vocab = a.vocab;
     x.ignore = a.ignore_index;
     return x;

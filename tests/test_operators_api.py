@@ -156,8 +156,19 @@ def test_linear_xent_sums_pieces_of_tokens_past_2_gib(lib, tokens, x_ld, pieces)
     a = _lib.LinearXentArgs(tokens, 256, 512, 4096, 4096, x_ld, 256, 4096, 8)
     a.num_cus = 8   # (no ranges of K)
     assert lib.dg_linear_xent_workspace_size(a, 1, ctypes.byref(need)) == 0
-    rest = need.value - (tokens + 8) * 512 * 2 - tokens * 256 * 4
+    rest = need.value - (tokens + 8) * 512 * 2 - tokens * 256 * 4 - tokens * 4
     assert (rest > 512 * 256 * 4 - small) == pieces and rest < 512 * 256 * 4 + small
+
+
+@pytest.mark.parametrize('tokens', [1, 9, 1001])
+def test_linear_xent_holds_no_rows_past_the_tokens(lib, tokens):
+    """The gradient's workspace: d over the tokens, d_x's fp32 sums, the tokens' rests, and little else."""
+    need = ctypes.c_int64()
+    a = _lib.LinearXentArgs(tokens, 64, 1 << 17, 4096, 4096, 64, 64, 4096, 8)
+    a.num_cus = 1   # (no ranges of K)
+    assert lib.dg_linear_xent_workspace_size(a, 1, ctypes.byref(need)) == 0
+    least = tokens * (1 << 17) * 2 + tokens * 64 * 4 + tokens * 4
+    assert least <= need.value < least + 5 * 256
 
 
 def test_python_refusals():
