@@ -845,6 +845,7 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
         if (a.alignment < 32 || a.alignment % 32 != 0) return dg_set_error("dg_gemm: alignment must be a multiple of 32");
     }
 
+    if (a.split_k < 0) return dg_set_error("dg_gemm: split_k must be >= 0");
     const int cus = a.num_cus > 0 ? a.num_cus : device_cus();
     // Few rows to an expert, e2m1 on both sides: the weights' bytes are all (32 x 8 pairs over 32 experts, N = 2048 K = 4096:
     // 33 us against 56 on the 384-row tiles and 59 on 32-row ones).
@@ -852,7 +853,6 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
         if (compile_only && info == nullptr) return DG_OK;
         return mx_experts(a, cus_capped(cus) ? cus : 0, reinterpret_cast<hipStream_t>(stream), info);
     }
-    if (a.split_k < 0) return dg_set_error("dg_gemm: split_k must be >= 0");
     const bool lib_ws = a.workspace == nullptr && a.library_workspace != 0;
     Plan plan = choose(a, cus, a.workspace != nullptr || lib_ws);
     void* workspace = a.workspace;

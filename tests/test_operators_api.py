@@ -119,6 +119,24 @@ def test_few_rows_to_an_expert_plan(lib):
     assert plan(2080) != 4 and plan(1248, _lib.DG_KIND_FP8_FP8) != 4 and plan(1248, gemm_type=_lib.DG_GEMM_MGROUPED_IDX) != 4
 
 
+def _experts_args(m=1248, alignment=32):
+    """A grouped e2m1 x e2m1 call over 32 experts, N = 2048, K = 4096, in a psum layout of m rows."""
+    a = _lib.GemmArgs()
+    a.kind, a.gemm_type, a.m, a.n, a.k, a.num_groups, a.alignment, a.alpha = \
+        _lib.DG_KIND_FP4_FP4, _lib.DG_GEMM_MGROUPED_PSUM, m, 2048, 4096, 32, alignment, 1.0
+    a.lda = a.ldb = a.ldd = 2048
+    a.batch_stride_b, a.sfa_ld, a.sfb_ld, a.num_cus = 2048 * 2048, m, 2048, 256
+    return a
+
+
+@pytest.mark.parametrize('m', [1248, 4096])
+def test_few_rows_to_an_expert_refuse_a_negative_split(lib, m):
+    info, a = _lib.LaunchInfo(), _experts_args(m)
+    assert lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)) == 0
+    a.split_k = -1
+    _refused(lib, lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)), 'split_k')
+
+
 def test_linear_xent_refusals(lib):
     def run(fn='dg_linear_xent_forward', **kw):
         a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 40, 0)
