@@ -57,7 +57,7 @@ int m_indices_runs(const int32_t* idx, int m, int alignment, int32_t* runs, cons
 
 // csrc/mx_product.hip: M-grouped psum GEMMs of e2m1 rows, a few to an expert
 bool mx_experts_fit(const dg_gemm_args& a);
-int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* info);
+int mx_experts(const dg_gemm_args& a, hipStream_t st, dg_launch_info* info);
 
 KernelFn lookup_quad_fp8(int bm, int bn, int epi);
 KernelFn lookup_quad_fp8_mn_a(int bm, int bn, int epi);
@@ -848,10 +848,12 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
     if (a.split_k < 0) return dg_set_error("dg_gemm: split_k must be >= 0");
     const int cus = a.num_cus > 0 ? a.num_cus : device_cus();
     // Few rows to an expert, e2m1 on both sides: the weights' bytes are all (32 x 8 pairs over 32 experts, N = 2048 K = 4096:
-    // 33 us against 56 on the 384-row tiles and 59 on 32-row ones).
-    if (mx_experts_fit(a) && k_rows == 0) {
+    // 33 us against 56 on the 384-row tiles and 59 on 32-row ones).  Not under a CU cap, where its workgroups of one to four waves
+    // go out in many small launches (384-row tiles and it, us: 200 CUs 32 x 8 over 32, 2048x4096, 98 and 112, 128 x 8 102 and 241, 16 x 8
+    // over 64, 2048x512, 48 and 123; 64 CUs 255 and 296, 288 and 572, 123 and 328).
+    if (k_rows == 0 && !cus_capped(cus) && mx_experts_fit(a)) {
         if (compile_only && info == nullptr) return DG_OK;
-        return mx_experts(a, cus_capped(cus) ? cus : 0, reinterpret_cast<hipStream_t>(stream), info);
+        return mx_experts(a, reinterpret_cast<hipStream_t>(stream), info);
     }
     const bool lib_ws = a.workspace == nullptr && a.library_workspace != 0;
     Plan plan = choose(a, cus, a.workspace != nullptr || lib_ws);

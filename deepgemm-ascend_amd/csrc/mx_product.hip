@@ -389,7 +389,7 @@ bool mx_experts_fit(const dg_gemm_args& a) {
            span32(kStrip, a.ldb) && span32(ceil_div(a.k, 64), a.sfa_ld * 2) && span32(ceil_div(a.k, 64), a.sfb_ld * 2);
 }
 
-int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* info) {
+int mx_experts(const dg_gemm_args& a, hipStream_t st, dg_launch_info* info) {
     MxProductParams p = {};
     p.a = reinterpret_cast<const uint8_t*>(a.a); p.w = reinterpret_cast<const uint8_t*>(a.b); p.d = reinterpret_cast<uint8_t*>(a.d);
     p.sfa = reinterpret_cast<const uint16_t*>(a.sfa); p.sfw = reinterpret_cast<const uint16_t*>(a.sfb);
@@ -403,14 +403,13 @@ int mx_experts(const dg_gemm_args& a, int cus, hipStream_t st, dg_launch_info* i
         const int64_t strips = ceil_div(a.n, kStrip), grid = strips * (a.num_groups + a.m / 64);
         info->block_m = 64;
         info->block_n = kStrip;
-        info->plan_workgroups = info->tiles = grid;
-        info->grid = cus > 0 ? std::min<int64_t>(grid, cus) : grid;
+        info->plan_workgroups = info->tiles = info->grid = grid;
         info->threads = 64 * k_waves(strips * a.num_groups, a.k, true);
         info->split_k = 1;
         info->skinny = 4;
         return DG_OK;
     }
-    return launch_product<kCodes>(p, st, cus);
+    return launch_product<kCodes>(p, st, 0);
 }
 
 }  // namespace dg

@@ -137,6 +137,15 @@ def test_few_rows_to_an_expert_refuse_a_negative_split(lib, m):
     _refused(lib, lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)), 'split_k')
 
 
+@pytest.mark.parametrize('cus,own', [(256, True), (200, False), (64, False)])
+def test_few_rows_to_an_expert_under_a_cap_take_tiles(lib, cus, own):
+    """Workgroups of a wave or a few are no use of a capped number of them."""
+    info, a = _lib.LaunchInfo(), _experts_args()
+    a.num_cus = cus
+    assert lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)) == 0
+    assert (info.skinny == 4) == own and info.grid <= (1 << 31 if own else cus)
+
+
 def test_linear_xent_refusals(lib):
     def run(fn='dg_linear_xent_forward', **kw):
         a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 40, 0)
