@@ -559,7 +559,12 @@ Plan select_plan(const dg_gemm_args& a, int cus, bool allow_split) {
     // 128, 64 of them, N=K=2048 50 and 70.  (Behind: 64 x 8 over 64, N=1024 K=2048, alignment 128 (134) 38 and 34.)  Past one and
     // a half tiles: 256 x 8 over 32, N=4096 K=7168, alignment 64 (126) 266 and 254, 768 x 8, N=2048 K=4096, 64 (254) 104 and
     // 86, 128 (316) 95 and 90.
-    if (a.kind == kFP4FP4 && a.gemm_type == kMGroupedPsum && a.alignment % 256 != 0 && a.alignment % 64 == 0) {
+    // Weights that no cache holds bring the sides closer: 32 x 8 over 32, N=2048 K=4096, 64 66 and 65, 128 81 and 66, 128 x 8 67 and 94, 89
+    // and 95; and all of 1024 rows on one expert, which the host does not see, take 41 and 32, 55 and 34.  Under a CU cap 64x128
+    // stays ahead (200 CUs: 70 and 101, 92 and 101; 64 CUs: 194 and 258, 258 and 285), 128x128 does not (96 and 102, 126 and 102; 270
+    // and 261, 300 and 292).
+    if (a.kind == kFP4FP4 && a.gemm_type == kMGroupedPsum && a.alignment % 256 != 0 && a.alignment % 64 == 0 &&
+        (a.alignment % 128 != 0 || !cus_capped(cus))) {
         const int rows = a.alignment % 128 == 0 ? 128 : 64;
         if (2 * (int64_t)a.m <= 3 * (int64_t)rows * a.num_groups)
             for (const TileCfg& tc : kTiles)

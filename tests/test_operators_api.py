@@ -146,6 +146,16 @@ def test_few_rows_to_an_expert_under_a_cap_take_tiles(lib, cus, own):
     assert (info.skinny == 4) == own and info.grid <= (1 << 31 if own else cus)
 
 
+@pytest.mark.parametrize('alignment,cus,tile', [(64, 200, (64, 128)), (128, 256, (128, 128)), (128, 200, (384, 128)), (128, 64, (384, 128))])
+def test_fp4_psum_layouts_under_a_cap(lib, alignment, cus, tile):
+    """128x128 tiles, which several CUs share a group's weights by, gain nothing where few CUs may run."""
+    a = _experts_args(4224 if alignment == 128 else 2240, alignment)
+    a.num_cus = cus
+    block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.dg_select_config(ctypes.byref(a), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
+    assert (block_m.value, block_n.value) == tile
+
+
 def test_linear_xent_refusals(lib):
     def run(fn='dg_linear_xent_forward', **kw):
         a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 40, 0)
