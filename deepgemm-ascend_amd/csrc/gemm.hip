@@ -516,6 +516,10 @@ Plan quad_plan(const dg_gemm_args& a, int cus, bool allow_split) {
             q.share *= q.mn_stage;
             if (bf16 && quad) q.fixed += kQuadMnFixedBf16;
         }
+        // Batched and masked FP4 x FP4: where a group's rows end inside every tile (M below the tile's height), a stage loads that
+        // much less.  Masked, 128 rows, 256x256 and 128x128 tiles, us: 32 groups, N=4096 K=7168 136 and 188, 64 groups,
+        // N=K=2048 52 and 61; but 32 groups, N=2048 K=512, one round of either, 12.9 and 12.6.
+        if (fp4 && (a.gemm_type == kBatched || a.gemm_type == kMasked)) q.share *= (double)(std::min(a.m, q.bm) + q.bn) / (q.bm + q.bn);
         const bool capped = bf16 && cus_capped(cus), walks = capped && !mn && a.gemm_type != kKGrouped && tile_persistable(tc);
         const int64_t tiles = plan_tiles(a, tc), slots = (int64_t)cus * q.occ;
         for (int sp = 1; sp <= 8 && sp <= ns; ++sp) {

@@ -156,6 +156,17 @@ def test_fp4_psum_layouts_under_a_cap(lib, alignment, cus, tile):
     assert (block_m.value, block_n.value) == tile
 
 
+@pytest.mark.parametrize('groups,n,k', [(32, 4096, 7168), (64, 2048, 2048)])
+def test_fp4_masked_groups_of_fewer_rows_than_a_tile(lib, groups, n, k):
+    """128 rows a group: a half-filled large tile loads half the rows, and reads the weights once."""
+    a = _lib.GemmArgs()
+    a.kind, a.gemm_type, a.m, a.n, a.k, a.num_groups, a.alignment, a.num_cus = \
+        _lib.DG_KIND_FP4_FP4, _lib.DG_GEMM_MASKED, 128, n, k, groups, 256, 256
+    block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.dg_select_config(ctypes.byref(a), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
+    assert (block_m.value, block_n.value) == (256, 256)
+
+
 def test_linear_xent_refusals(lib):
     def run(fn='dg_linear_xent_forward', **kw):
         a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 40, 0)
