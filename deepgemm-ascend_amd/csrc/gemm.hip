@@ -477,6 +477,12 @@ constexpr double kCutRow = 1.2, kUnalignedRows = 3.5;
 // of one tile per allowed CU, 3 us apart (bf16 4096x7168x2048 on 200 CUs: 256x224 120 us, 256x256 131; the e4m3 rates
 // choose the persistent tiles where they are the faster ones without it: 512x2112x2048 on 64 CUs 15.3, with it 20.9).
 constexpr double kLaunchGap = 3.0;
+// FP4 x FP4 (dense, batched and masked) alike, fitted to 129 capped problems on 64, 128 and 200 CUs: a persistent kernel pays
+// its fixed part about four fifths, and launches lie less far apart.  With 256x256 tiles, which have no persistent kernel, and as
+// planned by this, us: 2048x7168x2048 on 64 CUs 78 and 70, 16 groups of 1024^3 on 200 32 and 28, 3000x3000x512 on 64
+// 39 and 26.  (A stage of the persistent 256x160 kernel takes longer than the other one's: 512x2112x7168 on 64 CUs 47, 256x128
+// 43; 8 groups of 129x2048x4096 on 200 35 and 31.)  Grouped layouts, most of whose tiles may be padding, are planned without.
+constexpr double kLaunchGapFp4 = 1.35, kWalkFixedFp4 = 0.8, kWalk160Fp4 = 1.3;
 
 double quad_time(const QuadRate& q, int64_t tiles, int stages, int cus) {
     const int64_t slots = (int64_t)cus * q.occ, full = tiles / slots, rest = tiles % slots;
@@ -520,16 +526,18 @@ Plan quad_plan(const dg_gemm_args& a, int cus, bool allow_split) {
         // much less.  Masked, 128 rows, 256x256 and 128x128 tiles, us: 32 groups, N=4096 K=7168 136 and 188, 64 groups,
         // N=K=2048 52 and 61; but 32 groups, N=2048 K=512, one round of either, 12.9 and 12.6.
         if (fp4 && (a.gemm_type == kBatched || a.gemm_type == kMasked)) q.share *= (double)(std::min(a.m, q.bm) + q.bn) / (q.bm + q.bn);
-        const bool capped = bf16 && cus_capped(cus), walks = capped && !mn && a.gemm_type != kKGrouped && tile_persistable(tc);
+        const bool capped = (bf16 || (fp4 && (dense || a.gemm_type == kMasked))) && cus_capped(cus), walks = capped && !mn && a.gemm_type != kKGrouped && tile_persistable(tc);
+        if (fp4 && capped && !walks) q.occ = 1;   // (a workgroup per allowed CU a launch)
+        if (fp4 && walks && q.bn == 160) q.light *= kWalk160Fp4;
         const int64_t tiles = plan_tiles(a, tc), slots = (int64_t)cus * q.occ;
         for (int sp = 1; sp <= 8 && sp <= ns; ++sp) {
             if (sp > 1 && (!allow_split || !quad || tiles * sp > slots || tiles > kMaxSplitTiles || ns < 4 * sp)) break;
             const int sps = ceil_div(ns, sp);
             if (ceil_div(ns, sps) != sp) continue;
             QuadRate r = q;
-            if (sp == 1 && walks) r.fixed *= 0.5;
+            if (sp == 1 && walks) r.fixed *= fp4 ? kWalkFixedFp4 : 0.5;
             double t = quad_time(r, tiles * sp, sps, cus);
-            if (sp == 1 && capped && !walks) t += kLaunchGap * (ceil_div64(tiles, cus) - 1);
+            if (sp == 1 && capped && !walks) t += (fp4 ? kLaunchGapFp4 : kLaunchGap) * (ceil_div64(tiles, cus) - 1);
             if (quad && cut) t += a.n % 4 == 0 ? kCutRow : kUnalignedRows;
             if (sp > 1) t += 3.5 + 8.0 * sp * a.m * (double)a.n * groups / 7e6;
             if (t < best * (sp > 1 ? 0.97 : 1.0)) {

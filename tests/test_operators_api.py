@@ -167,6 +167,17 @@ def test_fp4_masked_groups_of_fewer_rows_than_a_tile(lib, groups, n, k):
     assert (block_m.value, block_n.value) == (256, 256)
 
 
+@pytest.mark.parametrize('gemm_type,groups,m,n,k,cus', [(_lib.DG_GEMM_NORMAL, 1, 2048, 7168, 2048, 64), (_lib.DG_GEMM_NORMAL, 1, 3000, 3000, 512, 64),
+                                                        (_lib.DG_GEMM_BATCHED, 16, 1024, 1024, 1024, 200)])
+def test_fp4_products_under_a_cap_take_tiles_that_walk(lib, gemm_type, groups, m, n, k, cus):
+    """One launch of a persistent kernel in place of launch after launch of a tile per allowed CU."""
+    a = _lib.GemmArgs()
+    a.kind, a.gemm_type, a.m, a.n, a.k, a.num_groups, a.alignment, a.num_cus = _lib.DG_KIND_FP4_FP4, gemm_type, m, n, k, groups, 256, cus
+    block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.dg_select_config(ctypes.byref(a), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
+    assert (block_m.value, block_n.value) == (256, 224)
+
+
 def test_linear_xent_refusals(lib):
     def run(fn='dg_linear_xent_forward', **kw):
         a = _lib.LinearXentArgs(4, 64, 100, 4096, 4096, 64, 64, 4096, 8, -100, 4096, 4096, 4096, 4096, 4096, 64, 64, 4096, 1 << 40, 0)
