@@ -681,9 +681,23 @@ int elem_bytes_times2(int kind, bool is_a) {
 
 }  // namespace dg
 
+namespace {
+// Whether the kernel of few e2m1 rows to an expert serves a call.  Not under a CU cap, where its workgroups of one to four waves
+// go out in many small launches (384-row tiles and it, us: 200 CUs 32 x 8 over 32, 2048x4096, 98 and 112, 128 x 8 102 and 241, 16 x 8
+// over 64, 2048x512, 48 and 123; 64 CUs 255 and 296, 288 and 572, 123 and 328).
+bool few_rows_kernel(const dg_gemm_args& a, int cus) { return !dg::cus_capped(cus) && dg::mx_experts_fit(a); }
+}  // namespace
+
 extern "C" int dg_select_config(const dg_gemm_args* args, int32_t* block_m, int32_t* block_n) {
     if (args == nullptr) return dg_set_error("dg_select_config: null args");
     const int cus = args->num_cus > 0 ? args->num_cus : dg::device_cus();
+    if (few_rows_kernel(*args, cus)) {
+        dg_launch_info info = {};
+        (void)dg::mx_experts(*args, nullptr, &info);
+        if (block_m) *block_m = info.block_m;
+        if (block_n) *block_n = info.block_n;
+        return DG_OK;
+    }
     const dg::Plan pl = dg::choose(*args, cus, args->workspace != nullptr || args->library_workspace != 0 || args->split_k > 1);
     if (pl.tile.bm == 0) return dg_set_error("no tile shape fits this problem (M-grouped alignment must be a multiple of 32)");
     if (block_m) *block_m = pl.tile.bm;
@@ -865,10 +879,9 @@ int gemm_impl(const dg_gemm_args* args, void* stream, bool compile_only, dg_laun
     if (a.split_k < 0) return dg_set_error("dg_gemm: split_k must be >= 0");
     const int cus = a.num_cus > 0 ? a.num_cus : device_cus();
     // Few rows to an expert, e2m1 on both sides: the weights' bytes are all (32 x 8 pairs over 32 experts, N = 2048 K = 4096:
-    // 33 us against 56 on the 384-row tiles and 59 on 32-row ones).  Not under a CU cap, where its workgroups of one to four waves
-    // go out in many small launches (384-row tiles and it, us: 200 CUs 32 x 8 over 32, 2048x4096, 98 and 112, 128 x 8 102 and 241, 16 x 8
-    // over 64, 2048x512, 48 and 123; 64 CUs 255 and 296, 288 and 572, 123 and 328).
-    if (k_rows == 0 && !cus_capped(cus) && mx_experts_fit(a)) {
+    // 33 us against 56 on the 384-row tiles and 59 on 32-row ones; weights out of any cache 34 and 65, 128 x 8 54 and 93; but 1024
+    // rows that are all of one expert, which the host does not see, 47 and 29).
+    if (k_rows == 0 && few_rows_kernel(a, cus)) {
         if (compile_only && info == nullptr) return DG_OK;
         return mx_experts(a, reinterpret_cast<hipStream_t>(stream), info);
     }

@@ -737,6 +737,7 @@ def select_config(m: int, n: int, k: int, kind: int = _lib.DG_KIND_FP8_FP8, gemm
     args.kind, args.gemm_type, args.m, args.n, args.k, args.num_groups = kind, gemm_type, m, n, k, num_groups
     args.alignment = get_mk_alignment_for_contiguous_layout()
     args.num_cus = get_num_sms()
+    args.alpha = 1.0
     import ctypes
     bm, bn = ctypes.c_int32(), ctypes.c_int32()
     lib = _lib.load()

@@ -137,6 +137,17 @@ def test_few_rows_to_an_expert_refuse_a_negative_split(lib, m):
     _refused(lib, lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)), 'split_k')
 
 
+@pytest.mark.parametrize('m,alignment,cus', [(1248, 32, 256), (1248, 32, 200), (2048, 64, 256), (2240, 64, 256), (4224, 128, 256)])
+def test_select_config_names_the_tile_that_runs(lib, m, alignment, cus):
+    """Also where the kernel of few rows to an expert runs."""
+    info, a = _lib.LaunchInfo(), _experts_args(m, alignment)
+    a.num_cus = cus
+    block_m, block_n = ctypes.c_int32(), ctypes.c_int32()
+    assert lib.dg_launch_plan(ctypes.byref(a), ctypes.byref(info)) == 0
+    assert lib.dg_select_config(ctypes.byref(a), ctypes.byref(block_m), ctypes.byref(block_n)) == 0
+    assert (block_m.value, block_n.value) == (info.block_m, info.block_n)
+
+
 @pytest.mark.parametrize('cus,own', [(256, True), (200, False), (64, False)])
 def test_few_rows_to_an_expert_under_a_cap_take_tiles(lib, cus, own):
     """Workgroups of a wave or a few are no use of a capped number of them."""
