@@ -15,7 +15,8 @@ typedef unsigned int u32;
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;   // (1024 threads: 32768 x 8 pairs 20.7 us in place of 17.2)
 constexpr int kMaxGroups = 1024;
 // Up to kSortOnePass pairs every workgroup counts all of them itself (one launch); past that a first launch counts
-// blocks of pairs.
+// blocks of pairs, and past kSortMaxBlocks blocks, whose counts each workgroup would read for itself, another one sums them
+// (256 groups, 2^23 pairs 156 us in place of 185, 2^26 1.19 ms in place of 3.9).
 constexpr int kSortOnePass = 8192;
 constexpr int kSortMaxBlocks = 256;
 // Pairs of a block past that (32768 x 8 pairs over 256 groups: 18.7 us with 1024, 17.3 with 2048, 18.7 with 4096, 28 with 8192).
@@ -28,7 +29,8 @@ struct SortParams {
     int pairs, groups, alignment, rows;
     int per_block, blocks;     // pairs of a block, blocks
     int32_t *slots, *source, *indices, *psum;
-    int32_t* counts;           // [blocks][groups] (two launches) or nullptr
+    int32_t* counts;           // [blocks][groups] (two launches) or nullptr; summed: of the blocks before, and [groups] of all
+    int summed;
     u32* status;
     int vbase;
 };
@@ -49,6 +51,33 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortPara
     for (int i = first + tid; i < last; i += kSortThreads) atomicAdd(&hist[key_of(p, i)], 1);
     __syncthreads();
     for (int g = tid; g < p.groups; g += kSortThreads) p.counts[(int64_t)b * p.groups + g] = hist[g];
+}
+
+// Counts of many blocks -> counts of the blocks before, in place, and of all blocks behind them.  A lane takes a group, a wave a run of
+// blocks, twice: its sum, then its rows under what the waves before have.
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void sort_sum_kernel(const SortParams p) {
+    __shared__ int part[kSumThreads / 64][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = kSumThreads / 64;
+    const int g = (blockIdx.x + p.vbase) * 64 + lane, per = ceil_div(p.blocks, waves);
+    const int b0 = min(p.blocks, wave * per), b1 = min(p.blocks, b0 + per);
+    const bool on = g < p.groups;
+    int sum = 0;
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += on ? p.counts[(int64_t)b * p.groups + g] : 0;
+    part[wave][lane] = sum;
+    __syncthreads();
+    int next = 0;
+    for (int w = 0; w < wave; ++w) next += part[w][lane];
+    if (!on) return;
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+        int32_t* const c = p.counts + (int64_t)b * p.groups + g;
+        const int n = *c;
+        *c = next;
+        next += n;
+    }
+    if (wave == waves - 1) p.counts[(int64_t)p.blocks * p.groups + g] = next;
 }
 
 // Lanes of the wave with this lane's key (keys of `bits` bits).
@@ -77,7 +106,13 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
     for (int w = 0; w < kSortWaves; ++w)
         for (int g = tid; g <= G; g += kSortThreads) wave_next[w][g] = 0;
     __syncthreads();
-    if (p.counts != nullptr) {
+    if (p.summed) {
+        for (int g = tid; g < G; g += kSortThreads) {
+            total[g] = p.counts[(int64_t)p.blocks * G + g];
+            before[g] = p.counts[(int64_t)b * G + g];
+        }
+        for (int i = first + tid; i < last; i += kSortThreads) keys[i - first] = (uint16_t)key_of(p, i);
+    } else if (p.counts != nullptr) {
         // a part of the blocks each, so that the loads of all parts are in flight
         const int parts = max(1, kSortThreads / G), part = tid / G;
         if (G >= kSortThreads) {
@@ -499,7 +534,8 @@ int layout_ok(const dg_moe_layout* l, const char* who) {
 
 extern "C" int dg_moe_sort_workspace_size(int32_t num_pairs, int32_t num_groups, int64_t* bytes) {
     if (bytes == nullptr || num_pairs < 0 || num_groups < 1) return dg_set_error("dg_moe_sort: invalid size");
-    *bytes = num_pairs <= dg::kSortOnePass ? 0 : (int64_t)dg::sort_blocks(num_pairs, 0) * num_groups * 4;
+    const int64_t blocks = dg::sort_blocks(num_pairs, 0);
+    *bytes = num_pairs <= dg::kSortOnePass ? 0 : (blocks + (blocks > dg::kSortMaxBlocks ? 1 : 0)) * num_groups * 4;
     return DG_OK;
 }
 
@@ -531,8 +567,11 @@ extern "C" int dg_moe_sort(const void* ids, int32_t id_bytes, const dg_moe_layou
     p.slots = l->slots; p.source = l->source; p.indices = l->m_indices; p.psum = l->psum;
     p.counts = need > 0 ? reinterpret_cast<int32_t*>(workspace) : nullptr;
     p.status = status_words_for(st);
+    p.summed = need > 0 && p.blocks > kSortMaxBlocks;
     if (need > 0)
         if (const int rc = launch_op(sort_count_kernel, p.blocks, kSortThreads, p, st, num_cus)) return rc;
+    if (p.summed)
+        if (const int rc = launch_op(sort_sum_kernel, ceil_div(p.groups, 64), kSumThreads, p, st, num_cus)) return rc;
     return launch_op(sort_place_kernel, p.blocks, kSortThreads, p, st, num_cus);
 }
 

@@ -52,6 +52,47 @@ def test_sort(t, k, n, alignment, kind):
     _sort(ids, n, alignment)
 
 
+@pytest.mark.parametrize('t,k,n,alignment', [(400000, 8, 7, 64), (262145, 8, 1000, 32), (1500001, 3, 65, 128), (2800000, 6, 256, 128)])
+def test_sort_of_millions_of_pairs(t, k, n, alignment):
+    """More blocks of pairs than each workgroup reads the counts of (2^21 pairs), against a stable sort; a third is dropped."""
+    ids = torch.randint(-n // 2, n, (t, k), generator=gen(t)).to(torch.int32)
+    ids[t // 2:t // 2 + 9000] = n - 1
+    deep_gemm.set_mk_alignment_for_contiguous_layout(alignment)
+    layout = deep_gemm.moe_sort(ids.cuda(), n)
+    key = torch.where(ids < 0, n, ids).reshape(-1)
+    counts = torch.bincount(key, minlength=n + 1)[:n]
+    padded = (counts + alignment - 1) // alignment * alignment
+    start = torch.cumsum(padded, 0) - padded
+    order = torch.sort(key, stable=True).indices[:int(counts.sum())]
+    group = key[order].long()
+    row = start[group] + torch.arange(len(order)) - (torch.cumsum(counts, 0) - counts)[group]
+    slots = torch.full((t * k,), -1, dtype=torch.int32)
+    slots[order] = row.int()
+    source = torch.full((layout.source.numel(),), -1, dtype=torch.int32)
+    m_indices = source.clone()
+    source[row], m_indices[row] = order.int(), group.int()
+    for got, ref in zip(layout, (slots.view(t, k), source, (start + counts).int(), m_indices)):
+        assert torch.equal(got.cpu(), ref)
+
+
+def test_sort_takes_time_in_proportion():
+    """2^26 pairs are eight times as many as 2^23: where every workgroup reads every block's counts they take 64 times as long."""
+    times = []
+    for t in (1 << 20, 1 << 23):
+        ids = torch.randint(0, 256, (t, 8), device='cuda', dtype=torch.int32)
+        best = float('inf')
+        for _ in range(4):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            deep_gemm.moe_sort(ids, 256)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        times.append(best)
+    print('2^23 and 2^26 pairs:', times)
+    assert times[1] < 16 * times[0]
+
+
 def test_sort_reports_ids_past_the_last_group():
     ids = torch.tensor([[0, 5], [3, -7], [2, 1]], dtype=torch.int32)
     _sort(ids, 4, 32)

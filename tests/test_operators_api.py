@@ -42,6 +42,14 @@ def test_sort_refusals(lib):
     _refused(lib, lib.dg_moe_sort_workspace_size(-1, 4, ctypes.byref(need)), 'invalid size')
 
 
+@pytest.mark.parametrize('pairs,rows_of_counts', [(8192, 0), (8193, 5), (1 << 21, 256), ((1 << 21) + 1, 258), (1 << 26, 8193)])
+def test_sort_workspace(lib, pairs, rows_of_counts):
+    """Counts of every block and, past 256 blocks, their sums."""
+    need = ctypes.c_int64()
+    assert lib.dg_moe_sort_workspace_size(pairs, 300, ctypes.byref(need)) == 0
+    assert need.value == rows_of_counts * 300 * 4
+
+
 def test_movement_refusals(lib):
     d = lambda layout=None, src=4096, sld=64, rb=64, dst=4096, dld=64, sf=None, sfo=None, oload=64: lib.dg_moe_dispatch(
         src, sld, rb, layout or _layout(), dst, dld, sf, 2, 1, sfo, oload, 1, 0, None)
