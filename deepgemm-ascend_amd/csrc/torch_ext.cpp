@@ -450,7 +450,8 @@ Tensors mx_dequantize(const at::Tensor& codes, const at::Tensor& sf, bool f32, i
         return {};
     const int64_t m = codes.size(0), k = codes.size(1) * (fp4 ? 2 : 1), k64 = ceil_div(k, 64);
     if (k % 32 != 0 || m > kMaxExtent || k > kMaxExtent || sf.scalar_type() != at::kShort || sf.dim() != 2 ||
-        sf.size(0) != m || sf.size(1) != k64 || sf.device() != codes.device() || !(m <= 1 || sf.stride(0) == 1))
+        sf.size(0) != m || sf.size(1) != k64 || sf.device() != codes.device() || !(m <= 1 || sf.stride(0) == 1) ||
+        (reinterpret_cast<uintptr_t>(sf.data_ptr()) & 3) || (k64 > 1 && (sf.stride(1) % 2 || sf.stride(1) < m)))
         return {};
     raise_pending();
     Tensors out = {at::empty({m, k}, codes.options().dtype(f32 ? at::kFloat : at::kBFloat16))};

@@ -81,9 +81,12 @@ def mx_dequantize(q: Tuple[torch.Tensor, torch.Tensor], dtype: torch.dtype = tor
     _assert(k % 32 == 0, f'K must be a multiple of the block of 32 values, got {k}')
     _assert(sf.dtype == torch.int16 and sf.shape == (*codes.shape[:-1], _ceil_div(k, 64)), 'sf must be int16 [.., M, ceil(K / 64)]')
     _assert(m <= 1 or sf.stride(-2) == 1, 'sf must be in the required layout (rows contiguous)')
-    if codes.size(-1) > 1 and (codes.stride(-1) != 1 or codes.stride(-2) % 8 or codes.data_ptr() % 8 or
+    # (copies whose rows lie as the kernel reads them, also of tensors that are contiguous but start anywhere)
+    if codes.size(-1) > 1 and (codes.stride(-1) != 1 or any(s % 8 for s in codes.stride()[:-1]) or codes.data_ptr() % 8 or
                                (m > 1 and codes.stride(-2) < codes.size(-1))):
-        codes = codes.contiguous()
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    if sf.data_ptr() % 4 or (sf.size(-1) > 1 and (sf.stride(-1) % 2 or sf.stride(-1) < m)) or (sf.dim() == 3 and sf.stride(0) % 2):
+        sf = torch.empty((*sf.shape[:-2], sf.size(-1), _align(m, 2)), dtype=torch.int16, device=sf.device)[..., :m].transpose(-1, -2).copy_(sf)
     out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=codes.device)
     _run('dg_mx_dequantize', out, codes, sf, fmt)
     return out

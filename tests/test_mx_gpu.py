@@ -52,6 +52,28 @@ def test_quantize_many_rows(fmt):
 
 
 @pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
+@pytest.mark.parametrize('out', [torch.bfloat16, torch.float32])
+def test_dequantize_rows_that_start_anywhere(fmt, out):
+    """Rows from an odd one on, single rows, scale factors of other strides and codes at an odd address give what the whole gives."""
+    x = torch.randn(2, 21, 160, generator=gen(6)).cuda()
+    codes, sf = deep_gemm.mx_quantize(x, fmt)
+    whole = deep_gemm.mx_dequantize((codes, sf), out)
+    for rows in (slice(1, 21), slice(3, 4), slice(20, 21), slice(2, 9)):
+        assert torch.equal(deep_gemm.mx_dequantize((codes[1, rows], sf[1, rows]), out), whole[1, rows])
+        assert torch.equal(deep_gemm.mx_dequantize((codes[:, rows], sf[:, rows]), out), whole[:, rows])
+    assert torch.equal(deep_gemm.mx_dequantize((codes[0, 5:6], sf[0, 5:6].contiguous()), out), whole[0, 5:6])
+    for held in (codes, codes[0]):
+        at = torch.empty(held.numel() + 1, dtype=torch.uint8, device='cuda')[1:].view(held.dtype).view(held.shape)
+        at.copy_(held)
+        assert at.is_contiguous() and at.data_ptr() % 8
+        assert torch.equal(deep_gemm.mx_dequantize((at, sf if held is codes else sf[0]), out), whole if held is codes else whole[0])
+    odd = torch.empty(2, 3, 23, dtype=torch.int16, device='cuda')[:, :, 1:22].transpose(1, 2)   # (rows 23 apart)
+    odd.copy_(sf)
+    assert torch.equal(deep_gemm.mx_dequantize((codes, odd), out), whole)
+    assert torch.equal(deep_gemm.mx_dequantize((codes[0], odd[0]), out), whole[0])
+
+
+@pytest.mark.parametrize('fmt', ['e2m1', 'e4m3'])
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 def test_edges(fmt, dtype):
     """Ties, block maxima on either side of the format's largest value, zeros of both signs, numbers near the ends of the
