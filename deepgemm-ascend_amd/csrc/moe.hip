@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(const DispatchPar
         u32 pair = 0;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const int s = r + x < p.rows ? p.source[r + x] : -1, t = s < 0 ? p.tokens : s / p.topk;
+            const int s = r + x < p.rows ? p.source[r + x] : -1, t = s < 0 || p.topk == 0 ? p.tokens : s / p.topk;
             if (t < p.tokens) pair |= (u32)(uint16_t)in[t] << (16 * x);
         }
         *reinterpret_cast<u32*>(p.sf_out + (int64_t)j * p.sf_out_ld + r) = pair;   // (an even leading dimension)
@@ -585,7 +585,7 @@ extern "C" int dg_moe_dispatch(const void* src, int64_t src_ld, int64_t row_byte
     if (sf != nullptr && (k64 < 0 || sf_ld < l->tokens || sf_out_ld < l->rows || sf_out_ld % 2 != 0 || sf_out == nullptr || !aligned_to(sf_out, 4)))
         return dg_set_error("dg_moe_dispatch: scale factors are [k64][ld], ld at least the rows and (out) even");
     if (l->rows == 0 || row_bytes == 0) return DG_OK;
-    if (dst == nullptr || l->source == nullptr || (l->tokens > 0 && (src == nullptr || l->slots == nullptr)))
+    if (dst == nullptr || l->source == nullptr || (l->tokens > 0 && (src == nullptr || (l->topk > 0 && l->slots == nullptr))))
         return dg_set_error("dg_moe_dispatch: null tensor");
     const int v = row_bytes >= 16 ? 16 : 1;
     if (row_bytes > 0x7fffffffLL) return dg_set_error("dg_moe_dispatch: row too long");

@@ -163,6 +163,23 @@ def test_dispatch_moves_scale_factors(t, k64):
     assert out.size(0) <= 1 or (out.stride(0) == 1 and out.stride(1) % 2 == 0)
 
 
+def test_layouts_of_no_choices():
+    """No row has a token: rows are padding, also where a layout's sources name pairs all the same."""
+    full = lambda *shape, v=0: torch.full(shape, v, dtype=torch.int32, device='cuda')
+    layout = deep_gemm.MoELayout(full(4, 0), full(64, v=3), full(2), full(64))
+    x, sf = torch.ones(4, 64, dtype=torch.int8, device='cuda'), full(2, 4, v=5).to(torch.int16).t()
+    rows, out = deep_gemm.moe_dispatch((x, sf), layout)
+    assert rows.shape == (64, 64) and out.shape == (64, 2) and (out == 0).all()
+    deep_gemm.set_mk_alignment_for_contiguous_layout(32)
+    layout = deep_gemm.moe_sort(full(4, 0), 2, num_rows=64)
+    for a in deep_gemm.moe_dispatch((x, sf), layout):
+        assert a.size(0) == 64 and (a == 0).all()
+    rows = torch.ones(64, 32, device='cuda')
+    assert (deep_gemm.moe_combine(rows, layout) == 0).all()
+    d_rows, d_weights = deep_gemm.moe_combine_backward(rows[:4], rows, layout, torch.ones(4, 0, device='cuda'))
+    assert (d_rows == 0).all() and d_weights.shape == (4, 0)
+
+
 def _close(got, ref, mag, n, dtype):
     """A sum of n products in fp32, in order, then rounded to dtype."""
     err = (got.double() - ref).abs()
