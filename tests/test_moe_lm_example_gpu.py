@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import deep_gemm
+from oracle import mx as ox
 
 pytestmark = pytest.mark.gpu
 
@@ -51,6 +52,35 @@ def test_training_step(tokens, alignment):
     assert abs(float(loss) - float(ref)) < 0.02
     for got, want in zip((*grads, d_x), (*ref_grads, ref_x)):
         assert (got.float() - want).norm() < 10 * 2.0 ** -8 / 3 ** 0.5 * want.norm()
+
+
+def _quantised(x):
+    """fp32 values of x after the oracle's e2m1 quantisation."""
+    flat = x.reshape(-1, x.size(-1)).cpu()
+    return ox.values(*ox.quantize(flat, 'e2m1'), 'e2m1').float().view(x.shape).to(x.device)
+
+
+@pytest.mark.parametrize('tokens,alignment', [(1, 32), (8, 32), (40, 32), (9, 64), (40, 256)])
+def test_decoding_step(tokens, alignment):
+    """The logits of the 4-bit step against fp32 products of dequantised weights and activations, token by token and expert by expert,
+    rounded to bf16 where the step holds bf16."""
+    deep_gemm.set_mk_alignment_for_contiguous_layout(alignment)
+    block = ex.Block(hidden=256, inner=128, experts=8, topk=3, vocab=1500)
+    g = torch.Generator(device='cuda')
+    g.manual_seed(4)
+    x = torch.randn(tokens, 256, generator=g, device='cuda').bfloat16()
+    got = ex.decode_step(ex.Quantised(block), x)
+    up, down, head = (_quantised(w) for w in (block.up, block.down, block.head))
+    ids, weights, _ = ex.route(block, x)
+    xq, out = _quantised(x), torch.zeros(tokens, 256, device='cuda')
+    for t in range(tokens):
+        for c in range(block.topk):
+            e = int(ids[t, c])
+            h = (xq[t:t + 1] @ up[e].t()).bfloat16()
+            out[t] += weights[t, c] * (_quantised(ex.swiglu(h)) @ down[e].t()).bfloat16().float()[0]
+    want = _quantised(x + out.bfloat16()) @ head.t()
+    # (what is left are sums in another order, and the few values that another last bit takes to the next 4-bit code)
+    assert (got - want).norm() < 10 * 2.0 ** -8 / 3 ** 0.5 * want.norm()
 
 
 def test_training_lowers_the_loss_and_decoding_follows():
