@@ -323,7 +323,7 @@ struct CastParams {
     int64_t ignore;
 };
 
-// d_x: the fp32 sums over the pieces as bf16, a chunk a thread (8192 x 4096: 31 us, 201 MB).  The target's entry of d, most of
+// d_x: the fp32 sums over the pieces as bf16, a chunk a thread (8192 x 4096: 43 us, 268 MB).  The target's entry of d, most of
 // its row, is joined by what its rounding left, so that it counts in fp32 whatever the weights of the losses.  In the launch of few tokens' d_w it
 // saves its own: the backward pass of 1 token, 4000 words of width 512 1.6 us, of 90, 11000 of 704 1.6, of 256, 1000 of 4096 1.9.
 __device__ __forceinline__ void cast_chunks(const CastParams& p, int block) {
@@ -359,6 +359,7 @@ __device__ __forceinline__ void cast_chunks(const CastParams& p, int block) {
 // tiles, us: 16 tokens, 131072 words of width 4096 757 and 799, 50257 of 1024 73 and 87, 100000 of 512 82 and 97, 32000 of 2048 85 and
 // 97; 128 tokens 930 and 937, 100 and 114, 117 and 131, 107 and 119; 200 tokens, 50257 of 1024 124 and 141; 300 tokens 1365 and
 // 1340, 170 and 189, 188 and 205, 182 and 189; 512 tokens 1665 and 1575, 209 and 220, 271 and 278, 221 and 223; 777 tokens 2581 and 2410.
+// The limit is where the widest d_w turns: past it, to about 500 tokens, narrow ones give up 1 to 10 % that the short tiles would still gain.
 constexpr int kShortTile = 128, kShortK = 32, kShortTokens = 256;
 
 struct ShortParams {
@@ -560,7 +561,8 @@ constexpr int kMaxTokens = 1 << 20;
 // whose products are summed in fp32 (a range of 2^31 - 1 bytes would end inside x, and the tokens past it read as zeros).
 bool x_in_one_range(const dg_linear_xent_args& a) { return (int64_t)a.tokens * a.x_ld * 2 <= 0x7fffffffLL; }
 
-// Tokens of such a piece: below 1 GiB of x and of d, as dg_gemm takes MN-major operands; whole stages.
+// Tokens of such a piece: below 1 GiB of x and of d, as dg_gemm takes MN-major operands; whole stages.  (The backward pass of width 4096
+// and 32000 words: 262143 tokens, the most in one range, 186 ms, 262144 in three pieces 194.)
 int piece_tokens(const dg_linear_xent_args& a, int words) {
     const int64_t row = 2 * std::max<int64_t>(a.x_ld, words);
     return (int)std::min<int64_t>(0x3fffffffLL / row / 64 * 64, a.tokens);

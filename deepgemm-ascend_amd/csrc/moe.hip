@@ -14,7 +14,8 @@ typedef unsigned int u32;
 // ------------------------------------------------------------------------------------------------ sorting
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;   // (1024 threads: 32768 x 8 pairs 20.7 us in place of 17.2)
 constexpr int kMaxGroups = 1024;
-// Up to kSortOnePass pairs every workgroup counts all of them itself (one launch); past that a first launch counts
+// Up to kSortOnePass pairs every workgroup counts all of them itself (one launch; us, and with a counting launch: 4096 pairs over 64
+// groups 6.0 and 9.5, 6126 over 40 7.5 and 9.3, 8000 over 256 8.0 and 11.2, 8192 over 8 7.7 and 9.1); past that a first launch counts
 // blocks of pairs, and past kSortMaxBlocks blocks, whose counts each workgroup would read for itself, another one sums them
 // (256 groups, 2^23 pairs 156 us in place of 185, 2^26 1.19 ms in place of 3.9).
 constexpr int kSortOnePass = 8192;

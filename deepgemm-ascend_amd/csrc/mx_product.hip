@@ -5,12 +5,14 @@
 // 16 bytes of one block of 32 codes of one row, so a wave's load is 16 rows x 64 bytes as they lie in memory, no two lanes
 // need the same bytes, and neither LDS nor a barrier stands between memory and the matrix unit.  A wave owns 32 rows of w and
 // a range of K, two to eight steps of 128 ahead in registers; the waves of a workgroup that share rows join their sums in LDS, in
-// order.  The few rows of a come the same way (from the caches).  One row of 4096 values against 7168: 6 to 7 us, a launch and a
-// wave's two dependent rounds of loads where the 15.6 MB alone would take 3.  32 x 8 pairs over 32 experts, N = 2048 K = 4096: 30 to
+// order.  The few rows of a come the same way (from the caches).  One row of 4096 values against 7168: 6 to 7 us where the 15.6 MB
+// alone would take 3, a launch whose steps wait for each other: one round of loads (a wave's four steps of w and behind them x, which
+// is there when all of them are), the quantisation, a barrier, the products and the join of eight waves' sums.  32 x 8 pairs over 32 experts, N = 2048 K = 4096: 30 to
 // 33 us (143 MB: 4.3 to 4.8 TB/s).
 //
 // The rows of a are e2m1 codes (an M-grouped layout: each expert's rows with its weights), or a few rows of bf16 / fp32 values
-// that every workgroup quantises into LDS, a block of 32 a thread, while its first weights are on their way.
+// that every workgroup quantises into LDS, a block of 32 a thread, once its first weights have arrived too (loads return in order, and
+// the values are asked for last).
 #include "gemm_kernel.hpp"
 #include "op_launch.hpp"
 #include "mx_scale.hpp"

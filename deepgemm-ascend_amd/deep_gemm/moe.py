@@ -7,7 +7,8 @@ A mixture-of-experts layer runs between two of these calls:
     m_grouped_bf16_gemm_nt_contiguous(rows, w, y, layout.psum)
     out = moe_combine(y, layout, topk_weights)                # [T, N] weighted sums of a token's rows
 
-and its gradient between ``moe_combine_backward`` and ``moe_dispatch_backward``.  Nothing synchronises with the host: the
+and its gradient between ``moe_combine_backward`` and ``moe_dispatch_backward``.  No autograd graph is recorded: results of inputs
+that require gradients have none, and a program chains the backward calls itself.  Nothing synchronises with the host: the
 number of rows M is a bound over every routing (``moe_num_rows``), and the rows past the last group are padding.
 """
 import ctypes

@@ -2,7 +2,7 @@
 of activations quantised on the way.
 
 ``mx_quantize`` returns what the GEMMs take as an operand with recipe (1, 32): codes (e4m3, or e2m1 packed two to an int8
-byte) and UE8M0 scale factors in the required layout.
+byte) and UE8M0 scale factors in the required layout.  No autograd graph is recorded.
 """
 from typing import Optional, Tuple
 
