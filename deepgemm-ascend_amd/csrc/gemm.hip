@@ -686,7 +686,7 @@ namespace {
 // Whether the kernel of few e2m1 rows to an expert serves a call.  Not under a CU cap, where its workgroups of one to four waves
 // go out in many small launches (384-row tiles and it, us: 200 CUs 32 x 8 over 32, 2048x4096, 98 and 112, 128 x 8 102 and 241, 16 x 8
 // over 64, 2048x512, 48 and 123; 64 CUs 255 and 296, 288 and 572, 123 and 328).
-bool few_rows_kernel(const dg_gemm_args& a, int cus) { return !dg::cus_capped(cus) && dg::mx_experts_fit(a); }
+bool few_rows_kernel(const dg_gemm_args& a, int cus) { return dg::mx_experts_fit(a) && !dg::cus_capped(cus); }
 }  // namespace
 
 extern "C" int dg_select_config(const dg_gemm_args* args, int32_t* block_m, int32_t* block_n) {
