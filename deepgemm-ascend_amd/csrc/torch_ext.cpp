@@ -70,7 +70,7 @@ std::string error_message(uint32_t bits) {
                "id < num_groups followed only by -1 padding)";
     }
     const std::pair<uint32_t, const char*> others[] = {
-        {DG_ERR_EXPERT_ID, "topk_idx holds an expert id >= num_groups"},
+        {DG_ERR_EXPERT_ID, "topk_idx holds an expert id >= num_groups, or a layout a group past the last adapter"},
         {DG_ERR_MOE_ROWS, "the pairs of topk_idx need more rows than num_rows"},
         {DG_ERR_TARGET, "target holds an index outside the vocabulary"},
     };
@@ -571,6 +571,342 @@ Tensors linear_xent_backward(const at::Tensor& d_loss, const at::Tensor& x, cons
     return out;
 }
 
+// ------------------------------------------------------------------------------------------------ what stands between the products
+// The same calls as deep_gemm/moe.py (routing), norm.py, activation.py and lora.py make.
+decltype(&dg_moe_route) g_route = nullptr;
+decltype(&dg_moe_route_backward) g_route_backward = nullptr;
+decltype(&dg_rms_norm_workspace_size) g_norm_workspace_size = nullptr;
+decltype(&dg_rms_norm_forward) g_norm = nullptr;
+decltype(&dg_rms_norm_backward) g_norm_backward = nullptr;
+decltype(&dg_swiglu_forward) g_swiglu = nullptr;
+decltype(&dg_swiglu_backward) g_swiglu_backward = nullptr;
+decltype(&dg_lora_workspace_size) g_lora_workspace_size = nullptr;
+decltype(&dg_lora_gemm) g_lora = nullptr;
+
+void init_blocks(int64_t route, int64_t route_backward, int64_t norm_workspace, int64_t norm, int64_t norm_backward, int64_t swiglu,
+                 int64_t swiglu_backward, int64_t lora_workspace, int64_t lora) {
+    g_route = reinterpret_cast<decltype(g_route)>(route);
+    g_route_backward = reinterpret_cast<decltype(g_route_backward)>(route_backward);
+    g_norm_workspace_size = reinterpret_cast<decltype(g_norm_workspace_size)>(norm_workspace);
+    g_norm = reinterpret_cast<decltype(g_norm)>(norm);
+    g_norm_backward = reinterpret_cast<decltype(g_norm_backward)>(norm_backward);
+    g_swiglu = reinterpret_cast<decltype(g_swiglu)>(swiglu);
+    g_swiglu_backward = reinterpret_cast<decltype(g_swiglu_backward)>(swiglu_backward);
+    g_lora_workspace_size = reinterpret_cast<decltype(g_lora_workspace_size)>(lora_workspace);
+    g_lora = reinterpret_cast<decltype(g_lora)>(lora);
+}
+
+// A plain matrix of `rows` x `cols` bf16 or fp32 values on `device` (negative sizes: any).
+bool matrix(const at::Tensor& t, int64_t rows, int64_t cols, const at::Device& device) {
+    return t.dim() == 2 && t.is_cuda() && t.device() == device && rows_dtype(t) >= 0 && (rows < 0 || t.size(0) == rows) &&
+           (cols < 0 || t.size(1) == cols) && plain(t) && t.size(0) <= kMaxExtent && t.size(1) <= kMaxExtent;
+}
+
+// A contiguous tensor of `dtype` on `device`.
+bool dense(const at::Tensor& t, at::ScalarType dtype, at::IntArrayRef sizes, const at::Device& device) {
+    return t.scalar_type() == dtype && t.sizes() == sizes && t.is_contiguous() && t.device() == device;
+}
+
+int64_t row_ld(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// Codes of `rows` x `k` values and their scale factors, to be written.
+struct Codes {
+    at::Tensor codes, sf;
+    int64_t ld;
+};
+Codes new_codes(const at::Tensor& like, bool fp4, int64_t rows, int64_t k) {
+    const int64_t ld = align_up(rows, 2);
+    return {at::empty({rows, fp4 ? k / 2 : k}, like.options().dtype(fp4 ? at::kChar : at::kFloat8_e4m3fn)),
+            at::empty({ceil_div(k, 64) * ld}, like.options().dtype(at::kShort)), ld};
+}
+
+bool route_args(const at::Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale, int64_t num_cus, dg_moe_route_args& a) {
+    if (g_route == nullptr || !logits.is_cuda() || !matrix(logits, -1, -1, logits.device()) || logits.numel() == 0 || logits.size(1) > 1024 || topk < 1 ||
+        topk > 16 || topk > logits.size(1))
+        return false;
+    a = {};
+    a.tokens = (int32_t)logits.size(0);
+    a.experts = (int32_t)logits.size(1);
+    a.topk = (int32_t)topk;
+    a.scores = sigmoid ? DG_SCORES_SIGMOID : DG_SCORES_SOFTMAX;
+    a.renormalize = renormalize;
+    a.scale = (float)scale;
+    a.dtype = rows_dtype(logits);
+    a.logits = logits.data_ptr();
+    a.logits_ld = row_ld(logits);
+    a.num_cus = (int32_t)num_cus;
+    return true;
+}
+
+Tensors moe_route(const at::Tensor& logits, int64_t topk, bool sigmoid, const c10::optional<at::Tensor>& bias, int64_t num_groups, int64_t topk_groups,
+                  int64_t group_top, bool renormalize, double scale, int64_t num_cus, int64_t stream) {
+    dg_moe_route_args a;
+    if (!route_args(logits, topk, sigmoid, renormalize, scale, num_cus, a) || num_groups < 1 || logits.size(1) % num_groups != 0 || topk_groups < 1 ||
+        topk_groups > num_groups || topk > topk_groups * (logits.size(1) / num_groups) || group_top < 1 || group_top > 2 ||
+        (bias.has_value() && !dense(*bias, at::kFloat, {logits.size(1)}, logits.device())))
+        return {};
+    raise_pending();
+    const c10::DeviceGuard guard(logits.device());
+    Tensors out = {at::empty({logits.size(0), topk}, logits.options().dtype(at::kInt)), at::empty({logits.size(0), topk}, logits.options().dtype(at::kFloat))};
+    a.num_groups = (int32_t)num_groups;
+    a.topk_groups = (int32_t)topk_groups;
+    a.group_top = (int32_t)group_top;
+    a.bias = bias.has_value() ? bias->data_ptr<float>() : nullptr;
+    a.ids = out[0].data_ptr<int32_t>();
+    a.weights = out[1].data_ptr<float>();
+    check_rc(g_route(&a, stream_ptr(stream)));
+    return out;
+}
+
+Tensors moe_route_backward(const at::Tensor& d_weights, const at::Tensor& logits, const at::Tensor& ids, bool sigmoid, bool renormalize, double scale,
+                           int64_t num_cus, int64_t stream) {
+    dg_moe_route_args a;
+    if (ids.dim() != 2 || !route_args(logits, ids.size(1), sigmoid, renormalize, scale, num_cus, a) ||
+        !dense(ids, at::kInt, {logits.size(0), ids.size(1)}, logits.device()) || !dense(d_weights, at::kFloat, ids.sizes(), logits.device()))
+        return {};
+    raise_pending();
+    const c10::DeviceGuard guard(logits.device());
+    Tensors out = {at::empty(logits.sizes(), logits.options())};
+    a.ids = ids.data_ptr<int32_t>();
+    a.d_weights = d_weights.data_ptr<float>();
+    a.d_logits = out[0].data_ptr();
+    a.d_logits_ld = logits.size(1);
+    check_rc(g_route_backward(&a, stream_ptr(stream)));
+    return out;
+}
+
+bool norm_args(const at::Tensor& x, const at::Tensor& weight, double eps, int64_t num_cus, dg_rms_norm_args& a) {
+    if (g_norm == nullptr || !x.is_cuda() || !matrix(x, -1, -1, x.device()) || x.numel() == 0 || x.size(1) > 32768 || rows_dtype(weight) < 0 ||
+        !dense(weight, weight.scalar_type(), {x.size(1)}, x.device()))
+        return false;
+    a = {};
+    a.tokens = (int32_t)x.size(0);
+    a.width = (int32_t)x.size(1);
+    a.dtype = rows_dtype(x);
+    a.weight_dtype = rows_dtype(weight);
+    a.eps = (float)eps;
+    a.format = -1;
+    a.weight = weight.data_ptr();
+    a.num_cus = (int32_t)num_cus;
+    return true;
+}
+
+// y (or codes and scale factors), rstd and, with a residual, h.  format: -1 values, DG_MX_*.
+Tensors rms_norm(const at::Tensor& x, const at::Tensor& weight, const c10::optional<at::Tensor>& residual, double eps, int64_t format, int64_t num_cus,
+                 int64_t stream) {
+    dg_rms_norm_args a;
+    if (!norm_args(x, weight, eps, num_cus, a) || (format != -1 && x.size(1) % 32 != 0) ||
+        (residual.has_value() && (!matrix(*residual, x.size(0), x.size(1), x.device()) || residual->scalar_type() != x.scalar_type())))
+        return {};
+    raise_pending();
+    const c10::DeviceGuard guard(x.device());
+    a.x = x.data_ptr();
+    a.x_ld = row_ld(x);
+    Tensors out;
+    int64_t ld = 0;
+    if (format == -1) {
+        out.push_back(at::empty(x.sizes(), x.options()));
+        a.y_ld = x.size(1);
+    } else {
+        Codes c = new_codes(x, format == DG_MX_E2M1, x.size(0), x.size(1));
+        a.format = (int32_t)format;
+        a.y_ld = c.codes.size(1);
+        a.sf = static_cast<int16_t*>(c.sf.data_ptr());
+        a.sf_ld = ld = c.ld;
+        out = {std::move(c.codes), std::move(c.sf)};
+    }
+    a.y = out[0].data_ptr();
+    out.push_back(at::empty({x.size(0)}, x.options().dtype(at::kFloat)));
+    a.rstd = out.back().data_ptr<float>();
+    if (residual.has_value()) {
+        out.push_back(at::empty(x.sizes(), x.options()));
+        a.residual = residual->data_ptr();
+        a.residual_ld = row_ld(*residual);
+        a.h = out.back().data_ptr();
+        a.h_ld = x.size(1);
+    }
+    check_rc(g_norm(&a, stream_ptr(stream)));
+    if (format != -1) out[1] = scale_view(std::move(out[1]), x.size(0), ceil_div(x.size(1), 64), ld);
+    return out;
+}
+
+Tensors rms_norm_backward(const at::Tensor& d_y, const at::Tensor& h, const at::Tensor& weight, const at::Tensor& rstd,
+                          const c10::optional<at::Tensor>& d_h, int64_t num_cus, int64_t stream) {
+    dg_rms_norm_args a;
+    if (!norm_args(h, weight, 0, num_cus, a) || !matrix(d_y, h.size(0), h.size(1), h.device()) || d_y.scalar_type() != h.scalar_type() ||
+        !dense(rstd, at::kFloat, {h.size(0)}, h.device()) ||
+        (d_h.has_value() && (!matrix(*d_h, h.size(0), h.size(1), h.device()) || d_h->scalar_type() != h.scalar_type())))
+        return {};
+    raise_pending();
+    const c10::DeviceGuard guard(h.device());
+    int64_t need = 0;
+    check_rc(g_norm_workspace_size(&a, &need));
+    Tensors out = {at::empty(h.sizes(), h.options()), at::empty({h.size(1)}, rstd.options())};
+    const at::Tensor ws = at::empty({need}, h.options().dtype(at::kByte));
+    a.h = h.data_ptr();
+    a.h_ld = row_ld(h);
+    a.rstd = rstd.data_ptr<float>();
+    a.d_y = d_y.data_ptr();
+    a.d_y_ld = row_ld(d_y);
+    if (d_h.has_value()) {
+        a.d_h = d_h->data_ptr();
+        a.d_h_ld = row_ld(*d_h);
+    }
+    a.d_x = out[0].data_ptr();
+    a.d_x_ld = h.size(1);
+    a.d_weight = out[1].data_ptr<float>();
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = need;
+    check_rc(g_norm_backward(&a, stream_ptr(stream)));
+    return out;
+}
+
+bool gate_args(int64_t rows, int64_t width, const at::Tensor& values, const c10::optional<at::Tensor>& m_indices, bool zero_padding, int64_t num_cus,
+               dg_swiglu_args& a) {
+    if (g_swiglu == nullptr || rows == 0 || width == 0 || (m_indices.has_value() && !dense(*m_indices, at::kInt, {rows}, values.device()))) return false;
+    a = {};
+    a.rows = (int32_t)rows;
+    a.width = (int32_t)width;
+    a.dtype = rows_dtype(values);
+    a.format = -1;
+    a.m_indices = m_indices.has_value() ? m_indices->data_ptr<int32_t>() : nullptr;
+    a.zero_padding = zero_padding;
+    a.num_cus = (int32_t)num_cus;
+    return true;
+}
+
+// act (or codes and scale factors) and, with `checkpoint`, h's codes and scale factors.
+Tensors swiglu(const at::Tensor& h, int64_t format, bool checkpoint, const c10::optional<at::Tensor>& m_indices, bool zero_padding, int64_t num_cus,
+               int64_t stream) {
+    dg_swiglu_args a;
+    if (!h.is_cuda() || !matrix(h, -1, -1, h.device()) || h.size(1) % 2 != 0) return {};
+    const int64_t rows = h.size(0), f = h.size(1) / 2;
+    if (!gate_args(rows, f, h, m_indices, zero_padding, num_cus, a) || ((format != -1 || checkpoint) && f % 32 != 0)) return {};
+    raise_pending();
+    const c10::DeviceGuard guard(h.device());
+    a.h = h.data_ptr();
+    a.h_ld = row_ld(h);
+    Tensors out;
+    if (format == -1) {
+        out.push_back(at::empty({rows, f}, h.options()));
+        a.act_ld = f;
+    } else {
+        Codes c = new_codes(h, format == DG_MX_E2M1, rows, f);
+        a.format = (int32_t)format;
+        a.act_ld = c.codes.size(1);
+        a.act_sf = static_cast<int16_t*>(c.sf.data_ptr());
+        a.act_sf_ld = c.ld;
+        out = {std::move(c.codes), std::move(c.sf)};
+    }
+    a.act = out[0].data_ptr();
+    if (checkpoint) {
+        Codes c = new_codes(h, false, rows, 2 * f);
+        a.saved = c.codes.data_ptr();
+        a.saved_ld = 2 * f;
+        a.saved_sf = static_cast<int16_t*>(c.sf.data_ptr());
+        a.saved_sf_ld = c.ld;
+        out.push_back(std::move(c.codes));
+        out.push_back(std::move(c.sf));
+    }
+    check_rc(g_swiglu(&a, stream_ptr(stream)));
+    const int64_t ld = align_up(rows, 2);
+    if (format != -1) out[1] = scale_view(std::move(out[1]), rows, ceil_div(f, 64), ld);
+    if (checkpoint) out.back() = scale_view(std::move(out.back()), rows, f / 32, ld);
+    return out;
+}
+
+Tensors swiglu_backward(const at::Tensor& d_act, const at::Tensor& saved, const c10::optional<at::Tensor>& sf, bool with_act,
+                        const c10::optional<at::Tensor>& m_indices, bool zero_padding, int64_t num_cus, int64_t stream) {
+    dg_swiglu_args a;
+    if (!d_act.is_cuda() || !matrix(d_act, -1, -1, d_act.device())) return {};
+    const int64_t rows = d_act.size(0), f = d_act.size(1);
+    if (!gate_args(rows, f, d_act, m_indices, zero_padding, num_cus, a)) return {};
+    if (sf.has_value()) {
+        if (f % 32 != 0 || saved.scalar_type() != at::kFloat8_e4m3fn || saved.dim() != 2 || saved.size(0) != rows || saved.size(1) != 2 * f ||
+            saved.device() != d_act.device() || !plain(saved) || row_ld(saved) % 8 != 0 || (reinterpret_cast<uintptr_t>(saved.data_ptr()) & 7) != 0)
+            return {};
+        const int64_t k64 = f / 32, ld = k64 > 1 ? sf->stride(1) : align_up(rows, 2);
+        if (sf->scalar_type() != at::kShort || sf->dim() != 2 || sf->size(0) != rows || sf->size(1) != k64 || sf->device() != d_act.device() ||
+            !(rows <= 1 || sf->stride(0) == 1) || ld % 2 != 0 || ld < rows || (reinterpret_cast<uintptr_t>(sf->data_ptr()) & 3) != 0)
+            return {};
+        a.saved = saved.data_ptr();
+        a.saved_ld = row_ld(saved);
+        a.saved_sf = static_cast<int16_t*>(sf->data_ptr());
+        a.saved_sf_ld = ld;
+    } else {
+        if (!matrix(saved, rows, 2 * f, d_act.device()) || saved.scalar_type() != d_act.scalar_type()) return {};
+        a.h = saved.data_ptr();
+        a.h_ld = row_ld(saved);
+    }
+    raise_pending();
+    const c10::DeviceGuard guard(d_act.device());
+    Tensors out = {at::empty({rows, 2 * f}, d_act.options())};
+    a.d_act = d_act.data_ptr();
+    a.d_act_ld = row_ld(d_act);
+    a.d_h = out[0].data_ptr();
+    a.d_h_ld = 2 * f;
+    if (with_act) {
+        out.push_back(at::empty({rows, f}, d_act.options()));
+        a.act = out[1].data_ptr();
+        a.act_ld = f;
+    }
+    check_rc(g_swiglu_backward(&a, stream_ptr(stream)));
+    return out;
+}
+
+bool aligned_rows(const at::Tensor& t) {
+    if (t.scalar_type() != at::kBFloat16 || t.stride(-1) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0) return false;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) % 8 != 0) return false;
+    return t.size(-2) <= 1 || t.stride(-2) >= t.size(-1);
+}
+
+// false: the general path
+bool lora_gemm(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const at::Tensor& d, const Tensors& layout,
+               const c10::optional<at::Tensor>& scales, const c10::optional<at::Tensor>& c, int64_t num_cus, int64_t stream) {
+    dg_moe_layout l;
+    if (g_lora == nullptr || !x.is_cuda() || x.dim() != 2 || a.dim() != 3 || b.dim() != 3 || x.numel() == 0 || a.numel() == 0 || b.numel() == 0 ||
+        !layout_of(layout, x.device(), l) || l.tokens != x.size(0) || l.topk != 1 || l.rows % 32 != 0 || !aligned_rows(x) || !aligned_rows(a) ||
+        !aligned_rows(b) || a.device() != x.device() || b.device() != x.device() || a.size(0) != b.size(0) || a.size(2) != x.size(1) ||
+        b.size(2) != a.size(1) || a.size(1) % 8 != 0 || a.size(1) > 256 || x.size(1) % 8 != 0 || x.size(0) > kMaxExtent || x.size(1) > kMaxExtent ||
+        a.size(0) > kMaxExtent || b.size(1) > kMaxExtent || !matrix(d, x.size(0), b.size(1), x.device()) ||
+        (scales.has_value() && !dense(*scales, at::kFloat, {a.size(0)}, x.device())) ||
+        (c.has_value() && (!matrix(*c, x.size(0), b.size(1), x.device()) || c->scalar_type() != d.scalar_type() ||
+                           (c->data_ptr() == d.data_ptr() && row_ld(*c) != row_ld(d)))))
+        return false;
+    raise_pending();
+    const c10::DeviceGuard guard(x.device());
+    dg_lora_args p = {};
+    p.tokens = (int32_t)x.size(0);
+    p.adapters = (int32_t)a.size(0);
+    p.rank = (int32_t)a.size(1);
+    p.n = (int32_t)b.size(1);
+    p.k = (int32_t)x.size(1);
+    p.x = x.data_ptr();
+    p.a = a.data_ptr();
+    p.b = b.data_ptr();
+    p.x_ld = row_ld(x);
+    p.a_ld = a.size(1) > 1 ? a.stride(1) : p.k;
+    p.a_stride = a.size(0) > 1 ? a.stride(0) : 0;
+    p.b_ld = b.size(1) > 1 ? b.stride(1) : p.rank;
+    p.b_stride = b.size(0) > 1 ? b.stride(0) : 0;
+    p.scales = scales.has_value() ? scales->data_ptr<float>() : nullptr;
+    p.c = c.has_value() ? c->data_ptr() : nullptr;
+    p.c_ld = c.has_value() ? row_ld(*c) : 0;
+    p.d = d.data_ptr();
+    p.d_ld = row_ld(d);
+    p.d_dtype = rows_dtype(d);
+    p.layout = &l;
+    p.num_cus = (int32_t)num_cus;
+    int64_t need = 0;
+    check_rc(g_lora_workspace_size(&p, &need));
+    const at::Tensor ws = at::empty({need}, x.options().dtype(at::kByte));
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = need;
+    check_rc(g_lora(&p, stream_ptr(stream)));
+    return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -586,5 +922,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("mx_gemm", &mx_gemm, "product of rows quantised on the way; false: the general path must handle the call");
     m.def("linear_xent", &linear_xent, "loss and log sums of a linear cross entropy");
     m.def("linear_xent_backward", &linear_xent_backward, "gradients of x and the weight");
+    m.def("init_blocks", &init_blocks, "hand over the entry points of what stands between the products");
+    m.def("moe_route", &moe_route, "experts and weights of the tokens");
+    m.def("moe_route_backward", &moe_route_backward, "gradient of the logits");
+    m.def("rms_norm", &rms_norm, "normalised rows (or codes and scale factors), rstd and the sum with the residual");
+    m.def("rms_norm_backward", &rms_norm_backward, "gradients of the rows and the weight");
+    m.def("swiglu", &swiglu, "gated activation (or codes and scale factors) and the input's 8-bit checkpoint");
+    m.def("swiglu_backward", &swiglu_backward, "gradient of the gated activation's input, and the activation again");
+    m.def("lora_gemm", &lora_gemm, "adapters of many requests; false: the general path must handle the call");
     m.def("gemm", &gemm, "validate and launch one GEMM; false: the general path must handle the call");
 }

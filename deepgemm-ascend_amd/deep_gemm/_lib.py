@@ -26,11 +26,14 @@ EXPORTED_SYMBOLS = ('dg_gemm', 'dg_transform_sf', 'dg_transform_k_grouped_sf', '
                     'dg_jit_stats', 'dg_launch_plan', 'dg_gemm_noalloc', 'dg_take_errors', 'dg_error_words',
                     'dg_stream_workspace', 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine',
                     'dg_moe_combine_backward', 'dg_mx_quantize', 'dg_mx_dequantize', 'dg_mx_gemm', 'dg_linear_xent_workspace_size',
-                    'dg_linear_xent_forward', 'dg_linear_xent_backward')
+                    'dg_linear_xent_forward', 'dg_linear_xent_backward', 'dg_moe_route', 'dg_moe_route_backward',
+                    'dg_rms_norm_workspace_size', 'dg_rms_norm_forward', 'dg_rms_norm_backward', 'dg_swiglu_forward',
+                    'dg_swiglu_backward', 'dg_lora_workspace_size', 'dg_lora_gemm')
 
 # Sticky error bits kernels report through host-mapped words (DG_ERR_* in the header)
 DG_ERR_SF_INVALID, DG_ERR_M_INDICES, DG_ERR_EXPERT_ID, DG_ERR_MOE_ROWS, DG_ERR_TARGET = 1, 2, 4, 8, 16
 DG_MX_E2M1, DG_MX_E4M3 = 0, 1
+DG_SCORES_SOFTMAX, DG_SCORES_SIGMOID = 0, 1
 DG_ENOKERNEL = -3   # dg_gemm: no compiled kernel for the requested configuration
 
 
@@ -94,6 +97,55 @@ class LinearXentArgs(ctypes.Structure):
         ('loss', ctypes.c_void_p), ('lse', ctypes.c_void_p), ('d_loss', ctypes.c_void_p),
         ('d_x', ctypes.c_void_p), ('d_w', ctypes.c_void_p), ('d_x_ld', ctypes.c_int64), ('d_w_ld', ctypes.c_int64),
         ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64), ('num_cus', ctypes.c_int32),
+    ]
+
+
+class MoERouteArgs(ctypes.Structure):
+    """Mirror of ``dg_moe_route_args`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('tokens', ctypes.c_int32), ('experts', ctypes.c_int32), ('topk', ctypes.c_int32), ('scores', ctypes.c_int32),
+        ('num_groups', ctypes.c_int32), ('topk_groups', ctypes.c_int32), ('group_top', ctypes.c_int32),
+        ('renormalize', ctypes.c_int32), ('scale', ctypes.c_float), ('dtype', ctypes.c_int32),
+        ('logits', ctypes.c_void_p), ('logits_ld', ctypes.c_int64), ('bias', ctypes.c_void_p), ('ids', ctypes.c_void_p),
+        ('weights', ctypes.c_void_p), ('d_weights', ctypes.c_void_p), ('d_logits', ctypes.c_void_p), ('d_logits_ld', ctypes.c_int64),
+        ('num_cus', ctypes.c_int32),
+    ]
+
+
+class RmsNormArgs(ctypes.Structure):
+    """Mirror of ``dg_rms_norm_args`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('tokens', ctypes.c_int32), ('width', ctypes.c_int32), ('dtype', ctypes.c_int32), ('weight_dtype', ctypes.c_int32),
+        ('eps', ctypes.c_float), ('format', ctypes.c_int32), ('x', ctypes.c_void_p), ('residual', ctypes.c_void_p),
+        ('x_ld', ctypes.c_int64), ('residual_ld', ctypes.c_int64), ('weight', ctypes.c_void_p), ('h', ctypes.c_void_p),
+        ('h_ld', ctypes.c_int64), ('rstd', ctypes.c_void_p), ('y', ctypes.c_void_p), ('y_ld', ctypes.c_int64),
+        ('sf', ctypes.c_void_p), ('sf_ld', ctypes.c_int64), ('d_y', ctypes.c_void_p), ('d_h', ctypes.c_void_p),
+        ('d_y_ld', ctypes.c_int64), ('d_h_ld', ctypes.c_int64), ('d_x', ctypes.c_void_p), ('d_x_ld', ctypes.c_int64),
+        ('d_weight', ctypes.c_void_p), ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64), ('num_cus', ctypes.c_int32),
+    ]
+
+
+class SwigluArgs(ctypes.Structure):
+    """Mirror of ``dg_swiglu_args`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('rows', ctypes.c_int32), ('width', ctypes.c_int32), ('dtype', ctypes.c_int32), ('format', ctypes.c_int32),
+        ('h', ctypes.c_void_p), ('h_ld', ctypes.c_int64), ('act', ctypes.c_void_p), ('act_ld', ctypes.c_int64),
+        ('act_sf', ctypes.c_void_p), ('act_sf_ld', ctypes.c_int64), ('saved', ctypes.c_void_p), ('saved_ld', ctypes.c_int64),
+        ('saved_sf', ctypes.c_void_p), ('saved_sf_ld', ctypes.c_int64), ('d_act', ctypes.c_void_p), ('d_act_ld', ctypes.c_int64),
+        ('d_h', ctypes.c_void_p), ('d_h_ld', ctypes.c_int64), ('m_indices', ctypes.c_void_p), ('zero_padding', ctypes.c_int32),
+        ('num_cus', ctypes.c_int32),
+    ]
+
+
+class LoraArgs(ctypes.Structure):
+    """Mirror of ``dg_lora_args`` (include/deep_gemm_amd.h)."""
+    _fields_ = [
+        ('tokens', ctypes.c_int32), ('adapters', ctypes.c_int32), ('rank', ctypes.c_int32), ('n', ctypes.c_int32), ('k', ctypes.c_int32),
+        ('x', ctypes.c_void_p), ('a', ctypes.c_void_p), ('b', ctypes.c_void_p), ('x_ld', ctypes.c_int64), ('a_ld', ctypes.c_int64),
+        ('a_stride', ctypes.c_int64), ('b_ld', ctypes.c_int64), ('b_stride', ctypes.c_int64), ('scales', ctypes.c_void_p),
+        ('c', ctypes.c_void_p), ('c_ld', ctypes.c_int64), ('d', ctypes.c_void_p), ('d_ld', ctypes.c_int64), ('d_dtype', ctypes.c_int32),
+        ('layout', ctypes.POINTER(MoELayoutArgs)), ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64),
+        ('num_cus', ctypes.c_int32),
     ]
 
 
@@ -173,7 +225,16 @@ def load(path=None) -> ctypes.CDLL:
                 ('dg_mx_gemm', [ptr, i32, i64, ptr, i64, ptr, i64, ptr, i32, i64, i32, i32, i32, i32, i32, ptr]),
                 ('dg_linear_xent_workspace_size', [ctypes.POINTER(LinearXentArgs), i32, ctypes.POINTER(i64)]),
                 ('dg_linear_xent_forward', [ctypes.POINTER(LinearXentArgs), ptr]),
-                ('dg_linear_xent_backward', [ctypes.POINTER(LinearXentArgs), ptr])):
+                ('dg_linear_xent_backward', [ctypes.POINTER(LinearXentArgs), ptr]),
+                ('dg_moe_route', [ctypes.POINTER(MoERouteArgs), ptr]),
+                ('dg_moe_route_backward', [ctypes.POINTER(MoERouteArgs), ptr]),
+                ('dg_rms_norm_workspace_size', [ctypes.POINTER(RmsNormArgs), ctypes.POINTER(i64)]),
+                ('dg_rms_norm_forward', [ctypes.POINTER(RmsNormArgs), ptr]),
+                ('dg_rms_norm_backward', [ctypes.POINTER(RmsNormArgs), ptr]),
+                ('dg_swiglu_forward', [ctypes.POINTER(SwigluArgs), ptr]),
+                ('dg_swiglu_backward', [ctypes.POINTER(SwigluArgs), ptr]),
+                ('dg_lora_workspace_size', [ctypes.POINTER(LoraArgs), ctypes.POINTER(i64)]),
+                ('dg_lora_gemm', [ctypes.POINTER(LoraArgs), ptr])):
             getattr(lib, name).argtypes = argtypes
             getattr(lib, name).restype = ctypes.c_int
         lib.dg_take_errors.restype = ctypes.c_uint32
@@ -196,7 +257,7 @@ def error_message(bits: int, where: str = 'an earlier deep_gemm call') -> str:
         parts.append('m_indices is not padded to the M-grouped alignment (every alignment-row block must hold one '
                      'group id < num_groups followed only by -1 padding)')
     if bits & DG_ERR_EXPERT_ID:
-        parts.append('topk_idx holds an expert id >= num_groups')
+        parts.append('topk_idx holds an expert id >= num_groups, or a layout a group past the last adapter')
     if bits & DG_ERR_MOE_ROWS:
         parts.append('the pairs of topk_idx need more rows than num_rows')
     if bits & DG_ERR_TARGET:
@@ -260,6 +321,9 @@ def ext():
                 'dg_moe_sort', 'dg_moe_sort_workspace_size', 'dg_moe_dispatch', 'dg_moe_combine', 'dg_moe_combine_backward',
                 'dg_mx_quantize', 'dg_mx_dequantize', 'dg_mx_gemm', 'dg_linear_xent_workspace_size', 'dg_linear_xent_forward',
                 'dg_linear_xent_backward')))
+            mod.init_blocks(*(addr(getattr(lib, f)) for f in (
+                'dg_moe_route', 'dg_moe_route_backward', 'dg_rms_norm_workspace_size', 'dg_rms_norm_forward', 'dg_rms_norm_backward',
+                'dg_swiglu_forward', 'dg_swiglu_backward', 'dg_lora_workspace_size', 'dg_lora_gemm')))
         _ext = mod
         _ext_tried = True
         return _ext

@@ -227,6 +227,14 @@ def _operators(t: torch.Tensor):
     return None if get_dry_run() or not t.is_cuda else _lib.ext()
 
 
+def _call(fn: str, args, t: torch.Tensor) -> None:
+    """An operator's library call on t's device and its current stream there."""
+    _lib.raise_pending()
+    lib = _lib.load()
+    with torch.cuda.device(t.device):
+        _lib.check(getattr(lib, fn)(args, _stream(t)), lib)
+
+
 def _fast_recipes(recipe, recipe_a, recipe_b):
     """operand_recipes flattened to (gran_a_mn, gran_a_k, gran_b_mn, gran_b_k), memoised."""
     key = (recipe, recipe_a, recipe_b)

@@ -1,13 +1,14 @@
 """Tokens sorted by expert, moved into the rows of an M-grouped contiguous layout and back, with the gradients.
 
-A mixture-of-experts layer runs between two of these calls:
+A mixture-of-experts layer runs between these calls:
 
+    topk_idx, topk_weights = moe_route(logits, topk)          # [T, E] router logits -> a token's experts and their weights
     layout = moe_sort(topk_idx, num_experts)                  # [T, K] expert ids -> rows of an M-grouped layout
     rows = moe_dispatch(x, layout)                            # [M, H] tokens in their rows (bf16, fp8, packed fp4, ...)
     m_grouped_bf16_gemm_nt_contiguous(rows, w, y, layout.psum)
     out = moe_combine(y, layout, topk_weights)                # [T, N] weighted sums of a token's rows
 
-and its gradient between ``moe_combine_backward`` and ``moe_dispatch_backward``.  No autograd graph is recorded: results of inputs
+and its gradient between ``moe_combine_backward`` and ``moe_dispatch_backward``, the router's from ``moe_route_backward``.  No autograd graph is recorded: results of inputs
 that require gradients have none, and a program chains the backward calls itself.  Nothing synchronises with the host: the
 number of rows M is a bound over every routing (``moe_num_rows``), and the rows past the last group are padding.
 """
@@ -17,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .gemm import _operators, _stream
+from .gemm import _call, _operators, _stream
 from .layout import _assert, _align
 from .runtime import cu_cap, get_dry_run, get_mk_alignment_for_contiguous_layout
 
@@ -38,6 +39,86 @@ def moe_num_rows(num_pairs: int, num_groups: int) -> int:
     alignment (set_mk_alignment_for_contiguous_layout)."""
     a = get_mk_alignment_for_contiguous_layout()
     return (num_pairs + min(num_groups, num_pairs) * (a - 1)) // a * a
+
+
+_SCORES = {'softmax': _lib.DG_SCORES_SOFTMAX, 'sigmoid': _lib.DG_SCORES_SIGMOID}
+MAX_EXPERTS, MAX_TOPK = 1024, 16
+
+
+def _route_args(logits: torch.Tensor, topk: int, scores: str, renormalize: bool, scale: float) -> Tuple[torch.Tensor, _lib.MoERouteArgs]:
+    _assert(logits.dim() == 2 and logits.is_cuda, 'logits must be a [T, E] device tensor')
+    _assert(logits.dtype in _DTYPES, 'logits must be bf16 or fp32')
+    _assert(1 <= logits.size(1) <= MAX_EXPERTS, f'between 1 and {MAX_EXPERTS} experts')
+    _assert(logits.size(0) <= 2 ** 30, 'at most 2^30 tokens')
+    _assert(0 <= topk <= min(MAX_TOPK, logits.size(1)), f'topk must be at most {MAX_TOPK} and at most the experts')
+    logits = _plain(logits)
+    a = _lib.MoERouteArgs()
+    a.tokens, a.experts, a.topk = logits.size(0), logits.size(1), topk
+    a.scores, a.renormalize, a.scale, a.dtype = _SCORES[scores], int(renormalize), scale, _DTYPES[logits.dtype]
+    a.logits, a.logits_ld, a.num_cus = logits.data_ptr(), logits.stride(0) if logits.size(0) > 1 else logits.size(1), cu_cap()
+    return logits, a
+
+
+def moe_route(logits: torch.Tensor, topk: int, scores: str = 'softmax', bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+              topk_groups: int = 1, group_top: int = 2, renormalize: bool = True, scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(ids [T, topk] int32, weights [T, topk] fp32): the experts of each token, as ``moe_sort`` and ``moe_combine`` take them, from the
+    router's ``logits`` [T, E] (bf16 or fp32, E at most 1024, topk at most 16).
+
+    Scores s are the ``softmax`` of a row or the ``sigmoid`` of each logit.  ``bias`` [E] (fp32; for balance) is added for the choice
+    alone.  With ``num_groups`` > 1 the experts lie in that many groups of equal size, and the ``topk_groups`` groups whose
+    ``group_top`` (1 or 2) best biased scores have the largest sum stay.  The topk best biased scores there are chosen, best first, equal
+    ones by the lowest index, compared as 64 bits give them (numbers nearer than 2^-42 relative count as equal).
+    ``renormalize``: weights s / (sum of the chosen s + 1e-20) instead of s; both times ``scale``.
+
+    An expert whose logit or bias is -inf is never chosen; where fewer than topk are left, ids are -1 (dropped pairs for ``moe_sort``)
+    and weights 0.  NaN counts as the largest number."""
+    _assert(scores in _SCORES, f'unknown scores {scores}: softmax or sigmoid')
+    ext = _operators(logits)
+    if ext is not None:
+        made = ext.moe_route(logits, topk, scores == 'sigmoid', bias, num_groups, topk_groups, group_top, renormalize, scale, cu_cap(),
+                             _stream(logits))
+        if made:
+            return made[0], made[1]
+    logits, a = _route_args(logits, topk, scores, renormalize, scale)
+    e = logits.size(1)
+    _assert(num_groups >= 1 and e % num_groups == 0, f'{num_groups} groups do not divide {e} experts')
+    _assert(1 <= topk_groups <= num_groups, 'topk_groups must be between 1 and num_groups')
+    _assert(group_top in (1, 2), 'group_top must be 1 or 2')
+    _assert(topk <= topk_groups * (e // num_groups), "topk must be at most the kept groups' experts")
+    if bias is not None:
+        _assert(bias.dtype == torch.float32 and bias.shape == (e,) and bias.device == logits.device, 'bias must be a [E] fp32 tensor')
+        bias = bias.contiguous()
+    ids = torch.empty((logits.size(0), topk), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((logits.size(0), topk), dtype=torch.float32, device=logits.device)
+    if not get_dry_run():
+        a.num_groups, a.topk_groups, a.group_top = num_groups, topk_groups, group_top
+        a.bias, a.ids, a.weights = bias.data_ptr() if bias is not None else None, ids.data_ptr(), weights.data_ptr()
+        _call('dg_moe_route', a, logits)
+    return ids, weights
+
+
+def moe_route_backward(d_weights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, scores: str = 'softmax', renormalize: bool = True,
+                       scale: float = 1.0) -> torch.Tensor:
+    """Gradient [T, E] of ``moe_route``'s logits, in their type, from that of its weights (fp32) and its ids; the bias has none.
+    Negative ids have no gradient; nor have ids past the last expert, which are reported (``check_errors``)."""
+    _assert(scores in _SCORES, f'unknown scores {scores}: softmax or sigmoid')
+    ext = _operators(logits)
+    if ext is not None:
+        made = ext.moe_route_backward(d_weights, logits, ids, scores == 'sigmoid', renormalize, scale, cu_cap(), _stream(logits))
+        if made:
+            return made[0]
+    _assert(ids.dim() == 2 and ids.dtype == torch.int32 and ids.size(0) == logits.size(0) and ids.device == logits.device,
+            'ids must be a [T, topk] int32 tensor')
+    logits, a = _route_args(logits, ids.size(1), scores, renormalize, scale)
+    _assert(d_weights.dtype == torch.float32 and d_weights.shape == ids.shape and d_weights.device == logits.device,
+            'd_weights must be a [T, topk] fp32 tensor')
+    ids, d_weights = ids.contiguous(), d_weights.contiguous()
+    d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if not get_dry_run():
+        a.ids, a.d_weights = ids.data_ptr(), d_weights.data_ptr()
+        a.d_logits, a.d_logits_ld = d_logits.data_ptr(), d_logits.size(1)
+        _call('dg_moe_route_backward', a, logits)
+    return d_logits
 
 
 def _args(layout: MoELayout, num_groups: int = 0, alignment: int = 1) -> _lib.MoELayoutArgs:

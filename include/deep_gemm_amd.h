@@ -388,6 +388,143 @@ int dg_linear_xent_workspace_size(const dg_linear_xent_args *args, int32_t backw
 int dg_linear_xent_forward(const dg_linear_xent_args *args, void *stream);
 int dg_linear_xent_backward(const dg_linear_xent_args *args, void *stream);
 
+/*
+ * Routing: the experts of a token from the router's logits l [tokens][experts] (bf16 or fp32, at most 1024 experts).
+ *   s = softmax(l) or 1 / (1 + exp(-l));   b = s + bias (NULL: 0)
+ *   With num_groups > 1 (a divisor of experts) a group's score is the sum of its group_top (1 or 2) largest b, and the topk_groups
+ *   groups of the largest scores stay.  ids = the topk (at most 16) experts of the largest b there, largest first;
+ *   weights = s[ids], renormalize: divided by (their sum + 1e-20), times scale.
+ * Equal numbers go to the lowest index; b and the scores are compared as 64 bits give them.  An expert whose logit or bias is -inf
+ * is out, and a group without experts too; a token that has fewer than topk left gets id -1 and weight 0 behind them.  NaN counts
+ * as the largest number.
+ * The gradient: d_logits [tokens][experts] of d_weights; ids that are negative or past the last expert (DG_ERR_EXPERT_ID) have
+ * none, ids of a token that repeat count as often.  ids and weights are [tokens][topk], without gaps.
+ */
+#define DG_SCORES_SOFTMAX 0
+#define DG_SCORES_SIGMOID 1
+typedef struct dg_moe_route_args {
+    int32_t tokens, experts, topk;
+    int32_t scores;               /* DG_SCORES_*                                                           */
+    int32_t num_groups, topk_groups, group_top;
+    int32_t renormalize;
+    float scale;
+    int32_t dtype;                /* of logits and d_logits: DG_DTYPE_BF16 or DG_DTYPE_F32                 */
+    const void *logits;
+    int64_t logits_ld;            /* elements                                                              */
+    const float *bias;            /* [experts] or NULL (forward)                                           */
+    int32_t *ids;                 /* forward: written; backward: read                                      */
+    float *weights;               /* forward: written                                                      */
+    const float *d_weights;       /* backward                                                              */
+    void *d_logits;               /* backward: written                                                     */
+    int64_t d_logits_ld;
+    int32_t num_cus;
+} dg_moe_route_args;
+int dg_moe_route(const dg_moe_route_args *args, void *stream);
+int dg_moe_route_backward(const dg_moe_route_args *args, void *stream);
+
+/*
+ * Root-mean-square norm of rows of `width` values (at most 32768), with the residual's addition before it:
+ *   h = x + residual, rounded to dtype (residual NULL: h is x, and is not written);
+ *   rstd = 1 / sqrt(mean(h^2) + eps);   y = h rstd weight
+ * y is written in dtype (format -1) or as codes and required-layout scale factors (DG_MX_*, width a multiple of 32, quantised from
+ * the fp32 values as dg_mx_quantize does it).
+ * Backward, from d_y and h (and d_h, the gradient that reaches h by the residual's path, or NULL), all of dtype:
+ *   d_x = rstd (weight d_y - h rstd^2 mean(weight d_y h)) + d_h, the gradient of x and of the residual;
+ *   d_weight = sum over the tokens of d_y h rstd, fp32.
+ * The workspace (dg_rms_norm_workspace_size bytes, backward only) holds nothing between calls.
+ */
+typedef struct dg_rms_norm_args {
+    int32_t tokens, width;
+    int32_t dtype, weight_dtype;  /* DG_DTYPE_BF16 or DG_DTYPE_F32                                         */
+    float eps;
+    int32_t format;               /* -1, DG_MX_E2M1 or DG_MX_E4M3                                          */
+    const void *x, *residual;
+    int64_t x_ld, residual_ld;    /* elements                                                              */
+    const void *weight;           /* [width]                                                               */
+    void *h;                      /* forward: written (with a residual); backward: read                    */
+    int64_t h_ld;
+    float *rstd;                  /* [tokens]; forward: written; backward: read                            */
+    void *y;                      /* values, or codes                                                      */
+    int64_t y_ld;                 /* elements, or bytes of codes (a multiple of 8)                         */
+    int16_t *sf;
+    int64_t sf_ld;                /* even                                                                  */
+    const void *d_y, *d_h;
+    int64_t d_y_ld, d_h_ld;
+    void *d_x;
+    int64_t d_x_ld;
+    float *d_weight;              /* [width]                                                               */
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t num_cus;
+} dg_rms_norm_args;
+int dg_rms_norm_workspace_size(const dg_rms_norm_args *args, int64_t *bytes);
+int dg_rms_norm_forward(const dg_rms_norm_args *args, void *stream);
+int dg_rms_norm_backward(const dg_rms_norm_args *args, void *stream);
+
+/*
+ * Gated activation of rows h = (gate | up) of 2 width values: act = gate / (1 + exp(-gate)) up, and its gradient.
+ * act is written in dtype (format -1) or as codes and required-layout scale factors (DG_MX_*, width a multiple of 32).
+ * saved (optional; width a multiple of 32): h as e4m3 codes [rows][2 width] and required-layout scale factors, as dg_mx_quantize
+ * gives them, from the same read.
+ * Backward, from d_act (dtype) and h, or saved where h is NULL: d_h = (d_act up s (1 + gate (1 - s)) | d_act gate s) with
+ * s = 1 / (1 + exp(-gate)), and act (dtype, optional) once more.
+ * m_indices (optional, [rows]): rows with a negative entry are padding; they are not read, and outputs there are zeros
+ * (zero_padding), or rows of act, saved codes and d_h are left as they are and scale factors are zeros.
+ */
+typedef struct dg_swiglu_args {
+    int32_t rows, width;
+    int32_t dtype;                /* DG_DTYPE_BF16 or DG_DTYPE_F32                                         */
+    int32_t format;               /* of act: -1, DG_MX_E2M1 or DG_MX_E4M3 (backward: -1)                   */
+    const void *h;
+    int64_t h_ld;                 /* elements                                                              */
+    void *act;                    /* values, or codes; backward: values or NULL                            */
+    int64_t act_ld;               /* elements, or bytes of codes (a multiple of 8)                         */
+    int16_t *act_sf;
+    int64_t act_sf_ld;            /* even                                                                  */
+    void *saved;                  /* forward: written, or NULL; backward: read where h is NULL             */
+    int64_t saved_ld;             /* bytes, a multiple of 8                                                */
+    int16_t *saved_sf;
+    int64_t saved_sf_ld;
+    const void *d_act;            /* backward                                                              */
+    int64_t d_act_ld;
+    void *d_h;
+    int64_t d_h_ld;
+    const int32_t *m_indices;
+    int32_t zero_padding;
+    int32_t num_cus;
+} dg_swiglu_args;
+int dg_swiglu_forward(const dg_swiglu_args *args, void *stream);
+int dg_swiglu_backward(const dg_swiglu_args *args, void *stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   d[t] = c[t] + scales[i] (x[t] a[i]^T) b[i]^T, i the adapter of token t; a token without one: d[t] = c[t]
+ * x [tokens][k], a [adapters][rank][k] and b [adapters][n][rank] bf16 (k and rank multiples of 8, rank at most 256, x, a and b
+ * 16-byte aligned rows), d and c of d_dtype, c NULL: 0, c = d: in place.  The layout is dg_moe_sort's of one choice a token over at
+ * least as many groups as there are adapters (a group past the last adapter: DG_ERR_EXPERT_ID, its tokens keep c).
+ * The inner products are summed in fp32 and enter the second product as the sum of two bf16 numbers (2^-17 relative).
+ * The workspace (dg_lora_workspace_size bytes) holds nothing between calls.
+ */
+typedef struct dg_lora_args {
+    int32_t tokens, adapters, rank, n, k;
+    const void *x, *a, *b;
+    int64_t x_ld;                 /* elements                                                              */
+    int64_t a_ld, a_stride;       /* elements: rows of an adapter, adapters                                */
+    int64_t b_ld, b_stride;
+    const float *scales;          /* [adapters] or NULL: 1                                                 */
+    const void *c;
+    int64_t c_ld;
+    void *d;
+    int64_t d_ld;
+    int32_t d_dtype;              /* DG_DTYPE_BF16 or DG_DTYPE_F32                                         */
+    const dg_moe_layout *layout;  /* slots, source, m_indices and rows are read                            */
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t num_cus;
+} dg_lora_args;
+int dg_lora_workspace_size(const dg_lora_args *args, int64_t *bytes);
+int dg_lora_gemm(const dg_lora_args *args, void *stream);
+
 /* Message of the last failing call on this thread ("" if none). */
 const char *dg_last_error(void);
 
