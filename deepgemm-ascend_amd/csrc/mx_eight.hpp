@@ -117,30 +117,56 @@ __device__ __forceinline__ float scale_value(u32 s) {
     return __builtin_bit_cast(float, s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23);
 }
 
-// n (at most 8) values of a row from x on, zeros behind them; 16-byte accesses where all eight are there.
+// Eight values of a row as they lie in memory, zeros behind the n-th; 16-byte accesses where all eight are there.
+template <typename E> struct Raw;
+template <>
+struct Raw<float> {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const float* x, int n) {
+        a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (n >= 8) {
+            a = reinterpret_cast<const f32x4_any*>(x)[0];
+            b = reinterpret_cast<const f32x4_any*>(x)[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+                if (i < n) (i < 4 ? a : b)[i & 3] = x[i];
+        }
+    }
+    __device__ __forceinline__ void values(Eight<float>& v) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v.v[i] = a[i];
+            v.v[4 + i] = b[i];
+        }
+    }
+};
+template <>
+struct Raw<uint16_t> {
+    i32x4 w;
+    __device__ __forceinline__ void load(const uint16_t* x, int n) {
+        w = i32x4{0, 0, 0, 0};
+        if (n >= 8) {
+            w = *reinterpret_cast<const i32x4_half*>(x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+                if (i < n) w[i >> 1] |= (int)((u32)x[i] << (i & 1 ? 16 : 0));
+        }
+    }
+    __device__ __forceinline__ void values(Eight<float>& v) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v.v[2 * i] = __builtin_bit_cast(float, (u32)w[i] << 16);
+            v.v[2 * i + 1] = __builtin_bit_cast(float, (u32)w[i] & 0xffff0000u);
+        }
+    }
+};
 template <typename E>
 __device__ __forceinline__ void load_eight(Eight<float>& v, const E* x, int n) {
-    if (n >= 8) {
-        if constexpr (sizeof(E) == 4) {
-            v.load(x);
-        } else {
-            const i32x4 w = *reinterpret_cast<const i32x4_half*>(x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v.v[2 * i] = __builtin_bit_cast(float, (u32)w[i] << 16);
-                v.v[2 * i + 1] = __builtin_bit_cast(float, (u32)w[i] & 0xffff0000u);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v.v[i] = 0.f;
-        if (i < n) {
-            if constexpr (sizeof(E) == 4) v.v[i] = x[i];
-            else v.v[i] = bf16_to_f32(x[i]);
-        }
-    }
+    Raw<E> r;
+    r.load(x, n);
+    r.values(v);
 }
 
 // The first n of eight values to a row of E (one rounding, to nearest even, for bf16).

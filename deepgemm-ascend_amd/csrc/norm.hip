@@ -7,11 +7,13 @@
 #include "mx_eight.hpp"
 #include "op_launch.hpp"
 
+#include <type_traits>
+
 namespace dg {
 namespace {
 
 constexpr int kMaxWidth = 32768;
-constexpr int kMaxPartials = 512;   // workgroups of the gradient, each of which leaves a partial d_weight
+constexpr int kMaxPartials = 256;   // workgroups of the gradient, each of which leaves a partial d_weight
 
 struct NormParams {
     const void *x, *residual, *weight;
@@ -27,7 +29,8 @@ struct NormParams {
     int64_t dy_ld, dh_ld;
     void* d_x;
     int64_t dx_ld;
-    float* partial;            // [groups][width] (gradient)
+    float* partial;            // [groups][partial_ld] (gradient)
+    int partial_ld;
     float* d_weight;
     int tokens, width, weight_f32;
     int groups;
@@ -35,23 +38,35 @@ struct NormParams {
     int vbase;
 };
 
+// The sum over a wave, the same in every lane: within rows of 16 lanes, then lane 15 to the next row and lane 31 to the upper half.
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-    return v;
+    auto moved = [](float x, auto ctrl, auto rows) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    v += moved(v, integral_constant<int, kXor1>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, kXor2>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, kMirror8>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, 0x140>(), integral_constant<int, 0xf>());   // row_mirror
+    v += moved(v, integral_constant<int, 0x142>(), integral_constant<int, 0xa>());   // row_bcast15 to rows 1 and 3
+    v += moved(v, integral_constant<int, 0x143>(), integral_constant<int, 0xc>());   // row_bcast31 to rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// The sum over the threads that hold a row; `turn` alternates between the two halves of `part`, so that one barrier does.
-template <int THREADS>
-__device__ __forceinline__ float row_sum(float v, float (*part)[16], int turn) {
+// The sum over the THREADS that hold a row, of TEAMS in a workgroup; `turn` alternates between two halves of `part`, so that one
+// barrier does.
+template <int THREADS, int TEAMS>
+__device__ __forceinline__ float row_sum(float v, float (&part)[2][16], int turn) {
     v = wave_sum(v);
     if constexpr (THREADS > 64) {
+        constexpr int WAVES = THREADS / 64;
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) part[turn][wave] = v;
         __syncthreads();
         v = 0.f;
+        const float* const mine = part[turn] + wave / WAVES * WAVES;
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; ++i) v += part[turn][i];
+        for (int i = 0; i < WAVES; ++i) v += mine[i];
     }
     return v;
 }
@@ -100,7 +115,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_kernel(con
 #pragma unroll
             for (int i = 0; i < 8; ++i) squares += v[j].v[i] * v[j].v[i];
         }
-        const float rstd = rsqrtf(row_sum<THREADS>(squares, part, r & 1) * p.inv_width + p.eps);
+        const float rstd = rsqrtf(row_sum<THREADS, AT_ONCE>(squares, part, r & 1) * p.inv_width + p.eps);
         if (on && at == 0) p.rstd[t] = rstd;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -127,8 +142,17 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_kernel(con
         __syncthreads();
         // two rows a thread: the leading dimension is even, and an odd last row's partner is written 0
         const int k64 = ceil_div(p.width, 64);
-        for (int e = threadIdx.x; e < k64 * (ROWS / 2); e += WG) {
-            const int j = e / (ROWS / 2), r = e % (ROWS / 2) * 2;
+        if constexpr (ROWS == 1) {
+            for (int j = threadIdx.x; j < k64; j += WG) {
+                int16_t* const to = p.sf + (int64_t)j * p.sf_ld + row0;
+                if (row0 % 2 == 0 && row0 + 1 == p.tokens) *reinterpret_cast<u32*>(to) = pairs[j][0];
+                else *to = (int16_t)pairs[j][0];
+            }
+            return;
+        }
+        constexpr int TWO = ROWS > 1 ? ROWS / 2 : 1;
+        for (int e = threadIdx.x; e < k64 * TWO; e += WG) {
+            const int j = e / TWO, r = e % TWO * 2;
             if (row0 + r >= p.tokens) continue;
             const u32 two = pairs[j][r] | (row0 + r + 1 < p.tokens ? (u32)pairs[j][r + 1] << 16 : 0u);
             *reinterpret_cast<u32*>(p.sf + (int64_t)j * p.sf_ld + row0 + r) = two;
@@ -136,61 +160,90 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_kernel(con
     }
 }
 
-// Rows t, t + step, ...: d_x as they come, d_weight summed over them in registers.
-template <typename E, int THREADS, int V>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_backward_kernel(const NormParams p) {
-    constexpr int WG = THREADS < 256 ? 256 : THREADS, AT_ONCE = WG / THREADS;
-    __shared__ float part[2][16];
-    __shared__ float joined[AT_ONCE > 1 ? THREADS * V * 8 : 1];
-    const int at = threadIdx.x % THREADS, which = threadIdx.x / THREADS, group = blockIdx.x + p.vbase;
-    Eight<float> w[V], sum[V];
+// What a thread holds of a token's h and d_y.
+template <typename E, int V>
+struct BackwardRow {
+    Raw<E> h[V], d[V];
+    float rstd;
+    template <int THREADS>
+    __device__ __forceinline__ void load(const NormParams& p, int64_t t, int at) {
+        const bool on = t < p.tokens;
+        rstd = on ? p.rstd[t] : 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int col = (j * THREADS + at) * 8;
-        load_weight(w[j], p, col, p.width - col);
+        for (int j = 0; j < V; ++j) {
+            const int col = (j * THREADS + at) * 8, n = on ? p.width - col : 0;
+            h[j].load(reinterpret_cast<const E*>(p.h) + t * p.h_ld + col, n);
+            d[j].load(reinterpret_cast<const E*>(p.d_y) + t * p.dy_ld + col, n);
+        }
+    }
+};
+
+// TEAMS of THREADS hold a row each and step through the tokens together; the next rows (bf16) are in flight while a row is summed.
+// d_weight is summed over a team's rows in registers, over the teams in LDS, in order.
+template <typename E, int THREADS, int TEAMS, int V>
+__global__ __launch_bounds__(THREADS * TEAMS) void norm_backward_kernel(const NormParams p) {
+    constexpr bool AHEAD = sizeof(E) == 2 && V <= 2;
+    __shared__ float part[2][16];
+    __shared__ float joined[TEAMS > 1 ? THREADS * V * 8 : 1];
+    const int at = threadIdx.x % THREADS, team = threadIdx.x / THREADS, group = blockIdx.x + p.vbase;
+    Eight<float> sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[j].v[i] = 0.f;
-    }
+    const int64_t step = (int64_t)p.groups * TEAMS;
+    int64_t t = (int64_t)group * TEAMS + team;
+    BackwardRow<E, V> row, next;
+    row.template load<THREADS>(p, t, at);
     int turn = 0;
+    // (a workgroup's teams take as many steps: that of the first team, whose tokens come first)
 #pragma unroll 1
-    for (int64_t t = (int64_t)group * AT_ONCE + which; t < p.tokens; t += (int64_t)p.groups * AT_ONCE) {
-        Eight<float> h[V], d[V];
-        const float rstd = p.rstd[t];
+    for (int64_t first = (int64_t)group * TEAMS; first < p.tokens; first += step, t += step) {
+        Raw<E> a[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int col = (j * THREADS + at) * 8;
+            a[j].load(reinterpret_cast<const E*>(p.d_h) + t * p.dh_ld + col, p.d_h != nullptr && t < p.tokens ? p.width - col : 0);
+        }
+        if constexpr (AHEAD) next.template load<THREADS>(p, t + step, at);
+        const float rstd = row.rstd;
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int col = (j * THREADS + at) * 8, n = p.width - col;
-            load_eight(h[j], reinterpret_cast<const E*>(p.h) + t * p.h_ld + col, n);
-            load_eight(d[j], reinterpret_cast<const E*>(p.d_y) + t * p.dy_ld + col, n);
+            const int col = (j * THREADS + at) * 8;
+            Eight<float> w, h, d;
+            load_weight(w, p, col, p.width - col);
+            row.h[j].values(h);
+            row.d[j].values(d);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                h[j].v[i] *= rstd;
-                sum[j].v[i] += d[j].v[i] * h[j].v[i];
-                d[j].v[i] *= w[j].v[i];
-                dot += d[j].v[i] * h[j].v[i];
+                h.v[i] *= rstd;
+                sum[j].v[i] += d.v[i] * h.v[i];
+                dot += d.v[i] * w.v[i] * h.v[i];
             }
         }
-        const float mean = row_sum<THREADS>(dot, part, turn) * p.inv_width;
+        const float mean = row_sum<THREADS, TEAMS>(dot, part, turn) * p.inv_width;
         turn ^= 1;
+        if (t < p.tokens) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int col = (j * THREADS + at) * 8, n = p.width - col;
-            Eight<float> g;
+            for (int j = 0; j < V; ++j) {
+                const int col = (j * THREADS + at) * 8, n = p.width - col;
+                Eight<float> w, h, d, g;
+                load_weight(w, p, col, n);
+                row.h[j].values(h);
+                row.d[j].values(d);
+                a[j].values(g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g.v[i] = rstd * (d[j].v[i] - h[j].v[i] * mean);
-            if (p.d_h != nullptr) {
-                Eight<float> a;
-                load_eight(a, reinterpret_cast<const E*>(p.d_h) + t * p.dh_ld + col, n);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) g.v[i] += a.v[i];
+                for (int i = 0; i < 8; ++i) g.v[i] += rstd * (d.v[i] * w.v[i] - h.v[i] * rstd * mean);
+                store_eight(reinterpret_cast<E*>(p.d_x) + t * p.dx_ld + col, g, n);
             }
-            store_eight(reinterpret_cast<E*>(p.d_x) + t * p.dx_ld + col, g, n);
         }
+        if constexpr (AHEAD) row = next;
+        else row.template load<THREADS>(p, t + step, at);
     }
-    // the waves of a workgroup one after another, in order
-    if constexpr (AT_ONCE > 1) {
-        for (int o = 0; o < AT_ONCE; ++o) {
-            if (which == o)
+    if constexpr (TEAMS > 1) {
+        for (int o = 0; o < TEAMS; ++o) {
+            if (team == o)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -200,13 +253,13 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_backward_k
                     }
             __syncthreads();
         }
-        if (which != 0) return;
+        if (team != 0) return;
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[j].v[i] = joined[(j * 8 + i) * THREADS + at];
     }
-    float* const to = p.partial + (int64_t)group * p.width;
+    float* const to = p.partial + (int64_t)group * p.partial_ld;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int col = (j * THREADS + at) * 8;
@@ -214,26 +267,43 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_backward_k
     }
 }
 
-// d_weight from the partial sums, in order: 16 columns a workgroup, 16 threads to a column.
+// d_weight from the partial sums, in order: 32 columns a workgroup, four a thread, 32 threads to a column.
 __global__ __launch_bounds__(256) void norm_weight_kernel(const NormParams p) {
-    __shared__ float part[16][17];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, col = (blockIdx.x + p.vbase) * 16 + c;
-    float sum = 0.f;
-    if (col < p.width)
-        for (int g = r; g < p.groups; g += 16) sum += p.partial[(int64_t)g * p.width + col];
+    __shared__ f32x4 part[32][8];
+    const int c = threadIdx.x & 7, r = threadIdx.x >> 3, col = (blockIdx.x + p.vbase) * 32 + c * 4;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (col < p.width) {
+#pragma unroll 8
+        for (int g = r; g < p.groups; g += 32) {
+            const f32x4 o = *reinterpret_cast<const f32x4*>(p.partial + (int64_t)g * p.partial_ld + col);   // (rows of whole fours)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum[q] += o[q];
+        }
+    }
     part[r][c] = sum;
     __syncthreads();
-    if (r != 0 || col >= p.width) return;
+    const int one = threadIdx.x, mine = (blockIdx.x + p.vbase) * 32 + one;
+    if (one >= 32 || mine >= p.width) return;
+    float all = 0.f;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) sum += part[i][c];
-    p.d_weight[col] = sum;
+    for (int i = 0; i < 32; ++i) all += part[i][one >> 2][one & 3];
+    p.d_weight[mine] = all;
 }
 
 typedef void (*NormKernel)(const NormParams);
 
-// A wave to a row up to 2048 values, a workgroup of 256 threads up to 16384, of 512 up to 32768.
+// Few tokens: a workgroup to a row, as wide as the row allows, one step or few.  Otherwise a wave to a row up to 2048 values, a workgroup
+// of 256 threads up to 16384, of 512 up to 32768, whose rows follow each other.
 template <typename E, int FMT>
-NormKernel pick_forward(int width, unsigned& threads, int& rows) {
+NormKernel pick_forward(int tokens, int width, unsigned& threads, int& rows) {
+    if (tokens <= 512) {
+        rows = 1;
+        threads = width <= 2048 ? 256 : 1024;
+        if (width <= 2048) return &norm_kernel<E, FMT, 256, 1, 1>;
+        if (width <= 8192) return &norm_kernel<E, FMT, 1024, 1, 1>;
+        if (width <= 16384) return &norm_kernel<E, FMT, 1024, 2, 1>;
+        return &norm_kernel<E, FMT, 1024, 4, 1>;
+    }
     constexpr int ROWS = FMT >= 0 ? 8 : 4;
     rows = ROWS;
     threads = width <= 16384 ? 256 : 512;
@@ -245,23 +315,33 @@ NormKernel pick_forward(int width, unsigned& threads, int& rows) {
     if (width <= 16384) return &norm_kernel<E, FMT, 256, 8, ROWS>;
     return &norm_kernel<E, FMT, 512, 8, ROWS>;
 }
+
+// Rows that a workgroup of the gradient holds at once.
+int teams(int width) { return width <= 1024 ? 16 : width <= 2048 ? 8 : width <= 4096 ? 4 : width <= 8192 ? 2 : 1; }
+
+// Few tokens: 512 threads to a workgroup where a row leaves that choice, so that more CUs have rows.
+bool few(int tokens, int width) { return width <= 4096 && tokens < kMaxPartials * teams(width); }
+
 template <typename E>
-NormKernel pick_backward(int width, unsigned& threads, int& at_once) {
-    at_once = width <= 2048 ? 4 : 1;
-    threads = width <= 16384 ? 256 : 512;
-    if (width <= 512) return &norm_backward_kernel<E, 64, 1>;
-    if (width <= 1024) return &norm_backward_kernel<E, 64, 2>;
-    if (width <= 2048) return &norm_backward_kernel<E, 64, 4>;
-    if (width <= 4096) return &norm_backward_kernel<E, 256, 2>;
-    if (width <= 8192) return &norm_backward_kernel<E, 256, 4>;
-    if (width <= 16384) return &norm_backward_kernel<E, 256, 8>;
-    return &norm_backward_kernel<E, 512, 8>;
+NormKernel pick_backward(int tokens, int width) {
+    if (few(tokens, width)) {
+        if (width <= 512) return &norm_backward_kernel<E, 64, 8, 1>;
+        if (width <= 1024) return &norm_backward_kernel<E, 64, 8, 2>;
+        if (width <= 2048) return &norm_backward_kernel<E, 128, 4, 2>;
+        return &norm_backward_kernel<E, 256, 2, 2>;
+    }
+    if (width <= 512) return &norm_backward_kernel<E, 64, 16, 1>;
+    if (width <= 1024) return &norm_backward_kernel<E, 64, 16, 2>;
+    if (width <= 2048) return &norm_backward_kernel<E, 128, 8, 2>;
+    if (width <= 4096) return &norm_backward_kernel<E, 256, 4, 2>;
+    if (width <= 8192) return &norm_backward_kernel<E, 512, 2, 2>;
+    if (width <= 16384) return &norm_backward_kernel<E, 1024, 1, 2>;
+    return &norm_backward_kernel<E, 1024, 1, 4>;
 }
 
-// Workgroups of the gradient: enough for every CU, few enough that their partial sums cost little.
+// Workgroups of the gradient: one to a CU, whose partial sums cost little.
 int partials(int tokens, int width) {
-    const int at_once = width <= 2048 ? 4 : 1;
-    return std::max(1, std::min(ceil_div(tokens, at_once), kMaxPartials));
+    return std::max(1, std::min(ceil_div(tokens, few(tokens, width) ? teams(width) / 2 : teams(width)), kMaxPartials));
 }
 
 int check(const dg_rms_norm_args* a, NormParams& p) {
@@ -315,11 +395,11 @@ int forward(const dg_rms_norm_args* a, void* stream) {
     int rows = 0;
     NormKernel kernel;
     if (a->dtype == DG_DTYPE_F32)
-        kernel = !quant ? pick_forward<float, -1>(a->width, threads, rows)
-                        : a->format == DG_MX_E2M1 ? pick_forward<float, DG_MX_E2M1>(a->width, threads, rows) : pick_forward<float, DG_MX_E4M3>(a->width, threads, rows);
+        kernel = !quant ? pick_forward<float, -1>(a->tokens, a->width, threads, rows)
+                        : a->format == DG_MX_E2M1 ? pick_forward<float, DG_MX_E2M1>(a->tokens, a->width, threads, rows) : pick_forward<float, DG_MX_E4M3>(a->tokens, a->width, threads, rows);
     else
-        kernel = !quant ? pick_forward<uint16_t, -1>(a->width, threads, rows)
-                        : a->format == DG_MX_E2M1 ? pick_forward<uint16_t, DG_MX_E2M1>(a->width, threads, rows) : pick_forward<uint16_t, DG_MX_E4M3>(a->width, threads, rows);
+        kernel = !quant ? pick_forward<uint16_t, -1>(a->tokens, a->width, threads, rows)
+                        : a->format == DG_MX_E2M1 ? pick_forward<uint16_t, DG_MX_E2M1>(a->tokens, a->width, threads, rows) : pick_forward<uint16_t, DG_MX_E4M3>(a->tokens, a->width, threads, rows);
     return launch_op(kernel, ceil_div64(a->tokens, rows), threads, p, reinterpret_cast<hipStream_t>(stream), a->num_cus);
 }
 
@@ -327,7 +407,7 @@ int workspace_size(const dg_rms_norm_args* a, int64_t* bytes) {
     NormParams p;
     if (bytes == nullptr) return dg_set_error("dg_rms_norm: null result");
     if (const int rc = check(a, p); rc != DG_OK) return rc;
-    *bytes = (int64_t)partials(a->tokens, a->width) * a->width * 4;
+    *bytes = (int64_t)partials(a->tokens, a->width) * align_up(a->width, 4) * 4;
     return DG_OK;
 }
 
@@ -341,10 +421,10 @@ int backward(const dg_rms_norm_args* a, void* stream) {
     if (some && (a->h_ld < a->width || a->d_y_ld < a->width || a->d_x_ld < a->width || (a->d_h != nullptr && a->d_h_ld < a->width)))
         return dg_set_error("dg_rms_norm: leading dimension smaller than the row");
     if (!aligned_to(a->h, size) || !aligned_to(a->d_y, size) || !aligned_to(a->d_h, size) || !aligned_to(a->d_x, size) || !aligned_to(a->rstd, 4) ||
-        !aligned_to(a->d_weight, 4) || !aligned_to(a->workspace, 4) || !aligned_to(a->weight, p.weight_f32 ? 4 : 2))
+        !aligned_to(a->d_weight, 4) || !aligned_to(a->workspace, 16) || !aligned_to(a->weight, p.weight_f32 ? 4 : 2))
         return dg_set_error("dg_rms_norm: tensors must be aligned");
     p.groups = partials(a->tokens, a->width);
-    if (a->workspace == nullptr || a->workspace_bytes < (int64_t)p.groups * a->width * 4) return dg_set_error("dg_rms_norm: workspace too small");
+    if (a->workspace == nullptr || a->workspace_bytes < (int64_t)p.groups * align_up(a->width, 4) * 4) return dg_set_error("dg_rms_norm: workspace too small");
     p.d_y = a->d_y;
     p.dy_ld = a->d_y_ld;
     p.d_h = a->d_h;
@@ -352,13 +432,12 @@ int backward(const dg_rms_norm_args* a, void* stream) {
     p.d_x = a->d_x;
     p.dx_ld = a->d_x_ld;
     p.partial = static_cast<float*>(a->workspace);
+    p.partial_ld = align_up(a->width, 4);
     p.d_weight = a->d_weight;
-    unsigned threads = 0;
-    int at_once = 0;
-    const NormKernel kernel = a->dtype == DG_DTYPE_F32 ? pick_backward<float>(a->width, threads, at_once) : pick_backward<uint16_t>(a->width, threads, at_once);
+    const NormKernel kernel = a->dtype == DG_DTYPE_F32 ? pick_backward<float>(a->tokens, a->width) : pick_backward<uint16_t>(a->tokens, a->width);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (const int rc = launch_op(kernel, p.groups, threads, p, st, a->num_cus); rc != DG_OK) return rc;
-    return launch_op(&norm_weight_kernel, ceil_div(a->width, 16), 256, p, st, a->num_cus);
+    if (const int rc = launch_op(kernel, p.groups, few(a->tokens, a->width) ? 512 : 1024, p, st, a->num_cus); rc != DG_OK) return rc;
+    return launch_op(&norm_weight_kernel, ceil_div(a->width, 32), 256, p, st, a->num_cus);
 }
 
 }  // namespace
