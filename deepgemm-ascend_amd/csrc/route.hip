@@ -4,10 +4,16 @@
 //   w = scale s[id] / (sum s[id] + 1e-20):
 //   d s[id_c] = scale (d_w_c - sum_j d_w_j s[id_j] / S) / S with S the sum and its 1e-20, then through softmax or sigmoid.
 //
-// LPT lanes hold a token's row, P experts each.  A key carries its expert's index in its low ten bits, so that all keys differ and
-// comparing them alone gives the order, equal numbers to the lowest index.  The lanes sort their keys and join lists of the KP largest
-// pairwise: max(a[i], b[KP - 1 - i]) of two descending lists are the KP largest of both, in an order that one bitonic merge sorts.
+// LPT lanes hold a token's row, P experts each.  A key is a number whose low bits gave way to its expert's index, so that all keys
+// differ and comparing them alone gives the order, equal numbers to the lowest index.  The lanes sort their keys and join lists of the KP
+// largest pairwise: max(a[i], b[KP - 1 - i]) of two descending lists are the KP largest of both, in an order that one bitonic merge sorts.
+//
+// Keys of 32 bits select quickly but not surely: 22 to 26 bits of a score in fp32.  The choice is then checked against the scores
+// themselves: every chosen one above the next, and the last above all others, by more than fp32 can be off.  A token that fails
+// (about one in a hundred, and rows with infinities or NaN) is done again in 64 bits.
 #include "op_launch.hpp"
+
+#include <utility>
 
 namespace dg {
 namespace {
@@ -18,6 +24,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 256;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 16;
+constexpr int kMaxGroups = 64;
 constexpr float kTiny = 1e-20f;
 
 struct RouteParams {
@@ -28,6 +35,8 @@ struct RouteParams {
     int groups, per_group, keep, group_top;
     u32 per_group_inv;         // ceil(2^21 / per_group): e / per_group = e * inv >> 21 for e < 1024
     int by_logit;              // the order of b is the logits' own
+    int exact_keys;            // keys of 32 bits hold all of b
+    int group_lanes;           // 1 + log2 of a group's lanes, where these are a power of two, at most 16; 0 otherwise
     int renormalize;
     float scale;
     const float* bias;
@@ -43,6 +52,13 @@ struct RouteParams {
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short u16x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
+// f of 0 ... N - 1 as constants: the arrays that they index are registers from the start (loops, unrolled later, leave the compiler
+// moving an array as a whole: 211 registers, and 36 us in place of 25 for 32768 tokens over 256 experts).
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+    [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, N>());
+}
+
 // A lane's expert i: runs of four, so that a token's lanes read side by side.
 template <int LPT>
 __device__ __forceinline__ int expert_of(int sub, int i) { return (i >> 2) * (4 * LPT) + sub * 4 + (i & 3); }
@@ -51,24 +67,25 @@ template <int LPT, int P>
 __device__ __forceinline__ void load_row(const RouteParams& p, int64_t t, int sub, float (&l)[P]) {
     const float* const f = reinterpret_cast<const float*>(p.logits) + t * p.ld;
     const uint16_t* const h = reinterpret_cast<const uint16_t*>(p.logits) + t * p.ld;
-#pragma unroll
-    for (int q = 0; q < P / 4; ++q) {
+    each<P / 4>([&](auto q) {
         const int e = expert_of<LPT>(sub, q * 4);
-        if (e + 4 <= p.experts) {
+        u32 v[4];
+        if (p.experts == LPT * P || e + 4 <= p.experts) {
             if (p.bf16) {
-                const u16x4_any v = *reinterpret_cast<const u16x4_any*>(h + e);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) l[q * 4 + i] = bf16_to_f32(v[i]);
+                const u16x4_any w = *reinterpret_cast<const u16x4_any*>(h + e);
+                each<4>([&](auto i) { v[i] = (u32)w[i.value] << 16; });
             } else {
-                const f32x4_any v = *reinterpret_cast<const f32x4_any*>(f + e);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) l[q * 4 + i] = v[i];
+                const f32x4_any w = *reinterpret_cast<const f32x4_any*>(f + e);
+                each<4>([&](auto i) { v[i] = __builtin_bit_cast(u32, (float)w[i.value]); });
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) l[q * 4 + i] = e + i >= p.experts ? -__builtin_inff() : p.bf16 ? bf16_to_f32(h[e + i]) : f[e + i];
+            each<4>([&](auto i) {
+                v[i] = 0xff800000u;
+                if (e + i < p.experts) v[i] = p.bf16 ? (u32)h[e + i] << 16 : __builtin_bit_cast(u32, f[e + i]);
+            });
         }
-    }
+        each<4>([&](auto i) { l[q * 4 + i] = __builtin_bit_cast(float, v[i]); });
+    });
 }
 
 __device__ __forceinline__ float logit_at(const RouteParams& p, int64_t t, int e) {
@@ -87,6 +104,8 @@ __device__ __forceinline__ u32 other(u32 v) {
 }
 template <int M>
 __device__ __forceinline__ float other(float v) { return __builtin_bit_cast(float, other<M>(__builtin_bit_cast(u32, v))); }
+template <int M>
+__device__ __forceinline__ int other(int v) { return (int)other<M>((u32)v); }
 template <int M>
 __device__ __forceinline__ double other(double v) {
     const u64 b = __builtin_bit_cast(u64, v);
@@ -196,65 +215,60 @@ __device__ __forceinline__ int expert_of_key(double k) {
     return (int)(v >> 32) < 0 ? (int)(v & 1023) : 1023 - (int)(v & 1023);
 }
 
-// s of a token's experts, in 64 bits.
-template <int LPT, int P>
-__device__ __forceinline__ void scores64(const RouteParams& p, const float (&l)[P], float top, double (&s)[P]) {
-    if (p.softmax) {
-        double sum = 0;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            s[i] = exp((double)l[i] - (double)top);
-            sum += s[i];
-        }
-        sum = lanes_sum<LPT>(sum);
-#pragma unroll
-        for (int i = 0; i < P; ++i) s[i] /= sum;
-    } else {
-#pragma unroll
-        for (int i = 0; i < P; ++i) s[i] = 1.0 / (1.0 + exp(-(double)l[i]));
-    }
+// What a token's lanes, all of one wave, wrote to LDS before is there for the others after.
+__device__ __forceinline__ void lanes_wait() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int LPT, int P, int KP>
-__global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
-    // b of the workgroup's tokens, and the scores of their groups (at most one an expert)
-    __shared__ double b_of[kThreads * P];
-    __shared__ double group_of[kThreads * P];
-    const int tid = threadIdx.x, sub = tid % LPT, mine = tid / LPT;
-    const int64_t t = (int64_t)(blockIdx.x + p.vbase) * (kThreads / LPT) + mine;
-    const int64_t row = t < p.tokens ? t : p.tokens - 1;   // (lanes past the last token keep the others company)
-    float l[P];
-    load_row<LPT>(p, row, sub, l);
-    float top = l[0];
-#pragma unroll
-    for (int i = 1; i < P; ++i) top = fmaxf(top, l[i]);
-    top = lanes_max<LPT>(top);
-    top = top == -__builtin_inff() ? 0.f : top;   // (every expert out)
-
+// The choices of one token in 64 bits, by the whole wave: lane c has the id of choice c, -1 for none.  logits, rows [N]: its logits, and
+// room for b; sums [kMaxGroups].
+template <int N, int KP, bool SOFTMAX>
+__device__ __forceinline__ int choose64(const RouteParams& p, const float* logits, double* rows, double* sums) {
+    constexpr int P = N / 64;
+    const int lane = threadIdx.x & 63;
     double b[P];
-    if (p.by_logit) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) b[i] = l[i];
-    } else {
-        scores64<LPT>(p, l, top, b);
+    for (int i = 0; i < P; ++i) b[i] = logits[i * 64 + lane];   // (-inf past the last expert)
+    if (!p.by_logit) {
+        if constexpr (SOFTMAX) {
+            double top = b[0], sum = 0;
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int e = expert_of<LPT>(sub, i);
-            if (l[i] == -__builtin_inff()) b[i] = -__builtin_inf();
-            else if (p.bias != nullptr) b[i] += (double)p.bias[min(e, p.experts - 1)];
+            for (int i = 1; i < P; ++i) top = fmax(top, b[i]);
+            top = fmax(top, other<1>(top)); top = fmax(top, other<2>(top)); top = fmax(top, other<4>(top));
+            top = fmax(top, other<8>(top)); top = fmax(top, other<16>(top)); top = fmax(top, other<32>(top));
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                b[i] = b[i] == -__builtin_inf() ? b[i] : exp(b[i] - top);
+                if (b[i] != -__builtin_inf()) sum += b[i];
+            }
+            sum = lanes_sum<64>(sum);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (b[i] != -__builtin_inf()) b[i] /= sum;
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (b[i] != -__builtin_inf()) b[i] = 1.0 / (1.0 + exp(-b[i]));
+        }
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) b[i] += (double)p.bias[min(i * 64 + lane, p.experts - 1)];   // (an expert that is out stays out)
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (logits[i * 64 + lane] == -__builtin_inff()) b[i] = -__builtin_inf();   // (whatever its bias)
         }
     }
     if (p.groups > 1) {
-        double* const rows = b_of + mine * (LPT * P);
-        double* const sums = group_of + mine * (LPT * P);
 #pragma unroll
-        for (int i = 0; i < P; ++i) rows[expert_of<LPT>(sub, i)] = b[i];
-        __syncthreads();
-        for (int g = sub; g < p.groups; g += LPT) {
+        for (int i = 0; i < P; ++i) rows[i * 64 + lane] = b[i];
+        lanes_wait();
+        if (lane < p.groups) {
             double first = -__builtin_inf(), second = first;
             bool nan = false;
             for (int j = 0; j < p.per_group; ++j) {
-                const double v = rows[g * p.per_group + j];
+                const double v = rows[lane * p.per_group + j];
                 nan = nan || v != v;
                 second = fmax(second, fmin(first, v));
                 first = fmax(first, v);
@@ -262,42 +276,207 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
             // (a group of one expert, or with one left, has that one's b; NaN is the largest here too)
             double sum = first;
             if (p.group_top > 1 && second != -__builtin_inf()) sum += second;
-            sums[g] = nan || sum != sum ? kNan : sum == __builtin_inf() ? kInf : sum;
+            sums[lane] = nan || sum != sum ? kNan : sum == __builtin_inf() ? kInf : sum;
         }
-        __syncthreads();
+        lanes_wait();
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int e = expert_of<LPT>(sub, i);
+            const int e = i * 64 + lane;
             if (e >= p.experts) continue;
             const int g = (int)((u32)e * p.per_group_inv >> 21);
-            const double mine_sum = sums[g];
+            const double mine = sums[g];
             int before = 0;
-            for (int o = 0; o < p.groups; ++o) before += sums[o] > mine_sum || (sums[o] == mine_sum && o < g);
+            for (int o = 0; o < p.groups; ++o) before += sums[o] > mine || (sums[o] == mine && o < g);
             if (before >= p.keep) b[i] = -__builtin_inf();
         }
     }
     double list[KP];
 #pragma unroll
-    for (int i = 0; i < P; ++i) b[i] = key_of(b[i], expert_of<LPT>(sub, i));
-    largest<LPT, P, KP>(b, list, kOut * 1.5);
-
+    for (int i = 0; i < P; ++i) b[i] = key_of(b[i], i * 64 + lane);
+    largest<64, P, KP>(b, list, kOut * 1.5);
     int id = -1;
 #pragma unroll
     for (int c = 0; c < KP; ++c)
-        if (sub == c) id = expert_of_key(list[c]);
-    if (sub >= p.topk || sub >= KP) id = -1;
-    float w = 0.f, sum = 1.f;
-    if (p.softmax) {
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < P; ++i) sum += expf(l[i] - top);
-        sum = lanes_sum<LPT>(sum);
+        if (lane == c) id = expert_of_key(list[c]);
+    return id;
+}
+
+// In fp32: a number that stands for "out", far below all others but finite.
+constexpr float kLow = -0x1.8p127f;
+
+// s of a logit; softmax: `top` and the inverse of the sum.
+template <bool SOFTMAX>
+__device__ __forceinline__ float score32(float l, float top, float inv) {
+    if constexpr (SOFTMAX) return __expf(l - top) * inv;
+    else return __builtin_amdgcn_rcpf(1.f + __expf(-l));
+}
+
+template <int LPT, int P, int KP, bool SOFTMAX>
+__global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
+    // for the tokens that need 64 bits, one of a wave at a time; and, of every token, the groups' scores
+    __shared__ double rows64[kThreads / 64][LPT * P], sums64[kThreads / 64][kMaxGroups];
+    __shared__ float logits64[kThreads / 64][LPT * P];
+    __shared__ float sums_of[kThreads / LPT][kMaxGroups];
+    const int tid = threadIdx.x, sub = tid % LPT, mine = tid / LPT, wave = tid >> 6;
+    const int64_t t = (int64_t)(blockIdx.x + p.vbase) * (kThreads / LPT) + mine;
+    const int64_t row = t < p.tokens ? t : p.tokens - 1;   // (lanes past the last token keep the others company)
+    float l[P], b[P];
+    load_row<LPT>(p, row, sub, l);
+    if (p.bias != nullptr) {
+        RouteParams as_row = p;
+        as_row.logits = p.bias;
+        as_row.ld = as_row.bf16 = 0;
+        load_row<LPT>(as_row, 0, sub, b);
+    } else {
+        each<P>([&](auto i) {
+            b[i] = 0.f;
+        });
     }
+    float top = 0.f, inv = 1.f;
+    if constexpr (SOFTMAX) {
+        top = l[0];
+        each<P - 1>([&](auto from_1) {
+            constexpr int i = from_1 + 1;
+            top = fmaxf(top, l[i]);
+        });
+        top = lanes_max<LPT>(top);
+        top = top == -__builtin_inff() ? 0.f : top;   // (every expert out)
+        float sum = 0.f;
+        each<P>([&](auto i) {
+            sum += __expf(l[i] - top);
+        });
+        inv = 1.f / lanes_sum<LPT>(sum);
+    }
+    // b in fp32, and whether the row has a NaN, +inf or a finite number as low as kLow (then odd is NaN)
+    float odd = 0.f;
+    if (p.by_logit) {
+        each<P>([&](auto i) {
+            b[i] = l[i];
+        });
+    } else {
+        each<P>([&](auto i) {
+            b[i] += score32<SOFTMAX>(l[i], top, inv);
+        });
+    }
+    each<P>([&](auto i) {
+        if (l[i] == -__builtin_inff() || b[i] == -__builtin_inff()) b[i] = kLow;
+        else if (b[i] <= kLow) b[i] = __builtin_inff();
+        odd = __builtin_fmaf(b[i], 0.f, odd);
+    });
+    if (SOFTMAX && !p.by_logit) odd = __builtin_fmaf(top, 0.f, odd);
+    bool sure = lanes_sum<LPT>(odd) == 0.f;
+    // How far a difference of two b can be off, beside 2^-21 of their size (score32's steps are within 2^-22 of s, and softmax's sum
+    // within 2^-19 of itself; twice that and more).
+    const float slack = p.by_logit ? 0.f : SOFTMAX ? __builtin_fmaf(0x1p-17f, inv, 0x1p-21f) : 0x1p-20f;
+    const float relative = p.by_logit ? 0.f : 0x1p-21f;
+
+    if (p.groups > 1) {
+        float* const sums = sums_of[mine];
+        const int lanes = p.per_group >> 2;   // of a group, where it lies in a run of them
+        const int shift = p.group_lanes - 1, in_run = LPT >> shift;   // log2 of these; groups side by side in a token's lanes
+        if (p.group_lanes) {
+            each<P / 4>([&](auto q) {
+                float first = fmaxf(b[4 * q], b[4 * q + 1]), second = fminf(b[4 * q], b[4 * q + 1]);
+                each<4 - 2>([&](auto from_2) {
+                    constexpr int i = from_2 + 2;
+                    second = fmaxf(second, fminf(first, b[4 * q + i]));
+                    first = fmaxf(first, b[4 * q + i]);
+                });
+                auto join = [&](float f, float s) {
+                    second = fmaxf(fminf(first, f), fmaxf(second, s));
+                    first = fmaxf(first, f);
+                };
+                if (lanes > 1) join(other<1>(first), other<1>(second));
+                if (lanes > 2) join(other<2>(first), other<2>(second));
+                if (lanes > 4) join(other<4>(first), other<4>(second));
+                if (lanes > 8) join(other<8>(first), other<8>(second));
+                const int g = q * in_run + (sub >> shift);
+                if ((sub & (lanes - 1)) == 0 && g < p.groups) sums[g] = p.group_top > 1 && second > kLow ? first + second : first;
+            });
+        } else {
+            sure = false;   // (groups that do not lie so: in 64 bits)
+        }
+        lanes_wait();
+        if (p.group_lanes) {
+            int better[P / 4], near[P / 4];
+            float own[P / 4];
+            each<P / 4>([&](auto q) {
+                own[q] = sums[min(q * in_run + (sub >> shift), p.groups - 1)];
+                better[q] = near[q] = 0;
+            });
+#pragma unroll 4
+            for (int o = 0; o < p.groups; ++o) {
+                const float v = sums[o];
+                each<P / 4>([&](auto q) {
+                    const float off = 2.f * slack + 2.f * relative * fabsf(own[q]);
+                    better[q] += v > own[q] + off;
+                    near[q] += v >= own[q] - off;   // (itself among them)
+                });
+            }
+            each<P / 4>([&](auto q) {
+                const bool gone = better[q] >= p.keep;
+                if (!gone && near[q] > p.keep && q * in_run + (sub >> shift) < p.groups) sure = false;
+                each<4>([&](auto i) {
+                    b[4 * q + i] = gone ? kLow : b[4 * q + i];
+                });
+            });
+        }
+    }
+
+    constexpr u32 kIndex = LPT * P - 1;
+    u32 key[P], list[KP];
+    each<P>([&](auto i) {
+        const u32 f = __builtin_bit_cast(u32, b[i]);
+        const u32 order = f ^ ((u32)((int)f >> 31) | 0x80000000u);   // (as whole numbers compare)
+        key[i] = (b[i] == kLow ? 0u : order & ~kIndex) | (kIndex - (u32)expert_of<LPT>(sub, i));
+    });
+    largest<LPT, P, KP>(key, list, 0u);
+    int id = -1;
+    each<KP>([&](auto c) {
+        if (sub == c && list[c] > kIndex) id = (int)(kIndex - (list[c] & kIndex));
+    });
+    if (sub >= p.topk) id = -1;
+    float s = 0.f, at = kLow;
     if (id >= 0) {
         const float v = logit_at(p, row, id);
-        w = p.softmax ? expf(v - top) / sum : 1.f / (1.f + expf(-v));
+        s = score32<SOFTMAX>(v, top, inv);
+        at = p.by_logit ? v : s + (p.bias != nullptr ? p.bias[id] : 0.f);
     }
-    if (p.renormalize) w /= lanes_sum<16>(w) + kTiny;   // (the choices lie in a token's first 16 lanes)
+    if (!p.exact_keys) {
+        const int base = (tid & 63) - sub;
+        const float after = __shfl(at, min(base + sub + 1, 63)), last = __shfl(at, base + p.topk - 1);
+        const float off = slack + relative * fabsf(at), off_last = slack + relative * fabsf(last);
+        if (sub + 1 < p.topk && after != kLow && !(at - after > off)) sure = false;
+        if (last != kLow) {
+            int from = 0;
+            each<P>([&](auto i) {
+                from += b[i] >= last - off_last;
+            });
+            if (lanes_sum<LPT>(from) != p.topk) sure = false;
+        }
+    }
+    // (a token's lanes agree)
+    const u64 unsure = __ballot(!sure);
+    if (unsure != 0) {
+        constexpr u64 kLanes = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
+#pragma unroll 1
+        for (int o = 0; o < 64 / LPT; ++o) {
+            if (!(unsure >> (o * LPT) & kLanes)) continue;
+            const bool its = (tid & 63) / LPT == o;
+            if (its)
+                each<P>([&](auto i) {
+                    logits64[wave][expert_of<LPT>(sub, i)] = l[i];
+                });
+            lanes_wait();
+            const int found = __shfl(choose64<LPT * P, KP, SOFTMAX>(p, logits64[wave], rows64[wave], sums64[wave]), sub);
+            lanes_wait();
+            if (!its) continue;
+            id = sub < p.topk ? found : -1;
+            s = id >= 0 ? score32<SOFTMAX>(logit_at(p, row, id), top, inv) : 0.f;
+        }
+    }
+    float w = s;
+    if (p.renormalize) w /= lanes_sum<16>(s) + kTiny;   // (the choices lie in a token's first 16 lanes)
     if (t < p.tokens && sub < p.topk) {
         p.ids[t * p.topk + sub] = id;
         p.weights[t * p.topk + sub] = id >= 0 ? w * p.scale : 0.f;
@@ -406,18 +585,19 @@ typedef void (*RouteKernel)(const RouteParams);
 
 // Lanes to a token and experts to a lane: 16 lanes are a row whose exchanges are single instructions; past 256 experts more lanes.
 template <bool BACKWARD, int LPT, int P>
-RouteKernel pick_topk(int topk) {
+RouteKernel pick_topk(int topk, bool softmax) {
     if constexpr (BACKWARD) return &route_backward_kernel<LPT, P>;
-    else return topk <= 4 ? &route_kernel<LPT, P, 4> : topk <= 8 ? &route_kernel<LPT, P, 8> : &route_kernel<LPT, P, 16>;
+    else if (softmax) return topk <= 4 ? &route_kernel<LPT, P, 4, true> : topk <= 8 ? &route_kernel<LPT, P, 8, true> : &route_kernel<LPT, P, 16, true>;
+    else return topk <= 4 ? &route_kernel<LPT, P, 4, false> : topk <= 8 ? &route_kernel<LPT, P, 8, false> : &route_kernel<LPT, P, 16, false>;
 }
 
 template <bool BACKWARD>
-RouteKernel pick(int experts, int topk, int& lanes) {
+RouteKernel pick(int experts, int topk, bool softmax, int& lanes) {
     lanes = experts <= 256 ? 16 : experts <= 512 ? 32 : 64;
-    if (experts <= 64) return pick_topk<BACKWARD, 16, 4>(topk);
-    if (experts <= 128) return pick_topk<BACKWARD, 16, 8>(topk);
-    if (experts <= 256) return pick_topk<BACKWARD, 16, 16>(topk);
-    return experts <= 512 ? pick_topk<BACKWARD, 32, 16>(topk) : pick_topk<BACKWARD, 64, 16>(topk);
+    if (experts <= 64) return pick_topk<BACKWARD, 16, 4>(topk, softmax);
+    if (experts <= 128) return pick_topk<BACKWARD, 16, 8>(topk, softmax);
+    if (experts <= 256) return pick_topk<BACKWARD, 16, 16>(topk, softmax);
+    return experts <= 512 ? pick_topk<BACKWARD, 32, 16>(topk, softmax) : pick_topk<BACKWARD, 64, 16>(topk, softmax);
 }
 
 template <bool BACKWARD>
@@ -431,6 +611,7 @@ int route_run(const dg_moe_route_args* a, void* stream) {
     if (a->logits_ld < a->experts || (BACKWARD && a->d_logits_ld < a->experts)) return dg_set_error("dg_moe_route: leading dimension smaller than the row");
     if (!BACKWARD) {
         if (a->num_groups < 1 || a->experts % a->num_groups != 0) return dg_set_error("dg_moe_route: the groups must divide the experts");
+        if (a->num_groups > kMaxGroups) return dg_set_error("dg_moe_route: at most 64 groups");
         if (a->topk_groups < 1 || a->topk_groups > a->num_groups) return dg_set_error("dg_moe_route: topk_groups must be between 1 and num_groups");
         if (a->group_top != 1 && a->group_top != 2) return dg_set_error("dg_moe_route: group_top is 1 or 2");
         if (a->topk > a->topk_groups * (a->experts / a->num_groups)) return dg_set_error("dg_moe_route: topk is more than the kept groups' experts");
@@ -468,10 +649,13 @@ int route_run(const dg_moe_route_args* a, void* stream) {
         p.group_top = a->group_top;
         p.bias = a->bias;
         p.by_logit = a->bias == nullptr && (p.groups == 1 || a->group_top == 1);
+        p.exact_keys = p.by_logit && p.bf16;
+        const int in_group = p.per_group >> 2;
+        if (p.per_group % 4 == 0 && (in_group & (in_group - 1)) == 0 && in_group <= 16) p.group_lanes = 1 + __builtin_ctz(in_group);
         p.weights = a->weights;
     }
     int lanes = 0;
-    const RouteKernel kernel = pick<BACKWARD>(a->experts, a->topk, lanes);
+    const RouteKernel kernel = pick<BACKWARD>(a->experts, a->topk, p.softmax, lanes);
     return launch_op(kernel, ceil_div64(a->tokens, kThreads / lanes), kThreads, p, st, a->num_cus);
 }
 
