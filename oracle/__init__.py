@@ -18,6 +18,7 @@ It restates, in plain CPU torch / numpy, the reference's own reference math:
 * ``moe``, ``mx``, ``loss`` -- the operators around the GEMMs (tokens sorted by expert and moved, quantisation in
                  blocks of 32, cross entropy of a linear layer) from their definitions in 64 bits; the
                  reference has none of them.
+* ``blocks``  -- what stands between the products (routing, the norm, the gated activation, adapters), likewise.
 * ``epilogue`` -- stochastic bf16 rounding (``tests/utils.py:70-92``) and FP8 output
                  quantisation (``tests/test_einsum.py:70-86``).
 
