@@ -292,28 +292,24 @@ __global__ __launch_bounds__(256) void norm_weight_kernel(const NormParams p) {
 
 typedef void (*NormKernel)(const NormParams);
 
-// Few tokens: a workgroup to a row, as wide as the row allows, one step or few.  Otherwise a wave to a row up to 2048 values, a workgroup
-// of 256 threads up to 16384, of 512 up to 32768, whose rows follow each other.
+// A workgroup to a row, as wide as the row allows; many short rows go to a wave each, four side by side (8192 x 1024 12.7 -> 11.1 us, to
+// e4m3 13.9 -> 11.8).  Rows that follow each other in a workgroup of 256 threads, whose exponent bytes then leave as runs of eight rows, wait
+// for each other's sums: 1024 x 7168 to e4m3 34.6 us in place of 11.3, 4096 x 7168 62 in place of 42.
 template <typename E, int FMT>
 NormKernel pick_forward(int tokens, int width, unsigned& threads, int& rows) {
-    if (tokens <= 512) {
-        rows = 1;
-        threads = width <= 2048 ? 256 : 1024;
-        if (width <= 2048) return &norm_kernel<E, FMT, 256, 1, 1>;
-        if (width <= 8192) return &norm_kernel<E, FMT, 1024, 1, 1>;
-        if (width <= 16384) return &norm_kernel<E, FMT, 1024, 2, 1>;
-        return &norm_kernel<E, FMT, 1024, 4, 1>;
+    if (width <= 1024 && tokens > 2048) {
+        rows = FMT >= 0 ? 8 : 4;
+        threads = 256;
+        if (width <= 512) return &norm_kernel<E, FMT, 64, 1, FMT >= 0 ? 8 : 4>;
+        return &norm_kernel<E, FMT, 64, 2, FMT >= 0 ? 8 : 4>;
     }
-    constexpr int ROWS = FMT >= 0 ? 8 : 4;
-    rows = ROWS;
-    threads = width <= 16384 ? 256 : 512;
-    if (width <= 512) return &norm_kernel<E, FMT, 64, 1, ROWS>;
-    if (width <= 1024) return &norm_kernel<E, FMT, 64, 2, ROWS>;
-    if (width <= 2048) return &norm_kernel<E, FMT, 64, 4, ROWS>;
-    if (width <= 4096) return &norm_kernel<E, FMT, 256, 2, ROWS>;
-    if (width <= 8192) return &norm_kernel<E, FMT, 256, 4, ROWS>;
-    if (width <= 16384) return &norm_kernel<E, FMT, 256, 8, ROWS>;
-    return &norm_kernel<E, FMT, 512, 8, ROWS>;
+    rows = 1;
+    threads = width <= 2048 ? 256 : width <= 4096 ? 512 : 1024;
+    if (width <= 2048) return &norm_kernel<E, FMT, 256, 1, 1>;
+    if (width <= 4096) return &norm_kernel<E, FMT, 512, 1, 1>;
+    if (width <= 8192) return &norm_kernel<E, FMT, 1024, 1, 1>;
+    if (width <= 16384) return &norm_kernel<E, FMT, 1024, 2, 1>;
+    return &norm_kernel<E, FMT, 1024, 4, 1>;
 }
 
 // Rows that a workgroup of the gradient holds at once.
