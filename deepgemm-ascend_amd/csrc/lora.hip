@@ -519,10 +519,11 @@ int64_t live_tiles(const dg_lora_args* a, int rows) {
     return std::max<int64_t>(1, std::min<int64_t>(ceil_div(a->layout->rows, rows), ceil_div(a->tokens, rows) + std::min(a->tokens, a->adapters)));
 }
 
-// One launch where what its strips read more than once is little, for a workgroup (a CU draws about 20 KB/us) and for all of them.
+// One launch where every strip has a CU to itself and reads little there for its inner products (a CU draws about 20 KB/us; 48 tokens over
+// 20 adapters, rank 16, K=7168 N=4096, 229 KB: 13.1 us, and by two launches 10.7; 511 tokens over 8, K=4096, 320 strips: 20.9 and 11.9).
 bool one_launch(const dg_lora_args* a) {
     const int64_t bytes = (int64_t)padded_rank(a->rank) * a->k * 2;
-    return padded_rank(a->rank) <= 64 && bytes <= (160 << 10) && live_tiles(a, 16) * ceil_div(a->n, 512) * bytes <= (int64_t(64) << 20);
+    return padded_rank(a->rank) <= 64 && bytes <= (160 << 10) && live_tiles(a, 16) * ceil_div(a->n, 512) <= 256;
 }
 
 // Ranges of k: enough that the tiles which hold tokens fill the card, at least 512 of k each.
