@@ -317,6 +317,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
     __shared__ double rows64[kThreads / 64][LPT * P], sums64[kThreads / 64][kMaxGroups];
     __shared__ float logits64[kThreads / 64][LPT * P];
     __shared__ float sums_of[kThreads / LPT][kMaxGroups];
+    __shared__ float rows_of[kThreads / LPT][LPT * P];   // b, for groups that are no run of lanes
     const int tid = threadIdx.x, sub = tid % LPT, mine = tid / LPT, wave = tid >> 6;
     const int64_t t = (int64_t)(blockIdx.x + p.vbase) * (kThreads / LPT) + mine;
     const int64_t row = t < p.tokens ? t : p.tokens - 1;   // (lanes past the last token keep the others company)
@@ -394,9 +395,46 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
                 if ((sub & (lanes - 1)) == 0 && g < p.groups) sums[g] = p.group_top > 1 && second > kLow ? first + second : first;
             });
         } else {
-            sure = false;   // (groups that do not lie so: in 64 bits)
+            float* const rows = rows_of[mine];
+            each<P>([&](auto i) { rows[expert_of<LPT>(sub, i)] = b[i]; });
+            lanes_wait();
+            for (int g = sub; g < p.groups; g += LPT) {
+                float first = kLow, second = kLow;
+                for (int j = 0; j < p.per_group; ++j) {
+                    const float v = rows[g * p.per_group + j];
+                    second = fmaxf(second, fminf(first, v));
+                    first = fmaxf(first, v);
+                }
+                sums[g] = p.group_top > 1 && second > kLow ? first + second : first;
+            }
         }
         lanes_wait();
+        if (!p.group_lanes) {
+            // a group's place, by the lane that has its score; then what becomes of it, in the place of the score
+            float state[kMaxGroups / LPT];
+            each<kMaxGroups / LPT>([&](auto q) {
+                const int g = q * LPT + sub;
+                state[q] = 0.f;
+                if (g >= p.groups) return;
+                const float own = sums[g], off = 2.f * slack + 2.f * relative * fabsf(own);
+                int better = 0, near = 0;
+                for (int o = 0; o < p.groups; ++o) {
+                    better += sums[o] > own + off;
+                    near += sums[o] >= own - off;   // (itself among them)
+                }
+                if (better < p.keep && near > p.keep) sure = false;
+                state[q] = better >= p.keep ? 1.f : 0.f;
+            });
+            lanes_wait();
+            each<kMaxGroups / LPT>([&](auto q) {
+                if (q * LPT + sub < p.groups) sums[q * LPT + sub] = state[q];
+            });
+            lanes_wait();
+            each<P>([&](auto i) {
+                const u32 e = (u32)min(expert_of<LPT>(sub, i), p.experts - 1);
+                if (sums[e * p.per_group_inv >> 21] != 0.f) b[i] = kLow;
+            });
+        }
         if (p.group_lanes) {
             int better[P / 4], near[P / 4];
             float own[P / 4];
