@@ -97,7 +97,8 @@ __device__ __forceinline__ void inner_products(const LoraParams& p, int i, const
     }
 }
 
-// v of TT times 16 rows of one adapter over a range of k: the four waves take a quarter each and join through LDS.
+// v of TT times 16 rows of one adapter over a range of k: the four waves take a quarter each and join through LDS.  4099 tokens, rank 32,
+// K=2048 9.4 us (17 MB of x); 48 tokens over 20 adapters, rank 16, K=7168 4.6.
 template <int NT, int TT>
 __global__ __launch_bounds__(kThreads) void lora_inner_kernel(const LoraParams p) {
     __shared__ f32x4 part[4][TT * NT][64];
@@ -351,7 +352,8 @@ __global__ __launch_bounds__(kThreads) void lora_outer_kernel(const LoraParams p
 }
 
 // Many tokens: d of 32 rows (one adapter's) in pieces of 256 columns, which pass through LDS so that half a wave reads and writes 256
-// columns of a token; the next piece of c is on its way meanwhile.
+// columns of a token; the next piece of c is on its way meanwhile.  4099 tokens over 8 adapters, rank 32, N=7168: 33 us (117 MB, 3.5 TB/s;
+// straight to memory in runs of 32 columns by 16 rows 43, by 64 rows 51, in LDS pieces of 512 columns without the next one 40).
 template <int NT, typename E>
 __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p) {
     __shared__ Operand<NT> operand[2];
@@ -429,7 +431,8 @@ __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p)
 }
 
 // Few tokens: both products in one launch.  Every strip of 512 columns computes its tile's inner products for itself (sixteen waves, a
-// sixteenth of k each, from the XCD's L2), which costs less than a second launch that waits for the first.
+// sixteenth of k each, from the XCD's L2), which costs less than a second launch that waits for the first: one token, rank 16, K=4096
+// N=7168 7.5 us.
 template <int NT, typename E>
 __global__ __launch_bounds__(1024) void lora_kernel(const LoraParams p) {
     __shared__ f32x4 part[16][NT][64];

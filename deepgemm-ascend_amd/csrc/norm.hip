@@ -77,7 +77,8 @@ __device__ __forceinline__ void load_weight(Eight<float>& w, const NormParams& p
 }
 
 // FMT: -1 values, DG_MX_*.  THREADS hold a row (64: the workgroup's four waves hold one each), V steps of eight values a thread.
-// ROWS rows to a workgroup, so that exponent bytes leave as runs of rows.
+// ROWS rows to a workgroup, so that exponent bytes leave as runs of rows.  Bound by the bytes: 8192 x 4096 bf16 with residual 44 us (6.1
+// TB/s), 4096 x 7168 to e4m3 40 (5.1); 16 x 7168 to e4m3 3.9, one chain of loads, sum and stores.
 template <typename E, int FMT, int THREADS, int V, int ROWS>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_kernel(const NormParams p) {
     constexpr int WG = THREADS < 256 ? 256 : THREADS, AT_ONCE = WG / THREADS;
@@ -179,7 +180,8 @@ struct BackwardRow {
 };
 
 // TEAMS of THREADS hold a row each and step through the tokens together; the next rows (bf16) are in flight while a row is summed.
-// d_weight is summed over a team's rows in registers, over the teams in LDS, in order.
+// d_weight is summed over a team's rows in registers, over the teams in LDS, in order.  8192 x 4096 bf16 52 us (5.2 TB/s; 82 with two
+// workgroups of one row a CU that read a row when they are done with the one before), and 5 for the partial sums.
 template <typename E, int THREADS, int TEAMS, int V>
 __global__ __launch_bounds__(THREADS * TEAMS) void norm_backward_kernel(const NormParams p) {
     constexpr bool AHEAD = sizeof(E) == 2 && V <= 2;

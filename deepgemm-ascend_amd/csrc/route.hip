@@ -303,6 +303,7 @@ __device__ __forceinline__ int choose64(const RouteParams& p, const float* logit
 
 // In fp32: a number that stands for "out", far below all others but finite.
 constexpr float kLow = -0x1.8p127f;
+constexpr float kHuge = 0x1p126f;   // (a group's sum past this may have left fp32)
 
 // s of a logit; softmax: `top` and the inverse of the sum.
 template <bool SOFTMAX>
@@ -422,7 +423,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
                     better += sums[o] > own + off;
                     near += sums[o] >= own - off;   // (itself among them)
                 }
-                if (better < p.keep && near > p.keep) sure = false;
+                if ((better < p.keep && near > p.keep) || (own != kLow && !(fabsf(own) < kHuge))) sure = false;
                 state[q] = better >= p.keep ? 1.f : 0.f;
             });
             lanes_wait();
@@ -453,7 +454,8 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
             }
             each<P / 4>([&](auto q) {
                 const bool gone = better[q] >= p.keep;
-                if (!gone && near[q] > p.keep && q * in_run + (sub >> shift) < p.groups) sure = false;
+                const bool doubt = (!gone && near[q] > p.keep) || (own[q] != kLow && !(fabsf(own[q]) < kHuge));
+                if (doubt && q * in_run + (sub >> shift) < p.groups) sure = false;
                 each<4>([&](auto i) {
                     b[4 * q + i] = gone ? kLow : b[4 * q + i];
                 });
@@ -619,6 +621,9 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(const RoutePar
     }
 }
 
+// 32768 tokens over 256 experts in 8 groups: 27 us (36 MB; the bytes take 7), of which the exponentials, the sorting of 16 keys a lane
+// and the joining of four times eight are most; 16 tokens 5.3, a chain of loads, sums and exchanges.  Logits in bf16 with a bias of
+// zeros have many equal scores, which go through 64 bits: 62.  Gradient: 8191 tokens over 160 experts 7.1.
 typedef void (*RouteKernel)(const RouteParams);
 
 // Lanes to a token and experts to a lane: 16 lanes are a row whose exchanges are single instructions; past 256 experts more lanes.

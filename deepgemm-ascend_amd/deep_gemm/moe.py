@@ -42,7 +42,7 @@ def moe_num_rows(num_pairs: int, num_groups: int) -> int:
 
 
 _SCORES = {'softmax': _lib.DG_SCORES_SOFTMAX, 'sigmoid': _lib.DG_SCORES_SIGMOID}
-MAX_EXPERTS, MAX_TOPK = 1024, 16
+MAX_EXPERTS, MAX_TOPK, MAX_EXPERT_GROUPS = 1024, 16, 64
 
 
 def _route_args(logits: torch.Tensor, topk: int, scores: str, renormalize: bool, scale: float) -> Tuple[torch.Tensor, _lib.MoERouteArgs]:
@@ -65,7 +65,7 @@ def moe_route(logits: torch.Tensor, topk: int, scores: str = 'softmax', bias: Op
     router's ``logits`` [T, E] (bf16 or fp32, E at most 1024, topk at most 16).
 
     Scores s are the ``softmax`` of a row or the ``sigmoid`` of each logit.  ``bias`` [E] (fp32; for balance) is added for the choice
-    alone.  With ``num_groups`` > 1 the experts lie in that many groups of equal size, and the ``topk_groups`` groups whose
+    alone.  With ``num_groups`` > 1 (at most 64) the experts lie in that many groups of equal size, and the ``topk_groups`` groups whose
     ``group_top`` (1 or 2) best biased scores have the largest sum stay.  The topk best biased scores there are chosen, best first, equal
     ones by the lowest index, compared as 64 bits give them (numbers nearer than 2^-42 relative count as equal).
     ``renormalize``: weights s / (sum of the chosen s + 1e-20) instead of s; both times ``scale``.
@@ -81,6 +81,7 @@ def moe_route(logits: torch.Tensor, topk: int, scores: str = 'softmax', bias: Op
             return made[0], made[1]
     logits, a = _route_args(logits, topk, scores, renormalize, scale)
     e = logits.size(1)
+    _assert(num_groups <= MAX_EXPERT_GROUPS, f'at most {MAX_EXPERT_GROUPS} groups of experts')
     _assert(num_groups >= 1 and e % num_groups == 0, f'{num_groups} groups do not divide {e} experts')
     _assert(1 <= topk_groups <= num_groups, 'topk_groups must be between 1 and num_groups')
     _assert(group_top in (1, 2), 'group_top must be 1 or 2')

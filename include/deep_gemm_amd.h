@@ -391,7 +391,7 @@ int dg_linear_xent_backward(const dg_linear_xent_args *args, void *stream);
 /*
  * Routing: the experts of a token from the router's logits l [tokens][experts] (bf16 or fp32, at most 1024 experts).
  *   s = softmax(l) or 1 / (1 + exp(-l));   b = s + bias (NULL: 0)
- *   With num_groups > 1 (a divisor of experts) a group's score is the sum of its group_top (1 or 2) largest b, and the topk_groups
+ *   With num_groups > 1 (a divisor of experts, at most 64) a group's score is the sum of its group_top (1 or 2) largest b, and the topk_groups
  *   groups of the largest scores stay.  ids = the topk (at most 16) experts of the largest b there, largest first;
  *   weights = s[ids], renormalize: divided by (their sum + 1e-20), times scale.
  * Equal numbers go to the lowest index; b and the scores are compared as 64 bits give them.  An expert whose logit or bias is -inf
