@@ -230,7 +230,7 @@ __device__ __forceinline__ int choose64(const RouteParams& p, const float* logit
     const int lane = threadIdx.x & 63;
     double b[P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) b[i] = logits[i * 64 + lane];   // (-inf past the last expert)
+    for (int i = 0; i < P; ++i) b[i] = (double)logits[i * 64 + lane] + 0.0;   // (-inf past the last expert; -0 becomes +0)
     if (!p.by_logit) {
         if constexpr (SOFTMAX) {
             double top = b[0], sum = 0;
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
     float odd = 0.f;
     if (p.by_logit) {
         each<P>([&](auto i) {
-            b[i] = l[i];
+            b[i] = l[i] + 0.f;   // (-0 becomes +0: keys tell them apart, numbers do not)
         });
     } else {
         each<P>([&](auto i) {

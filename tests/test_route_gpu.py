@@ -188,3 +188,22 @@ def test_nothing_to_do_and_dropped_rows():
     ids, w = deep_gemm.moe_route(out, 2)
     for kind in ('softmax', 'sigmoid'):
         assert (deep_gemm.moe_route_backward(torch.ones(4, 2, device='cuda'), out, ids, kind) == 0).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('kind', ['softmax', 'sigmoid'])
+def test_zeros_of_either_sign_are_equal(dtype, kind):
+    """As logits that were multiplied by a mask hold them: the lowest index among them, of experts and of groups."""
+    g = gen(11)
+    zero = torch.where(torch.rand(40, 96, generator=g) < 0.5, -0.0, 0.0)
+    logits = torch.where(torch.rand(40, 96, generator=g) < 0.3, zero, -torch.rand(40, 96, generator=g) - 0.1).to(dtype)
+    logits[0], logits[1] = -1, -1
+    logits[0, [3, 10]], logits[1, [3, 10]] = torch.tensor([-0.0, 0.0]).to(dtype), torch.tensor([0.0, -0.0]).to(dtype)
+    logits[2] = zero[2]
+    for topk in (1, 8):
+        _check(logits, topk, kind)
+        for groups in (8, 12, 16):   # (12: groups that are a run of lanes; 8 and 16: that are none)
+            for group_top in (1, 2):
+                _check(logits, min(topk, 3 * (96 // groups)), kind, num_groups=groups, topk_groups=3, group_top=group_top)
+    ids, _ = deep_gemm.moe_route(logits[:2].cuda(), 2, kind)
+    assert ids.tolist() == [[3, 10], [3, 10]]
