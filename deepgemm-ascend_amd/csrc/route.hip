@@ -303,7 +303,7 @@ __device__ __forceinline__ int choose64(const RouteParams& p, const float* logit
 
 // In fp32: a number that stands for "out", far below all others but finite.
 constexpr float kLow = -0x1.8p127f;
-constexpr float kHuge = 0x1p126f;   // (a group's sum past this may have left fp32)
+constexpr float kHuge = 0x1p126f;   // (a group's sum of numbers past this may have left fp32)
 
 // s of a logit; softmax: `top` and the inverse of the sum.
 template <bool SOFTMAX>
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
     // for the tokens that need 64 bits, one of a wave at a time; and, of every token, the groups' scores
     __shared__ double rows64[kThreads / 64][LPT * P], sums64[kThreads / 64][kMaxGroups];
     __shared__ float logits64[kThreads / 64][LPT * P];
-    __shared__ float sums_of[kThreads / LPT][kMaxGroups];
+    __shared__ f32x2 sums_of[kThreads / LPT][kMaxGroups];
     __shared__ float rows_of[kThreads / LPT][LPT * P];   // b, for groups that are no run of lanes
     const int tid = threadIdx.x, sub = tid % LPT, mine = tid / LPT, wave = tid >> 6;
     const int64_t t = (int64_t)(blockIdx.x + p.vbase) * (kThreads / LPT) + mine;
@@ -373,7 +373,15 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
     const float relative = p.by_logit ? 0.f : 0x1p-21f;
 
     if (p.groups > 1) {
-        float* const sums = sums_of[mine];
+        // A group's sum, as the least and the most that it can be.  Its terms may cancel, so the size of these counts, not of the sum.
+        f32x2* const sums = sums_of[mine];
+        auto put = [&](int g, float first, float second) {
+            const bool two = p.group_top > 1 && second > kLow;
+            const float sum = two ? first + second : first, size = fabsf(first) + (two ? fabsf(second) : 0.f);
+            const float off = slack + relative * size;
+            sums[g] = f32x2{sum - off, sum + off};
+            if (first != kLow && !(size < kHuge)) sure = false;
+        };
         const int lanes = p.per_group >> 2;   // of a group, where it lies in a run of them
         const int shift = p.group_lanes - 1, in_run = LPT >> shift;   // log2 of these; groups side by side in a token's lanes
         if (p.group_lanes) {
@@ -393,7 +401,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
                 if (lanes > 4) join(other<4>(first), other<4>(second));
                 if (lanes > 8) join(other<8>(first), other<8>(second));
                 const int g = q * in_run + (sub >> shift);
-                if ((sub & (lanes - 1)) == 0 && g < p.groups) sums[g] = p.group_top > 1 && second > kLow ? first + second : first;
+                if ((sub & (lanes - 1)) == 0 && g < p.groups) put(g, first, second);
             });
         } else {
             float* const rows = rows_of[mine];
@@ -406,7 +414,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
                     second = fmaxf(second, fminf(first, v));
                     first = fmaxf(first, v);
                 }
-                sums[g] = p.group_top > 1 && second > kLow ? first + second : first;
+                put(g, first, second);
             }
         }
         lanes_wait();
@@ -417,45 +425,43 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
                 const int g = q * LPT + sub;
                 state[q] = 0.f;
                 if (g >= p.groups) return;
-                const float own = sums[g], off = 2.f * slack + 2.f * relative * fabsf(own);
+                const f32x2 own = sums[g];
                 int better = 0, near = 0;
                 for (int o = 0; o < p.groups; ++o) {
-                    better += sums[o] > own + off;
-                    near += sums[o] >= own - off;   // (itself among them)
+                    better += sums[o][0] > own[1];
+                    near += sums[o][1] >= own[0];   // (itself among them)
                 }
-                if ((better < p.keep && near > p.keep) || (own != kLow && !(fabsf(own) < kHuge))) sure = false;
+                if (better < p.keep && near > p.keep) sure = false;
                 state[q] = better >= p.keep ? 1.f : 0.f;
             });
             lanes_wait();
             each<kMaxGroups / LPT>([&](auto q) {
-                if (q * LPT + sub < p.groups) sums[q * LPT + sub] = state[q];
+                if (q * LPT + sub < p.groups) sums[q * LPT + sub][0] = state[q];
             });
             lanes_wait();
             each<P>([&](auto i) {
                 const u32 e = (u32)min(expert_of<LPT>(sub, i), p.experts - 1);
-                if (sums[e * p.per_group_inv >> 21] != 0.f) b[i] = kLow;
+                if (sums[e * p.per_group_inv >> 21][0] != 0.f) b[i] = kLow;
             });
         }
         if (p.group_lanes) {
             int better[P / 4], near[P / 4];
-            float own[P / 4];
+            f32x2 own[P / 4];
             each<P / 4>([&](auto q) {
                 own[q] = sums[min(q * in_run + (sub >> shift), p.groups - 1)];
                 better[q] = near[q] = 0;
             });
 #pragma unroll 4
             for (int o = 0; o < p.groups; ++o) {
-                const float v = sums[o];
+                const f32x2 v = sums[o];
                 each<P / 4>([&](auto q) {
-                    const float off = 2.f * slack + 2.f * relative * fabsf(own[q]);
-                    better[q] += v > own[q] + off;
-                    near[q] += v >= own[q] - off;   // (itself among them)
+                    better[q] += v[0] > own[q][1];
+                    near[q] += v[1] >= own[q][0];   // (itself among them)
                 });
             }
             each<P / 4>([&](auto q) {
                 const bool gone = better[q] >= p.keep;
-                const bool doubt = (!gone && near[q] > p.keep) || (own[q] != kLow && !(fabsf(own[q]) < kHuge));
-                if (doubt && q * in_run + (sub >> shift) < p.groups) sure = false;
+                if (!gone && near[q] > p.keep && q * in_run + (sub >> shift) < p.groups) sure = false;
                 each<4>([&](auto i) {
                     b[4 * q + i] = gone ? kLow : b[4 * q + i];
                 });

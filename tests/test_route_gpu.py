@@ -207,3 +207,15 @@ def test_zeros_of_either_sign_are_equal(dtype, kind):
                 _check(logits, min(topk, 3 * (96 // groups)), kind, num_groups=groups, topk_groups=3, group_top=group_top)
     ids, _ = deep_gemm.moe_route(logits[:2].cuda(), 2, kind)
     assert ids.tolist() == [[3, 10], [3, 10]]
+
+
+@pytest.mark.parametrize('experts,groups', [(4, 2), (64, 8), (256, 8), (60, 10), (96, 16)])
+@pytest.mark.parametrize('kind', ['softmax', 'sigmoid'])
+def test_sums_of_groups_that_cancel(experts, groups, kind):
+    """The two best of a group lie far from each other and from zero: their sum is small, its rounding in fp32 is not."""
+    per = experts // groups
+    logits = _logits(600, experts, seed=21)
+    for big in (2.0 ** 12, 2.0 ** 16, 1e6, 2.0 ** 20):
+        bias = torch.full((experts,), -big)
+        bias[torch.arange(groups) * per + torch.arange(groups) % per] = big
+        _check(logits, 1, kind, bias, num_groups=groups, topk_groups=1)
