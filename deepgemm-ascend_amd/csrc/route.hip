@@ -254,10 +254,12 @@ __device__ __forceinline__ int choose64(const RouteParams& p, const float* logit
         }
         if (p.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) b[i] += (double)p.bias[min(i * 64 + lane, p.experts - 1)];   // (an expert that is out stays out)
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-                if (logits[i * 64 + lane] == -__builtin_inff()) b[i] = -__builtin_inf();   // (whatever its bias)
+            for (int i = 0; i < P; ++i) {
+                // (an expert that is out by its logit or its bias stays out, whatever the other is and beside NaN)
+                const float bias = p.bias[min(i * 64 + lane, p.experts - 1)];
+                b[i] += (double)bias;
+                if (logits[i * 64 + lane] == -__builtin_inff() || bias == -__builtin_inff()) b[i] = -__builtin_inf();
+            }
         }
     }
     if (p.groups > 1) {

@@ -219,3 +219,22 @@ def test_sums_of_groups_that_cancel(experts, groups, kind):
         bias = torch.full((experts,), -big)
         bias[torch.arange(groups) * per + torch.arange(groups) % per] = big
         _check(logits, 1, kind, bias, num_groups=groups, topk_groups=1)
+
+
+@pytest.mark.parametrize('kind', ['softmax', 'sigmoid'])
+def test_closed_experts_beside_nan_stay_closed(kind):
+    closed = torch.randn(64, generator=gen(8)) * 0.1
+    closed[:20] = -INF
+    closed[40:48] = -INF                 # (a whole group of eight among them)
+    logits = _logits(6, 64)
+    logits[1, 3] = float('nan')          # a closed expert's own logit
+    logits[2, [3, 30]] = float('nan')
+    logits[3, [5, 33]] = INF
+    logits[4] = float('nan')
+    logits[5, 21:] = float('nan')
+    logits[5, 25] = -INF
+    for groups, keep in ((1, 1), (8, 3), (16, 6)):
+        ids, _ = deep_gemm.moe_route(logits.cuda(), 6, kind, closed.cuda(), groups, keep)
+        want, _ = ob.route(logits, 6, kind, closed, groups, keep)
+        assert torch.equal(ids.cpu(), want)
+        assert (closed[ids[ids >= 0].long().cpu()] > -INF).all()
