@@ -10,7 +10,7 @@
 //
 // Keys of 32 bits select quickly but not surely: 22 to 26 bits of a score in fp32.  The choice is then checked against the scores
 // themselves: every chosen one above the next, and the last above all others, by more than fp32 can be off.  A token that fails
-// (about one in a hundred, and rows with infinities or NaN) is done again in 64 bits.
+// (about one in a hundred, and rows with infinities or NaN) is done again in 64 bits, whose keys' choice is checked likewise, exactly.
 #include "op_launch.hpp"
 
 #include <utility>
@@ -112,6 +112,13 @@ __device__ __forceinline__ double other(double v) {
     return __builtin_bit_cast(double, (u64)other<M>((u32)(b >> 32)) << 32 | other<M>((u32)b));
 }
 
+// The next lane's value, within a row of 16 lanes.
+__device__ __forceinline__ int after(int v) { return __builtin_amdgcn_mov_dpp(v, 0x101, 0xf, 0xf, true); }   // row_shl:1
+__device__ __forceinline__ double after(double v) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    return __builtin_bit_cast(double, (u64)(u32)after((int)(b >> 32)) << 32 | (u32)after((int)b));
+}
+
 template <int LPT, typename T>
 __device__ __forceinline__ T lanes_sum(T v) {
     v += other<1>(v); v += other<2>(v); v += other<4>(v); v += other<8>(v);
@@ -199,15 +206,16 @@ __device__ __forceinline__ void largest(const T (&key)[P], T (&top)[KP], T none)
     if constexpr (LPT > 32) join_lanes<32>(top);
 }
 
-// A number as a key: its low ten bits give way to the expert's index (the lower, the larger).  Finite numbers here are far from a
-// double's largest, where experts that are out, infinity and NaN (the largest) have their places.
+// Finite numbers here are far from a double's largest, where experts that are out, infinity and NaN (the largest) have their places.
 constexpr double kOut = -0x1p1023, kInf = 0x1p1022, kNan = 0x1p1023;
+__device__ __forceinline__ double placed(double b) {
+    return b != b ? kNan : b == -__builtin_inf() ? kOut : b == __builtin_inf() ? kInf : b;
+}
+__device__ __forceinline__ double key_bits(double b, u32 low) { return __builtin_bit_cast(double, (__builtin_bit_cast(u64, b) & ~1023ull) | low); }
+// A number as a key: its low ten bits give way to the expert's index (the lower, the larger).
 __device__ __forceinline__ double key_of(double b, int e) {
-    if (b != b) b = kNan;
-    else if (b == -__builtin_inf()) b = kOut;
-    else if (b == __builtin_inf()) b = kInf;
     const u64 v = __builtin_bit_cast(u64, b);
-    return __builtin_bit_cast(double, (v & ~1023ull) | (u32)((int)(v >> 32) < 0 ? e : 1023 - e));
+    return key_bits(b, (int)(v >> 32) < 0 ? e : 1023 - e);
 }
 __device__ __forceinline__ int expert_of_key(double k) {
     const u64 v = __builtin_bit_cast(u64, k);
@@ -294,12 +302,68 @@ __device__ __forceinline__ int choose64(const RouteParams& p, const float* logit
     }
     double list[KP];
 #pragma unroll
-    for (int i = 0; i < P; ++i) b[i] = key_of(b[i], i * 64 + lane);
+    for (int i = 0; i < P; ++i) {
+        b[i] = placed(b[i]);
+        rows[i * 64 + lane] = b[i];
+        b[i] = key_of(b[i], i * 64 + lane);
+    }
     largest<64, P, KP>(b, list, kOut * 1.5);
-    int id = -1;
+    double key = kOut, last_key = kOut;
 #pragma unroll
-    for (int c = 0; c < KP; ++c)
-        if (lane == c) id = expert_of_key(list[c]);
+    for (int c = 0; c < KP; ++c) {
+        if (lane == c) key = list[c];
+        if (c == p.topk - 1) last_key = list[c];
+    }
+    int id = expert_of_key(key);
+    if (p.by_logit) return id;
+    // Keys are numbers without their last bits (those of logits end before).  The choice is held against the numbers: each above the next,
+    // or equal to it by a lower index; and where experts beside the choices share the last one's bits, as many at or above it as choices.
+    lanes_wait();
+    const double at = id >= 0 ? rows[id] : kOut, next = after(at);
+    const int next_id = after(id);
+    bool wrong = lane + 1 < p.topk && next_id >= 0 && !(at > next || (at == next && id < next_id));
+    if (last_key > kOut) {
+        const double from = fmin(key_bits(last_key, 0), key_bits(last_key, 1023));
+        int near = 0;
+#pragma unroll
+        for (int i = 0; i < P; ++i) near += __popcll(__ballot(b[i] >= from));
+        if (near > p.topk) {
+            const u64 bits = __builtin_bit_cast(u64, at);
+            const u32 high = (u32)__builtin_amdgcn_readlane((int)(bits >> 32), p.topk - 1), low = (u32)__builtin_amdgcn_readlane((int)bits, p.topk - 1);
+            const double last = __builtin_bit_cast(double, (u64)high << 32 | low);
+            const int last_id = expert_of_key(last_key);
+            near = 0;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const double v = rows[i * 64 + lane];
+                near += __popcll(__ballot(v > last || (v == last && i * 64 + lane <= last_id)));
+            }
+            wrong = wrong || near != p.topk;
+        }
+    }
+    if (__ballot(wrong) != 0) {   // (numbers nearer than 2^-42 of their size and not equal, such as sigmoids near 1)
+#pragma unroll 1
+        for (int c = 0; c < p.topk; ++c) {
+            double best = kOut;
+            int who = N;
+#pragma unroll 1
+            for (int e = lane; e < N; e += 64)
+                if (rows[e] > best) {
+                    best = rows[e];
+                    who = e;
+                }
+            auto join = [&](double o, int w) {
+                if (o > best || (o == best && w < who)) {
+                    best = o;
+                    who = w;
+                }
+            };
+            join(other<1>(best), other<1>(who)); join(other<2>(best), other<2>(who)); join(other<4>(best), other<4>(who));
+            join(other<8>(best), other<8>(who)); join(other<16>(best), other<16>(who)); join(other<32>(best), other<32>(who));
+            if (lane == c) id = who < N ? who : -1;
+            if (who < N && (who & 63) == lane) rows[who] = kOut;   // (which this lane alone reads)
+        }
+    }
     return id;
 }
 
@@ -318,9 +382,8 @@ template <int LPT, int P, int KP, bool SOFTMAX>
 __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
     // for the tokens that need 64 bits, one of a wave at a time; and, of every token, the groups' scores
     __shared__ double rows64[kThreads / 64][LPT * P], sums64[kThreads / 64][kMaxGroups];
-    __shared__ float logits64[kThreads / 64][LPT * P];
     __shared__ f32x2 sums_of[kThreads / LPT][kMaxGroups];
-    __shared__ float rows_of[kThreads / LPT][LPT * P];   // b, for groups that are no run of lanes
+    __shared__ float rows_of[kThreads / LPT][LPT * P];   // b, for groups that are no run of lanes; then the logits, for 64 bits
     const int tid = threadIdx.x, sub = tid % LPT, mine = tid / LPT, wave = tid >> 6;
     const int64_t t = (int64_t)(blockIdx.x + p.vbase) * (kThreads / LPT) + mine;
     const int64_t row = t < p.tokens ? t : p.tokens - 1;   // (lanes past the last token keep the others company)
@@ -507,16 +570,13 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
     const u64 unsure = __ballot(!sure);
     if (unsure != 0) {
         constexpr u64 kLanes = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
+        each<P>([&](auto i) { rows_of[mine][expert_of<LPT>(sub, i)] = l[i]; });
+        lanes_wait();
 #pragma unroll 1
         for (int o = 0; o < 64 / LPT; ++o) {
             if (!(unsure >> (o * LPT) & kLanes)) continue;
             const bool its = (tid & 63) / LPT == o;
-            if (its)
-                each<P>([&](auto i) {
-                    logits64[wave][expert_of<LPT>(sub, i)] = l[i];
-                });
-            lanes_wait();
-            const int found = __shfl(choose64<LPT * P, KP, SOFTMAX>(p, logits64[wave], rows64[wave], sums64[wave]), sub);
+            const int found = __shfl(choose64<LPT * P, KP, SOFTMAX>(p, rows_of[wave * (64 / LPT) + o], rows64[wave], sums64[wave]), sub);
             lanes_wait();
             if (!its) continue;
             id = sub < p.topk ? found : -1;

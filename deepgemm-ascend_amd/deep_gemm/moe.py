@@ -67,7 +67,7 @@ def moe_route(logits: torch.Tensor, topk: int, scores: str = 'softmax', bias: Op
     Scores s are the ``softmax`` of a row or the ``sigmoid`` of each logit.  ``bias`` [E] (fp32; for balance) is added for the choice
     alone.  With ``num_groups`` > 1 (at most 64) the experts lie in that many groups of equal size, and the ``topk_groups`` groups whose
     ``group_top`` (1 or 2) best biased scores have the largest sum stay.  The topk best biased scores there are chosen, best first, equal
-    ones by the lowest index, compared as 64 bits give them (numbers nearer than 2^-42 relative count as equal).
+    ones by the lowest index, compared as 64 bits give them (without a bias, and with one group or ``group_top`` 1, as the logits are).
     ``renormalize``: weights s / (sum of the chosen s + 1e-20) instead of s; both times ``scale``.
 
     An expert whose logit or bias is -inf is never chosen; where fewer than topk are left, ids are -1 (dropped pairs for ``moe_sort``)

@@ -394,9 +394,10 @@ int dg_linear_xent_backward(const dg_linear_xent_args *args, void *stream);
  *   With num_groups > 1 (a divisor of experts, at most 64) a group's score is the sum of its group_top (1 or 2) largest b, and the topk_groups
  *   groups of the largest scores stay.  ids = the topk (at most 16) experts of the largest b there, largest first;
  *   weights = s[ids], renormalize: divided by (their sum + 1e-20), times scale.
- * Equal numbers go to the lowest index; b and the scores are compared as 64 bits give them.  An expert whose logit or bias is -inf
- * is out, and a group without experts too; a token that has fewer than topk left gets id -1 and weight 0 behind them.  NaN counts
- * as the largest number.
+ * Equal numbers go to the lowest index (-0 equals +0); b and the scores are compared as 64 bits give them, and where only the order
+ * of the logits counts (no bias; one group, or group_top 1) as these are.  An expert whose logit or bias is -inf is out, and a group
+ * without experts too (one with a single expert left has that one's b as its score); a token that has fewer than topk left gets id -1
+ * and weight 0 behind them.  NaN counts as the largest number.
  * The gradient: d_logits [tokens][experts] of d_weights; ids that are negative or past the last expert (DG_ERR_EXPERT_ID) have
  * none, ids of a token that repeat count as often.  ids and weights are [tokens][topk], without gaps.
  */

@@ -238,3 +238,18 @@ def test_closed_experts_beside_nan_stay_closed(kind):
         want, _ = ob.route(logits, 6, kind, closed, groups, keep)
         assert torch.equal(ids.cpu(), want)
         assert (closed[ids[ids >= 0].long().cpu()] > -INF).all()
+
+
+def test_numbers_in_64_bits_to_their_last():
+    """Scores that differ by a few of a double's last bits, or in none: sigmoids near 1, alone and under a bias."""
+    g = gen(31)
+    logits = 28 + 12 * torch.rand(60, 128, generator=g)
+    logits[::2] = logits[::2].round()
+    for bias in (torch.zeros(128), torch.randint(0, 3, (128,), generator=g) * 0.5):
+        _check(logits, 8, 'sigmoid', bias)
+        _check(logits, 16, 'sigmoid', bias)
+        _check(logits, 3, 'sigmoid', bias, num_groups=8, topk_groups=2)
+        _check(logits, 3, 'sigmoid', bias, num_groups=32, topk_groups=5)
+    far = torch.cat((logits, -logits), 1)   # (and among others far below)
+    _check(far, 16, 'sigmoid', torch.zeros(256), num_groups=4, topk_groups=3)
+    _check(torch.cat((far, far, far), 1), 16, 'sigmoid', torch.zeros(768))
