@@ -30,11 +30,11 @@ constexpr int64_t kMaxExtent = int64_t(1) << 30;
 inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // Workgroups [0, grid) of a kernel whose parameters hold the first one of a launch (vbase).  `cus` > 0 (set_num_sms
-// below the device's count): at most that many at a time, in launches one after another.
+// below the device's count): at most that many at a time, in launches one after another.  A launch has fewer than 2^32 threads.
 template <typename P>
 int launch_op(void (*kernel)(const P), int64_t grid, unsigned threads, P p, hipStream_t st, int cus, unsigned lds = 0) {
     if (grid > 0x7fffffffLL) return dg_set_error("too many workgroups");
-    const int64_t most = cus > 0 ? cus : std::max<int64_t>(grid, 1);
+    const int64_t most = std::min<int64_t>(cus > 0 ? cus : std::max<int64_t>(grid, 1), 0xffffffffLL / threads);
     for (int64_t base = 0; base < grid; base += most) {
         p.vbase = (int)base;
         hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(most, grid - base)), dim3(threads), lds, st, p);

@@ -178,3 +178,39 @@ def test_the_layers_decoding_step(tokens):
 
 def test_example_runs():
     ex.main(tokens=100)
+
+
+def _ends(n, k=5):
+    """The first rows, those around the end of a first launch of 2^32 threads, and the last."""
+    return [slice(0, k), slice(n // 2, n // 2 + k), slice(n - 40, n)]
+
+
+def test_routes_of_more_threads_than_one_launch_has():
+    t = (1 << 28) + 37                     # (16 threads to a token)
+    logits = torch.empty(t, 2, dtype=torch.bfloat16, device='cuda').normal_()
+    ids, w = deep_gemm.moe_route(logits, 1)
+    assert torch.equal(ids[:, 0] == 1, logits[:, 1] > logits[:, 0]) and (w == 1).all()
+    d = torch.ones(t, 1, device='cuda')
+    d_logits = deep_gemm.moe_route_backward(d, logits, ids, renormalize=False)
+    for part in _ends(t):
+        assert torch.equal(d_logits[part], deep_gemm.moe_route_backward(d[part], logits[part], ids[part], renormalize=False))
+
+
+def test_norms_of_more_threads_than_one_launch_has():
+    t, h = (1 << 22) + 41, 4104            # (1024 threads to a row)
+    x = torch.ones(t, h, dtype=torch.bfloat16, device='cuda')
+    for part in _ends(t):
+        x[part].normal_()
+    w = torch.ones(h, dtype=torch.bfloat16, device='cuda')
+    y, _, rstd = deep_gemm.rms_norm(x, w)
+    for part in _ends(t):
+        want = deep_gemm.rms_norm(x[part], w)
+        assert torch.equal(y[part], want[0]) and torch.equal(rstd[part], want[2])
+
+
+def test_activations_of_more_threads_than_one_launch_has():
+    m = 1 << 30                            # (four threads to a row)
+    h = torch.empty(m, 2, dtype=torch.bfloat16, device='cuda').normal_()
+    act = deep_gemm.swiglu(h)
+    for part in _ends(m):
+        assert torch.equal(act[part], deep_gemm.swiglu(h[part]))
