@@ -5,8 +5,9 @@
 // their readers), a second one multiplies them by b.  Both put the adapter's matrix on the side of the matrix instruction whose
 // results a lane holds four of, and the tokens on the other: a lane has consecutive values of one token.
 //
-// v enters the second product as the sum of two bf16 numbers, 2^-17 of it lost: an instruction of depth 32 takes 16 of them twice, the
-// high parts in its first half and the low parts in its second, against the same 16 columns of b.
+// v enters the second product as a sum of bf16 numbers: an instruction of depth 32 takes 16 of the rank twice, the high parts in its
+// first half and the low parts in its second, against the same 16 columns of b.  Two parts lose 2^-17, which the rounding of a bf16 d
+// hides; for an fp32 d the rest of v, which a third part holds whole, takes further instructions.
 #include "dg_common.hpp"
 #include "op_launch.hpp"
 
@@ -131,29 +132,43 @@ __global__ __launch_bounds__(kThreads) void lora_inner_kernel(const LoraParams p
     }
 }
 
-// The operand of the second product in LDS: high and low parts of 16 rows' v, [part][16 of the rank][token][16].
-template <int NT>
+// The operand of the second product in LDS: the parts of 16 rows' v, [part][16 of the rank][token][16], two for a d of bf16, three for
+// fp32.
+template <int NT, typename E>
 struct Operand {
-    uint16_t v[2][NT][16][16];
+    static constexpr int PARTS = sizeof(E) == 4 ? 3 : 2;
+    alignas(16) uint16_t v[PARTS][NT][16][16];
 
     // Four values of token lane & 15, from (lane >> 4) * 4 of the j-th sixteen on; zeros past the rank.
     __device__ __forceinline__ void put(int j, int lane, f32x4 s, float scale, int rank) {
         if (j * 16 + (lane >> 4) * 4 >= rank) s = f32x4{0.f, 0.f, 0.f, 0.f};
-        u32 high[2], low[2];
+        float rest[4];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float a = s[2 * q] * scale, b = s[2 * q + 1] * scale;
-            const u32 h = pack_bf16x2(a, b);
-            const float la = a - __builtin_bit_cast(float, h << 16), lb = b - __builtin_bit_cast(float, h & 0xffff0000u);
-            high[q] = h;
-            // (the low part beside an infinity is 0, not NaN)
-            low[q] = pack_bf16x2(fabsf(la) < __builtin_inff() ? la : 0.f, fabsf(lb) < __builtin_inff() ? lb : 0.f);
+        for (int q = 0; q < 4; ++q) rest[q] = s[q] * scale;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            u32 w[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float &a = rest[2 * q], &b = rest[2 * q + 1];
+                w[q] = pack_bf16x2(a, b);
+                a -= __builtin_bit_cast(float, w[q] << 16);
+                b -= __builtin_bit_cast(float, w[q] & 0xffff0000u);
+                // (the other parts beside an infinity are 0, not NaN)
+                a = fabsf(a) < __builtin_inff() ? a : 0.f;
+                b = fabsf(b) < __builtin_inff() ? b : 0.f;
+            }
+            *reinterpret_cast<i32x2*>(&v[part][j][lane & 15][(lane >> 4) * 4]) = i32x2{(int)w[0], (int)w[1]};
         }
-        *reinterpret_cast<i32x2*>(&v[0][j][lane & 15][(lane >> 4) * 4]) = i32x2{(int)high[0], (int)high[1]};
-        *reinterpret_cast<i32x2*>(&v[1][j][lane & 15][(lane >> 4) * 4]) = i32x2{(int)low[0], (int)low[1]};
     }
     __device__ __forceinline__ bf16x8 get(int j, int lane) const {
         return __builtin_bit_cast(bf16x8, *reinterpret_cast<const i32x4*>(&v[lane >> 5][j][lane & 15][((lane >> 4) & 1) * 8]));
+    }
+    // The third parts: of one sixteen of the rank, with zeros for the instruction's second half, or of two, one to each half.
+    static constexpr int THIRDS = NT >= 8 ? 2 : 1;
+    __device__ __forceinline__ bf16x8 third(int j, int lane) const {
+        const i32x4 w = *reinterpret_cast<const i32x4*>(&v[PARTS - 1][THIRDS > 1 ? j + (lane >> 5) : j][lane & 15][((lane >> 4) & 1) * 8]);
+        return __builtin_bit_cast(bf16x8, THIRDS > 1 || lane < 32 ? w : i32x4{0, 0, 0, 0});
     }
 };
 
@@ -237,16 +252,33 @@ __device__ __forceinline__ void load_columns(const LoraParams& p, int i, bool so
     }
 }
 
-template <int NT>
-__device__ __forceinline__ void outer_products(const bf16x8 (&b)[2][NT], const bf16x8 (&vs)[NT], float (&out)[8]) {
+// Third parts come from LDS as they are needed (held beside the others they cost waves: 4096 tokens, K=N=4096, fp32 d, rank 64 62 us in place
+// of 73, rank 128 106 of 120, and two sixteens to an instruction there: 106 of 108, rank 256 215 of 227; without third parts 72, 104 and 202).
+template <int NT, typename E>
+__device__ __forceinline__ void outer_products(const bf16x8 (&b)[2][NT], const bf16x8 (&vs)[NT], const Operand<NT, E>& operand, int lane, float (&out)[8]) {
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[h][j], vs[j], acc, 0, 0, 0);
+        for (int j = 0; j < NT; ++j) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[h][j], vs[j], acc[h], 0, 0, 0);
+    if constexpr (Operand<NT, E>::PARTS == 3) {
+        if constexpr (NT >= 4) __builtin_amdgcn_sched_barrier(0);
+        constexpr int AT_ONCE = Operand<NT, E>::THIRDS;
+        const bool upper = AT_ONCE > 1 && lane >= 32;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) out[h * 4 + q] = acc[q];
+        for (int j = 0; j < NT; j += AT_ONCE) {
+            const bf16x8 rest = operand.third(j, lane);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const i32x4 b0 = __builtin_bit_cast(i32x4, b[h][j]), b1 = __builtin_bit_cast(i32x4, b[h][j + AT_ONCE - 1]);
+                acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, upper ? b1 : b0), rest, acc[h], 0, 0, 0);
+            }
+        }
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) out[h * 4 + q] = acc[h][q];
 }
 
 // Those columns of 16 rows, straight from and to memory (t: the token of row lane & 15): for few tokens.
@@ -263,10 +295,10 @@ struct Columns {
         if (p.c != nullptr && n0 + 32 <= p.n) c.load(from);
         else c.load(from, p.c != nullptr ? p.n - at : 0);
     }
-    __device__ __forceinline__ void finish(const LoraParams& p, int t, int lane, int n0, const bf16x8 (&vs)[NT]) const {
+    __device__ __forceinline__ void finish(const LoraParams& p, int t, int lane, int n0, const bf16x8 (&vs)[NT], const Operand<NT, E>& operand) const {
         const int n = n0 + (lane >> 4) * 8;
         float out[8];
-        outer_products<NT>(b, vs, out);
+        outer_products<NT, E>(b, vs, operand, lane, out);
 #pragma unroll
         for (int q = 0; q < 8; ++q) out[q] += c.value(q);
         if (t >= 0) store_columns(reinterpret_cast<E*>(p.d) + t * p.d_ld + n, out, p.n - n);
@@ -296,8 +328,8 @@ __device__ __forceinline__ void copy_rows(const LoraParams& p, int64_t t) {
 }
 
 // The operands of TT times 16 rows of adapter i from the ranges' inner products, in order.
-template <int NT, int TT>
-__device__ __forceinline__ void gather_operand(const LoraParams& p, int i, bool some, int row0, Operand<NT> (&operand)[TT]) {
+template <int NT, int TT, typename E>
+__device__ __forceinline__ void gather_operand(const LoraParams& p, int i, bool some, int row0, Operand<NT, E> (&operand)[TT]) {
     const int lane = threadIdx.x & 63;
     const float scale = !some ? 0.f : p.scales != nullptr ? p.scales[i] : 1.f;
     for (int e = threadIdx.x; e < TT * NT * 64; e += kThreads) {
@@ -320,7 +352,7 @@ __device__ __forceinline__ void gather_operand(const LoraParams& p, int i, bool 
 // where these have no adapter.
 template <int NT, typename E>
 __global__ __launch_bounds__(kThreads) void lora_outer_kernel(const LoraParams p) {
-    __shared__ Operand<NT> operand[1];
+    __shared__ Operand<NT, E> operand[1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, index = blockIdx.x + p.vbase - p.copies;
     if (index < 0) {
         copy_rows<E>(p, (int64_t)(blockIdx.x + p.vbase) * 4 + wave);
@@ -338,14 +370,14 @@ __global__ __launch_bounds__(kThreads) void lora_outer_kernel(const LoraParams p
     int n0 = strip * p.strip_cols + wave * 32;
     Columns<NT, E> now, next;
     if (n0 < end) now.load(p, i, some, t, lane, n0);
-    gather_operand<NT, 1>(p, i, some, row0, operand);
+    gather_operand<NT, 1, E>(p, i, some, row0, operand);
     __syncthreads();
     bf16x8 vs[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) vs[j] = operand[0].get(j, lane);
     for (; n0 < end; n0 += 128) {
         if (AHEAD && n0 + 128 < end) next.load(p, i, some, t, lane, n0 + 128);
-        now.finish(p, t, lane, n0, vs);
+        now.finish(p, t, lane, n0, vs, operand[0]);
         if constexpr (AHEAD) now = next;
         else if (n0 + 128 < end) now.load(p, i, some, t, lane, n0 + 128);
     }
@@ -356,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void lora_outer_kernel(const LoraParams p
 // straight to memory in runs of 32 columns by 16 rows 43, by 64 rows 51, in LDS pieces of 512 columns without the next one 40).
 template <int NT, typename E>
 __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p) {
-    __shared__ Operand<NT> operand[2];
+    __shared__ Operand<NT, E> operand[2];
     __shared__ float delta[32][256 + 8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, index = blockIdx.x + p.vbase - p.copies;
     if (index < 0) {
@@ -385,7 +417,7 @@ __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p)
     };
     int n0 = strip * p.strip_cols;
     load(c, n0);
-    gather_operand<NT, 2>(p, i, some, row0, operand);
+    gather_operand<NT, 2, E>(p, i, some, row0, operand);
     __syncthreads();
     for (; n0 < end; n0 += 256) {
 #pragma unroll
@@ -400,7 +432,7 @@ __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) vs[j] = operand[s].get(j, lane);
                 float out[8];
-                outer_products<NT>(b, vs, out);
+                outer_products<NT, E>(b, vs, operand[s], lane, out);
                 f32x4* const to = reinterpret_cast<f32x4*>(&delta[s * 16 + (lane & 15)][at + (lane >> 4) * 8]);
                 to[0] = f32x4{out[0], out[1], out[2], out[3]};
                 to[1] = f32x4{out[4], out[5], out[6], out[7]};
@@ -436,7 +468,7 @@ __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p)
 template <int NT, typename E>
 __global__ __launch_bounds__(1024) void lora_kernel(const LoraParams p) {
     __shared__ f32x4 part[16][NT][64];
-    __shared__ Operand<NT> operand;
+    __shared__ Operand<NT, E> operand;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, index = blockIdx.x + p.vbase - p.copies;
     if (index < 0) {
         copy_rows<E>(p, (int64_t)(blockIdx.x + p.vbase) * 16 + wave);
@@ -475,7 +507,7 @@ __global__ __launch_bounds__(1024) void lora_kernel(const LoraParams p) {
     bf16x8 vs[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) vs[j] = operand.get(j, lane);
-    columns.finish(p, t, lane, n0, vs);
+    columns.finish(p, t, lane, n0, vs, operand);
 }
 
 typedef void (*LoraKernel)(const LoraParams);

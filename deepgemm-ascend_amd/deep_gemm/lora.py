@@ -35,7 +35,7 @@ def lora_gemm_nt(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, d: torch.Ten
     ``x`` [T, K], ``a`` [L, R, K] and ``b`` [L, N, R] are bf16, K and R multiples of 8, R at most 256 (adapters of lower rank have zeros);
     ``d`` [T, N] is bf16 or fp32, ``c`` (of its type) is d itself, a tensor that does not overlap it, or None for 0; ``scales`` [L] fp32 (None:
     1).  ``layout`` is ``moe_sort``'s of the tokens' adapter ids [T, 1], sorted once for every projection of a step; a small alignment
-    (32) suits few tokens.  The inner products are held in fp32 and enter the second product to 2^-17."""
+    (32) suits few tokens.  The inner products are held in fp32 and enter the second product whole for an fp32 d, to 2^-17 for a bf16 one."""
     ext = _operators(x)
     if ext is not None and ext.lora_gemm(x, a, b, d, layout, scales, c, cu_cap(), _stream(x)):
         return

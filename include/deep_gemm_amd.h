@@ -503,7 +503,8 @@ int dg_swiglu_backward(const dg_swiglu_args *args, void *stream);
  * x [tokens][k], a [adapters][rank][k] and b [adapters][n][rank] bf16 (k and rank multiples of 8, rank at most 256, x, a and b
  * 16-byte aligned rows), d and c of d_dtype, c NULL: 0, c = d: in place.  The layout is dg_moe_sort's of one choice a token over at
  * least as many groups as there are adapters (a group past the last adapter: DG_ERR_EXPERT_ID, its tokens keep c).
- * The inner products are summed in fp32 and enter the second product as the sum of two bf16 numbers (2^-17 relative).
+ * The inner products are summed in fp32 and enter the second product whole for an fp32 d, as the sum of two bf16 numbers (2^-17 relative) for
+ * a bf16 one.
  * The workspace (dg_lora_workspace_size bytes) holds nothing between calls.
  */
 typedef struct dg_lora_args {

@@ -141,3 +141,21 @@ def test_outputs_past_4_gib():
     for part in (torch.arange(3), torch.arange(t - 3, t)):
         want, mag = ob.lora(x[part], a, b, ids[part], scales, torch.ones(3, n))
         assert ((d[part].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + (90 * U32 + 2.0 ** -17) * mag).all()
+
+
+@pytest.mark.parametrize('t,adapters,rank,k,n', [(3, 3, 8, 64, 40), (40, 4, 24, 128, 300), (60, 20, 16, 8192, 256), (600, 3, 40, 96, 260),
+                                                 (520, 2, 128, 64, 300), (700, 40, 16, 64, 64), (12, 2, 256, 64, 72)])
+def test_fp32_outputs_hold_the_inner_products_in_full(t, adapters, rank, k, n):
+    """Two products of bf16 to an inner product, and one of the rank to a column: no sum hides what is cut on the way."""
+    g = gen(t + n)
+    x, a, b = torch.zeros(t, k), torch.randn(adapters, rank, k, generator=g), torch.zeros(adapters, n, rank)
+    x[:, 1], x[:, k - 3] = torch.randn(t, generator=g), torch.randn(t, generator=g)
+    b[:, torch.arange(n), torch.arange(n) % rank] = torch.randn(adapters, n, generator=g)
+    x, a, b = x.bfloat16(), a.bfloat16(), b.bfloat16()
+    ids, scales = torch.randint(0, adapters, (t,), generator=g), 0.5 + torch.rand(adapters, generator=g)
+    d = torch.empty(t, n, device='cuda')
+    deep_gemm.lora_gemm_nt(x.cuda(), a.cuda(), b.cuda(), d, _layout(ids, adapters), scales.cuda())
+    want, mag = ob.lora(x, a, b, ids, scales)
+    # The sum of two and its scale; the products of the inner product's parts (exact) in as many additions: at most eight steps of at
+    # most an unit in the last place each.
+    assert ((d.cpu().double() - want).abs() <= 16 * U32 * mag).all()
