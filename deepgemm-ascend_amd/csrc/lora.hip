@@ -575,6 +575,7 @@ int check(const dg_lora_args* a) {
     if (a->d_dtype != DG_DTYPE_BF16 && a->d_dtype != DG_DTYPE_F32) return dg_set_error("dg_lora: D is bf16 or fp32");
     if (a->layout->tokens != a->tokens || a->layout->topk != 1) return dg_set_error("dg_lora: the layout must be of one choice a token");
     if (a->layout->rows < 0 || a->layout->rows > kMaxExtent || a->layout->rows % 32 != 0) return dg_set_error("dg_lora: the layout's rows must be a multiple of 32");
+    if (a->layout->alignment % 32 != 0) return dg_set_error("dg_lora: the layout's alignment must be a multiple of 32");
     return DG_OK;
 }
 

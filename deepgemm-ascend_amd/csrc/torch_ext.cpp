@@ -876,6 +876,7 @@ bool lora_gemm(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, co
         return false;
     raise_pending();
     const c10::DeviceGuard guard(x.device());
+    l.alignment = 32;   // (every alignment that can be set is a multiple of it)
     dg_lora_args p = {};
     p.tokens = (int32_t)x.size(0);
     p.adapters = (int32_t)a.size(0);

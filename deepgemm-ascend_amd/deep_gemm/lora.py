@@ -73,7 +73,7 @@ def lora_gemm_nt(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, d: torch.Ten
     p.scales = scales.data_ptr() if scales is not None else None
     p.c, p.c_ld = (c.data_ptr(), _ld(c)) if c is not None else (None, 0)
     p.d, p.d_ld, p.d_dtype = d.data_ptr(), _ld(d), _DTYPES[d.dtype]
-    held = _layout_args(layout)
+    held = _layout_args(layout, alignment=32)   # (every alignment that can be set is a multiple of it)
     p.layout, p.num_cus = ctypes.pointer(held), cu_cap()
     lib, need = _lib.load(), ctypes.c_int64()
     _lib.check(lib.dg_lora_workspace_size(p, ctypes.byref(need)), lib)

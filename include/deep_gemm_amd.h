@@ -501,8 +501,9 @@ int dg_swiglu_backward(const dg_swiglu_args *args, void *stream);
  * Low-rank adapters of many requests beside a shared projection:
  *   d[t] = c[t] + scales[i] (x[t] a[i]^T) b[i]^T, i the adapter of token t; a token without one: d[t] = c[t]
  * x [tokens][k], a [adapters][rank][k] and b [adapters][n][rank] bf16 (k and rank multiples of 8, rank at most 256, x, a and b
- * 16-byte aligned rows), d and c of d_dtype, c NULL: 0, c = d: in place.  The layout is dg_moe_sort's of one choice a token over at
- * least as many groups as there are adapters (a group past the last adapter: DG_ERR_EXPERT_ID, its tokens keep c).
+ * 16-byte aligned rows), d and c of d_dtype, c NULL: 0, c = d: in place.  The layout is dg_moe_sort's of one choice a token, with an
+ * alignment and rows that are multiples of 32, over at least as many groups as there are adapters (a group past the last adapter:
+ * DG_ERR_EXPERT_ID, its tokens keep c).
  * The inner products are summed in fp32 and enter the second product whole for an fp32 d, as the sum of two bf16 numbers (2^-17 relative) for
  * a bf16 one.
  * The workspace (dg_lora_workspace_size bytes) holds nothing between calls.
@@ -519,7 +520,7 @@ typedef struct dg_lora_args {
     void *d;
     int64_t d_ld;
     int32_t d_dtype;              /* DG_DTYPE_BF16 or DG_DTYPE_F32                                         */
-    const dg_moe_layout *layout;  /* slots, source, m_indices and rows are read                            */
+    const dg_moe_layout *layout;  /* sizes, alignment, slots, source and m_indices are read                */
     void *workspace;
     int64_t workspace_bytes;
     int32_t num_cus;

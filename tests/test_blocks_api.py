@@ -229,3 +229,17 @@ def test_oracle_lora():
     for e in range(3):
         want = want + torch.where(ids == e, s[e], 0.0).double().unsqueeze(1) * (x.double() @ a[e].double().t() @ b[e].double().t())
     assert torch.allclose(ob.lora(x, a, b, ids, s, c)[0], want)
+
+
+def test_lora_refuses_layouts_whose_groups_start_anywhere(lib):
+    """A tile of 16 or 32 rows belongs to one adapter only where groups start at multiples of 32."""
+    a = _lib.LoraArgs()
+    for name in ('x', 'a', 'b', 'd', 'workspace'):
+        setattr(a, name, 4096)
+    a.tokens, a.adapters, a.rank, a.n, a.k = 64, 3, 16, 64, 128
+    a.x_ld, a.a_ld, a.a_stride, a.b_ld, a.b_stride, a.c_ld, a.d_ld = 128, 128, 2048, 16, 1024, 64, 64
+    for alignment in (1, 8, 16, 48):
+        held = _lib.MoELayoutArgs(64, 1, 3, 96, alignment, 4096, 4096, 4096, 4096)
+        a.layout = ctypes.pointer(held)
+        _refused(lib, lib.dg_lora_gemm(a, None), 'alignment')
+        _refused(lib, lib.dg_lora_workspace_size(a, ctypes.byref(ctypes.c_int64())), 'alignment')
