@@ -253,3 +253,17 @@ def test_numbers_in_64_bits_to_their_last():
     far = torch.cat((logits, -logits), 1)   # (and among others far below)
     _check(far, 16, 'sigmoid', torch.zeros(256), num_groups=4, topk_groups=3)
     _check(torch.cat((far, far, far), 1), 16, 'sigmoid', torch.zeros(768))
+
+
+@pytest.mark.parametrize('kind', ['softmax', 'sigmoid'])
+def test_small_weights_are_as_exact_as_large_ones(kind):
+    logits = -80 * torch.rand(200, 16, generator=gen(41))
+    logits[:, 3] = torch.rand(200, generator=gen(42))
+    ids, w = deep_gemm.moe_route(logits.cuda(), 16, kind, renormalize=False)
+    want = ob.scores(logits, kind).gather(1, ids.cpu().long())
+    # The exponential (2 units), softmax's sum of 16 (20 units at most, its largest terms exact to 4), a quotient and a product.  Softmax's
+    # exponent is a difference in fp32, off by half a step, 2^-24 |l - top| at most; exp(x + e) = exp(x) (1 + e), so by |l - top| units.
+    units = torch.tensor(8.0)
+    if kind == 'softmax':
+        units = 28 + (logits.max(1, keepdim=True).values - logits).double().gather(1, ids.cpu().long())
+    assert ((w.cpu().double() - want).abs() <= units * U32 * want).all()
