@@ -37,6 +37,9 @@ struct GateParams {
     int vbase;
 };
 
+// By the hardware's exponential of x / ln 2, whose argument's rounding costs up to |x| units of 2^-24 where x is negative (9 for x between -8
+// and -2, 30 down to -30); 0 below 2^-126.  With a full exponential 3 units, but few rows take 5.2 us in place of 4.5 (1248 x 2048 bf16)
+// and many to e4m3 70.3 in place of 67.4 (fp32 rows the same 152).  Rows of both types have the same fp32 values before they are rounded.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 
 // Exponent bytes of a tile, [block][row], to scale factors whose pairs start at any block (`block0`: the tile's first): as runs of two

@@ -38,6 +38,7 @@ def swiglu(h: torch.Tensor, fmt: Optional[str] = None, checkpoint: bool = False,
            zero_padding: bool = True):
     """act [M, F] = gate / (1 + exp(-gate)) * up of the rows ``h`` = (gate | up) [M, 2 F] (bf16 or fp32), in fp32, rounded once to their
     type; with ``fmt`` 'e4m3' or 'e2m1' the pair (codes, sf) that ``mx_quantize`` would give of the fp32 values (F a multiple of 32).
+    The fp32 values are off by up to |gate| + 4 units of 2^-24 for negative gates, and by 4 for others.
 
     ``checkpoint``: (act, saved), where saved is what ``mx_quantize(h, 'e4m3')`` gives, from the same read (F a multiple of 32).
     ``m_indices`` [M] int32 (as ``moe_sort`` gives it): rows with a negative entry are padding; they are not read, and are zeros in the
