@@ -463,8 +463,8 @@ __global__ __launch_bounds__(kThreads) void lora_rows_kernel(const LoraParams p)
 }
 
 // Few tokens: both products in one launch.  Every strip of 512 columns computes its tile's inner products for itself (sixteen waves, a
-// sixteenth of k each, from the XCD's L2), which costs less than a second launch that waits for the first: one token, rank 16, K=4096
-// N=7168 7.5 us.
+// sixteenth of k each, from the XCD's L2), which costs less than a second launch that waits for the first: one token, rank 16, K=2048
+// N=7168 5.5 us, by two launches 7.8.
 template <int NT, typename E>
 __global__ __launch_bounds__(1024) void lora_kernel(const LoraParams p) {
     __shared__ f32x4 part[16][NT][64];
@@ -554,8 +554,11 @@ int64_t live_tiles(const dg_lora_args* a, int rows) {
     return std::max<int64_t>(1, std::min<int64_t>(ceil_div(a->layout->rows, rows), ceil_div(a->tokens, rows) + std::min(a->tokens, a->adapters)));
 }
 
-// One launch where every strip has a CU to itself and reads little there for its inner products (a CU draws about 20 KB/us; 48 tokens over
-// 20 adapters, rank 16, K=7168 N=4096, 229 KB: 13.1 us, and by two launches 10.7; 511 tokens over 8, K=4096, 320 strips: 20.9 and 11.9).
+// One launch where every strip has a CU to itself and reads little there for its inner products: the adapter's matrix, once a strip.  By its
+// size, one launch and two in us on the device (adapters from HBM): 1 token, rank 16, N=7168 64 KB 5.5 and 7.8, 112 KB 7.1 and 8.6, 128 KB 7.8
+// and 7.3, 160 KB 9.1 and 7.7, 224 KB 11.2 and 8.6; 16 tokens, rank 32, N=4096 112 KB 9.1 and 10.0, 160 KB 11.4 and 10.3.  The second launch
+// costs the host 3 us (one token, 128 KB, calls behind each other from Python 7.9 and 11.2), so the limit lies past where the device
+// would have it.  511 tokens over 8 adapters, rank 16, K=N=4096, 320 strips: 21.5 and 11.4.
 bool one_launch(const dg_lora_args* a) {
     const int64_t bytes = (int64_t)padded_rank(a->rank) * a->k * 2;
     return padded_rank(a->rank) <= 64 && bytes <= (160 << 10) && live_tiles(a, 16) * ceil_div(a->n, 512) <= 256;
