@@ -180,8 +180,9 @@ struct BackwardRow {
 };
 
 // TEAMS of THREADS hold a row each and step through the tokens together; the next rows (bf16) are in flight while a row is summed.
-// d_weight is summed over a team's rows in registers, over the teams in LDS, in order.  8192 x 4096 bf16 52 us (5.2 TB/s; 82 with two
-// workgroups of one row a CU that read a row when they are done with the one before), and 5 for the partial sums.
+// d_weight is summed over a team's rows in registers, over the teams in LDS, in order.  8192 x 4096 bf16 51 us (5.2 TB/s, 32 bytes a lane
+// in scratch at the 128 registers that 1024 threads leave; 82 with two workgroups of one row a CU that read a row when they are done with
+// the one before), and 5 for the partial sums.
 template <typename E, int THREADS, int TEAMS, int V>
 __global__ __launch_bounds__(THREADS * TEAMS) void norm_backward_kernel(const NormParams p) {
     constexpr bool AHEAD = sizeof(E) == 2 && V <= 2;
