@@ -696,10 +696,10 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(const RoutePar
     }
 }
 
-// 32768 tokens over 256 experts in 8 groups: 27 us (36 MB; the bytes take 7), 16 of them or more VALU instructions (74 a logit: the exponentials, the
-// sorting of 16 keys a lane and the joining of four times eight are most), the rest the loads of two rounds of workgroups at four waves a
-// SIMD; 16 tokens 5.7, a chain of loads, sums and exchanges.  Logits in bf16 with a bias of zeros have many equal scores, which go through
-// 64 bits: 61.  Gradient: 8191 tokens over 160 experts 7.2.
+// 32768 tokens over 256 experts in 8 groups: 27 us (36 MB; the bytes take 7), 16 of them or more VALU instructions (74 a logit: the
+// exponentials, the sorting of 16 keys a lane and the joining of four times eight are most), the rest the loads of two rounds of workgroups
+// at four waves a SIMD; 16 tokens 5.7, a chain of loads, sums and exchanges.  Logits in bf16 with a bias of zeros have many equal scores,
+// which go through 64 bits: 61.  Gradient: 8191 tokens over 160 experts 7.2.
 typedef void (*RouteKernel)(const RouteParams);
 
 // Lanes to a token and experts to a lane: 16 lanes are a row whose exchanges are single instructions; past 256 experts more lanes.
